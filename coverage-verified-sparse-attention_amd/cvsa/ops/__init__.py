@@ -44,6 +44,13 @@ __all__ = [
     "quest_scores",
     "quest_refresh_scores",
     "QuestPageMeta",
+    "ChunkLayout",
+    "RotaryTable",
+    "qk_norm_rope",
+    "append_chunk_kv",
+    "prepare_append_chunk",
+    "reserve_chunk",
+    "chunk_attention",
 ]
 
 _DTYPE_CODE = {
@@ -1305,3 +1312,8 @@ class AppendCall:
         args[12] = n
         args[13] = next_free_block
         check(self.fn(*args), "append_kv")
+
+
+# Chunks of new tokens (uses the helpers above).
+from .chunk import (ChunkLayout, RotaryTable, append_chunk_kv, chunk_attention,  # noqa: E402
+                    prepare_append_chunk, qk_norm_rope, reserve_chunk)

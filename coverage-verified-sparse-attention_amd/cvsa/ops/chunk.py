@@ -1,0 +1,370 @@
+"""Chunks of new tokens: several per sequence, taken into the paged cache and
+attended from it.
+
+A prompt, a piece of one, a draft to be verified or a decode step is a ragged
+batch of new tokens (:class:`ChunkLayout`).  :func:`append_chunk_kv` writes
+its keys, normed and rotated on the way, and its values to the cache, and can
+rotate the queries in the same launch; :func:`chunk_attention` attends the
+queries over the cache.  :func:`qk_norm_rope` is the norm and rotation alone,
+for keys that stay outside the cache.
+
+None of these has a counterpart in the reference, whose harness leaves
+prefill to the model it wraps.  They serve; there is no backward pass.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_seqs, _device_of,
+               _i32, _lib, _ptr, _stream, check)
+
+
+class ChunkLayout:
+    """Which rows of a chunk's q, k and v belong to which sequence.
+
+    ``query_lens[b]`` new tokens of sequence b, 0 allowed; their rows follow
+    each other.  Made once per step and kept by the caller for all layers:
+    ``cu_seqlens`` ([B + 1] int32) on the device and the same offsets on the
+    host, from which the launches are shaped.
+    """
+
+    __slots__ = ("lens", "batch", "total", "longest", "cu_seqlens", "cu_host", "device")
+
+    def __init__(self, query_lens: Sequence[int], device="cuda"):
+        lens = tuple(int(n) for n in query_lens)
+        if not lens:
+            raise ValueError("chunk layout: no sequences")
+        if min(lens) < 0:
+            raise ValueError(f"chunk layout: negative chunk length {min(lens)}")
+        if sum(lens) > 1 << 24:
+            raise ValueError(f"chunk layout: {sum(lens)} tokens (at most {1 << 24})")
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        self.lens = lens
+        self.batch = len(lens)
+        self.total = cu[-1]
+        self.longest = max(lens)
+        self.cu_host = (ctypes.c_int32 * len(cu))(*cu)
+        self.cu_seqlens = torch.tensor(cu, dtype=torch.int32, device=device)
+        self.device = self.cu_seqlens.device
+
+
+class RotaryTable:
+    """Cosines and sines of every position's angles, kept by the caller.
+
+    ``table``: [positions, rot_dim] fp32, the cosines of the rot_dim / 2
+    angles, then their sines.  ``rot_dim`` is a multiple of 16; a head's
+    dimensions past it are not rotated.  Pair i is (i, i + rot_dim / 2) of
+    the head, or (2i, 2i + 1) with ``interleaved``.
+    """
+
+    __slots__ = ("table", "rot_dim", "max_positions", "interleaved")
+
+    def __init__(self, table: torch.Tensor, interleaved: bool = False):
+        if table.dim() != 2 or table.dtype != torch.float32:
+            raise ValueError("rotary table must be [positions, rot_dim] float32, got "
+                             f"{tuple(table.shape)} {table.dtype}")
+        if table.shape[0] < 1:
+            raise ValueError("rotary table holds no position")
+        if table.shape[1] < 16 or table.shape[1] % 16:
+            raise NotImplementedError(f"rotary table: rot_dim {table.shape[1]} is not a "
+                                      "multiple of 16")
+        self.table = table.contiguous()
+        if self.table.data_ptr() % 16:
+            self.table = self.table.clone()
+        self.max_positions, self.rot_dim = table.shape
+        self.interleaved = bool(interleaved)
+
+    @classmethod
+    def build(cls, rot_dim: int, max_positions: int, base: float = 10000.0, device="cuda",
+              interleaved: bool = False) -> "RotaryTable":
+        """Angles position * base^(-2i / rot_dim), taken in 64 bits (32 lose
+        the angle of far positions) and rounded once."""
+        i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
+        ang = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] \
+            * base ** (-i / rot_dim)
+        return cls(torch.cat([ang.cos(), ang.sin()], 1).to(torch.float32), interleaved)
+
+
+def _call(dev: torch.device, who: str, fn, *args) -> None:
+    """fn(*args, stream) on dev's current stream, whatever the current device."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, _stream(dev)), who)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(dev)), who)
+
+
+def _rows(who: str, name: str, t: torch.Tensor, rows: Optional[int], heads: Optional[int], D: int,
+          dtype=None) -> torch.Tensor:
+    """t as [>= rows, heads, D] rows that the kernels can read."""
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != D \
+            or (rows is not None and t.shape[0] < rows):
+        raise ValueError(f"{who}: {name} must be [{'tokens' if rows is None else rows}, "
+                         f"{'heads' if heads is None else heads}, {D}], got {tuple(t.shape)}")
+    if t.dtype not in _DTYPE_CODE or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{who}: {name} must be {dtype or 'bfloat16, float16 or float32'}, "
+                         f"got {t.dtype}")
+    unit = 4 if t.dtype == torch.float32 else 8
+    s = t.stride()
+    if s[2] != 1 or s[0] % unit or s[1] % unit or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _weights(who: str, D: int, *weights):
+    """Norm weights [D] of one dtype (None: no norm), and its code."""
+    dtype = None
+    out = []
+    for name, w in zip(("q_weight", "k_weight"), weights):
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != D or w.dtype not in _DTYPE_CODE:
+                raise ValueError(f"{who}: {name} must be [{D}] of a float dtype, got "
+                                 f"{tuple(w.shape)} {w.dtype}")
+            if dtype is not None and w.dtype != dtype:
+                raise ValueError(f"{who}: q_weight and k_weight differ in dtype")
+            dtype = w.dtype
+            w = w.contiguous()
+            if w.data_ptr() % 16:
+                w = w.clone()
+        out.append(w)
+    return out[0], out[1], _DTYPE_CODE[dtype or torch.float32]
+
+
+def _rotary(who: str, rotary: Optional[RotaryTable], D: int):
+    if rotary is None:
+        return None, 0, 0, 0
+    if rotary.rot_dim > D:
+        raise ValueError(f"{who}: rot_dim {rotary.rot_dim} exceeds the head dimension {D}")
+    return (rotary.table.data_ptr(), rotary.max_positions, rotary.rot_dim,
+            int(rotary.interleaved))
+
+
+def _check_layout(who: str, layout: ChunkLayout, dev: torch.device, batch: int) -> None:
+    if layout.device != dev:
+        raise ValueError(f"{who}: the layout is on {layout.device}, the tensors on {dev}")
+    if layout.batch != batch:
+        raise ValueError(f"{who}: the layout has {layout.batch} sequences, the tables {batch}")
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
+                 positions: Optional[torch.Tensor], rotary: Optional[RotaryTable] = None,
+                 q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """Norms of queries and keys for each head, with the position rotation.
+
+    q [T, H_q, D] and k [T, H_kv, D] (or None), bf16, fp16 or fp32, any token
+    and head strides (views of a fused projection are read in place).  Every
+    head's row becomes x * rsqrt(mean(x^2) + eps) * weight where a weight [D]
+    is given, then is rotated by ``rotary``'s entry of positions[t] ([T]
+    integers; None without rotation); a position outside the table gives NaN.
+    In 32 bits, rounded once to the inputs' dtype.  Returns contiguous
+    (q_out, k_out).
+    """
+    who = "qk_norm_rope"
+    dev = _device_of(q, k, positions, rotary.table if rotary else None, q_weight, k_weight)
+    q = _rows(who, "q", q, None, None, q.shape[-1])
+    T, H_q, D = q.shape
+    H_kv = 0
+    if k is not None:
+        k = _rows(who, "k", k, T, None, D, q.dtype)
+        if k.shape[0] != T:
+            raise ValueError(f"{who}: k has {k.shape[0]} tokens, q {T}")
+        H_kv = k.shape[1]
+    elif k_weight is not None:
+        raise ValueError(f"{who}: k_weight without k")
+    if rotary is None and q_weight is None and k_weight is None:
+        raise ValueError(f"{who}: neither a rotation nor a norm is asked for")
+    qw, kw, wcode = _weights(who, D, q_weight, k_weight)
+    rot = _rotary(who, rotary, D)
+    if rotary is not None:
+        if positions is None or positions.dim() != 1 or positions.is_floating_point():
+            raise ValueError(f"{who}: positions must be [{T}] integers")
+        _check_count(who, "positions", positions, T)
+        positions = _i32(positions)
+    q_out = torch.empty(T, H_q, D, device=dev, dtype=q.dtype)
+    k_out = None if k is None else torch.empty(T, H_kv, D, device=dev, dtype=k.dtype)
+    if T:
+        ks = (0, 0) if k is None else (k.stride(0), k.stride(1))
+        _call(dev, who, _lib.load().cvsa_qk_norm_rope, q.data_ptr(), q.stride(0), q.stride(1),
+              _ptr(k), *ks, _DTYPE_CODE[q.dtype], _ptr(positions) if rotary else None, *rot,
+              _ptr(qw), _ptr(kw), wcode, float(eps), T, H_q, H_kv, D, q_out.data_ptr(),
+              _ptr(k_out))
+    return q_out, k_out
+
+
+def _check_caches(who, k_cache, v_cache, block_size):
+    _check_cache(k_cache)
+    _check_cache(v_cache, "v_cache")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache shapes differ")
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"{who}: cache block_size mismatch")
+
+
+def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, layout, block_size,
+                         rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None):
+    """The checks of :func:`append_chunk_kv` without its launch: returns
+    (launch, q_out); launch() enqueues it."""
+    who = "append_chunk_kv"
+    dev = _device_of(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
+                     rotary.table if rotary else None)
+    _check_caches(who, k_cache, v_cache, block_size)
+    H_kv, D = k_cache.shape[2], k_cache.shape[3]
+    bt = _block_tables(block_tables)
+    ctx = _i32(context_lens)
+    B, W = bt.shape
+    _check_seqs(who, B, bt, ctx)
+    _check_layout(who, layout, dev, B)
+    T = layout.total
+    k = _rows(who, "k", k, T, H_kv, D)
+    v = _rows(who, "v", v, T, H_kv, D, k.dtype)
+    if q is None and q_weight is not None:
+        raise ValueError(f"{who}: q_weight without q")
+    qw, kw, wcode = _weights(who, D, q_weight, k_weight)
+    rot = _rotary(who, rotary, D)
+    q_out, H_q, qs = None, 0, (0, 0)
+    if q is not None:
+        q = _rows(who, "q", q, T, None, D, k.dtype)
+        H_q, qs = q.shape[1], (q.stride(0), q.stride(1))
+        q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        if q.shape[0] > T:
+            q_out[T:].zero_()
+    if D not in (32, 64, 128, 256):
+        raise NotImplementedError(f"{who}: D={D} not in {{32, 64, 128, 256}}")
+
+    def launch():
+        if T == 0:
+            return
+        _call(dev, who, _lib.load().cvsa_append_chunk_kv, k.data_ptr(), k.stride(0), k.stride(1),
+              v.data_ptr(), v.stride(0), v.stride(1), _ptr(q), *qs, _DTYPE_CODE[k.dtype],
+              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bt.data_ptr(),
+              bt.stride(0), W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T, *rot, _ptr(qw),
+              _ptr(kw), wcode, float(eps), H_q, H_kv, D, block_size, _ptr(q_out))
+    return launch, q_out
+
+
+def append_chunk_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, block_tables: torch.Tensor,
+                    context_lens: torch.Tensor, layout: ChunkLayout, block_size: int,
+                    rotary: Optional[RotaryTable] = None,
+                    k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                    q: Optional[torch.Tensor] = None,
+                    q_weight: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write a chunk's keys and values [T, H_kv, D] to the paged cache.
+
+    ``context_lens`` counts the chunk's tokens already and the block tables
+    hold their pages (SequenceKVManager.reserve_chunk, or a scheduler of the
+    caller's): token i of sequence b goes to position context_lens[b] -
+    layout.lens[b] + i.  Nothing but the cache rows is changed, so one layout
+    and one set of tables serve all layers.  Keys are normed (``k_weight``)
+    and rotated (``rotary``) on the way as in :func:`qk_norm_rope`, and with
+    ``q`` ([T, H_q, D]) the queries' norm and rotation by the same positions
+    are returned.  bf16, fp16 or fp32 rows, any token and head strides; the
+    cache is bf16.  A token whose position is negative, past the block table
+    or in a block outside the pool is not written.  Rows past layout.total
+    are not read; the returned q is zero there.
+    """
+    launch, q_out = prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens,
+                                         layout, block_size, rotary, k_weight, eps, q, q_weight)
+    launch()
+    return q_out
+
+
+def reserve_chunk(block_tables: torch.Tensor, context_lens: torch.Tensor,
+                  pages_allocated: torch.Tensor, layout: ChunkLayout, next_free_block: int,
+                  num_blocks: int, block_size: int) -> None:
+    """Pages for a chunk, by the rule of append_token_kv
+    (cvsa/runtime/kv_cache.py:133-150) for each of its tokens: context_lens
+    grows by the chunk's lengths and new pages take the blocks from
+    next_free_block on.  The three tensors are contiguous int32 and updated in
+    place; the caller has checked that tables and pool hold the chunk
+    (SequenceKVManager.reserve_chunk does)."""
+    who = "reserve_chunk"
+    dev = _device_of(block_tables, context_lens, pages_allocated)
+    for name, t in (("block_tables", block_tables), ("context_lens", context_lens),
+                    ("pages_allocated", pages_allocated)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous int32")
+    B = block_tables.shape[0] if block_tables.dim() == 2 else -1
+    _check_seqs(who, B, block_tables, context_lens)
+    _check_count(who, "pages_allocated", pages_allocated, B)
+    _check_layout(who, layout, dev, B)
+    _call(dev, who, _lib.load().cvsa_reserve_chunk, block_tables.data_ptr(),
+          block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+          pages_allocated.data_ptr(), layout.cu_seqlens.data_ptr(), B, next_free_block,
+          num_blocks, block_size)
+
+
+def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_tables: torch.Tensor, context_lens: torch.Tensor,
+                    layout: ChunkLayout, num_kv_heads: int, num_q_per_kv: int, block_size: int,
+                    causal: bool = True, scale: Optional[float] = None,
+                    max_context_len: int = 0, return_lse: bool = False,
+                    out: Optional[torch.Tensor] = None):
+    """Attention of a chunk's queries over the paged cache -> [T, H_q, D] bf16.
+
+    q [T, H_q, D] bf16, any token and head strides.  ``context_lens`` counts
+    the chunk's tokens: query i of sequence b has position context_lens[b] -
+    layout.lens[b] + i and sees the keys up to it, or with ``causal=False``
+    the whole context (an encoder's states, a bidirectional chunk).  Keys of
+    blocks outside the pool or past the block table take no part; a query
+    that sees no key gives zeros and a log-sum-exp of -inf.  ``scale``
+    defaults to D^-0.5.  ``max_context_len`` (most keys of a sequence, where
+    the caller knows) only shapes the launch.  With ``return_lse`` the natural
+    log-sum-exps [T, H_q] fp32 of the scaled scores are returned too.  Rows
+    past layout.total are zero in a new output and left as they are in ``out``
+    (contiguous bf16 of q's shape).
+
+    Scores, sums and outputs are held in 32 bits; the weights of the second
+    product are rounded to bf16.
+    """
+    who = "chunk_attention"
+    dev = _device_of(q, k_cache, v_cache, block_tables, context_lens, out)
+    _check_caches(who, k_cache, v_cache, block_size)
+    D = k_cache.shape[3]
+    if k_cache.shape[2] != num_kv_heads:
+        raise ValueError(f"{who}: head counts do not match the caches")
+    bt = _block_tables(block_tables)
+    ctx = _i32(context_lens)
+    B, W = bt.shape
+    _check_seqs(who, B, bt, ctx)
+    _check_layout(who, layout, dev, B)
+    T, H_q = layout.total, num_kv_heads * num_q_per_kv
+    q = _rows(who, "q", q, T, H_q, D, torch.bfloat16)
+    max_context_len = int(max_context_len)
+    if max_context_len < 0:
+        raise ValueError(f"{who}: max_context_len must not be negative")
+    scale = D ** -0.5 if scale is None else float(scale)
+    rows = q.shape[0]
+    if out is None:
+        out = torch.empty(rows, H_q, D, device=dev, dtype=torch.bfloat16)
+        if rows > T:
+            out[T:].zero_()
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        raise ValueError(f"{who}: out must be contiguous bfloat16 {tuple(q.shape)}")
+    lse = None
+    if return_lse:
+        lse = torch.empty(rows, H_q, device=dev, dtype=torch.float32)
+        if rows > T:
+            lse[T:].zero_()
+    if T:
+        L = _lib.load()
+        # Allocated for the call, so no two calls, streams or captured graphs
+        # share it.
+        need = L.cvsa_chunk_attention_workspace_bytes(layout.cu_host, B, H_q, num_kv_heads, D,
+                                                      block_size, W, max_context_len)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        _call(dev, who, L.cvsa_chunk_attention, q.data_ptr(), q.stride(0), q.stride(1),
+              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bt.data_ptr(),
+              bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(), layout.cu_host, B, H_q,
+              num_kv_heads, D, block_size, W, max_context_len, scale, int(bool(causal)),
+              out.data_ptr(), _ptr(lse), _ptr(ws), need)
+    return (out, lse) if return_lse else out

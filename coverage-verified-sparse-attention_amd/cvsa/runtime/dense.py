@@ -36,3 +36,13 @@ class DenseAttentionBackend:
         return ops.dense_decode(q, k_cache, v_cache, block_tables, context_lens,
                                 self.num_kv_heads, self.num_q_per_kv, self.block_size,
                                 work=work)
+
+    def prefill(self, q, k_cache, v_cache, block_tables, context_lens, layout, layer_idx=0,
+                causal=True, scale=None, max_context_len=0):
+        """Attention of a chunk of new tokens already in the cache:
+        [T, H_q, D] queries laid out by ``layout`` (ops.ChunkLayout) ->
+        [T, H_q, D].  No counterpart in the reference's backends, which only
+        decode."""
+        return ops.chunk_attention(q, k_cache, v_cache, block_tables, context_lens, layout,
+                                   self.num_kv_heads, self.num_q_per_kv, self.block_size,
+                                   causal=causal, scale=scale, max_context_len=max_context_len)

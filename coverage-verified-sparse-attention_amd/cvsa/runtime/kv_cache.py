@@ -9,7 +9,8 @@ a bump allocator hands out consecutive block ids, ``block_tables`` is
 MI355X differences: the manager keeps a host mirror of every context length
 and allocated-page count, so appending a decode token needs no device->host
 read; ``append_token_kv`` / ``append_tokens_kv`` launch the HIP append kernel
-(one launch for a whole batch) instead of per-sequence ``.item()`` calls.
+(one launch for a whole batch) instead of per-sequence ``.item()`` calls;
+``append_chunk_kv`` takes several tokens per sequence, rotated on the way.
 Block tables accept any block ids, so randomly permuted physical pages work.
 If ``block_tables`` / ``context_lens`` are edited directly, call
 ``sync_host_state()`` before the next append.
@@ -260,3 +261,56 @@ class SequenceKVManager:
             ops.append_kv(k, v, *buffers, seq_begin, self.cache._reserve(need),
                           self.block_size)
         self._commit_append(seqs)
+
+    def reserve_chunk(self, layout: "ops.ChunkLayout") -> None:
+        """Take a chunk's tokens into the tables: each context grows by its
+        chunk length and new pages get blocks, by append_token_kv's rule
+        (kv_cache.py:133-150).  One launch, no device read; the rows are
+        written by ops.append_chunk_kv."""
+        need, pages = self._plan_chunk(layout)
+        ops.reserve_chunk(self.block_tables, self.context_lens, self._pages_allocated_dev, layout,
+                          self.cache._next_free, self.cache._total_blocks, self.block_size)
+        self.cache._reserve(need)
+        self._pages_allocated = pages
+        self._ctx_host = [c + n for c, n in zip(self._ctx_host, layout.lens)]
+
+    def _plan_chunk(self, layout):
+        """(blocks a chunk takes, pages allocated after it); refuses a chunk
+        that the tables or the pool cannot hold."""
+        if layout.batch != self.batch_size:
+            raise ValueError(f"the layout has {layout.batch} sequences, the manager "
+                             f"{self.batch_size}")
+        bs, need, pages = self.block_size, 0, []
+        for s, (ctx, n, have) in enumerate(zip(self._ctx_host, layout.lens,
+                                               self._pages_allocated)):
+            last = -(-(ctx + n) // bs)
+            if last > self.max_pages:
+                raise IndexError(f"sequence {s}: context {ctx} + {n} exceeds the block table "
+                                 f"({self.max_pages} pages)")
+            new = max(0, last - max(have, -(-ctx // bs))) if n else 0
+            need += new
+            pages.append(have + new)
+        free = self.cache._total_blocks - self.cache._next_free
+        if need > free:
+            raise AssertionError(f"Out of blocks: need {need}, have {free}")
+        return need, pages
+
+    def append_chunk_kv(self, k: torch.Tensor, v: torch.Tensor, layout: "ops.ChunkLayout",
+                        rotary=None, k_weight=None, eps: float = 1e-6, q=None, q_weight=None):
+        """Append layout.lens[b] tokens to every sequence b: k, v
+        [T, H_kv, D], the keys normed and rotated on the way; with q
+        [T, H_q, D] its norm and rotation at the same positions are returned
+        (ops.append_chunk_kv).  Everything is checked before any state
+        changes."""
+        self._plan_chunk(layout)
+        if rotary is not None:
+            top = max((c + n for c, n in zip(self._ctx_host, layout.lens) if n), default=0)
+            if top > rotary.max_positions:
+                raise ValueError(f"position {top - 1} is outside the rotary table of "
+                                 f"{rotary.max_positions}")
+        launch, q_out = ops.prepare_append_chunk(
+            k, v, self.cache.k_cache, self.cache.v_cache, self.block_tables, self.context_lens,
+            layout, self.block_size, rotary, k_weight, eps, q, q_weight)
+        self.reserve_chunk(layout)
+        launch()
+        return q_out

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define CVSA_ABI_VERSION 14
+#define CVSA_ABI_VERSION 15
 
 enum {
   CVSA_OK = 0,
@@ -640,6 +640,90 @@ int cvsa_step_plan_run_append(cvsa_step_plan *plan, const uint16_t *q, void *out
                               const int32_t *slots, const int32_t *slots_dev,
                               int32_t *slot_errors, void *stream);
 void cvsa_step_plan_destroy(cvsa_step_plan *plan);
+
+/* ---------------------------------------------- chunks of new tokens
+ *
+ * A chunk is a ragged batch of new tokens: sequence b brings the rows
+ * [cu_seqlens[b], cu_seqlens[b + 1]) of q, k and v (cu_seqlens: [B + 1] int32,
+ * cu_seqlens[0] = 0; a sequence may bring none).  context_lens counts the
+ * chunk's tokens: token i of sequence b has position
+ * context_lens[b] - (cu_seqlens[b + 1] - cu_seqlens[b]) + i.  The block tables
+ * hold the blocks of its pages (cvsa_reserve_chunk).
+ *
+ * Rotation: `table` is [table_len, rot_dim] fp32, for each position the
+ * cosines of its rot_dim / 2 angles, then their sines; NULL: no rotation.
+ * rot_dim is a multiple of 16, at most D; dimensions past it are not rotated.
+ * Pair i is (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved = 1.  A
+ * position outside the table gives NaN.  Weights: [D] of weight_dtype; a
+ * NULL weight means no norm of that side.  Strides are in elements; rows and
+ * strides must be 16-byte aligned.  The arithmetic is fp32, rounded once.
+ */
+
+/* Norm x * rsqrt(mean(x^2) + eps) * weight of every head's row of q
+ * [tokens, H_q, D] and k [tokens, H_kv, D] (or NULL), then the rotation by
+ * the token's entry of positions ([tokens] int32, unused without a table).
+ * q_out / k_out: contiguous, of the inputs' dtype (CVSA_DTYPE_*). */
+int cvsa_qk_norm_rope(const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                      const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                      int32_t dtype, const int32_t *positions, const float *table,
+                      int64_t table_len, int32_t rot_dim, int32_t interleaved,
+                      const void *q_weight, const void *k_weight, int32_t weight_dtype,
+                      float eps, int32_t tokens, int32_t H_q, int32_t H_kv, int32_t D,
+                      void *q_out, void *k_out, void *stream);
+
+/* Writes the chunk's keys (normed and rotated on the way) and values to their
+ * rows of the paged cache, rounded to bf16; with q, its norm and rotation to
+ * q_out ([tokens, H_q, D] of dtype) in the same launch.  `tokens` is
+ * cu_seqlens[B].  context_lens and block_tables are read, not changed; a token
+ * whose position is negative, past the table or in a block outside the pool is
+ * not written. */
+int cvsa_append_chunk_kv(const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                         const void *v, int64_t v_stride_t, int64_t v_stride_h,
+                         const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                         int32_t dtype, uint16_t *k_cache, uint16_t *v_cache,
+                         int64_t num_blocks, const int32_t *block_tables,
+                         int64_t bt_stride_b, int32_t W, const int32_t *context_lens,
+                         const int32_t *cu_seqlens, int32_t B, int32_t tokens,
+                         const float *table, int64_t table_len, int32_t rot_dim,
+                         int32_t interleaved, const void *q_weight, const void *k_weight,
+                         int32_t weight_dtype, float eps, int32_t H_q, int32_t H_kv,
+                         int32_t D, int32_t block_size, void *q_out, void *stream);
+
+/* Pages for a chunk: adds each sequence's chunk length to context_lens and
+ * gives its new pages the blocks from next_free_block on, by the rule of
+ * append_token_kv (kv_cache.py:133-150) applied to each token, sequence after
+ * sequence.  pages_allocated ([B] int32) is updated; entries past W or
+ * num_blocks are not written (the caller checks both first). */
+int cvsa_reserve_chunk(int32_t *block_tables, int64_t bt_stride_b, int32_t W,
+                       int32_t *context_lens, int32_t *pages_allocated,
+                       const int32_t *cu_seqlens, int32_t B, int32_t next_free_block,
+                       int64_t num_blocks, int32_t block_size, void *stream);
+
+/* Bytes of the workspace of cvsa_chunk_attention (0: none needed, or a shape
+ * that it refuses).  cu_host: cu_seqlens in host memory; max_context_len: most
+ * keys of a sequence, or 0 when only the block table bounds them. */
+size_t cvsa_chunk_attention_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
+                                            int32_t H_kv, int32_t D, int32_t block_size,
+                                            int32_t W, int32_t max_context_len);
+
+/* Attention of the chunk's queries q ([cu[B], H_q, D] bf16) over the paged
+ * cache, softmax(scale q k^T) v over the keys at positions up to the query's
+ * (causal) or over the whole context.  Keys of blocks outside the pool do not
+ * take part; a row without keys gives zeros and a log-sum-exp of -inf.  A value
+ * that a row does not see (infinite or NaN ones too) does not touch it.
+ * cu_host: the same offsets in host memory.  out: [cu[B], H_q, D] bf16
+ * contiguous; lse: [cu[B], H_q] fp32 (natural logarithm) or NULL.  The
+ * workspace needs no initialisation and is free again when the call's kernels
+ * have run.  max_context_len only shapes the launch. */
+int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
+                         const uint16_t *k_cache, const uint16_t *v_cache,
+                         int64_t num_blocks, const int32_t *block_tables,
+                         int64_t bt_stride_b, const int32_t *context_lens,
+                         const int32_t *cu_seqlens, const int32_t *cu_host, int32_t B,
+                         int32_t H_q, int32_t H_kv, int32_t D, int32_t block_size,
+                         int32_t W, int32_t max_context_len, float scale, int32_t causal,
+                         uint16_t *out, float *lse, void *workspace,
+                         size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
