@@ -60,7 +60,7 @@ static void launch_chunk(const ChunkArgs &a, int row_waves, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.tiles * a.H_kv * a.splits));
   auto go = [&](auto rw) {
     constexpr int RW = decltype(rw)::value;
-    if constexpr (RW < 8 || D < 256)
+    if constexpr (RW < 8 || D == 64 || D == 128)
       hipLaunchKernelGGL((chunk_attention_kernel<D, RW>), grid,
                          dim3(RW * chunk_key_tiles<D>(RW) * 64), 0, s, a);
   };
@@ -84,7 +84,7 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_kv, int G, int D, in
   int64_t longest = 0;
   for (int b = 0; b < B; ++b) longest = std::max<int64_t>(longest, cu[b + 1] - cu[b]);
   const int64_t rows = longest * G;
-  p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || D == 256 ? 4 : 8;
+  p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || D == 256 || D == 32 ? 4 : 8;
   const int64_t tile_rows = p.row_waves * 32;
   int64_t tiles = 0;
   for (int b = 0; b < B; ++b)
@@ -160,6 +160,8 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
   CVSA_REQUIRE(chunk_shape_ok(cu_host, B, H_q, H_kv, D, block_size, W) && num_blocks > 0 &&
                    bt_stride_b >= W,
                CVSA_ERR_INVALID, "chunk_attention: bad sizes or chunk offsets (B=%d W=%d)", B, W);
+  CVSA_REQUIRE((int64_t)block_size * H_kv * D < (1 << 30), CVSA_ERR_UNSUPPORTED,
+               "chunk_attention: a block of %d tokens of %d heads is too large", block_size, H_kv);
   CVSA_REQUIRE(scale > 0.f && scale < INFINITY, CVSA_ERR_INVALID,
                "chunk_attention: scale must be positive and finite");
   CVSA_REQUIRE(max_context_len >= 0 && (causal == 0 || causal == 1), CVSA_ERR_INVALID,
@@ -182,7 +184,7 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
                "chunk_attention: too many row tiles");
   ChunkArgs a = {};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
-  a.k_cache = k_cache; a.v_cache = v_cache; a.num_blocks = num_blocks;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.num_blocks = (int)std::min<int64_t>(num_blocks, INT32_MAX);
   a.block_tables = block_tables; a.bt_sb = bt_stride_b; a.W = W;
   a.context_lens = context_lens; a.cu = cu_seqlens;
   a.B = B; a.H_q = H_q; a.H_kv = H_kv; a.G = H_q / H_kv; a.tokens = tokens;
