@@ -1,109 +1,228 @@
 // Attention of a chunk of new tokens over the paged cache: the join of split
-// keys, the launch plan and the entry points.  Kernel: chunk_attention.h.
-#include "chunk_attention.h"
+// keys, the launch plan and the entry points.  Sequences that bring few rows
+// (chunk_stream.h) and many (chunk_prefill.h) get a launch each.
+#include "chunk_prefill.h"
+#include "chunk_stream.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace cvsa {
 
 constexpr int kJoinThreads = 256;
 
-// The states of a row's splits joined in the order of the keys: a workgroup
-// per token, D / 4 threads per row.
+// The states of a row's splits joined in the order of the keys.  D / 4 threads
+// have a float4 of the row each; with few rows `groups` such groups share a
+// row's splits, and their sums are joined in LDS.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArgs a,
-                                                                  int tile_rows) {
-  const int tok = blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  int b = 0, n = a.B;
-  while (n > 1) {  // the last sequence with cu[b] <= tok, 64 candidates a look
-    const int step = (n + 63) / 64;
-    const bool le = lane * step < n && a.cu[b + lane * step] <= tok;
-    const int k = __popcll(__ballot(le)) - 1;
-    b += k * step;
-    n = min(step, n - k * step);
-  }
-  const int first = a.cu[b], len = a.cu[b + 1] - first, ctx = a.context_lens[b];
-  const int64_t rows = (int64_t)a.tokens * a.H_q;
-  for (int i = threadIdx.x; i < a.H_q * (D / 4); i += kJoinThreads) {
-    const int head = i / (D / 4), d = i % (D / 4) * 4;
-    const int row0 = ((tok - first) * a.G + head % a.G) / tile_rows * tile_rows;
-    const int keys = chunk_tile_keys(a, ctx - len, ctx, len * a.G, row0, tile_rows);
-    const int parts = min((keys + a.split_len - 1) / a.split_len, a.splits);
-    const int64_t at = (int64_t)tok * a.H_q + head;
-    float m = -INFINITY;
-    for (int s = 0; s < parts; ++s) m = fmaxf(m, a.part_ml[s * rows + at].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < parts; ++s) {
-      const float2 ml = a.part_ml[s * rows + at];
-      const float w = __builtin_amdgcn_exp2f(ml.x - ref);
-      const float4 v = *reinterpret_cast<const float4 *>(a.part_o + (s * rows + at) * D + d);
-      l = fmaf(ml.y, w, l);
-      o.x = fmaf(v.x, w, o.x);
-      o.y = fmaf(v.y, w, o.y);
-      o.z = fmaf(v.z, w, o.z);
-      o.w = fmaf(v.w, w, o.w);
+                                                                  const ChunkClass c,
+                                                                  int groups) {
+  constexpr int L = D / 4, NG = kJoinThreads / L;
+  __shared__ float4 s_o[NG][L];
+  __shared__ float2 s_ml[NG];
+  const int group = threadIdx.x / L, d = threadIdx.x % L * 4;
+  const int per_wg = NG / groups, part = group % groups;
+  const int64_t rows = (int64_t)c.tokens * a.H_q;
+  const int64_t want = (int64_t)blockIdx.x * per_wg + group / groups;
+  const int64_t from = min(want, rows - 1);
+  // The row's token in its class: its sequence and place in it.  The rows of a
+  // workgroup may be of several tokens; each lane looks for its own, a wave's
+  // lanes over the same sequences.
+  const int class_tok = (int)(from / a.H_q), head = (int)(from % a.H_q);
+  int tok = class_tok, first = 0, len = 0, seq = 0;
+  {
+    const int lane = threadIdx.x & 63;
+    int base = 0;  // tokens of the class before b0
+    for (int b0 = 0; b0 < a.B; b0 += kWave) {
+      const int b = b0 + lane;
+      const int lo = b < a.B ? a.cu[b] : 0;
+      int n = b < a.B ? a.cu[b + 1] - lo : 0;
+      if (n * a.G < c.min_rows || n * a.G > c.max_rows) n = 0;
+      const int end = base + (int)wave_incl_scan_u32((uint32_t)n);
+      const int total = __builtin_amdgcn_readlane(end, 63);
+      // the first sequence that ends past the token, by bisection over lanes
+      int l = 0;
+#pragma unroll
+      for (int step = 32; step > 0; step >>= 1)
+        if (__shfl(end, l + step - 1, 64) <= class_tok) l += step;
+      const int e = __shfl(end, l & 63, 64), m = __shfl(n, l & 63, 64),
+                f = __shfl(lo, l & 63, 64);
+      if (class_tok >= base && class_tok < total) {
+        seq = b0 + l;
+        first = f;
+        len = m;
+        tok = class_tok - (e - m);
+      }
+      base = total;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2 *>(a.out + at * D + d) =
-        make_uint2(chunk_cvt_bf16x2(o.x * inv, o.y * inv), chunk_cvt_bf16x2(o.z * inv, o.w * inv));
-    if (a.lse && d == 0)
-      a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
+  const int ctx = a.context_lens[seq];
+  const int row0 = (tok * a.G + head % a.G) / c.tile_rows * c.tile_rows;
+  const int keys = chunk_tile_keys(a, ctx - len, ctx, len * a.G, row0, c.tile_rows);
+  const int parts = min((keys + c.split_len - 1) / c.split_len, c.splits);
+  float m = -INFINITY;
+  for (int s = part; s < parts; s += groups) m = fmaxf(m, c.part_ml[s * rows + from].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float w, float sum, const float4 &v) {
+    l = fmaf(sum, w, l);
+    o.x = fmaf(v.x, w, o.x);
+    o.y = fmaf(v.y, w, o.y);
+    o.z = fmaf(v.z, w, o.z);
+    o.w = fmaf(v.w, w, o.w);
+  };
+#pragma unroll 4
+  for (int s = part; s < parts; s += groups) {
+    const float2 ml = c.part_ml[s * rows + from];
+    add(__builtin_amdgcn_exp2f(ml.x - ref), ml.y,
+        *reinterpret_cast<const float4 *>(c.part_o + (s * rows + from) * D + d));
+  }
+  if (groups > 1) {  // the same in every thread
+    s_o[group][d / 4] = o;
+    if (d == 0) s_ml[group] = make_float2(m, l);
+    __syncthreads();
+    if (part > 0) return;
+    for (int g = 1; g < groups; ++g) m = fmaxf(m, s_ml[group + g].x);
+    const float top = m == -INFINITY ? 0.f : m;
+    const float2 own = s_ml[group];
+    const float4 mine = o;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    add(__builtin_amdgcn_exp2f(own.x - top), own.y, mine);
+    for (int g = 1; g < groups; ++g) {
+      const float2 ml = s_ml[group + g];
+      add(__builtin_amdgcn_exp2f(ml.x - top), ml.y, s_o[group + g][d / 4]);
+    }
+  }
+  if (want >= rows) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = (int64_t)(first + tok) * a.H_q + head;
+  *reinterpret_cast<uint2 *>(a.out + at * D + d) =
+      make_uint2(chunk_cvt_bf16x2(o.x * inv, o.y * inv), chunk_cvt_bf16x2(o.z * inv, o.w * inv));
+  if (a.lse && d == 0)
+    a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// Groups of threads that share a row: as many as keep the GPU's CUs busy when
+// rows are few (one row of 64 splits: 64 loads in a row by one group, or 8 by
+// eight).
 template <int D>
-static void launch_chunk(const ChunkArgs &a, int row_waves, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.tiles * a.H_kv * a.splits));
-  auto go = [&](auto rw) {
-    constexpr int RW = decltype(rw)::value;
-    if constexpr (RW < 8 || D == 64 || D == 128)
-      hipLaunchKernelGGL((chunk_attention_kernel<D, RW>), grid,
-                         dim3(RW * chunk_key_tiles<D>(RW) * 64), 0, s, a);
-  };
-  if (row_waves == 1) go(std::integral_constant<int, 1>());
-  else if (row_waves == 2) go(std::integral_constant<int, 2>());
-  else if (row_waves == 4) go(std::integral_constant<int, 4>());
-  else go(std::integral_constant<int, 8>());
-  if (a.splits > 1)
-    hipLaunchKernelGGL(chunk_join_kernel<D>, dim3(a.tokens), dim3(kJoinThreads), 0, s, a,
-                       row_waves * 32);
+static void launch_join(const ChunkArgs &a, const ChunkClass &c, hipStream_t s) {
+  constexpr int NG = kJoinThreads / (D / 4);
+  const int64_t rows = (int64_t)c.tokens * a.H_q;
+  int groups = 1;
+  while (groups < NG && groups * 2 <= c.splits && rows * groups < 1024 * NG) groups *= 2;
+  const int per_wg = NG / groups;
+  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((unsigned)((rows + per_wg - 1) / per_wg)),
+                     dim3(kJoinThreads), 0, s, a, c, groups);
+}
+
+// Rows of a sequence and KV head that the stream kernel takes at most: two
+// tiles of a wave (one at D = 256, whose two tiles' outputs alone would fill a
+// wave's registers).
+template <int D>
+constexpr int chunk_few_rows() {
+  return D == 256 ? 32 : 64;
 }
 
 struct ChunkPlan {
-  int row_waves, tiles, splits, split_len;
+  ChunkClass few, many;  // tiles 0: no such sequence
+  size_t bytes;          // of the workspace
 };
 
-// Row waves of a workgroup and splits of the keys, from the chunk lengths and
-// the most keys a sequence can hold.
-static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_kv, int G, int D, int64_t max_keys) {
-  ChunkPlan p;
-  int64_t longest = 0;
-  for (int b = 0; b < B; ++b) longest = std::max<int64_t>(longest, cu[b + 1] - cu[b]);
-  const int64_t rows = longest * G;
-  p.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || D == 256 || D == 32 ? 4 : 8;
-  const int64_t tile_rows = p.row_waves * 32;
-  int64_t tiles = 0;
-  for (int b = 0; b < B; ++b)
-    tiles += ((int64_t)(cu[b + 1] - cu[b]) * G + tile_rows - 1) / tile_rows;
-  p.tiles = (int)tiles;
-  const int64_t items = std::max<int64_t>(1, tiles * H_kv);
-  // Splits of at least 512 keys, enough of them for four workgroups per CU.
-  const int64_t want = std::min<int64_t>((1024 + items - 1) / items, 64);
-  int64_t len = std::max<int64_t>(512, (max_keys + want - 1) / want);
+// Keys of a split: so many that the class makes about `want` workgroups, at
+// least `least` of them.  Two a CU: 8 sequences of 32K keys, 4 heads 110 us, 1024
+// workgroups 118, 2048 143; 32 ragged sequences of 8K, 8 heads 133, 141, 136.
+static void plan_splits(ChunkClass &c, int H_kv, int64_t max_keys, int64_t want, int64_t least) {
+  const int64_t items = (int64_t)c.tiles * H_kv;
+  int64_t len = std::max<int64_t>(least, (max_keys * items + want - 1) / want);
   len = (len + 127) / 128 * 128;
-  p.split_len = (int)len;
-  p.splits = items >= 512 ? 1 : (int)std::max<int64_t>(1, (max_keys + len - 1) / len);
+  c.split_len = (int)std::min<int64_t>(len, 1 << 30);
+  c.splits = (int)std::max<int64_t>(1, (max_keys + len - 1) / len);
+}
+
+template <int D>
+static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t max_keys) {
+  const int G = H_q / H_kv;
+  ChunkPlan p = {};
+  p.few.min_rows = 1;
+  p.few.max_rows = chunk_few_rows<D>();
+  p.many.min_rows = p.few.max_rows + 1;
+  p.many.max_rows = 0x7fffffff;
+  p.many.tile_rows = chunk_row_waves<D>() * 32;
+  int64_t most_few = 0;
+  for (int b = 0; b < B; ++b) {
+    const int64_t rows = (int64_t)(cu[b + 1] - cu[b]) * G;
+    if (rows <= p.few.max_rows) most_few = std::max(most_few, rows);
+  }
+  p.few.tile_rows = most_few > 32 ? 64 : 32;
+  for (int b = 0; b < B; ++b) {
+    const int n = cu[b + 1] - cu[b];
+    ChunkClass &c = (int64_t)n * G <= p.few.max_rows ? p.few : p.many;
+    c.tiles += (int)(((int64_t)n * G + c.tile_rows - 1) / c.tile_rows);
+    c.tokens += n;
+  }
+  plan_splits(p.few, H_kv, max_keys, 512, 256);
+  // Many rows: the number of splits whose rounds of 256 workgroups (one a CU)
+  // take least, at 1.4 us for 64 keys, 5 us for a workgroup's start and end and
+  // 4 TB/s for writing and joining the parts.
+  const double items = (double)p.many.tiles * H_kv;
+  double best = 1e30;
+  int64_t splits = 1;
+  for (int64_t n = 1; n <= 64 && (n == 1 || max_keys / n >= 512); ++n) {
+    const double rounds = std::ceil(items * n / 256);
+    const double us = rounds * ((double)max_keys / n / 64 * 1.4 + 5) +
+                      (n > 1 ? 4 + (double)p.many.tokens * H_q * n * D * 8 / 4e6 : 0);
+    if (us < best) {
+      best = us;
+      splits = n;
+    }
+  }
+  p.many.split_len = (int)(((max_keys + splits - 1) / splits + 127) / 128 * 128);
+  p.many.splits = (int)std::max<int64_t>(1, (max_keys + p.many.split_len - 1) / p.many.split_len);
+  for (ChunkClass *c : {&p.few, &p.many}) {
+    if (c->tiles == 0 || c->splits <= 1) continue;
+    const size_t rows = (size_t)c->splits * c->tokens * H_q;
+    c->part_ml = (float2 *)p.bytes;  // offsets until there is a workspace
+    p.bytes += (rows * sizeof(float2) + 255) / 256 * 256;
+    c->part_o = (float *)p.bytes;
+    p.bytes += (rows * D * sizeof(float) + 255) / 256 * 256;
+  }
   return p;
 }
 
-static size_t chunk_part_bytes(const ChunkPlan &p, int64_t rows, int D) {
-  if (p.splits <= 1) return 0;
-  const size_t ml = ((size_t)p.splits * rows * sizeof(float2) + 255) / 256 * 256;
-  return ml + (size_t)p.splits * rows * D * sizeof(float);
+static ChunkPlan plan_chunk_d(const int32_t *cu, int B, int H_q, int H_kv, int D,
+                              int64_t max_keys) {
+  if (D == 32) return plan_chunk<32>(cu, B, H_q, H_kv, max_keys);
+  if (D == 64) return plan_chunk<64>(cu, B, H_q, H_kv, max_keys);
+  if (D == 128) return plan_chunk<128>(cu, B, H_q, H_kv, max_keys);
+  return plan_chunk<256>(cu, B, H_q, H_kv, max_keys);
+}
+
+static int64_t chunk_grid(const ChunkClass &c, int H_kv) {
+  return (int64_t)c.tiles * H_kv * c.splits;
+}
+
+template <int D>
+static void launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
+  if (p.many.tiles > 0) {
+    hipLaunchKernelGGL(chunk_prefill_kernel<D>, dim3((unsigned)chunk_grid(p.many, a.H_kv)),
+                       dim3(chunk_row_waves<D>() * 64), 0, s, a, p.many);
+    if (p.many.splits > 1) launch_join<D>(a, p.many, s);
+  }
+  if (p.few.tiles > 0) {
+    const dim3 grid((unsigned)chunk_grid(p.few, a.H_kv)), block(chunk_stream_waves<D>() * 64);
+    if constexpr (chunk_few_rows<D>() > 32) {
+      if (p.few.tile_rows > 32)
+        hipLaunchKernelGGL((chunk_stream_kernel<D, 2>), grid, block, 0, s, a, p.few);
+    }
+    if (p.few.tile_rows <= 32)
+      hipLaunchKernelGGL((chunk_stream_kernel<D, 1>), grid, block, 0, s, a, p.few);
+    if (p.few.splits > 1) launch_join<D>(a, p.few, s);
+  }
 }
 
 static bool chunk_shape_ok(const int32_t *cu, int32_t B, int32_t H_q, int32_t H_kv, int32_t D,
@@ -131,9 +250,8 @@ extern "C" size_t cvsa_chunk_attention_workspace_bytes(const int32_t *cu_host, i
                                                        int32_t block_size, int32_t W,
                                                        int32_t max_context_len) {
   if (!chunk_shape_ok(cu_host, B, H_q, H_kv, D, block_size, W) || cu_host[B] == 0) return 0;
-  const ChunkPlan p = plan_chunk(cu_host, B, H_kv, H_q / H_kv, D,
-                                 chunk_max_keys(W, block_size, max_context_len));
-  return chunk_part_bytes(p, (int64_t)cu_host[B] * H_q, D);
+  return plan_chunk_d(cu_host, B, H_q, H_kv, D, chunk_max_keys(W, block_size, max_context_len))
+      .bytes;
 }
 
 extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
@@ -172,36 +290,32 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
                CVSA_ERR_INVALID, "chunk_attention: rows must be 16-byte aligned");
   const int32_t tokens = cu_host[B];
   if (tokens == 0) return CVSA_OK;
-  const ChunkPlan p = plan_chunk(cu_host, B, H_kv, H_q / H_kv, D,
-                                 chunk_max_keys(W, block_size, max_context_len));
-  const int64_t rows = (int64_t)tokens * H_q;
-  const size_t need = chunk_part_bytes(p, rows, D);
-  CVSA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need &&
-                             ((uintptr_t)workspace & 255) == 0),
+  ChunkPlan p = plan_chunk_d(cu_host, B, H_q, H_kv, D,
+                             chunk_max_keys(W, block_size, max_context_len));
+  CVSA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes &&
+                                ((uintptr_t)workspace & 255) == 0),
                CVSA_ERR_WORKSPACE,
-               "chunk_attention: needs a 256-byte aligned workspace of %zu bytes", need);
-  CVSA_REQUIRE((int64_t)p.tiles * H_kv * p.splits < (1LL << 31), CVSA_ERR_UNSUPPORTED,
-               "chunk_attention: too many row tiles");
+               "chunk_attention: needs a 256-byte aligned workspace of %zu bytes", p.bytes);
+  CVSA_REQUIRE(chunk_grid(p.few, H_kv) < (1LL << 31) && chunk_grid(p.many, H_kv) < (1LL << 31),
+               CVSA_ERR_UNSUPPORTED, "chunk_attention: too many row tiles");
+  for (ChunkClass *c : {&p.few, &p.many}) {
+    c->part_ml = (float2 *)((char *)workspace + (size_t)c->part_ml);
+    c->part_o = (float *)((char *)workspace + (size_t)c->part_o);
+  }
   ChunkArgs a = {};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
   a.k_cache = k_cache; a.v_cache = v_cache; a.num_blocks = (int)std::min<int64_t>(num_blocks, INT32_MAX);
   a.block_tables = block_tables; a.bt_sb = bt_stride_b; a.W = W;
   a.context_lens = context_lens; a.cu = cu_seqlens;
-  a.B = B; a.H_q = H_q; a.H_kv = H_kv; a.G = H_q / H_kv; a.tokens = tokens;
+  a.B = B; a.H_q = H_q; a.H_kv = H_kv; a.G = H_q / H_kv;
   a.bs_log2 = __builtin_ctz(block_size);
   a.c = scale * 1.4426950408889634f;
   a.causal = causal;
   a.out = out; a.lse = lse;
-  a.tiles = p.tiles; a.splits = p.splits; a.split_len = p.split_len;
-  if (p.splits > 1) {
-    a.part_ml = (float2 *)workspace;
-    a.part_o = (float *)((char *)workspace +
-                         ((size_t)p.splits * rows * sizeof(float2) + 255) / 256 * 256);
-  }
   const hipStream_t s = (hipStream_t)stream;
-  if (D == 32) launch_chunk<32>(a, p.row_waves, s);
-  else if (D == 64) launch_chunk<64>(a, p.row_waves, s);
-  else if (D == 128) launch_chunk<128>(a, p.row_waves, s);
-  else launch_chunk<256>(a, p.row_waves, s);
+  if (D == 32) launch_chunk<32>(a, p, s);
+  else if (D == 64) launch_chunk<64>(a, p, s);
+  else if (D == 128) launch_chunk<128>(a, p, s);
+  else launch_chunk<256>(a, p, s);
   return cvsa_host::check_launch("chunk_attention");
 }

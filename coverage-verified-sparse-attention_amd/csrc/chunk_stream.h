@@ -1,0 +1,244 @@
+// Chunk attention of few rows (up to 64 of a sequence and KV head): single
+// tokens, drafts, short chunks.  Reading K and V bounds it, so the kernel is
+// made to keep loads in flight.
+//
+// Every wave of a workgroup has all the rows (RT tiles of 32) and takes its own
+// tiles of 32 keys, in buffers of its own: two of K and two of V, no barrier
+// in the walk.  K of tile s + 2 is requested once tile s has been multiplied, V
+// likewise, so one to two tiles are under way at any time (64 to 128 KiB a CU
+// at D = 128).  The waves' states are joined at the end.
+#pragma once
+#include "chunk_common.h"
+
+namespace cvsa {
+
+template <int D>
+constexpr int chunk_stream_waves() {
+  return D == 256 ? 2 : 4;
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(chunk_stream_waves<D>() * 64, D * RT >= 256 ? 1 : 2) void
+chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
+  constexpr int NW = chunk_stream_waves<D>(), NT = NW * 64, KT = 32;
+  constexpr int CPR = D / 8, RPL = 64 / CPR;  // rows of a load
+  constexpr int P = KT / RPL;                 // loads of a tile of K or V
+  constexpr int KS = D / 16, DB = D / 32;
+  constexpr int kTile = KT * D;
+  __shared__ __align__(16) uint16_t s_k0[NW * kTile], s_k1[NW * kTile], s_v0[NW * kTile],
+      s_v1[NW * kTile];
+  __shared__ float2 s_ml[NW - 1][RT * 32];
+  __shared__ ChunkTaken<D> s_taken;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, half = lane >> 5;
+
+  int id = blockIdx.x;
+  const int h = id % a.H_kv;
+  id /= a.H_kv;
+  const int split = id % cl.splits;
+  const ChunkTile t = chunk_find_tile(a, cl, id / cl.splits);
+  const int k0 = split * cl.split_len;
+  // The last split also takes keys past the plan's bound.
+  const int k1 = split < cl.splits - 1 ? min(t.keys, k0 + cl.split_len) : t.keys;
+  if (cl.splits > 1 && k0 >= k1) return;
+
+  ChunkRow row[RT];
+  chunk_bf16x8_t q[RT][KS];
+  ChunkState<D> state[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    row[r] = chunk_row(a, t, h, t.row0 + r * 32 + l31, k1);
+    chunk_load_q<D>(a, t, row[r], q[r]);
+    state[r].init();
+  }
+  const int full_keys = a.causal ? min(t.pos0 + t.row0 / a.G + 1, k1) : k1;  // all rows see
+
+  const int32_t *const bt = a.block_tables + t.seq * a.bt_sb;
+  const int bs_mask = (1 << a.bs_log2) - 1;
+  const int row_bytes = a.H_kv * D * 2;
+  const uint32_t block_bytes = (uint32_t)row_bytes << a.bs_log2;
+
+  // The wave's s-th tile; lane i (mod 32) looks up its key i.
+  auto first_key = [&](int s) { return k0 + (s * NW + wave) * KT; };
+  const int mine = k1 - k0 - wave * KT;
+  const int steps = mine > 0 ? (mine + NW * KT - 1) / (NW * KT) : 0;
+  auto lookup = [&](int s) { return bt[min(first_key(s) + l31, k1 - 1) >> a.bs_log2]; };
+
+  uint32_t row_off[P];  // of the lane's vector of each load, in the block of the load's rows
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int r = p * RPL + lane / CPR;
+    row_off[p] = lane / CPR * row_bytes + (h * D + chunk_swizzle<D>(r, lane % CPR) * 8) * 2;
+  }
+  // A tile's K or V: block 0 in place of keys that are none (`at` in the key's
+  // lane).  The rows of a load lie in one block, but for 16 rows of 8-token
+  // pages (D = 32).
+  auto request = [&](const uint16_t *cache, int s, int at, uint16_t *lds) {
+    const uint32_t readable = s < steps ? block_bytes : 0;  // past the last tile: no fetch
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint16_t *const to = lds + wave * kTile + p * 512;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (RPL <= 8) {
+        chunk_load_lds(cache, __builtin_amdgcn_readlane(at, p * RPL), block_bytes, readable,
+                       row_off[p], ((first_key(s) + p * RPL) & bs_mask) * row_bytes, to);
+      } else {
+        const int r = p * RPL + lane / CPR;
+        const uint32_t blk = __shfl(at, r, 64);
+        const char *from = (const char *)cache + (uint64_t)blk * block_bytes +
+                           (uint32_t)(((first_key(s) + r) & bs_mask) * row_bytes) +
+                           (h * D + chunk_swizzle<D>(r, lane % CPR) * 8) * 2;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+      }
+    }
+  };
+
+  uint32_t ka[KS], va[DB][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) ka[ks] = wave * kTile * 2 + chunk_k_place<D>(ks);
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) va[d][i] = wave * kTile * 2 + chunk_v_place<D>(d, i);
+
+  s_taken.clear(NT);
+  __syncthreads();
+
+  int at2;                    // blocks of tile s + 2
+  uint64_t key0, key1, key2;  // keys of tiles s to s + 2
+  int found;                  // looked up of tile s + 3
+  auto locate = [&](int s, int looked_up, int &at) {
+    const bool ok = first_key(s) + l31 < k1 && (uint32_t)looked_up < (uint32_t)a.num_blocks;
+    at = ok ? looked_up : 0;
+    return __ballot(ok);
+  };
+  auto step = [&](int s, uint16_t *k_cur, uint16_t *v_cur) {
+    // The places as new values in each step: the buffer's address then goes
+    // into the instruction, where it would take registers of its own.
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(ka[ks]));
+#pragma unroll
+    for (int d = 0; d < DB; ++d) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
+    const int ahead = lookup(s + 3);
+    f32x16_t st[RT][1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint4 k = chunk_read_k((const char *)k_cur + ka[ks]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        st[r][0] = chunk_mfma(k, __builtin_bit_cast(uint4, q[r][ks]), ks ? st[r][0] : f32x16_t{});
+    }
+    __builtin_amdgcn_sched_barrier(0);  // K has been read
+    key2 = locate(s + 2, found, at2);
+    request(a.k_cache, s + 2, at2, k_cur);
+    found = ahead;
+    const bool whole = first_key(s) + KT <= full_keys && ~key0 == 0;
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) chunk_mask(st[r], key0, first_key(s), row[r].last_key);
+    }
+    uint4 pw[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) state[r].weights(st[r], a.c, pw[r], [](int) {});
+    if (!whole) {
+      // The wave's vectors of V, as they were loaded; they have arrived once
+      // the first of them has been waited for here.
+#pragma unroll 1
+      for (int p = 0; p < P; ++p) {
+        const int r = p * RPL + lane / CPR;
+        s_taken.clean(reinterpret_cast<uint4 *>(v_cur + wave * kTile + p * 512 + lane * 8),
+                      key0 >> r & 1, first_key(s) + r, chunk_swizzle<D>(r, lane % CPR) * 8);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const uint4 v = chunk_read_v((char *)v_cur + va[d][0] + 32 * j * D,
+                                     (char *)v_cur + va[d][1] + 32 * j * D);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) state[r].o[d] = chunk_mfma(v, pw[r][j], state[r].o[d]);
+      }
+    __builtin_amdgcn_sched_barrier(0);  // V has been read
+    request(a.v_cache, s + 2, at2, v_cur);
+    key0 = key1;
+    key1 = key2;
+  };
+  if (steps > 0) {
+    int at;
+    const int f0 = lookup(0), f1 = lookup(1);
+    found = lookup(2);
+    key0 = locate(0, f0, at);
+    request(a.k_cache, 0, at, s_k0);
+    request(a.v_cache, 0, at, s_v0);
+    key1 = locate(1, f1, at);
+    request(a.k_cache, 1, at, s_k1);
+    request(a.v_cache, 1, at, s_v1);
+    for (int s = 0; s < steps; s += 2) {
+      step(s, s_k0, s_v0);
+      if (s + 1 < steps) step(s + 1, s_k1, s_v1);
+    }
+    // No load may reach the buffers once they are the join's.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+  }
+
+  // The waves' states, joined in order by the first: an array of K or V for
+  // each other wave, float4 i of row r at place i ^ (r % 8).
+  static_assert(NW <= 4 && NW * kTile * 2 >= RT * 32 * D * 4, "room to join");
+  auto room = [&](int w) {
+    return reinterpret_cast<float4 *>(w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
+  };
+  auto place = [&](int r, int d, int g) {
+    return (r * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
+  };
+#pragma unroll
+  for (int r = 0; r < RT; ++r) state[r].finish();
+  __syncthreads();
+  if (wave > 0) {
+    float4 *const so = room(wave);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      if (half == 0) s_ml[wave - 1][r * 32 + l31] = make_float2(state[r].m, state[r].l);
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          so[place(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
+                                           state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
+    }
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    for (int w = 1; w < NW; ++w) {
+      const float4 *const so = room(w);
+      const float2 ml = s_ml[w - 1][r * 32 + l31];
+      const float nm = fmaxf(state[r].m, ml.x);
+      const float a0 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[r].m - nm);
+      const float a1 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - nm);
+      state[r].m = nm;
+      state[r].l = state[r].l * a0 + ml.y * a1;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 v = so[place(r, d, g)];
+          state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
+          state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
+          state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
+          state[r].o[d][4 * g + 3] = state[r].o[d][4 * g + 3] * a0 + v.w * a1;
+        }
+      }
+    }
+    s_taken.restore(row[r].last_key, state[r].o);
+    state[r].store(a, cl, t, row[r], split);
+  }
+}
+
+}  // namespace cvsa
