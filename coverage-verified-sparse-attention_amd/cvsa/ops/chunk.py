@@ -19,7 +19,9 @@ from typing import Optional, Sequence
 import torch
 
 from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_seqs, _device_of,
-               _i32, _lib, _ptr, _stream, check)
+               _i32, _lib, _ptr, check)
+
+_BF16 = torch.bfloat16
 
 
 class ChunkLayout:
@@ -31,7 +33,8 @@ class ChunkLayout:
     host, from which the launches are shaped.
     """
 
-    __slots__ = ("lens", "batch", "total", "longest", "cu_seqlens", "cu_host", "device")
+    __slots__ = ("lens", "batch", "total", "longest", "cu_seqlens", "cu_host", "device",
+                 "_workspace_bytes")
 
     def __init__(self, query_lens: Sequence[int], device="cuda"):
         lens = tuple(int(n) for n in query_lens)
@@ -51,6 +54,7 @@ class ChunkLayout:
         self.cu_host = (ctypes.c_int32 * len(cu))(*cu)
         self.cu_seqlens = torch.tensor(cu, dtype=torch.int32, device=device)
         self.device = self.cu_seqlens.device
+        self._workspace_bytes = {}  # of chunk_attention, by the call's sizes
 
 
 class RotaryTable:
@@ -90,51 +94,70 @@ class RotaryTable:
         return cls(torch.cat([ang.cos(), ang.sin()], 1).to(torch.float32), interleaved)
 
 
-def _call(dev: torch.device, who: str, fn, *args) -> None:
-    """fn(*args, stream) on dev's current stream, whatever the current device."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, _stream(dev)), who)
+def _same_device(*tensors: Optional[torch.Tensor]) -> torch.device:
+    """_device_of for the calls of every step: one look at each tensor."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            return _device_of(*tensors)  # raises
+    return tensors[0].device
+
+
+def _call(dev: torch.device, who: str, fn, *args, keep=None) -> None:
+    """fn(*args, stream) on dev's current stream, whatever the current device;
+    `keep` lives until the launch."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, _stream(dev)), who)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, who)
 
 
 def _rows(who: str, name: str, t: torch.Tensor, rows: Optional[int], heads: Optional[int], D: int,
-          dtype=None) -> torch.Tensor:
-    """t as [>= rows, heads, D] rows that the kernels can read."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != D \
-            or (rows is not None and t.shape[0] < rows):
+          dtype=None):
+    """t as [>= rows, heads, D] rows that the kernels can read: (t, address,
+    token stride, head stride)."""
+    shape, dt = t.shape, t.dtype
+    if len(shape) != 3 or shape[2] != D or (heads is not None and shape[1] != heads) \
+            or (rows is not None and shape[0] < rows):
         raise ValueError(f"{who}: {name} must be [{'tokens' if rows is None else rows}, "
-                         f"{'heads' if heads is None else heads}, {D}], got {tuple(t.shape)}")
-    if t.dtype not in _DTYPE_CODE or (dtype is not None and t.dtype != dtype):
+                         f"{'heads' if heads is None else heads}, {D}], got {tuple(shape)}")
+    if (dt is not dtype) if dtype is not None else (dt not in _DTYPE_CODE):
         raise ValueError(f"{who}: {name} must be {dtype or 'bfloat16, float16 or float32'}, "
-                         f"got {t.dtype}")
-    unit = 4 if t.dtype == torch.float32 else 8
-    s = t.stride()
-    if s[2] != 1 or s[0] % unit or s[1] % unit or t.data_ptr() % 16:
+                         f"got {dt}")
+    st, sh, sd = t.stride()
+    at = t.data_ptr()
+    if sd != 1 or (st | sh) & (3 if dt is torch.float32 else 7) or at & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-    return t
+        st, sh, sd = t.stride()
+        at = t.data_ptr()
+    return t, at, st, sh
 
 
-def _weights(who: str, D: int, *weights):
+def _weights(who: str, D: int, q_weight, k_weight):
     """Norm weights [D] of one dtype (None: no norm), and its code."""
-    dtype = None
-    out = []
-    for name, w in zip(("q_weight", "k_weight"), weights):
-        if w is not None:
-            if w.dim() != 1 or w.shape[0] != D or w.dtype not in _DTYPE_CODE:
-                raise ValueError(f"{who}: {name} must be [{D}] of a float dtype, got "
-                                 f"{tuple(w.shape)} {w.dtype}")
-            if dtype is not None and w.dtype != dtype:
-                raise ValueError(f"{who}: q_weight and k_weight differ in dtype")
-            dtype = w.dtype
-            w = w.contiguous()
-            if w.data_ptr() % 16:
-                w = w.clone()
-        out.append(w)
-    return out[0], out[1], _DTYPE_CODE[dtype or torch.float32]
+    if q_weight is None and k_weight is None:
+        return None, None, 0
+    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
+        raise ValueError(f"{who}: q_weight and k_weight differ in dtype")
+    return (_weight(who, "q_weight", q_weight, D), _weight(who, "k_weight", k_weight, D),
+            _DTYPE_CODE[(k_weight if q_weight is None else q_weight).dtype])
+
+
+def _weight(who: str, name: str, w, D: int):
+    if w is None:
+        return None
+    if w.dim() != 1 or w.shape[0] != D or w.dtype not in _DTYPE_CODE:
+        raise ValueError(f"{who}: {name} must be [{D}] of a float dtype, got "
+                         f"{tuple(w.shape)} {w.dtype}")
+    if not w.is_contiguous() or w.data_ptr() & 15:
+        w = w.contiguous().clone()
+    return w
 
 
 def _rotary(who: str, rotary: Optional[RotaryTable], D: int):
@@ -146,11 +169,22 @@ def _rotary(who: str, rotary: Optional[RotaryTable], D: int):
             int(rotary.interleaved))
 
 
-def _check_layout(who: str, layout: ChunkLayout, dev: torch.device, batch: int) -> None:
+def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, context_lens):
+    """Block tables and context lengths as the kernels read them."""
+    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 \
+            or block_tables.stride(1) != 1:
+        block_tables = _block_tables(block_tables)
+    if context_lens.dtype is not torch.int32 or not context_lens.is_contiguous():
+        context_lens = _i32(context_lens)
+    B = layout.batch
     if layout.device != dev:
         raise ValueError(f"{who}: the layout is on {layout.device}, the tensors on {dev}")
-    if layout.batch != batch:
-        raise ValueError(f"{who}: the layout has {layout.batch} sequences, the tables {batch}")
+    if block_tables.shape[0] != B:
+        raise ValueError(f"{who}: the layout has {B} sequences, the tables "
+                         f"{block_tables.shape[0]}")
+    if context_lens.dim() != 1 or context_lens.shape[0] != B:
+        _check_seqs(who, B, None, context_lens)
+    return block_tables, context_lens
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
@@ -168,12 +202,12 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
     (q_out, k_out).
     """
     who = "qk_norm_rope"
-    dev = _device_of(q, k, positions, rotary.table if rotary else None, q_weight, k_weight)
-    q = _rows(who, "q", q, None, None, q.shape[-1])
+    dev = _same_device(q, k, positions, rotary.table if rotary else None, q_weight, k_weight)
+    q, *q_at = _rows(who, "q", q, None, None, q.shape[-1])
     T, H_q, D = q.shape
-    H_kv = 0
+    H_kv, k_at = 0, (None, 0, 0)
     if k is not None:
-        k = _rows(who, "k", k, T, None, D, q.dtype)
+        k, *k_at = _rows(who, "k", k, T, None, D, q.dtype)
         if k.shape[0] != T:
             raise ValueError(f"{who}: k has {k.shape[0]} tokens, q {T}")
         H_kv = k.shape[1]
@@ -187,25 +221,29 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
         if positions is None or positions.dim() != 1 or positions.is_floating_point():
             raise ValueError(f"{who}: positions must be [{T}] integers")
         _check_count(who, "positions", positions, T)
-        positions = _i32(positions)
-    q_out = torch.empty(T, H_q, D, device=dev, dtype=q.dtype)
-    k_out = None if k is None else torch.empty(T, H_kv, D, device=dev, dtype=k.dtype)
+        if positions.dtype is not torch.int32 or not positions.is_contiguous():
+            positions = _i32(positions)
+    q_out = q.new_empty((T, H_q, D))
+    k_out = None if k is None else q.new_empty((T, H_kv, D))
     if T:
-        ks = (0, 0) if k is None else (k.stride(0), k.stride(1))
-        _call(dev, who, _lib.load().cvsa_qk_norm_rope, q.data_ptr(), q.stride(0), q.stride(1),
-              _ptr(k), *ks, _DTYPE_CODE[q.dtype], _ptr(positions) if rotary else None, *rot,
-              _ptr(qw), _ptr(kw), wcode, float(eps), T, H_q, H_kv, D, q_out.data_ptr(),
-              _ptr(k_out))
+        _call(dev, who, _lib.load().cvsa_qk_norm_rope, *q_at, *k_at, _DTYPE_CODE[q.dtype],
+              _ptr(positions) if rotary else None, *rot, _ptr(qw), _ptr(kw), wcode, float(eps), T,
+              H_q, H_kv, D, q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
 def _check_caches(who, k_cache, v_cache, block_size):
-    _check_cache(k_cache)
-    _check_cache(v_cache, "v_cache")
-    if k_cache.shape != v_cache.shape:
+    """The caches' (num_blocks, H_kv, D)."""
+    shape = k_cache.shape
+    if len(shape) != 4 or k_cache.dtype is not _BF16 or v_cache.dtype is not _BF16 \
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        _check_cache(k_cache)
+        _check_cache(v_cache, "v_cache")
+    if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache shapes differ")
-    if k_cache.shape[1] != block_size:
+    if shape[1] != block_size:
         raise ValueError(f"{who}: cache block_size mismatch")
+    return shape[0], shape[2], shape[3]
 
 
 def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, layout, block_size,
@@ -213,28 +251,24 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
     """The checks of :func:`append_chunk_kv` without its launch: returns
     (launch, q_out); launch() enqueues it."""
     who = "append_chunk_kv"
-    dev = _device_of(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
-                     rotary.table if rotary else None)
-    _check_caches(who, k_cache, v_cache, block_size)
-    H_kv, D = k_cache.shape[2], k_cache.shape[3]
-    bt = _block_tables(block_tables)
-    ctx = _i32(context_lens)
+    dev = _same_device(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
+                       rotary.table if rotary else None)
+    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
+    bt, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
-    _check_seqs(who, B, bt, ctx)
-    _check_layout(who, layout, dev, B)
     T = layout.total
-    k = _rows(who, "k", k, T, H_kv, D)
-    v = _rows(who, "v", v, T, H_kv, D, k.dtype)
+    k, *k_at = _rows(who, "k", k, T, H_kv, D)
+    v, *v_at = _rows(who, "v", v, T, H_kv, D, k.dtype)
     if q is None and q_weight is not None:
         raise ValueError(f"{who}: q_weight without q")
     qw, kw, wcode = _weights(who, D, q_weight, k_weight)
     rot = _rotary(who, rotary, D)
-    q_out, H_q, qs = None, 0, (0, 0)
+    q_out, H_q, q_at = None, 0, (None, 0, 0)
     if q is not None:
-        q = _rows(who, "q", q, T, None, D, k.dtype)
-        H_q, qs = q.shape[1], (q.stride(0), q.stride(1))
-        q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        if q.shape[0] > T:
+        q, *q_at = _rows(who, "q", q, T, None, D, k.dtype)
+        rows, H_q, _ = q.shape
+        q_out = q.new_empty((rows, H_q, D))
+        if rows > T:
             q_out[T:].zero_()
     if D not in (32, 64, 128, 256):
         raise NotImplementedError(f"{who}: D={D} not in {{32, 64, 128, 256}}")
@@ -242,11 +276,12 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
     def launch():
         if T == 0:
             return
-        _call(dev, who, _lib.load().cvsa_append_chunk_kv, k.data_ptr(), k.stride(0), k.stride(1),
-              v.data_ptr(), v.stride(0), v.stride(1), _ptr(q), *qs, _DTYPE_CODE[k.dtype],
-              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bt.data_ptr(),
-              bt.stride(0), W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T, *rot, _ptr(qw),
-              _ptr(kw), wcode, float(eps), H_q, H_kv, D, block_size, _ptr(q_out))
+        # k, v and q are held here: they may be copies.
+        _call(dev, who, _lib.load().cvsa_append_chunk_kv, *k_at, *v_at, *q_at,
+              _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
+              bt.data_ptr(), bt.stride(0), W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
+              *rot, _ptr(qw), _ptr(kw), wcode, float(eps), H_q, H_kv, D, block_size,
+              _ptr(q_out), keep=(k, v, q))
     return launch, q_out
 
 
@@ -292,10 +327,9 @@ def reserve_chunk(block_tables: torch.Tensor, context_lens: torch.Tensor,
                     ("pages_allocated", pages_allocated)):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be contiguous int32")
-    B = block_tables.shape[0] if block_tables.dim() == 2 else -1
-    _check_seqs(who, B, block_tables, context_lens)
+    block_tables, context_lens = _tables(who, layout, dev, block_tables, context_lens)
+    B = layout.batch
     _check_count(who, "pages_allocated", pages_allocated, B)
-    _check_layout(who, layout, dev, B)
     _call(dev, who, _lib.load().cvsa_reserve_chunk, block_tables.data_ptr(),
           block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
           pages_allocated.data_ptr(), layout.cu_seqlens.data_ptr(), B, next_free_block,
@@ -326,25 +360,21 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     product are rounded to bf16.
     """
     who = "chunk_attention"
-    dev = _device_of(q, k_cache, v_cache, block_tables, context_lens, out)
-    _check_caches(who, k_cache, v_cache, block_size)
-    D = k_cache.shape[3]
-    if k_cache.shape[2] != num_kv_heads:
+    dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out)
+    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
+    if H_kv != num_kv_heads:
         raise ValueError(f"{who}: head counts do not match the caches")
-    bt = _block_tables(block_tables)
-    ctx = _i32(context_lens)
+    bt, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
-    _check_seqs(who, B, bt, ctx)
-    _check_layout(who, layout, dev, B)
     T, H_q = layout.total, num_kv_heads * num_q_per_kv
-    q = _rows(who, "q", q, T, H_q, D, torch.bfloat16)
+    q, *q_at = _rows(who, "q", q, T, H_q, D, _BF16)
     max_context_len = int(max_context_len)
     if max_context_len < 0:
         raise ValueError(f"{who}: max_context_len must not be negative")
     scale = D ** -0.5 if scale is None else float(scale)
     rows = q.shape[0]
     if out is None:
-        out = torch.empty(rows, H_q, D, device=dev, dtype=torch.bfloat16)
+        out = q.new_empty((rows, H_q, D))
         if rows > T:
             out[T:].zero_()
     elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() \
@@ -359,12 +389,14 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         L = _lib.load()
         # Allocated for the call, so no two calls, streams or captured graphs
         # share it.
-        need = L.cvsa_chunk_attention_workspace_bytes(layout.cu_host, B, H_q, num_kv_heads, D,
-                                                      block_size, W, max_context_len)
+        sizes = (H_q, H_kv, D, block_size, W, max_context_len)
+        need = layout._workspace_bytes.get(sizes)
+        if need is None:
+            need = L.cvsa_chunk_attention_workspace_bytes(layout.cu_host, B, *sizes)
+            layout._workspace_bytes[sizes] = need
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-        _call(dev, who, L.cvsa_chunk_attention, q.data_ptr(), q.stride(0), q.stride(1),
-              k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], bt.data_ptr(),
-              bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(), layout.cu_host, B, H_q,
+        _call(dev, who, L.cvsa_chunk_attention, *q_at, k_cache.data_ptr(), v_cache.data_ptr(),
+              num_blocks, bt.data_ptr(), bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(), layout.cu_host, B, H_q,
               num_kv_heads, D, block_size, W, max_context_len, scale, int(bool(causal)),
               out.data_ptr(), _ptr(lse), _ptr(ws), need)
     return (out, lse) if return_lse else out

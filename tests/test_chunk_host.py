@@ -20,7 +20,8 @@ def calls(monkeypatch):
     """Ops on CPU tensors whose launches are only recorded."""
     made = []
     monkeypatch.setattr(chunk, "_device_of", lambda *t: torch.device("cpu"))
-    monkeypatch.setattr(chunk, "_call", lambda dev, who, fn, *args: made.append((who, args)))
+    monkeypatch.setattr(chunk, "_same_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(chunk, "_call", lambda dev, who, fn, *args, keep=None: made.append((who, args)))
 
     class Lib:
         cvsa_qk_norm_rope = cvsa_append_chunk_kv = cvsa_reserve_chunk = None
