@@ -198,6 +198,41 @@ __device__ __forceinline__ uint4 chunk_read_v(char *lo, char *hi) {
       __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((chunk_lds_short4 *)hi));
   return make_uint4(x.x, x.y, y.x, y.y);
 }
+
+// The places of a lane's reads, from a tile's start.  At D = 256 the second half
+// of the columns is 256 bytes on.
+template <int D>
+struct ChunkPlaces {
+  static constexpr int KU = D == 256 ? 8 : D / 16, DU = D == 256 ? 4 : D / 32;
+  uint32_t k[KU], v[DU][2];
+
+  __device__ __forceinline__ void init(uint32_t tile) {
+#pragma unroll
+    for (int ks = 0; ks < KU; ++ks) k[ks] = tile + chunk_k_place<D>(ks);
+#pragma unroll
+    for (int d = 0; d < DU; ++d)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[d][i] = tile + chunk_v_place<D>(d, i);
+  }
+  // As new values (in each step): the buffer's address then goes into the
+  // instruction, where it would take registers of its own.
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int ks = 0; ks < KU; ++ks) asm volatile("" : "+v"(k[ks]));
+#pragma unroll
+    for (int d = 0; d < DU; ++d) asm volatile("" : "+v"(v[d][0]), "+v"(v[d][1]));
+  }
+  // Keys 32 kb .. + 32 of columns 16 ks .. + 16; columns 32 d .. + 32 of keys 16 j
+  // .. + 16.
+  __device__ __forceinline__ uint4 read_k(const char *tile, int kb, int ks) const {
+    return chunk_read_k(tile + k[ks % KU] + (64 * kb * D + ks / KU * 256));
+  }
+  __device__ __forceinline__ uint4 read_v(char *tile, int j, int d) const {
+    const int at = 32 * j * D + d / DU * 256;
+    return chunk_read_v(tile + v[d % DU][0] + at, tile + v[d % DU][1] + at);
+  }
+};
+
 __device__ __forceinline__ f32x16_t chunk_mfma(const uint4 &x, const uint4 &y, const f32x16_t &c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(chunk_bf16x8_t, x),
                                                  __builtin_bit_cast(chunk_bf16x8_t, y), c, 0, 0,
@@ -330,7 +365,12 @@ struct ChunkState {
   template <int KB, class F>
   __device__ __forceinline__ void weights(const f32x16_t (&st)[KB], float c, uint4 (&pw)[2 * KB],
                                           F before) {
-    float sum = weigh(st, c, neg_m, pw, before);
+    settle(st, c, pw, weigh(st, c, neg_m, pw, before));
+  }
+  // The rest of weights(), given their sum for the present reference.
+  template <int KB>
+  __device__ __forceinline__ void settle(const f32x16_t (&st)[KB], float c, uint4 (&pw)[2 * KB],
+                                         float sum) {
     if (__ballot(!(sum < 1048576.f)) != 0) {
       float top[4] = {st[0][0], st[0][1], st[0][2], st[0][3]};
 #pragma unroll

@@ -17,7 +17,8 @@
 //    lane, no 64-bit arithmetic in lanes;
 //  - no maximum in a step (see weights()).
 //
-// D = 32 and 256: a workgroup takes 128 rows, four waves in step.
+// D = 32 and 256: a workgroup takes 128 rows, four waves in step, each its own
+// overlap.
 #pragma once
 #include "chunk_common.h"
 
@@ -33,7 +34,7 @@ constexpr int chunk_step_keys() {
 }
 
 template <int D>
-__global__ __launch_bounds__(chunk_row_waves<D>() * 64, D == 256 ? 1 : 2) void
+__global__ __launch_bounds__(chunk_row_waves<D>() * 64, D == 256 ? 1 : D == 32 ? 3 : 2) void
 chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   constexpr int NW = chunk_row_waves<D>(), NT = NW * 64, KT = chunk_step_keys<D>();
   constexpr int CPR = D / 8, NC = KT * CPR;
@@ -111,36 +112,26 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
     __builtin_amdgcn_s_waitcnt(0x0f70);
     asm volatile("" ::: "memory");
   };
-  uint32_t ka[KS], va[DB][2];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) ka[ks] = chunk_k_place<D>(ks);
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) va[d][i] = chunk_v_place<D>(d, i);
+  ChunkPlaces<D> at;
+  at.init(0);
 
   if constexpr (NW == 8) {
     // V of one step, then K of the next.  The order is the source's: the LDS
     // reads run kAhead products ahead, and between(i) follows product i.
     auto multiply = [&](char *v, const char *k, const uint4 (&pw)[2 * KB], f32x16_t (&st)[KB],
                         auto between) {
-      // The places as new values in each step: the buffer's address then goes
-      // into the instruction, where it would take registers of its own.
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(ka[ks]));
-#pragma unroll
-      for (int d = 0; d < DB; ++d) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
+      at.renew();
       constexpr int NV = 2 * KB * DB, N = NV + KB * KS, kAhead = 4;
       uint4 f[kAhead + 1];
-      auto fetch = [&](auto at) {
-        constexpr int i = decltype(at)::value;
+      auto fetch = [&](auto n) {
+        constexpr int i = decltype(n)::value;
         if constexpr (i < NV) {
           constexpr int j = i / DB, d = i % DB;
           f[i % (kAhead + 1)] =
-              chunk_read_v(v + va[d][0] + 32 * j * D, v + va[d][1] + 32 * j * D);
+              at.read_v(v, j, d);
         } else if constexpr (i < N) {
           constexpr int ks = (i - NV) / KB, kb = (i - NV) % KB;
-          f[i % (kAhead + 1)] = chunk_read_k(k + ka[ks] + 64 * kb * D);
+          f[i % (kAhead + 1)] = at.read_k(k, kb, ks);
         }
       };
       unrolled<kAhead>(fetch);
@@ -165,7 +156,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          st[kb] = chunk_mfma(chunk_read_k((const char *)lds + ka[ks] + 64 * kb * D),
+          st[kb] = chunk_mfma(at.read_k((const char *)lds, kb, ks),
                               __builtin_bit_cast(uint4, q[ks]), ks ? st[kb] : f32x16_t{});
     };
 
@@ -289,68 +280,145 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       else walk(std::false_type());
     }
   } else {
-    // Step s: once its K and V are there, those of step s + 1 follow into the
-    // other buffers, whose readers have passed the barrier.  The rows of a load
-    // may lie in several blocks (D = 32, 8-token pages), so lanes carry whole
-    // addresses.
-    auto load = [&](const uint16_t *cache, int s, int at, uint16_t *lds) {
+    // One wave to a SIMD, so its own instructions have to fill both pipes: in
+    // step s the products of K of step s + 1 stand between the exponentials of
+    // step s; then V of step s is added.  K of step s + 2 and V of step s + 1
+    // are under way meanwhile.  The rows of a load lie in one block, but for 16
+    // rows of 8-token pages (D = 32), where lanes carry whole addresses.
+    constexpr int RPL = 64 / CPR;
+    uint32_t row_off[P];  // of the lane's vector of each load, in the block of the load's rows
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < P; ++p) {
+      const int r = (p * NT + tid) / CPR;
+      row_off[p] = lane / CPR * row_bytes + (h * D + chunk_swizzle<D>(r, lane % CPR) * 8) * 2;
+    }
+    auto load_one = [&](const uint16_t *cache, int s, int at, uint16_t *lds, int p) {
+      uint16_t *const to = lds + (p * NT + wave * 64) * 8;
+      if constexpr (RPL <= 8) {
+        const int r = (p * NT + wave * 64) / CPR;
+        chunk_load_lds(cache, __builtin_amdgcn_readlane(at, r), block_bytes,
+                       s < steps ? block_bytes : 0, row_off[p],
+                       ((k0 + s * KT + r) & bs_mask) * row_bytes, to);
+      } else {
         const int c = tid + p * NT, r = c / CPR;
         const uint32_t blk = __shfl(at, r, 64);
         const char *from = (const char *)cache + (uint64_t)blk * block_bytes +
                            (uint32_t)(((k0 + s * KT + r) & bs_mask) * row_bytes) +
                            (h * D + chunk_swizzle<D>(r, c % CPR) * 8) * 2;
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)from,
-            (__attribute__((address_space(3))) void *)(lds + (p * NT + wave * 64) * 8), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
       }
     };
-    int found;      // blocks of step s + 1
-    uint64_t keys;  // of step s
-    auto step = [&](int s, uint16_t *k_cur, uint16_t *v_cur, uint16_t *k_next,
-                    uint16_t *v_next) {
-      arrived();
-      clean(s, keys, v_cur);
-      barrier();
-      const uint64_t now = keys;
-      const bool ok = in_pool(s + 1, found);
-      keys = __ballot(ok);
-      if (s + 1 < steps) {
-        load(a.k_cache, s + 1, ok ? found : 0, k_next);
-        load(a.v_cache, s + 1, ok ? found : 0, v_next);
-      }
-      found = lookup_keys(s + 2);
-      if (!live) return;
-      f32x16_t st[KB];
-      uint4 pw[2 * KB];
+    auto load = [&](const uint16_t *cache, int s, int at, uint16_t *lds) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-          st[kb] = chunk_mfma(chunk_read_k((const char *)k_cur + ka[ks] + 64 * kb * D),
-                              __builtin_bit_cast(uint4, q[ks]), ks ? st[kb] : f32x16_t{});
-      if (!whole(s, now)) chunk_mask(st, now, k0 + s * KT, row.last_key);
-      state.weights(st, a.c, pw, [](int) {});
+      for (int p = 0; p < P; ++p) load_one(cache, s, at, lds, p);
+    };
+    constexpr int NK = KB * KS, NV = 2 * KB * DB, NE = 16 * KB, kAhead = 4;
+    uint4 f[kAhead + 1];
+    auto fetch_k = [&](const char *k, auto n) {
+      constexpr int i = decltype(n)::value, ks = i / KB, kb = i % KB;
+      if constexpr (i < NK) f[i % (kAhead + 1)] = at.read_k(k, kb, ks);
+    };
+    auto k_product = [&](auto at, f32x16_t (&st)[KB]) {
+      constexpr int i = decltype(at)::value, ks = i / KB, kb = i % KB;
+      st[kb] = chunk_mfma(f[i % (kAhead + 1)], __builtin_bit_cast(uint4, q[ks]),
+                          ks ? st[kb] : f32x16_t{});
+    };
+    auto scores = [&](const uint16_t *k, f32x16_t (&st)[KB]) {
+      unrolled<kAhead>([&](auto i) { fetch_k((const char *)k, i); });
+      unrolled<NK>([&](auto at) {
+        k_product(at, st);
+        fetch_k((const char *)k, std::integral_constant<int, decltype(at)::value + kAhead>());
+      });
+    };
+    // Weights of st between the products of the next scores.
+    auto weights_and_scores = [&](const f32x16_t (&st)[KB], uint4 (&pw)[2 * KB], const char *k,
+                                  f32x16_t (&nxt)[KB]) {
+      unrolled<kAhead>([&](auto i) { fetch_k(k, i); });
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, even = 0.f;
+      uint32_t words[NE / 2];
+      unrolled<NE>([&](auto at) {
+        constexpr int e = decltype(at)::value;
+        // products e NK / NE up to (e + 1) NK / NE
+        constexpr int i0 = e * NK / NE, i1 = (e + 1) * NK / NE;
+        unrolled<i1 - i0>([&](auto n) {
+          constexpr int i = i0 + decltype(n)::value;
+          k_product(std::integral_constant<int, i>(), nxt);
+          fetch_k(k, std::integral_constant<int, i + kAhead>());
+        });
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[e / 16][e % 16], a.c, state.neg_m));
+        sum[e % 4] += p;
+        if constexpr (e % 2 == 0) even = p;
+        else words[e / 2] = chunk_cvt_bf16x2(even, p);
+        __builtin_amdgcn_sched_barrier(0);
+      });
 #pragma unroll
       for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          state.o[d] = chunk_mfma(chunk_read_v((char *)v_cur + va[d][0] + 32 * j * D,
-                                               (char *)v_cur + va[d][1] + 32 * j * D),
-                                  pw[j], state.o[d]);
+        pw[j] = make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
+      state.settle(st, a.c, pw, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    };
+    auto accumulate = [&](char *v, const uint4 (&pw)[2 * KB]) {
+      auto fetch = [&](auto n) {
+        constexpr int i = decltype(n)::value, j = i / DB, d = i % DB;
+        if constexpr (i < NV)
+          f[i % (kAhead + 1)] =
+              at.read_v(v, j, d);
+      };
+      unrolled<kAhead>(fetch);
+      __builtin_amdgcn_sched_barrier(0);
+      unrolled<NV>([&](auto at) {
+        constexpr int i = decltype(at)::value, j = i / DB, d = i % DB;
+        state.o[d] = chunk_mfma(f[i % (kAhead + 1)], pw[j], state.o[d]);
+        fetch(std::integral_constant<int, i + kAhead>());
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    int at1, found;             // blocks of step s + 1; looked up of step s + 2
+    uint64_t key0, key1, key2;  // keys of steps s to s + 2
+    auto locate = [&](int s, int looked_up, int &at) {
+      const bool ok = in_pool(s, looked_up);
+      at = ok ? looked_up : 0;
+      return __ballot(ok);
+    };
+    auto step = [&](int s, uint16_t *k_cur, uint16_t *k_next, uint16_t *v_cur, uint16_t *v_next,
+                    f32x16_t (&cur)[KB], f32x16_t (&nxt)[KB]) {
+      at.renew();
+      arrived();
+      clean(s, key0, v_cur);
+      barrier();
+      int at2;
+      key2 = locate(s + 2, found, at2);
+      found = lookup_keys(s + 3);
+      load(a.v_cache, s + 1, at1, v_next);
+      load(a.k_cache, s + 2, at2, k_cur);
+      at1 = at2;
+      if (live) {
+        if (!whole(s, key0)) chunk_mask(cur, key0, k0 + s * KT, row.last_key);
+        uint4 pw[2 * KB];
+        weights_and_scores(cur, pw, (const char *)k_next, nxt);
+        accumulate((char *)v_cur, pw);
+      }
+      key0 = key1;
+      key1 = key2;
     };
     if (steps > 0) {
-      found = lookup_keys(0);
-      const bool ok = in_pool(0, found);
-      keys = __ballot(ok);
-      load(a.k_cache, 0, ok ? found : 0, s_k0);
-      load(a.v_cache, 0, ok ? found : 0, s_v0);
-      found = lookup_keys(1);
+      f32x16_t st0[KB], st1[KB];
+      int at0;
+      const int f0 = lookup_keys(0), f1 = lookup_keys(1);
+      found = lookup_keys(2);
+      key0 = locate(0, f0, at0);
+      key1 = locate(1, f1, at1);
+      load(a.k_cache, 0, at0, s_k0);
+      load(a.v_cache, 0, at0, s_v0);
+      if (steps > 1) load(a.k_cache, 1, at1, s_k1);
+      arrived();
+      barrier();
+      if (live) scores(s_k0, st0);
       for (int s = 0; s < steps; s += 2) {
-        step(s, s_k0, s_v0, s_k1, s_v1);
-        if (s + 1 < steps) step(s + 1, s_k1, s_v1, s_k0, s_v0);
+        step(s, s_k0, s_k1, s_v0, s_v1, st0, st1);
+        if (s + 1 < steps) step(s + 1, s_k1, s_k0, s_v1, s_v0, st1, st0);
       }
+      arrived();  // no load may outlive the workgroup's LDS
     }
   }
   __syncthreads();  // the last note of a taken-out value

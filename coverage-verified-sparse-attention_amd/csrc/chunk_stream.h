@@ -18,7 +18,7 @@ constexpr int chunk_stream_waves() {
 }
 
 template <int D, int RT>
-__global__ __launch_bounds__(chunk_stream_waves<D>() * 64, D * RT >= 256 ? 1 : 2) void
+__global__ __launch_bounds__(chunk_stream_waves<D>() * 64, D >= 128 ? 1 : 2) void
 chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   constexpr int NW = chunk_stream_waves<D>(), NT = NW * 64, KT = 32;
   constexpr int CPR = D / 8, RPL = 64 / CPR;  // rows of a load
@@ -95,13 +95,8 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     }
   };
 
-  uint32_t ka[KS], va[DB][2];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) ka[ks] = wave * kTile * 2 + chunk_k_place<D>(ks);
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) va[d][i] = wave * kTile * 2 + chunk_v_place<D>(d, i);
+  ChunkPlaces<D> place;
+  place.init(wave * kTile * 2);
 
   s_taken.clear(NT);
   __syncthreads();
@@ -115,17 +110,12 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     return __ballot(ok);
   };
   auto step = [&](int s, uint16_t *k_cur, uint16_t *v_cur) {
-    // The places as new values in each step: the buffer's address then goes
-    // into the instruction, where it would take registers of its own.
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(ka[ks]));
-#pragma unroll
-    for (int d = 0; d < DB; ++d) asm volatile("" : "+v"(va[d][0]), "+v"(va[d][1]));
+    place.renew();
     const int ahead = lookup(s + 3);
     f32x16_t st[RT][1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const uint4 k = chunk_read_k((const char *)k_cur + ka[ks]);
+      const uint4 k = place.read_k((const char *)k_cur, 0, ks);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
         st[r][0] = chunk_mfma(k, __builtin_bit_cast(uint4, q[r][ks]), ks ? st[r][0] : f32x16_t{});
@@ -156,8 +146,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const uint4 v = chunk_read_v((char *)v_cur + va[d][0] + 32 * j * D,
-                                     (char *)v_cur + va[d][1] + 32 * j * D);
+        const uint4 v = place.read_v((char *)v_cur, j, d);
 #pragma unroll
         for (int r = 0; r < RT; ++r) state[r].o[d] = chunk_mfma(v, pw[r][j], state[r].o[d]);
       }
@@ -192,7 +181,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   auto room = [&](int w) {
     return reinterpret_cast<float4 *>(w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
   };
-  auto place = [&](int r, int d, int g) {
+  auto spot = [&](int r, int d, int g) {
     return (r * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
   };
 #pragma unroll
@@ -207,7 +196,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          so[place(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
+          so[spot(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
                                            state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
     }
   }
@@ -228,7 +217,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
         __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float4 v = so[place(r, d, g)];
+          const float4 v = so[spot(r, d, g)];
           state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
           state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
           state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
