@@ -12,10 +12,11 @@ namespace cvsa {
 
 constexpr int kJoinThreads = 256;
 
-// The states of a row's splits joined in the order of the keys.  D / 4 threads
+// The parts of a row joined in the order of the keys: of few rows (RANGES) those
+// of the ranges that its sequence spans, of many rows its splits.  D / 4 threads
 // have a float4 of the row each; with few rows `groups` such groups share a
-// row's splits, and their sums are joined in LDS.
-template <int D>
+// row's parts, and their sums are joined in LDS.
+template <int D, bool RANGES>
 __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArgs a,
                                                                   const ChunkClass c,
                                                                   int groups) {
@@ -23,47 +24,66 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
   __shared__ float4 s_o[NG][L];
   __shared__ float2 s_ml[NG];
   const int group = threadIdx.x / L, d = threadIdx.x % L * 4;
-  const int per_wg = NG / groups, part = group % groups;
-  const int64_t rows = (int64_t)c.tokens * a.H_q;
-  const int64_t want = (int64_t)blockIdx.x * per_wg + group / groups;
-  const int64_t from = min(want, rows - 1);
+  const int per_wg = NG / groups, mine = group % groups;
+  const uint32_t rows = (uint32_t)c.tokens * a.H_q;  // below 2^31
+  const uint32_t want = blockIdx.x * per_wg + group / groups;
+  const uint32_t row = min(want, rows - 1);
   // The row's token in its class: its sequence and place in it.  The rows of a
   // workgroup may be of several tokens; each lane looks for its own, a wave's
   // lanes over the same sequences.
-  const int class_tok = (int)(from / a.H_q), head = (int)(from % a.H_q);
-  int tok = class_tok, first = 0, len = 0, seq = 0;
-  {
-    const int lane = threadIdx.x & 63;
-    int base = 0;  // tokens of the class before b0
-    for (int b0 = 0; b0 < a.B; b0 += kWave) {
-      const int b = b0 + lane;
-      const int lo = b < a.B ? a.cu[b] : 0;
-      int n = b < a.B ? a.cu[b + 1] - lo : 0;
-      if (n * a.G < c.min_rows || n * a.G > c.max_rows) n = 0;
-      const int end = base + (int)wave_incl_scan_u32((uint32_t)n);
-      const int total = __builtin_amdgcn_readlane(end, 63);
-      // the first sequence that ends past the token, by bisection over lanes
-      int l = 0;
+  const int class_tok = (int)(row / a.H_q), head = (int)(row % a.H_q);
+  int tok = 0, first = 0, len = 0, ctx = 0;
+  uint32_t unit0 = 0, units = 0, total = 0;  // of the sequence, of all
+  const int lane = threadIdx.x & 63;
+  int base = 0;  // tokens of the class before b0
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const ChunkSeq s = chunk_look(a, c, b0 + lane);
+    const int end = base + (int)wave_incl_scan_u32((uint32_t)s.len);
+    const int unit_end = (int)wave_incl_scan_u32((uint32_t)s.units);
+    const int last = __builtin_amdgcn_readlane(end, 63);
+    // the first sequence that ends past the token, by bisection over lanes
+    int l = 0;
 #pragma unroll
-      for (int step = 32; step > 0; step >>= 1)
-        if (__shfl(end, l + step - 1, 64) <= class_tok) l += step;
-      const int e = __shfl(end, l & 63, 64), m = __shfl(n, l & 63, 64),
-                f = __shfl(lo, l & 63, 64);
-      if (class_tok >= base && class_tok < total) {
-        seq = b0 + l;
-        first = f;
-        len = m;
-        tok = class_tok - (e - m);
-      }
-      base = total;
+    for (int step = 32; step > 0; step >>= 1)
+      if (__shfl(end, l + step - 1, 64) <= class_tok) l += step;
+    l &= 63;
+    const int n = __shfl(s.len, l, 64), u = __shfl(s.units, l, 64);
+    const int before = __shfl(end, l, 64) - n, u0 = __shfl(unit_end, l, 64) - u;
+    const int f = __shfl(s.first, l, 64), x = __shfl(s.ctx, l, 64);
+    if (class_tok >= base && class_tok < last) {
+      first = f;
+      len = n;
+      ctx = x;
+      tok = class_tok - before;
+      unit0 = total + u0;
+      units = u;
     }
+    base = last;
+    total += __builtin_amdgcn_readlane(unit_end, 63);
   }
-  const int ctx = a.context_lens[seq];
-  const int row0 = (tok * a.G + head % a.G) / c.tile_rows * c.tile_rows;
-  const int keys = chunk_tile_keys(a, ctx - len, ctx, len * a.G, row0, c.tile_rows);
-  const int parts = min((keys + c.split_len - 1) / c.split_len, c.splits);
+  int parts;
+  int64_t part0, stride;  // the row's first part, from its second to the next
+  int64_t second;
+  if (RANGES) {
+    const ChunkRanges ranges(c, total);
+    const int r0 = ranges.of(unit0), r1 = ranges.of(unit0 + units - 1);
+    const int h = head / a.G, place = tok * a.G + head % a.G;
+    parts = r1 - r0 + 1;
+    part0 = ((int64_t)(2 * r0 + 1) * a.H_kv + h) * c.tile_rows + place;
+    second = part0 + (int64_t)a.H_kv * c.tile_rows;
+    stride = (int64_t)2 * a.H_kv * c.tile_rows;
+  } else {
+    const int row0 = (tok * a.G + head % a.G) / c.tile_rows * c.tile_rows;
+    const int keys = chunk_tile_keys(a, ctx - len, ctx, len * a.G, row0, c.tile_rows);
+    parts = min((keys + c.split_len - 1) / c.split_len, c.splits);
+    part0 = row;
+    second = (int64_t)rows + row;
+    stride = rows;
+  }
+  auto part = [&](int s) { return s == 0 ? part0 : second + (s - 1) * stride; };
   float m = -INFINITY;
-  for (int s = part; s < parts; s += groups) m = fmaxf(m, c.part_ml[s * rows + from].x);
+#pragma unroll 4
+  for (int s = mine; s < parts; s += groups) m = fmaxf(m, c.part_ml[part(s)].x);
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -74,30 +94,31 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
     o.z = fmaf(v.z, w, o.z);
     o.w = fmaf(v.w, w, o.w);
   };
+  const bool whole = RANGES && parts == 1;  // complete already
 #pragma unroll 4
-  for (int s = part; s < parts; s += groups) {
-    const float2 ml = c.part_ml[s * rows + from];
+  for (int s = mine; s < parts && !whole; s += groups) {
+    const float2 ml = c.part_ml[part(s)];
     add(__builtin_amdgcn_exp2f(ml.x - ref), ml.y,
-        *reinterpret_cast<const float4 *>(c.part_o + (s * rows + from) * D + d));
+        *reinterpret_cast<const float4 *>(c.part_o + part(s) * D + d));
   }
   if (groups > 1) {  // the same in every thread
     s_o[group][d / 4] = o;
     if (d == 0) s_ml[group] = make_float2(m, l);
     __syncthreads();
-    if (part > 0) return;
+    if (mine > 0) return;
     for (int g = 1; g < groups; ++g) m = fmaxf(m, s_ml[group + g].x);
     const float top = m == -INFINITY ? 0.f : m;
     const float2 own = s_ml[group];
-    const float4 mine = o;
+    const float4 have = o;
     l = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
-    add(__builtin_amdgcn_exp2f(own.x - top), own.y, mine);
+    add(__builtin_amdgcn_exp2f(own.x - top), own.y, have);
     for (int g = 1; g < groups; ++g) {
       const float2 ml = s_ml[group + g];
       add(__builtin_amdgcn_exp2f(ml.x - top), ml.y, s_o[group + g][d / 4]);
     }
   }
-  if (want >= rows) return;
+  if (want >= rows || whole) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t at = (int64_t)(first + tok) * a.H_q + head;
   *reinterpret_cast<uint2 *>(a.out + at * D + d) =
@@ -107,16 +128,17 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
 }
 
 // Groups of threads that share a row: as many as keep the GPU's CUs busy when
-// rows are few (one row of 64 splits: 64 loads in a row by one group, or 8 by
+// rows are few (one row of 64 parts: 64 loads in a row by one group, or 8 by
 // eight).
-template <int D>
+template <int D, bool RANGES>
 static void launch_join(const ChunkArgs &a, const ChunkClass &c, hipStream_t s) {
   constexpr int NG = kJoinThreads / (D / 4);
   const int64_t rows = (int64_t)c.tokens * a.H_q;
+  const int parts = RANGES ? c.splits / c.tiles + 1 : c.splits;  // of a row, about
   int groups = 1;
-  while (groups < NG && groups * 2 <= c.splits && rows * groups < 1024 * NG) groups *= 2;
+  while (groups < NG && groups * 2 <= parts && rows * groups < 1024 * NG) groups *= 2;
   const int per_wg = NG / groups;
-  hipLaunchKernelGGL(chunk_join_kernel<D>, dim3((unsigned)((rows + per_wg - 1) / per_wg)),
+  hipLaunchKernelGGL((chunk_join_kernel<D, RANGES>), dim3((unsigned)((rows + per_wg - 1) / per_wg)),
                      dim3(kJoinThreads), 0, s, a, c, groups);
 }
 
@@ -130,19 +152,9 @@ constexpr int chunk_few_rows() {
 
 struct ChunkPlan {
   ChunkClass few, many;  // tiles 0: no such sequence
-  size_t bytes;          // of the workspace
+  bool join_few, join_many;
+  size_t bytes;  // of the workspace
 };
-
-// Keys of a split: so many that the class makes about `want` workgroups, at
-// least `least` of them.  Two a CU: 8 sequences of 32K keys, 4 heads 110 us, 1024
-// workgroups 118, 2048 143; 32 ragged sequences of 8K, 8 heads 133, 141, 136.
-static void plan_splits(ChunkClass &c, int H_kv, int64_t max_keys, int64_t want, int64_t least) {
-  const int64_t items = (int64_t)c.tiles * H_kv;
-  int64_t len = std::max<int64_t>(least, (max_keys * items + want - 1) / want);
-  len = (len + 127) / 128 * 128;
-  c.split_len = (int)std::min<int64_t>(len, 1 << 30);
-  c.splits = (int)std::max<int64_t>(1, (max_keys + len - 1) / len);
-}
 
 template <int D>
 static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t max_keys) {
@@ -154,18 +166,31 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   p.many.max_rows = 0x7fffffff;
   p.many.tile_rows = chunk_row_waves<D>() * 32;
   int64_t most_few = 0;
+  bool same = true;
   for (int b = 0; b < B; ++b) {
     const int64_t rows = (int64_t)(cu[b + 1] - cu[b]) * G;
     if (rows <= p.few.max_rows) most_few = std::max(most_few, rows);
+    same = same && cu[b + 1] - cu[b] == cu[1];
   }
   p.few.tile_rows = most_few > 32 ? 64 : 32;
+  p.few.same_len = p.many.same_len = same ? cu[1] : 0;
   for (int b = 0; b < B; ++b) {
     const int n = cu[b + 1] - cu[b];
     ChunkClass &c = (int64_t)n * G <= p.few.max_rows ? p.few : p.many;
     c.tiles += (int)(((int64_t)n * G + c.tile_rows - 1) / c.tile_rows);
     c.tokens += n;
   }
-  plan_splits(p.few, H_kv, max_keys, 512, 256);
+  // Few rows: a range for each workgroup that fits the GPU, of one unit at least;
+  // up to 256 keys, a step or two of the waves, are not worth a join.
+  const int unit_log2 = D == 256 ? 6 : 7;
+  static_assert(chunk_stream_waves<D>() * 32 == (D == 256 ? 64 : 128), "a step of the waves");
+  const bool whole = max_keys <= 256;
+  p.few.unit_log2 = p.many.unit_log2 = whole ? 31 : unit_log2;
+  const int64_t units =
+      (int64_t)p.few.tiles * (whole ? 1 : (max_keys + (1 << unit_log2) - 1) >> unit_log2);
+  const int fit = most_few > 32 ? chunk_stream_fit<D, 2>() : chunk_stream_fit<D, 1>();
+  p.few.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 * (fit) / H_kv, units));
+  p.join_few = p.few.tiles > 0 && p.few.splits > 1 && !whole;
   // Many rows: the number of splits whose rounds of 256 workgroups (one a CU)
   // take least, at 1.4 us for 64 keys, 5 us for a workgroup's start and end and
   // 4 TB/s for writing and joining the parts.
@@ -183,9 +208,11 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   }
   p.many.split_len = (int)(((max_keys + splits - 1) / splits + 127) / 128 * 128);
   p.many.splits = (int)std::max<int64_t>(1, (max_keys + p.many.split_len - 1) / p.many.split_len);
+  p.join_many = p.many.tiles > 0 && p.many.splits > 1;
   for (ChunkClass *c : {&p.few, &p.many}) {
-    if (c->tiles == 0 || c->splits <= 1) continue;
-    const size_t rows = (size_t)c->splits * c->tokens * H_q;
+    if (!(c == &p.few ? p.join_few : p.join_many)) continue;
+    const size_t rows = c == &p.few ? (size_t)2 * c->splits * H_kv * c->tile_rows
+                                    : (size_t)c->splits * c->tokens * H_q;
     c->part_ml = (float2 *)p.bytes;  // offsets until there is a workspace
     p.bytes += (rows * sizeof(float2) + 255) / 256 * 256;
     c->part_o = (float *)p.bytes;
@@ -203,7 +230,7 @@ static ChunkPlan plan_chunk_d(const int32_t *cu, int B, int H_q, int H_kv, int D
 }
 
 static int64_t chunk_grid(const ChunkClass &c, int H_kv) {
-  return (int64_t)c.tiles * H_kv * c.splits;
+  return (int64_t)c.tiles * H_kv * c.splits;  // of many rows
 }
 
 template <int D>
@@ -211,17 +238,17 @@ static void launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) 
   if (p.many.tiles > 0) {
     hipLaunchKernelGGL(chunk_prefill_kernel<D>, dim3((unsigned)chunk_grid(p.many, a.H_kv)),
                        dim3(chunk_row_waves<D>() * 64), 0, s, a, p.many);
-    if (p.many.splits > 1) launch_join<D>(a, p.many, s);
+    if (p.join_many) launch_join<D, false>(a, p.many, s);
   }
   if (p.few.tiles > 0) {
-    const dim3 grid((unsigned)chunk_grid(p.few, a.H_kv)), block(chunk_stream_waves<D>() * 64);
+    const dim3 grid((unsigned)(p.few.splits * a.H_kv)), block(chunk_stream_waves<D>() * 64);
     if constexpr (chunk_few_rows<D>() > 32) {
       if (p.few.tile_rows > 32)
         hipLaunchKernelGGL((chunk_stream_kernel<D, 2>), grid, block, 0, s, a, p.few);
     }
     if (p.few.tile_rows <= 32)
       hipLaunchKernelGGL((chunk_stream_kernel<D, 1>), grid, block, 0, s, a, p.few);
-    if (p.few.splits > 1) launch_join<D>(a, p.few, s);
+    if (p.join_few) launch_join<D, true>(a, p.few, s);
   }
 }
 
@@ -233,7 +260,8 @@ static bool chunk_shape_ok(const int32_t *cu, int32_t B, int32_t H_q, int32_t H_
     return false;
   for (int b = 0; b < B; ++b)
     if (cu[b + 1] < cu[b]) return false;
-  return cu[B] <= (1 << 24) && (int64_t)cu[B] * (H_q / H_kv) < (1 << 30);
+  return cu[B] <= (1 << 24) && (int64_t)cu[B] * (H_q / H_kv) < (1 << 30) &&
+         (int64_t)cu[B] * H_q < (1LL << 31);
 }
 
 static int64_t chunk_max_keys(int32_t W, int32_t block_size, int32_t max_context_len) {
@@ -296,8 +324,9 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
                                 ((uintptr_t)workspace & 255) == 0),
                CVSA_ERR_WORKSPACE,
                "chunk_attention: needs a 256-byte aligned workspace of %zu bytes", p.bytes);
-  CVSA_REQUIRE(chunk_grid(p.few, H_kv) < (1LL << 31) && chunk_grid(p.many, H_kv) < (1LL << 31),
-               CVSA_ERR_UNSUPPORTED, "chunk_attention: too many row tiles");
+  CVSA_REQUIRE(chunk_grid(p.many, H_kv) < (1LL << 31) &&
+                   (int64_t)p.few.tiles * ((int64_t)W * block_size / 64 + 1) < (1LL << 31),
+               CVSA_ERR_UNSUPPORTED, "chunk_attention: too many row tiles or keys");
   for (ChunkClass *c : {&p.few, &p.many}) {
     c->part_ml = (float2 *)((char *)workspace + (size_t)c->part_ml);
     c->part_o = (float *)((char *)workspace + (size_t)c->part_o);

@@ -37,15 +37,21 @@
 
 namespace cvsa {
 
-// The row tiles of the sequences that bring min_rows to max_rows rows (tokens
-// times G), and how their keys are split.
+// The sequences that bring min_rows to max_rows rows (tokens times G), their row
+// tiles, and how their keys are spread over workgroups: many rows by splits of
+// split_len keys, few rows by `splits` equal ranges of all their keys, sequence
+// after sequence.  Parts of a row that several workgroups have are joined: of
+// many rows part [split][token of the class * H_q + head], of few rows
+// [2 * range + (the part starts its sequence)][KV head][row].
 struct ChunkClass {
   int min_rows, max_rows;
   int tile_rows, tiles;
   int splits, split_len;
+  int unit_log2;    // few rows: keys of a unit, 31: a unit has all of a sequence
   int tokens;       // of these sequences
-  float *part_o;    // [splits, tokens * H_q, D]: sums of weighted values
-  float2 *part_ml;  // [splits, tokens * H_q]: reference (base 2), sum
+  int same_len;     // what every sequence brings, 0: they differ
+  float *part_o;    // [parts, D]: sums of weighted values
+  float2 *part_ml;  // [parts]: reference (base 2), sum
 };
 
 struct ChunkArgs {
@@ -101,7 +107,14 @@ __device__ __forceinline__ ChunkTile chunk_find_tile(const ChunkArgs &a, const C
   ChunkTile t;
   int first = 0, len = 0, before = 0, part0 = 0;
   t.seq = a.B - 1;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+  if (c.same_len > 0) {  // no need to look
+    const int nt = (c.same_len * a.G + c.tile_rows - 1) / c.tile_rows;
+    t.seq = id / nt;
+    len = c.same_len;
+    first = part0 = t.seq * len;
+    before = t.seq * nt;
+  }
+  for (int b0 = 0; c.same_len == 0 && b0 < a.B; b0 += kWave) {
     const int b = b0 + lane;
     const int lo = b < a.B ? a.cu[b] : 0;
     int n = b < a.B ? a.cu[b + 1] - lo : 0;
@@ -131,6 +144,40 @@ __device__ __forceinline__ ChunkTile chunk_find_tile(const ChunkArgs &a, const C
   t.keys = chunk_tile_keys(a, t.pos0, ctx, t.rows, t.row0, c.tile_rows);
   return t;
 }
+
+// Sequence b, without tokens if it is not of the class (or there is none); at
+// least one unit if it has tokens.
+struct ChunkSeq {
+  int first, len, ctx, keys, units;
+};
+__device__ __forceinline__ ChunkSeq chunk_look(const ChunkArgs &a, const ChunkClass &c, int b) {
+  ChunkSeq s = {0, 0, 0, 0, 0};
+  if (b >= a.B) return s;
+  s.first = c.same_len > 0 ? b * c.same_len : a.cu[b];
+  s.len = c.same_len > 0 ? c.same_len : a.cu[b + 1] - s.first;
+  s.ctx = a.context_lens[b];
+  s.keys = max(0, min(s.ctx, a.W << a.bs_log2));
+  if (s.len * a.G < c.min_rows || s.len * a.G > c.max_rows) s.len = 0;
+  else s.units = (max(s.keys - 1, 0) >> c.unit_log2) + 1;
+  return s;
+}
+
+// The ranges of few rows' units (fewer than 2^31 in all): n, none of them empty,
+// the first `more` one unit longer than the others.
+struct ChunkRanges {
+  uint32_t n, len, more;
+
+  __device__ __forceinline__ ChunkRanges(const ChunkClass &c, uint32_t units) {
+    n = min(units, (uint32_t)c.splits);
+    len = units / max(n, 1u);
+    more = units - len * n;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t r) const { return r * len + min(r, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t unit) const {
+    const uint32_t longer = more * (len + 1);
+    return unit < longer ? unit / (len + 1) : more + (unit - longer) / max(len, 1u);
+  }
+};
 
 // A lane's row of a tile.
 struct ChunkRow {
@@ -400,23 +447,11 @@ struct ChunkState {
     l = x + y;
   }
 
-  __device__ __forceinline__ void store(const ChunkArgs &a, const ChunkClass &c,
-                                        const ChunkTile &t, const ChunkRow &r, int split) const {
+  // The row's output.
+  __device__ __forceinline__ void store(const ChunkArgs &a, const ChunkTile &t,
+                                        const ChunkRow &r) const {
     if (!r.ok) return;
     const int half = (threadIdx.x >> 5) & 1;
-    if (c.splits > 1) {
-      const int64_t at =
-          ((int64_t)split * c.tokens + t.part0 + r.tok) * a.H_q + r.head;
-      float *po = c.part_o + at * D + 4 * half;
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4 *>(po + d * 32 + 8 * g) =
-              make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
-      if (half == 0) c.part_ml[at] = make_float2(m, l);
-      return;
-    }
     const int64_t at = (int64_t)(t.first + r.tok) * a.H_q + r.head;
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
     uint16_t *po = a.out + at * D + 4 * half;
@@ -429,6 +464,20 @@ struct ChunkState {
                        chunk_cvt_bf16x2(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
     if (a.lse && half == 0)
       a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  // The row's state as part `at`, for a join.
+  __device__ __forceinline__ void store_part(const ChunkClass &c, const ChunkRow &r,
+                                             int64_t at) const {
+    if (!r.ok) return;
+    const int half = (threadIdx.x >> 5) & 1;
+    float *po = c.part_o + at * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4 *>(po + d * 32 + 8 * g) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    if (half == 0) c.part_ml[at] = make_float2(m, l);
   }
 };
 

@@ -83,7 +83,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   // of the loads; where there is no key or no block of the pool, its bit of the
   // step's key mask is clear and block 0 is read in its place.
   auto lookup_keys = [&](int s) {
-    return bt[min(k0 + s * KT + (lane & (KT - 1)), k1 - 1) >> a.bs_log2];
+    return bt[min((k0 + s * KT + (lane & (KT - 1))) >> a.bs_log2, a.W - 1)];
   };
   auto in_pool = [&](int s, int found) {
     return k0 + s * KT + (lane & (KT - 1)) < k1 && (uint32_t)found < (uint32_t)a.num_blocks;
@@ -425,7 +425,10 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
 
   state.finish();
   s_taken.restore(row.last_key, state.o);
-  state.store(a, cl, t, row, split);
+  if (cl.splits > 1)
+    state.store_part(cl, row, ((int64_t)split * cl.tokens + t.part0 + row.tok) * a.H_q + row.head);
+  else
+    state.store(a, t, row);
 }
 
 }  // namespace cvsa
