@@ -333,7 +333,8 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
   }
   ChunkArgs a = {};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
-  a.k_cache = k_cache; a.v_cache = v_cache; a.num_blocks = (int)std::min<int64_t>(num_blocks, INT32_MAX);
+  a.k_cache = k_cache; a.v_cache = v_cache;
+  a.num_blocks = (int)std::min<int64_t>(num_blocks, INT32_MAX);
   a.block_tables = block_tables; a.bt_sb = bt_stride_b; a.W = W;
   a.context_lens = context_lens; a.cu = cu_seqlens;
   a.B = B; a.H_q = H_q; a.H_kv = H_kv; a.G = H_q / H_kv;

@@ -9,11 +9,18 @@
 // at D = 128).  The waves' states are joined at the end.
 //
 // Sequences differ in length, so the keys of all of them are laid end to end (in
-// units of 32 keys a wave, or of a sequence if none is longer) and cut into as many equal ranges as workgroups
-// fit the GPU; a workgroup walks its range, sequence by sequence, for one KV head
-// (the heads' workgroups read the same rows at about the same time).  Sequences
-// that lie in one range are complete there; parts of the others are joined by a
-// second kernel.
+// units of 32 keys a wave, or of a sequence if none is longer) and cut into as
+// many equal ranges as workgroups fit the GPU; a workgroup walks its range,
+// sequence by sequence, for one KV head (the heads' workgroups read the same
+// rows at about the same time).  Sequences that lie in one range are complete
+// there; parts of the others are joined by a second kernel.  (Splits of equal
+// length for each sequence, with rounds of workgroups, took 133 us where ranges
+// take 113: 32 sequences of up to 8 K keys, 32 heads on 8 of 128.)
+//
+// Measured with the join, heads of 128: 32 sequences of 8 K keys, one token each,
+// 193 us, 5.6 TB/s (a copy of 1 GB reaches 5.1); one sequence of 128 K keys 104 us,
+// 5.2 TB/s; 8 drafts of 5 tokens at 32 K keys 112 us, 4.8 TB/s.  What is left is
+// the kernel's start (6 us to the first products) and the join (5 to 7 us).
 #pragma once
 #include "chunk_common.h"
 

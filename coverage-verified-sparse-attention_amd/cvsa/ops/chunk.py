@@ -354,7 +354,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the caller knows) only shapes the launch.  With ``return_lse`` the natural
     log-sum-exps [T, H_q] fp32 of the scaled scores are returned too.  Rows
     past layout.total are zero in a new output and left as they are in ``out``
-    (contiguous bf16 of q's shape).
+    (contiguous bf16 of q's shape; a contiguous q itself will do).
 
     Scores, sums and outputs are held in 32 bits; the weights of the second
     product are rounded to bf16.
@@ -396,7 +396,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             layout._workspace_bytes[sizes] = need
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
         _call(dev, who, L.cvsa_chunk_attention, *q_at, k_cache.data_ptr(), v_cache.data_ptr(),
-              num_blocks, bt.data_ptr(), bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(), layout.cu_host, B, H_q,
-              num_kv_heads, D, block_size, W, max_context_len, scale, int(bool(causal)),
-              out.data_ptr(), _ptr(lse), _ptr(ws), need)
+              num_blocks, bt.data_ptr(), bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(),
+              layout.cu_host, B, H_q, num_kv_heads, D, block_size, W, max_context_len, scale,
+              int(bool(causal)), out.data_ptr(), _ptr(lse), _ptr(ws), need)
     return (out, lse) if return_lse else out

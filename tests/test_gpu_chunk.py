@@ -359,6 +359,61 @@ def test_scores_of_any_size(gpu):
         ref.check_attend(out, ref.attend(qq, kc, vc, bt, ctx, lens, 2, scale=scale), lse)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B", [65, 150])
+def test_chunk_attention_many_sequences(gpu, D, B):
+    """More sequences than a wave has lanes: single tokens, drafts, longer
+    chunks and none, over contexts from none to many; each class finds its own."""
+    g = _gen(B + D)
+    kinds = torch.tensor([0, 1, 1, 1, 3, 16, 33])
+    lens = kinds[torch.randint(0, 7, (B,), generator=g)].tolist()
+    lens[0], lens[-1] = 0, 40
+    before = torch.randint(0, 200, (B,), generator=g).tolist()
+    before[3] = before[B - 2] = 900
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, 16, 2, 4)
+    out, lse = _attend(gpu, q, kc, vc, bt, ctx, lens, 4, return_lse=True)
+    ref.check_attend(out, ref.attend(q, kc, vc, bt, ctx, lens, 4), lse)
+
+
+@pytest.mark.parametrize("D,Hk,G,n", [(128, 2, 4, 1), (64, 1, 7, 5), (256, 1, 8, 1),
+                                      (32, 300, 1, 2)])
+@pytest.mark.parametrize("B", [3, 66])
+def test_chunk_attention_equal_chunks(gpu, D, Hk, G, n, B):
+    """Every sequence brings as many tokens (their places are computed); more
+    KV heads than CUs; contexts of one range, several, or a part of one."""
+    g = _gen(B + D + n)
+    before = torch.randint(0, 60, (B,), generator=g).tolist()
+    if Hk < 300:
+        before[1] = 1500
+    q, kc, vc, bt, ctx = _attend_inputs(g, [n] * B, before, D, 16, Hk, G)
+    want = ref.attend(q, kc, vc, bt, ctx, [n] * B, G)
+    for bound in (0, 100):  # 100: short contexts promised, without a join
+        out, lse = _attend(gpu, q, kc, vc, bt, ctx, [n] * B, G, return_lse=True,
+                           max_context_len=bound)
+        ref.check_attend(out, want, lse)
+
+
+@pytest.mark.parametrize("D,n,G", [(32, 2, 4), (64, 5, 7), (128, 1, 8), (256, 3, 4),
+                                   (32, 40, 4), (64, 40, 4), (128, 40, 4), (256, 40, 4)])
+def test_scores_that_rise_and_fall(gpu, D, n, G):
+    """The reference of a row has to move when later scores outgrow it, by
+    little or by far, and to stay when they fall."""
+    g = _gen(D + n)
+    lens, before, bs = [n], [900], 16
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, 1, G)
+    q = q * 0.25 + 2
+    at = torch.arange(int(ctx[0]))
+    steps = {"rise": at * 0.25, "fall": -at * 0.25, "jump": (at >= 500) * 40.0,
+             "steps": at // 130 * 16.0, "far": (at >= 300) * 3000.0 + (at >= 800) * 1.0}
+    for score in steps.values():
+        k = kc.clone()
+        # q . k / sqrt(D) is score, about
+        k[bt[0, at // bs].long(), at % bs, 0] = (
+            (score / (2 * math.sqrt(D)))[:, None] + 0.1 * _randn(g, at.numel(), D)).bfloat16()
+        out, lse = _attend(gpu, q, k, vc, bt, ctx, lens, G, return_lse=True)
+        ref.check_attend(out, ref.attend(q, k, vc, bt, ctx, lens, G), lse)
+
+
 def test_strided_queries_padded_rows_and_out(gpu):
     g = _gen(9)
     lens, before, G, Hk, D = [5, 9], [20, 0], 2, 2, 64
@@ -373,6 +428,9 @@ def test_strided_queries_padded_rows_and_out(gpu):
     mine = torch.full((18, 4, D), 7.0, dtype=torch.bfloat16, device=gpu)
     assert _attend(gpu, view, kc, vc, bt, ctx, lens, G, out=mine) is mine
     assert torch.equal(mine[:14], want) and (mine[14:] == 7).all()
+    over = q.to(gpu)
+    assert _attend(gpu, over, kc, vc, bt, ctx, lens, G, out=over) is over
+    assert torch.equal(over, want)
     none = _attend(gpu, view, kc, vc, bt, ctx, [0, 0], G)
     assert none.shape == (18, 4, D) and (none == 0).all()
     wide = torch.full((2, 40), -1, dtype=torch.int32)
