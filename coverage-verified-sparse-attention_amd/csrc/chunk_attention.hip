@@ -164,7 +164,11 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   p.few.max_rows = chunk_few_rows<D>();
   p.many.min_rows = p.few.max_rows + 1;
   p.many.max_rows = 0x7fffffff;
-  p.many.tile_rows = chunk_row_waves<D>() * 32;
+  int longest = 0;
+  for (int b = 0; b < B; ++b) longest = std::max(longest, cu[b + 1] - cu[b]);
+  // 4 or 8 waves: see the kernel.
+  const bool start = max_keys <= 4096 && longest >= max_keys / 4;
+  p.many.tile_rows = D == 128 || (D == 64 && !start) ? 256 : 128;
   int64_t most_few = 0;
   bool same = true;
   for (int b = 0; b < B; ++b) {
@@ -174,12 +178,20 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   }
   p.few.tile_rows = most_few > 32 ? 64 : 32;
   p.few.same_len = p.many.same_len = same ? cu[1] : 0;
+  p.many.only = -1;
+  int sequences = 0;  // of many rows
   for (int b = 0; b < B; ++b) {
     const int n = cu[b + 1] - cu[b];
     ChunkClass &c = (int64_t)n * G <= p.few.max_rows ? p.few : p.many;
     c.tiles += (int)(((int64_t)n * G + c.tile_rows - 1) / c.tile_rows);
     c.tokens += n;
+    if (&c == &p.many && ++sequences == 1) {
+      c.only = b;
+      c.only_first = cu[b];
+      c.only_len = n;
+    }
   }
+  if (sequences > 1) p.many.only = -1;
   // Few rows: a range for each workgroup that fits the GPU, of one unit at least;
   // up to 256 keys, a step or two of the waves, are not worth a join.
   const int unit_log2 = D == 256 ? 6 : 7;
@@ -236,8 +248,15 @@ static int64_t chunk_grid(const ChunkClass &c, int H_kv) {
 template <int D>
 static void launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
   if (p.many.tiles > 0) {
-    hipLaunchKernelGGL(chunk_prefill_kernel<D>, dim3((unsigned)chunk_grid(p.many, a.H_kv)),
-                       dim3(chunk_row_waves<D>() * 64), 0, s, a, p.many);
+    const dim3 grid((unsigned)chunk_grid(p.many, a.H_kv));
+    if constexpr (D == 64 || D == 128) {
+      if (p.many.tile_rows == 256)
+        hipLaunchKernelGGL((chunk_prefill_kernel<D, 8>), grid, dim3(512), 0, s, a, p.many);
+    }
+    if constexpr (D != 128) {
+      if (p.many.tile_rows == 128)
+        hipLaunchKernelGGL((chunk_prefill_kernel<D, 4>), grid, dim3(256), 0, s, a, p.many);
+    }
     if (p.join_many) launch_join<D, false>(a, p.many, s);
   }
   if (p.few.tiles > 0) {

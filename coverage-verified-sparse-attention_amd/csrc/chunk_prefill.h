@@ -18,25 +18,25 @@
 //  - no maximum in a step (see weights()).
 //
 // D = 32 and 256: a workgroup takes 128 rows, four waves in step, each its own
-// overlap.
+// overlap.  So it does at D = 64 for prompts from near their start: smaller
+// tiles waste less of the causal mask and end closer together, though a step takes
+// longer: 2048 tokens from the start 34 us for 40, 16 prompts of up to 1000 after
+// 2000 175 for 189, but 4096 tokens after as many 243 for 231 (32 heads on 8).
 #pragma once
 #include "chunk_common.h"
 
 namespace cvsa {
 
 template <int D>
-constexpr int chunk_row_waves() {
-  return D == 64 || D == 128 ? 8 : 4;
-}
-template <int D>
 constexpr int chunk_step_keys() {
   return D == 256 ? 32 : 64;
 }
 
-template <int D>
-__global__ __launch_bounds__(chunk_row_waves<D>() * 64, D == 256 ? 1 : D == 32 ? 3 : 2) void
+// NW waves with 32 rows each.
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : D == 32 ? 3 : 2) void
 chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
-  constexpr int NW = chunk_row_waves<D>(), NT = NW * 64, KT = chunk_step_keys<D>();
+  constexpr int NT = NW * 64, KT = chunk_step_keys<D>();
   constexpr int CPR = D / 8, NC = KT * CPR;
   constexpr int P = NC / NT;  // vectors of K and of V per thread and step
   constexpr int KB = KT / 32, KS = D / 16, DB = D / 32;
@@ -49,35 +49,22 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // KV heads vary fastest: workgroups go round the XCDs, so one XCD's cache
-  // sees the keys of few heads.  Late row tiles, whose rows see most keys,
-  // start first.
+  // sees the keys of few heads.
   int id = blockIdx.x;
   const int h = id % a.H_kv;
   id /= a.H_kv;
   const int split = id % cl.splits;
-  const ChunkTile t = chunk_find_tile(a, cl, cl.tiles - 1 - id / cl.splits);
+  const ChunkTile t = chunk_find_tile<NW * 32>(a, cl, id / cl.splits);
   const int k0 = split * cl.split_len;
   // The last split also takes keys past the plan's bound.
   const int k1 = split < cl.splits - 1 ? min(t.keys, k0 + cl.split_len) : t.keys;
   if (cl.splits > 1 && k0 >= k1) return;
   const int steps = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
-  const bool live = t.row0 + wave * 32 < t.rows;  // the wave has rows
-  const ChunkRow row = chunk_row(a, t, h, t.row0 + wave * 32 + (lane & 31), k1);
-  const int full_keys = a.causal ? min(t.pos0 + t.row0 / a.G + 1, k1) : k1;  // all rows see
-  chunk_bf16x8_t q[KS];
-  chunk_load_q<D>(a, t, row, q);
-
   const int32_t *const bt = a.block_tables + t.seq * a.bt_sb;
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int row_bytes = a.H_kv * D * 2;
   const uint32_t block_bytes = (uint32_t)row_bytes << a.bs_log2;
-
-  s_taken.clear(NT);
-  __syncthreads();
-
-  ChunkState<D> state;
-  state.init();
 
   // Blocks.  Lane i looks up key i of a step for the whole wave, a step ahead
   // of the loads; where there is no key or no block of the pool, its bit of the
@@ -85,6 +72,29 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   auto lookup_keys = [&](int s) {
     return bt[min((k0 + s * KT + (lane & (KT - 1))) >> a.bs_log2, a.W - 1)];
   };
+  // All of the first lookups are under way before the first is waited for, and
+  // before Q.
+  const int found0 = lookup_keys(0), found1 = lookup_keys(1), found2 = lookup_keys(2);
+
+  const bool live = t.row0 + wave * 32 < t.rows;  // the wave has rows
+  const ChunkRow row = chunk_row(a, t, h, t.row0 + wave * 32 + (lane & 31), k1);
+  const int full_keys = a.causal ? min(t.pos0 + t.row0 / a.G + 1, k1) : k1;  // all rows see
+  chunk_bf16x8_t q[KS];
+  chunk_load_q<D>(a, t, row, q);
+
+  // Barrier after the wave's LDS accesses, its loads left in flight.
+  auto barrier = []() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  s_taken.clear(NT);
+  barrier();
+
+  ChunkState<D> state;
+  state.init();
+
   auto in_pool = [&](int s, int found) {
     return k0 + s * KT + (lane & (KT - 1)) < k1 && (uint32_t)found < (uint32_t)a.num_blocks;
   };
@@ -98,13 +108,6 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       s_taken.clean(reinterpret_cast<uint4 *>(lds + c * 8), keys >> r & 1, k0 + s * KT + r,
                     chunk_swizzle<D>(r, c % CPR) * 8);
     });
-  };
-  // Barrier after the wave's LDS accesses, its loads left in flight.
-  auto barrier = []() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
   };
   // Every load of this wave has arrived.
   auto arrived = []() {
@@ -252,16 +255,16 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
         key0 = key1;
         key1 = key2;
       };
-      key0 = locate(0, lookup_keys(0), blk2);
+      key0 = locate(0, found0, blk2);
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         load(a.k_cache, blk2[p], 0, s_k0, p);
         load(a.v_cache, blk2[p], 0, s_v0, p);
       }
-      key1 = locate(1, lookup_keys(1), blk1);
+      key1 = locate(1, found1, blk1);
 #pragma unroll
       for (int p = 0; p < P; ++p) load(a.k_cache, blk1[p], 1, s_k1, p);
-      found = lookup_keys(2);
+      found = found2;
       arrived();
       if (LATE) clean(0, key0, s_v0);
       barrier();
@@ -404,10 +407,9 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
     if (steps > 0) {
       f32x16_t st0[KB], st1[KB];
       int at0;
-      const int f0 = lookup_keys(0), f1 = lookup_keys(1);
-      found = lookup_keys(2);
-      key0 = locate(0, f0, at0);
-      key1 = locate(1, f1, at1);
+      found = found2;
+      key0 = locate(0, found0, at0);
+      key1 = locate(1, found1, at1);
       load(a.k_cache, 0, at0, s_k0);
       load(a.v_cache, 0, at0, s_v0);
       if (steps > 1) load(a.k_cache, 1, at1, s_k1);

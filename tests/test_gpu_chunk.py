@@ -244,11 +244,13 @@ def test_chunk_attention(gpu, D, lens, before):
 @pytest.mark.parametrize("D,bs,Hk,G,n", [(128, 16, 1, 128, 3), (64, 32, 2, 16, 40),
                                          (128, 128, 1, 4, 300), (256, 16, 1, 8, 33),
                                          (32, 16, 2, 12, 30), (128, 16, 1, 1, 260)])
-def test_chunk_attention_row_tiles(gpu, D, bs, Hk, G, n):
-    """Several row tiles and every number of row waves."""
+@pytest.mark.parametrize("W", [None, 5000])
+def test_chunk_attention_row_tiles(gpu, D, bs, Hk, G, n, W):
+    """Several row tiles and every number of row waves; a wide table takes
+    larger tiles and splits."""
     g = _gen(n)
     lens, before = [n, 1], [57, 90]
-    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, Hk, G)
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, Hk, G, W)
     out = _attend(gpu, q, kc, vc, bt, ctx, lens, G)
     ref.check_attend(out, ref.attend(q, kc, vc, bt, ctx, lens, G))
 
@@ -281,15 +283,15 @@ def test_chunk_attention_equals_dense_decode_for_single_tokens(gpu):
     ref.check_attend(dense, want)
 
 
-@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("D,W", [(64, None), (128, None), (256, None), (64, 300)])
 @pytest.mark.parametrize("n", [1, 6, 50])
-def test_rows_without_keys(gpu, D, n):
+def test_rows_without_keys(gpu, D, n, W):
     """Blocks outside the pool take no part; rows that see no key are zero
     with a log-sum-exp of -inf: a context shorter than the chunk, an empty
     context, a table of bad blocks only."""
     g = _gen(n)
     lens = [n, n, n, n]
-    q, kc, vc, bt, ctx = _attend_inputs(g, lens, [40, 40, 40, 40], D, 16, 2, 4)
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, [40, 40, 40, 40], D, 16, 2, 4, W)
     nb = kc.shape[0]
     bt[0, 1] = -1
     bt[1, :] = nb
@@ -314,14 +316,16 @@ def test_context_past_the_table(gpu):
 
 
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
-@pytest.mark.parametrize("D,n,G", [(128, 40, 4), (64, 9, 1), (256, 12, 2), (128, 3, 8)])
-def test_values_that_no_row_sees_do_not_touch_it(gpu, value, D, n, G):
+@pytest.mark.parametrize("D,n,G,W", [(128, 40, 4, None), (64, 9, 1, None), (256, 12, 2, None),
+                                     (128, 3, 8, None), (64, 40, 4, None), (64, 40, 4, 300),
+                                     (32, 40, 4, None)])
+def test_values_that_no_row_sees_do_not_touch_it(gpu, value, D, n, G, W):
     """Behind the context's end, in bad blocks, and keys and values of later
     tokens of the chunk: only the rows that see them feel them."""
     g = _gen(n)
     lens, before = [n, n], [21, 0]
     bs = 16
-    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, 2, G)
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, 2, G, W)
     used = torch.zeros(kc.shape[:2], dtype=torch.bool)
     for b in range(2):
         p = torch.arange(int(ctx[b]))
@@ -394,7 +398,8 @@ def test_chunk_attention_equal_chunks(gpu, D, Hk, G, n, B):
 
 
 @pytest.mark.parametrize("D,n,G", [(32, 2, 4), (64, 5, 7), (128, 1, 8), (256, 3, 4),
-                                   (32, 40, 4), (64, 40, 4), (128, 40, 4), (256, 40, 4)])
+                                   (32, 40, 4), (64, 40, 4), (128, 40, 4), (256, 40, 4),
+                                   (64, 300, 4)])
 def test_scores_that_rise_and_fall(gpu, D, n, G):
     """The reference of a row has to move when later scores outgrow it, by
     little or by far, and to stay when they fall."""
@@ -412,6 +417,25 @@ def test_scores_that_rise_and_fall(gpu, D, n, G):
             (score / (2 * math.sqrt(D)))[:, None] + 0.1 * _randn(g, at.numel(), D)).bfloat16()
         out, lse = _attend(gpu, q, k, vc, bt, ctx, lens, G, return_lse=True)
         ref.check_attend(out, ref.attend(q, k, vc, bt, ctx, lens, G), lse)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunk_attention_order_of_tiles(gpu, D, causal):
+    """Prompts of many row tiles whose order goes by their keys: alike ones,
+    contexts far apart, none, a chunk cut off by its table, and more sequences
+    than a wave has lanes; no tile is left out or done twice."""
+    g = _gen(D)
+    G, bs = 8, 16
+    for lens, before in (([100, 100, 100], [0, 0, 0]), ([90, 1, 130, 64], [300, 700, 0, 900]),
+                         ([33] * 70, [(37 * b) % 200 for b in range(70)])):
+        q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, 1, G)
+        if len(lens) == 4:
+            ctx[0], bt = 1500, bt[:, :50].contiguous()  # positions past the table
+            ctx[3] = -5
+        out = torch.full(q.shape, math.nan, dtype=torch.bfloat16, device=gpu)
+        _attend(gpu, q, kc, vc, bt, ctx, lens, G, causal=causal, out=out)
+        ref.check_attend(out, ref.attend(q, kc, vc, bt, ctx, lens, G, causal))
 
 
 def test_strided_queries_padded_rows_and_out(gpu):
