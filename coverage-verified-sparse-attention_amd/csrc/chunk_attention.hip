@@ -81,11 +81,8 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
     stride = rows;
   }
   auto part = [&](int s) { return s == 0 ? part0 : second + (s - 1) * stride; };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int s = mine; s < parts; s += groups) m = fmaxf(m, c.part_ml[part(s)].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  const bool whole = RANGES && parts == 1;  // complete already
+  float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float w, float sum, const float4 &v) {
     l = fmaf(sum, w, l);
@@ -94,12 +91,30 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
     o.z = fmaf(v.z, w, o.z);
     o.w = fmaf(v.w, w, o.w);
   };
-  const bool whole = RANGES && parts == 1;  // complete already
-#pragma unroll 4
-  for (int s = mine; s < parts && !whole; s += groups) {
-    const float2 ml = c.part_ml[part(s)];
-    add(__builtin_amdgcn_exp2f(ml.x - ref), ml.y,
-        *reinterpret_cast<const float4 *>(c.part_o + part(s) * D + d));
+  // Four parts at a time, all of their loads under way at once.
+  for (int s0 = mine; s0 < parts && !whole; s0 += 4 * groups) {
+    float2 ml[4];
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * groups;
+      const int64_t at = part(s < parts ? s : s0);
+      ml[i] = c.part_ml[at];
+      v[i] = *reinterpret_cast<const float4 *>(c.part_o + at * D + d);
+    }
+    float nm = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nm = fmaxf(nm, ml[i].x);
+    const float ref = nm == -INFINITY ? 0.f : nm, alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = nm;
+    l *= alpha;
+    o.x *= alpha;
+    o.y *= alpha;
+    o.z *= alpha;
+    o.w *= alpha;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (s0 + i * groups < parts) add(__builtin_amdgcn_exp2f(ml[i].x - ref), ml[i].y, v[i]);
   }
   if (groups > 1) {  // the same in every thread
     s_o[group][d / 4] = o;
