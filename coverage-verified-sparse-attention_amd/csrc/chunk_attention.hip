@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
     stride = rows;
   }
   auto part = [&](int s) { return s == 0 ? part0 : second + (s - 1) * stride; };
-  const bool whole = RANGES && parts == 1;  // complete already
+  const bool whole = parts == 1;  // complete already
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float w, float sum, const float4 &v) {
@@ -171,6 +171,56 @@ struct ChunkPlan {
   size_t bytes;  // of the workspace
 };
 
+// Splits of many rows' keys: the number with the shortest estimate of rounds of
+// workgroups, joined (rounds of the longest at one rate for all head sizes took
+// 380 us for 215: 10 prompts of up to 4792 tokens, 8 heads on 2 of 64; 2460 for
+// 1767: 5 of 2127 after 22 K keys, 32 on 16 of 32).  chunk: tokens of a chunk
+// (its tiles' mean), whose tiles are taken to see from max_keys - chunk to
+// max_keys keys.
+template <int D>
+static int plan_splits(const ChunkClass &c, int H_q, int H_kv, int64_t max_keys, double chunk) {
+  // us for 64 keys of a tile on a full CU; workgroups that fill one (two of eight
+  // waves fit at D = 64, but one alone is as fast), of which a single one has less
+  // than its share of the time.
+  const double step = D == 32 ? 0.52 : D == 256 ? 2.8 : D == 128 ? 1.45
+                              : c.tile_rows == 256 ? 1.15 : 0.6;
+  const int fit = D == 32 ? 3 : c.tile_rows == 128 && D == 64 ? 2 : 1;
+  const double hi = (double)max_keys, lo = std::max(hi - chunk, 0.), mean = (lo + hi) / 2;
+  const double items = (double)c.tiles * H_kv;
+  double best = 1e30;
+  int splits = 1;
+  // 1 to 8, as many as fill one to four rounds, and the most: 256 keys each.
+  const double most = std::max(1., std::min(64., std::floor(hi / 256)));
+  for (int i = 1; i <= 14; ++i) {
+    const double want = i <= 8 ? i : i <= 12 ? (i - 8) * 256 * fit / items : most / (i - 12);
+    const int n = (int)std::max(1., std::min(most, want));
+    const double len = hi / n;
+    // Mean of ceil(keys / len) from lo to hi.
+    auto area = [&](double x) {
+      const double q = std::floor(x / len);
+      return len * q * (q + 1) / 2 + (q + 1) * (x - q * len);
+    };
+    const double parts = n == 1 || hi - lo < 1 ? n : (area(hi) - area(lo)) / (hi - lo);
+    const double wgs = items * parts;
+    const double share = std::min<double>(fit, std::max((fit + 2) / 3., wgs / 256));
+    // 8 us for a workgroup's start and end, 12 if it writes a part.  Alike ones
+    // take whole rounds; of different ones the long start first and the short
+    // fill up.
+    const double ends = n == 1 ? 8 : 12, wg = mean / 64 * step * share / parts + ends;
+    const double rounds = wgs / (256 * fit), whole = std::ceil(rounds - 1e-6);
+    double us = std::max(len / 64 * step * share + ends,
+                         wg * (whole - (whole - rounds) * (hi - lo) / hi));
+    // The rows in several parts are written and read once more, at 3 TB/s.
+    if (n > 1)
+      us += 8 + std::min(parts, 2 * (parts - 1)) * c.tokens * H_q * D * 8 / 3e6;
+    if (us < best * (splits == 1 ? 0.95 : 1)) {
+      best = us;
+      splits = n;
+    }
+  }
+  return splits;
+}
+
 template <int D>
 static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t max_keys) {
   const int G = H_q / H_kv;
@@ -194,13 +244,16 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   p.few.tile_rows = most_few > 32 ? 64 : 32;
   p.few.same_len = p.many.same_len = same ? cu[1] : 0;
   p.many.only = -1;
-  int sequences = 0;  // of many rows
+  int sequences = 0;     // of many rows
+  int64_t weighted = 0;  // tokens of a tile's chunk, over all tiles
   for (int b = 0; b < B; ++b) {
     const int n = cu[b + 1] - cu[b];
     ChunkClass &c = (int64_t)n * G <= p.few.max_rows ? p.few : p.many;
     c.tiles += (int)(((int64_t)n * G + c.tile_rows - 1) / c.tile_rows);
     c.tokens += n;
-    if (&c == &p.many && ++sequences == 1) {
+    if (&c != &p.many) continue;
+    weighted += (int64_t)n * (((int64_t)n * G + c.tile_rows - 1) / c.tile_rows);
+    if (++sequences == 1) {
       c.only = b;
       c.only_first = cu[b];
       c.only_len = n;
@@ -216,23 +269,11 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   const int64_t units =
       (int64_t)p.few.tiles * (whole ? 1 : (max_keys + (1 << unit_log2) - 1) >> unit_log2);
   const int fit = most_few > 32 ? chunk_stream_fit<D, 2>() : chunk_stream_fit<D, 1>();
-  p.few.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 * (fit) / H_kv, units));
+  p.few.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 * fit / H_kv, units));
   p.join_few = p.few.tiles > 0 && p.few.splits > 1 && !whole;
-  // Many rows: the number of splits whose rounds of 256 workgroups (one a CU)
-  // take least, at 1.4 us for 64 keys, 5 us for a workgroup's start and end and
-  // 4 TB/s for writing and joining the parts.
-  const double items = (double)p.many.tiles * H_kv;
-  double best = 1e30;
   int64_t splits = 1;
-  for (int64_t n = 1; n <= 64 && (n == 1 || max_keys / n >= 512); ++n) {
-    const double rounds = std::ceil(items * n / 256);
-    const double us = rounds * ((double)max_keys / n / 64 * 1.4 + 5) +
-                      (n > 1 ? 4 + (double)p.many.tokens * H_q * n * D * 8 / 4e6 : 0);
-    if (us < best) {
-      best = us;
-      splits = n;
-    }
-  }
+  if (p.many.tiles > 0)
+    splits = plan_splits<D>(p.many, H_q, H_kv, max_keys, (double)weighted / p.many.tiles);
   p.many.split_len = (int)(((max_keys + splits - 1) / splits + 127) / 128 * 128);
   p.many.splits = (int)std::max<int64_t>(1, (max_keys + p.many.split_len - 1) / p.many.split_len);
   p.join_many = p.many.tiles > 0 && p.many.splits > 1;

@@ -427,7 +427,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
 
   state.finish();
   s_taken.restore(row.last_key, state.o);
-  if (cl.splits > 1)
+  if (cl.splits > 1 && (k0 > 0 || k1 < t.keys))
     state.store_part(cl, row, ((int64_t)split * cl.tokens + t.part0 + row.tok) * a.H_q + row.head);
   else
     state.store(a, t, row);
