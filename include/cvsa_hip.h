@@ -1,6 +1,7 @@
 /*
  * cvsa_hip.h - C ABI of libcvsa_hip.so, the MI355X (gfx950) implementation of
- * the CVSA decode-step attention path.
+ * the CVSA decode-step attention path, and of chunks of new tokens over the
+ * same cache.
  *
  * Conventions shared by every entry point:
  *  - Pointers are device pointers unless stated otherwise.  bf16 tensors are
