@@ -129,10 +129,10 @@ __device__ __forceinline__ int chunk_longer(const ChunkArgs &a, const ChunkSeq &
   return x <= 0 ? nt : nt - x * a.G / TR;
 }
 
-// Row tile `id` of a class in the order of their keys (to 64), the longest first:
-// tiles differ, by the causal mask and the contexts, and one that starts late
-// should be short.  4 prompts of 1024 tokens, 32 heads on 8 of 128: 51 us, in
-// the order of the sequences 62.
+// Row tile `id` of a class, of up to 64 sequences in the order of their keys (to
+// 64), the longest first: tiles differ, by the causal mask and the contexts, and
+// one that starts late should be short.  4 prompts of 1024 tokens, 32 heads on 8
+// of 128: 51 us, in the order of the sequences 62.
 template <int TR>
 __device__ __forceinline__ ChunkTile chunk_find_tile(const ChunkArgs &a, const ChunkClass &c,
                                                      int id) {
@@ -152,16 +152,15 @@ __device__ __forceinline__ ChunkTile chunk_find_tile(const ChunkArgs &a, const C
     auto longer = [&](const ChunkSeq &s, int level) {
       return level < 0 ? (s.len * a.G + TR - 1) / TR : chunk_longer<TR>(a, s, 64 * level + 63);
     };
-    // The lowest level that at most id tiles pass.
-    int low = 0, high = a.W << a.bs_log2 >> 6;  // none passes this one
-    if (a.B <= kWave)
+    // The lowest level that at most id tiles pass.  Past 64 sequences, where each
+    // try would read all of them again, their own order does.
+    const bool sorted = a.B <= kWave;
+    int low = 0, high = 0, above = 0;  // tiles that pass level high
+    if (sorted)
       high = __builtin_amdgcn_readfirstlane(wave_max_u32(own.len > 0 ? own.keys : 0)) >> 6;
-    int above = 0;  // tiles that pass level high
     while (low < high) {
       const int mid = (low + high) >> 1;
-      int n = 0;
-      for (int b0 = 0; b0 < a.B; b0 += kWave)
-        n += __builtin_amdgcn_readfirstlane(wave_sum_u32(longer(look(b0), mid)));
+      const int n = __builtin_amdgcn_readfirstlane(wave_sum_u32(longer(own, mid)));
       if (n <= id) {
         high = mid;
         above = n;
@@ -175,7 +174,8 @@ __device__ __forceinline__ ChunkTile chunk_find_tile(const ChunkArgs &a, const C
     first = len = ctx = tile = 0;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
       const ChunkSeq s = look(b0);
-      const int over = longer(s, low), nt = longer(s, -1), n = longer(s, low - 1) - over;
+      const int nt = longer(s, -1), over = sorted ? longer(s, low) : 0;
+      const int n = (sorted ? longer(s, low - 1) : nt) - over;
       const int incl = (int)wave_incl_scan_u32((uint32_t)n);
       const int toks = (int)wave_incl_scan_u32((uint32_t)s.len);
       const int total = __builtin_amdgcn_readlane(incl, 63);
