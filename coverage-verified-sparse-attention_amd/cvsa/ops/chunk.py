@@ -22,6 +22,9 @@ from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_se
                _i32, _lib, _ptr, check)
 
 _BF16 = torch.bfloat16
+_OUTSIDE = (1 << 31) - 1  # a position past every table
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.uint16,
+             torch.uint32, torch.uint64)
 
 
 class ChunkLayout:
@@ -77,6 +80,9 @@ class RotaryTable:
         if table.shape[1] < 16 or table.shape[1] % 16:
             raise NotImplementedError(f"rotary table: rot_dim {table.shape[1]} is not a "
                                       "multiple of 16")
+        if table.shape[0] > _OUTSIDE:
+            raise NotImplementedError(f"rotary table: {table.shape[0]} positions (at most "
+                                      f"{_OUTSIDE})")
         self.table = table.contiguous()
         if self.table.data_ptr() % 16:
             self.table = self.table.clone()
@@ -187,6 +193,17 @@ def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, cont
     return block_tables, context_lens
 
 
+def _positions(t: torch.Tensor) -> torch.Tensor:
+    """Positions as the kernels read them.  Those that int32 cannot hold stay
+    outside every table instead of wrapping to another position."""
+    if t.dtype in (torch.uint32, torch.uint64):
+        # Read as signed, what is past their range is negative.
+        t = t.view(torch.int32 if t.dtype is torch.uint32 else torch.int64)
+    if t.dtype is torch.int64:
+        t = t.clamp(-1, _OUTSIDE)
+    return _i32(t)
+
+
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
                  positions: Optional[torch.Tensor], rotary: Optional[RotaryTable] = None,
                  q_weight: Optional[torch.Tensor] = None,
@@ -218,11 +235,11 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
     qw, kw, wcode = _weights(who, D, q_weight, k_weight)
     rot = _rotary(who, rotary, D)
     if rotary is not None:
-        if positions is None or positions.dim() != 1 or positions.is_floating_point():
+        if positions is None or positions.dim() != 1 or positions.dtype not in _INTEGERS:
             raise ValueError(f"{who}: positions must be [{T}] integers")
         _check_count(who, "positions", positions, T)
         if positions.dtype is not torch.int32 or not positions.is_contiguous():
-            positions = _i32(positions)
+            positions = _positions(positions)
     q_out = q.new_empty((T, H_q, D))
     k_out = None if k is None else q.new_empty((T, H_kv, D))
     if T:

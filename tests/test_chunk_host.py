@@ -324,3 +324,58 @@ def test_manager_refuses_a_head_dimension_first(calls):
     with pytest.raises(NotImplementedError):
         m.append_chunk_kv(_bf(3, HK, 48), _bf(3, HK, 48), ops.ChunkLayout([3], "cpu"))
     assert not calls and m._ctx_host == [0]
+
+
+# ------------------------------------------------------------ positions
+
+def _position_reader(monkeypatch):
+    """qk_norm_rope on CPU tensors; the positions that its launch was given."""
+    seen = []
+    at = 7  # after three arguments of q, three of k and the dtype code
+
+    def call(dev, who, fn, *args, keep=None):
+        seen.append(list((ctypes.c_int32 * args[16]).from_address(args[at])))
+
+    monkeypatch.setattr(chunk, "_call", call)
+    return seen
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64])
+def test_positions_past_32_bits_stay_outside_the_table(calls, monkeypatch, dtype):
+    """A position that int32 cannot hold must not come back as another one."""
+    seen = _position_reader(monkeypatch)
+    far = [7, 2 ** 32 + 5, 2 ** 31, 2 ** 62 + 1, 79]
+    if dtype == torch.int64:
+        far += [-1, -2 ** 32 + 5, -2 ** 63]
+    else:
+        far += [2 ** 63 + 5, 2 ** 64 - 1]
+    T = len(far)
+    pos = torch.tensor(far, dtype=dtype)
+    table = ops.RotaryTable.build(D, 80, device="cpu")
+    for p in (pos, torch.stack([pos, pos], 1)[:, 0]):  # strided too
+        ops.qk_norm_rope(_bf(T, 1, D), None, p, table)
+    for got in seen:
+        for x, y in zip(far, got):
+            assert y == x if 0 <= x < 80 else not 0 <= y < 80
+    assert [len(got) for got in seen] == [T, T]
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32])
+def test_narrow_positions_are_kept(calls, monkeypatch, dtype):
+    seen = _position_reader(monkeypatch)
+    pos = torch.tensor([0, 5, 79], dtype=dtype)
+    ops.qk_norm_rope(_bf(3, 1, D), None, pos, ops.RotaryTable.build(D, 80, device="cpu"))
+    assert seen == [[0, 5, 79]]
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.complex64, torch.float32])
+def test_positions_that_are_no_integers_are_refused(calls, dtype):
+    with pytest.raises(ValueError, match="positions"):
+        ops.qk_norm_rope(_bf(3, 1, D), None, torch.zeros(3, dtype=dtype),
+                         ops.RotaryTable.build(D, 80, device="cpu"))
+    assert not calls
+
+
+def test_a_table_of_more_positions_than_int32_is_refused():
+    with pytest.raises(NotImplementedError, match="positions"):
+        ops.RotaryTable(torch.empty(1 << 31, 16, device="meta"))

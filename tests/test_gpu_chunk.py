@@ -112,6 +112,18 @@ def test_strided_rows_are_read_in_place(gpu):
         assert torch.equal(ops.qk_norm_rope(q, None, pos[:q.shape[0]], table)[0], want)
 
 
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64])
+def test_positions_past_32_bits_are_outside_the_table(gpu, dtype):
+    """2^32 + 5 is not position 5."""
+    q = torch.ones(4, 2, 64, dtype=torch.bfloat16, device=gpu)
+    table = ops.RotaryTable.build(32, 8, device=gpu)
+    pos = torch.tensor([2 ** 32 + 5, 5, 2 ** 31, 2 ** 62 + 1], dtype=dtype).to(gpu)
+    out = ops.qk_norm_rope(q, None, pos, table)[0].float()
+    assert out[[0, 2, 3], :, :32].isnan().all() and out[1].isfinite().all()
+    want = ops.qk_norm_rope(q, None, torch.full((4,), 5, dtype=torch.int32, device=gpu), table)[0]
+    assert torch.equal(out[1], want[1].float())
+
+
 # ------------------------------------------------------------ append
 
 def _tables(g, totals, bs, W=None, spare=3):
