@@ -140,7 +140,8 @@ def _rows(who: str, name: str, t: torch.Tensor, rows: Optional[int], heads: Opti
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()
-        st, sh, sd = t.stride()
+        # Not t's own: the stride of a single token or head can be any number.
+        st, sh = shape[1] * D, D
         at = t.data_ptr()
     return t, at, st, sh
 
@@ -176,7 +177,8 @@ def _rotary(who: str, rotary: Optional[RotaryTable], D: int):
 
 
 def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, context_lens):
-    """Block tables and context lengths as the kernels read them."""
+    """Block tables, their row stride and context lengths as the kernels read
+    them."""
     if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 \
             or block_tables.stride(1) != 1:
         block_tables = _block_tables(block_tables)
@@ -190,7 +192,8 @@ def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, cont
                          f"{block_tables.shape[0]}")
     if context_lens.dim() != 1 or context_lens.shape[0] != B:
         _check_seqs(who, B, None, context_lens)
-    return block_tables, context_lens
+    # The stride of a single row can be any number.
+    return block_tables, block_tables.stride(0) if B > 1 else block_tables.shape[1], context_lens
 
 
 def _positions(t: torch.Tensor) -> torch.Tensor:
@@ -271,7 +274,7 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
     dev = _same_device(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
                        rotary.table if rotary else None)
     num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
-    bt, ctx = _tables(who, layout, dev, block_tables, context_lens)
+    bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
     T = layout.total
     k, *k_at = _rows(who, "k", k, T, H_kv, D)
@@ -296,7 +299,7 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
         # k, v and q are held here: they may be copies.
         _call(dev, who, _lib.load().cvsa_append_chunk_kv, *k_at, *v_at, *q_at,
               _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
-              bt.data_ptr(), bt.stride(0), W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
+              bt.data_ptr(), bt_stride, W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
               *rot, _ptr(qw), _ptr(kw), wcode, float(eps), H_q, H_kv, D, block_size,
               _ptr(q_out), keep=(k, v, q))
     return launch, q_out
@@ -344,11 +347,11 @@ def reserve_chunk(block_tables: torch.Tensor, context_lens: torch.Tensor,
                     ("pages_allocated", pages_allocated)):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be contiguous int32")
-    block_tables, context_lens = _tables(who, layout, dev, block_tables, context_lens)
+    block_tables, bt_stride, context_lens = _tables(who, layout, dev, block_tables, context_lens)
     B = layout.batch
     _check_count(who, "pages_allocated", pages_allocated, B)
     _call(dev, who, _lib.load().cvsa_reserve_chunk, block_tables.data_ptr(),
-          block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+          bt_stride, block_tables.shape[1], context_lens.data_ptr(),
           pages_allocated.data_ptr(), layout.cu_seqlens.data_ptr(), B, next_free_block,
           num_blocks, block_size)
 
@@ -381,8 +384,10 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
     if H_kv != num_kv_heads:
         raise ValueError(f"{who}: head counts do not match the caches")
-    bt, ctx = _tables(who, layout, dev, block_tables, context_lens)
+    bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
+    if bt_stride < W:  # a row that sequences share
+        bt, bt_stride = bt.contiguous(), W
     T, H_q = layout.total, num_kv_heads * num_q_per_kv
     q, *q_at = _rows(who, "q", q, T, H_q, D, _BF16)
     max_context_len = int(max_context_len)
@@ -413,7 +418,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             layout._workspace_bytes[sizes] = need
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
         _call(dev, who, L.cvsa_chunk_attention, *q_at, k_cache.data_ptr(), v_cache.data_ptr(),
-              num_blocks, bt.data_ptr(), bt.stride(0), ctx.data_ptr(), layout.cu_seqlens.data_ptr(),
+              num_blocks, bt.data_ptr(), bt_stride, ctx.data_ptr(), layout.cu_seqlens.data_ptr(),
               layout.cu_host, B, H_q, num_kv_heads, D, block_size, W, max_context_len, scale,
               int(bool(causal)), out.data_ptr(), _ptr(lse), _ptr(ws), need)
     return (out, lse) if return_lse else out

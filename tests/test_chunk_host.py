@@ -379,3 +379,50 @@ def test_positions_that_are_no_integers_are_refused(calls, dtype):
 def test_a_table_of_more_positions_than_int32_is_refused():
     with pytest.raises(NotImplementedError, match="positions"):
         ops.RotaryTable(torch.empty(1 << 31, 16, device="meta"))
+
+
+# ------------------------------------------------------------ strides
+
+def _bent(t, stride):
+    """t (one entry along its first dimension) with another stride there: torch
+    calls it contiguous, whatever the stride is."""
+    assert t.shape[0] == 1
+    return t.as_strided(t.shape, (stride, *t.stride()[1:]))
+
+
+def test_the_stride_of_one_token_and_of_one_sequence_does_not_matter(calls):
+    """One token of rows that are no multiple of 16 bytes apart, and the table
+    of one sequence: no second row is read, so no stride refuses them."""
+    a = _append_args()
+    a["layout"] = ops.ChunkLayout([1], "cpu")
+    a["block_tables"] = _bent(torch.zeros(1, W, dtype=torch.int32), 1)
+    a["context_lens"] = torch.ones(1, dtype=torch.int32)
+    a.update(k=_bent(_bf(1, HK, D), HK * D + 3), v=_bent(_bf(1, HK, D), 1),
+             q=_bent(_bf(1, HK * G, D), HK * G * D + 1))
+    ops.append_chunk_kv(**a)
+    b = _attend_args()
+    b.update({n: a[n] for n in ("q", "layout", "block_tables", "context_lens")})
+    ops.chunk_attention(**b)
+    r = _rope_args()
+    # one head: its stride is none either
+    one = _bf(1, 1, D).as_strided((1, 1, D), (D + 5, 7, 1))
+    r.update(q=a["q"], k=one, positions=torch.zeros(1, dtype=torch.int64))
+    ops.qk_norm_rope(**r)
+    ops.reserve_chunk(a["block_tables"], a["context_lens"], torch.zeros(1, dtype=torch.int32),
+                      a["layout"], 0, NB, BS)
+    got = {who: dict(zip(range(len(args)), args)) for who, args in calls}
+    # (stride of the tokens, stride of the heads) in elements, multiples of 8
+    for who, places in (("append_chunk_kv", (1, 4, 7)), ("chunk_attention", (1,)),
+                        ("qk_norm_rope", (1, 4))):
+        for i in places:
+            assert got[who][i] % 8 == 0 and got[who][i + 1] % 8 == 0
+    assert got["append_chunk_kv"][14] >= W and got["append_chunk_kv"][15] == W
+    assert got["chunk_attention"][7] >= W and got["reserve_chunk"][1] >= W
+
+
+def test_a_table_that_sequences_share_is_read(calls):
+    """One row of blocks for every sequence, as a broadcast view."""
+    b = _attend_args()
+    b["block_tables"] = torch.zeros(1, W, dtype=torch.int32).expand(3, W)
+    ops.chunk_attention(**b)
+    assert calls[0][1][7] >= W

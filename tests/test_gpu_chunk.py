@@ -474,6 +474,36 @@ def test_strided_queries_padded_rows_and_out(gpu):
     assert torch.equal(_attend(gpu, q, kc, vc, wide[:, ::2], ctx, lens, G), want)
 
 
+def test_one_token_and_one_sequence_of_any_stride(gpu):
+    """A single token's row, and a single sequence's table, whose (unused)
+    strides are odd; and a table that sequences share."""
+    g = _gen(14)
+    Hk, G, D, bs, before = 2, 4, 64, 16, 40
+    q, kc, vc, bt, ctx = (x.to(gpu) for x in _attend_inputs(g, [1], [before], D, bs, Hk, G))
+    k, v = (_randn(g, 1, Hk, D).bfloat16().to(gpu) for _ in range(2))
+    layout, table = ops.ChunkLayout([1], gpu), ops.RotaryTable.build(D, 64, device=gpu)
+
+    def bent(t):
+        return t.as_strided(t.shape, (t.stride(0) + 1, *t.stride()[1:]))
+
+    def step(q, k, v, bt):
+        c = kc.clone(), vc.clone()
+        qr = ops.append_chunk_kv(k, v, *c, bt, ctx, layout, bs, table, q=q)
+        qn, kn = ops.qk_norm_rope(q, k, ctx - 1, table)
+        return (qr, *c, qn, kn,
+                ops.chunk_attention(qr, *c, bt, ctx, layout, Hk, G, bs))
+
+    want = step(q, k, v, bt)
+    got = step(bent(q), bent(k), bent(v), bt.as_strided(bt.shape, (1, 1)))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    three = ops.ChunkLayout([1] * 3, gpu)
+    shared = [bt.expand(3, -1), bt.repeat(3, 1)]
+    outs = [ops.chunk_attention(q.expand(3, -1, -1), *want[1:3], b, ctx.repeat(3), three, Hk, G, bs)
+            for b in shared]
+    assert torch.equal(*outs)
+
+
 def test_offsets_past_32_bits(gpu):
     """A pool of more than 2^32 elements: blocks at its far end."""
     Hk, D, bs = 8, 256, 128
