@@ -276,7 +276,7 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
     num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
     bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
-    T = layout.total
+    T, eps = layout.total, float(eps)
     k, *k_at = _rows(who, "k", k, T, H_kv, D)
     v, *v_at = _rows(who, "v", v, T, H_kv, D, k.dtype)
     if q is None and q_weight is not None:
@@ -292,6 +292,8 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
             q_out[T:].zero_()
     if D not in (32, 64, 128, 256):
         raise NotImplementedError(f"{who}: D={D} not in {{32, 64, 128, 256}}")
+    if max(H_q, H_kv) > 65536:
+        raise ValueError(f"{who}: {H_q} and {H_kv} heads (at most 65536)")
 
     def launch():
         if T == 0:
@@ -300,7 +302,7 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
         _call(dev, who, _lib.load().cvsa_append_chunk_kv, *k_at, *v_at, *q_at,
               _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
               bt.data_ptr(), bt_stride, W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
-              *rot, _ptr(qw), _ptr(kw), wcode, float(eps), H_q, H_kv, D, block_size,
+              *rot, _ptr(qw), _ptr(kw), wcode, eps, H_q, H_kv, D, block_size,
               _ptr(q_out), keep=(k, v, q))
     return launch, q_out
 

@@ -426,3 +426,18 @@ def test_a_table_that_sequences_share_is_read(calls):
     b["block_tables"] = torch.zeros(1, W, dtype=torch.int32).expand(3, W)
     ops.chunk_attention(**b)
     assert calls[0][1][7] >= W
+
+
+# ------------------------------------------------------------ before any state changes
+
+@pytest.mark.parametrize("error,bad", [
+    (TypeError, dict(eps=None)), (ValueError, dict(eps="small")),
+    (ValueError, dict(q=_bf(1, 1, D).expand(T, 65537, D))),
+])
+def test_manager_refuses_before_pages_are_taken(calls, error, bad):
+    """What only the launch looked at: by then the pages were taken."""
+    m = _manager()
+    before = _state(m)
+    with pytest.raises(error):
+        m.append_chunk_kv(_bf(T, HK, D), _bf(T, HK, D), ops.ChunkLayout(LENS, "cpu"), **bad)
+    assert _state(m) == before and not calls
