@@ -269,7 +269,8 @@ def _check_caches(who, k_cache, v_cache, block_size):
 def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, layout, block_size,
                          rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None):
     """The checks of :func:`append_chunk_kv` without its launch: returns
-    (launch, q_out); launch() enqueues it."""
+    (launch, q_out); launch() enqueues it, on the same stream.  The tables may
+    change in place in between; k, v, q and the weights may not."""
     who = "append_chunk_kv"
     dev = _same_device(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
                        rotary.table if rotary else None)
@@ -294,16 +295,20 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
         raise NotImplementedError(f"{who}: D={D} not in {{32, 64, 128, 256}}")
     if max(H_q, H_kv) > 65536:
         raise ValueError(f"{who}: {H_q} and {H_kv} heads (at most 65536)")
+    copied = bt is not block_tables or ctx is not context_lens
 
-    def launch():
+    def launch(at_once: bool = False):
         if T == 0:
             return
+        b, stride, c = bt, bt_stride, ctx
+        if copied and not at_once:
+            b, stride, c = _tables(who, layout, dev, block_tables, context_lens)
         # k, v and q are held here: they may be copies.
         _call(dev, who, _lib.load().cvsa_append_chunk_kv, *k_at, *v_at, *q_at,
               _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
-              bt.data_ptr(), bt_stride, W, ctx.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
+              b.data_ptr(), stride, W, c.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
               *rot, _ptr(qw), _ptr(kw), wcode, eps, H_q, H_kv, D, block_size,
-              _ptr(q_out), keep=(k, v, q))
+              _ptr(q_out), keep=(k, v, q, rotary))
     return launch, q_out
 
 
@@ -330,7 +335,7 @@ def append_chunk_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     """
     launch, q_out = prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens,
                                          layout, block_size, rotary, k_weight, eps, q, q_weight)
-    launch()
+    launch(at_once=True)
     return q_out
 
 

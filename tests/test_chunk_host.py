@@ -441,3 +441,22 @@ def test_manager_refuses_before_pages_are_taken(calls, error, bad):
     with pytest.raises(error):
         m.append_chunk_kv(_bf(T, HK, D), _bf(T, HK, D), ops.ChunkLayout(LENS, "cpu"), **bad)
     assert _state(m) == before and not calls
+
+
+def test_a_prepared_append_reads_the_tables_at_its_launch(calls, monkeypatch):
+    """The tables that grow between the checks and the launch, in a form that
+    the kernel needs copied: the copy is the launch's."""
+    a = _append_args()
+    a["context_lens"], a["block_tables"] = a["context_lens"].long(), a["block_tables"].long()
+    launch, _ = ops.prepare_append_chunk(**a)
+    a["context_lens"] += 9
+    a["block_tables"] += 4
+    got = []
+
+    def call(dev, who, fn, *args, keep=None):
+        got.append((list((ctypes.c_int32 * 3).from_address(args[16])),
+                    list((ctypes.c_int32 * (3 * W)).from_address(args[13]))))
+
+    monkeypatch.setattr(chunk, "_call", call)
+    launch()
+    assert got == [([n + 9 for n in LENS], [4] * (3 * W))]
