@@ -109,6 +109,14 @@ def _same_device(*tensors: Optional[torch.Tensor]) -> torch.device:
     return tensors[0].device
 
 
+def capturing(dev: torch.device) -> bool:
+    """Whether dev's current stream records a graph."""
+    if dev.type != "cuda":
+        return False
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _call(dev: torch.device, who: str, fn, *args, keep=None) -> None:
     """fn(*args, stream) on dev's current stream, whatever the current device;
     `keep` lives until the launch."""
@@ -347,7 +355,9 @@ def reserve_chunk(block_tables: torch.Tensor, context_lens: torch.Tensor,
     grows by the chunk's lengths and new pages take the blocks from
     next_free_block on.  The three tensors are contiguous int32 and updated in
     place; the caller has checked that tables and pool hold the chunk
-    (SequenceKVManager.reserve_chunk does)."""
+    (SequenceKVManager.reserve_chunk does).  next_free_block is the call's own
+    number: replays of a captured call give the same blocks out again, so
+    capture it only where no sequence needs a new page (pages_allocated)."""
     who = "reserve_chunk"
     dev = _device_of(block_tables, context_lens, pages_allocated)
     for name, t in (("block_tables", block_tables), ("context_lens", context_lens),

@@ -694,7 +694,9 @@ int cvsa_append_chunk_kv(const void *k, int64_t k_stride_t, int64_t k_stride_h,
  * gives its new pages the blocks from next_free_block on, by the rule of
  * append_token_kv (kv_cache.py:133-150) applied to each token, sequence after
  * sequence.  pages_allocated ([B] int32) is updated; entries past W or
- * num_blocks are not written (the caller checks both first). */
+ * num_blocks are not written (the caller checks both first).  next_free_block
+ * is a number of this call: replays of a captured call give the same blocks
+ * out again, unless no sequence needs a new page. */
 int cvsa_reserve_chunk(int32_t *block_tables, int64_t bt_stride_b, int32_t W,
                        int32_t *context_lens, int32_t *pages_allocated,
                        const int32_t *cu_seqlens, int32_t B, int32_t next_free_block,

@@ -460,3 +460,22 @@ def test_a_prepared_append_reads_the_tables_at_its_launch(calls, monkeypatch):
     monkeypatch.setattr(chunk, "_call", call)
     launch()
     assert got == [([n + 9 for n in LENS], [4] * (3 * W))]
+
+
+# ------------------------------------------------------------ captured graphs
+
+def test_manager_refuses_to_be_captured(calls, monkeypatch):
+    """A replay would hand out the same blocks again, and the manager's
+    lengths would stay behind."""
+    m = _manager()
+    before = _state(m)
+    lay = ops.ChunkLayout(LENS, "cpu")
+    monkeypatch.setattr(chunk, "capturing", lambda dev: True)
+    with pytest.raises(RuntimeError, match="captur"):
+        m.reserve_chunk(lay)
+    with pytest.raises(RuntimeError, match="captur"):
+        m.append_chunk_kv(_bf(T, HK, D), _bf(T, HK, D), lay)
+    assert _state(m) == before and not calls
+    ops.append_chunk_kv(**_append_args())  # over tables of the caller's: may be captured
+    ops.chunk_attention(**_attend_args())
+    assert len(calls) == 2

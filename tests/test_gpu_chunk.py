@@ -667,6 +667,44 @@ def test_graph_replays_and_other_streams(gpu, lens, W):
         assert torch.equal(other, eager)
 
 
+def test_a_managers_pages_are_not_taken_in_a_graph(gpu):
+    """The manager's calls are refused while a graph is captured and leave no
+    trace; the append over pages that it reserved before is captured, and
+    replays with new rows."""
+    g = _gen(15)
+    lens, bs, Hk, D = [5, 20], 16, 2, 64
+    T = sum(lens)
+    mgr = SequenceKVManager(PagedKVCache(8, bs, Hk, D, device=gpu), 2, 64)
+    mgr.cache.k_cache.zero_()
+    mgr.cache.v_cache.zero_()
+    layout, table = ops.ChunkLayout(lens, gpu), ops.RotaryTable.build(D, 64, device=gpu)
+    k, v = (torch.zeros(T, Hk, D, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    mgr.reserve_chunk(layout)
+    held = (list(mgr._ctx_host), list(mgr._pages_allocated), mgr.cache._next_free)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    args = (mgr.block_tables, mgr.context_lens, layout, bs, table)
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="captur"):
+            mgr.reserve_chunk(layout)
+        with pytest.raises(RuntimeError, match="captur"):
+            mgr.append_chunk_kv(k, v, layout, table)
+        ops.append_chunk_kv(k, v, mgr.cache.k_cache, mgr.cache.v_cache, *args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert held == (mgr._ctx_host, mgr._pages_allocated, mgr.cache._next_free)
+    for _ in range(3):
+        k.copy_(_randn(g, T, Hk, D).bfloat16())
+        v.copy_(_randn(g, T, Hk, D).bfloat16())
+        graph.replay()
+        torch.cuda.synchronize()
+        want = [torch.zeros_like(mgr.cache.k_cache) for _ in range(2)]
+        ops.append_chunk_kv(k, v, *want, *args)
+        assert torch.equal(mgr.cache.k_cache, want[0])
+        assert torch.equal(mgr.cache.v_cache, want[1])
+    assert mgr.context_lens.tolist() == lens
+
+
 def test_calls_on_two_streams_at_once(gpu):
     """Split calls that overlap share no workspace."""
     g = _gen(13)
