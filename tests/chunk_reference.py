@@ -115,3 +115,14 @@ def check_attend(got, ref, lse=None):
         assert torch.equal(lse.isfinite(), fin)
         assert (lse[~fin] == want_lse[~fin]).all() or want_lse[~fin].isnan().any()
         assert not ((lse - want_lse).abs() > lse_slack)[fin].any()
+
+
+def check_kinds(got, ref):
+    """check_attend, and that each output is of its kind: the same infinity, or
+    NaN."""
+    want = ref[0]
+    check_attend(got, ref)
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    inf = want.isinf()
+    assert inf.any() and torch.equal(got[inf], want[inf])

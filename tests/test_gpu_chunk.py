@@ -1,6 +1,7 @@
 """Chunks of new tokens on the GPU: norms with rotation, the append to the
 paged cache and the attention over it, each against its formula in 64 bits,
 and a run of them together as a serving loop makes it."""
+import ctypes
 import math
 
 import pytest
@@ -361,6 +362,63 @@ def test_values_that_no_row_sees_do_not_touch_it(gpu, value, D, n, G, W):
     early[n - 2:n] = False
     err = (out - want[0]).abs()
     assert not (err > want[2])[early].any()
+
+
+def _splits(lens, Hk, G, D, bs, W):
+    """(splits, keys of one) that the plan has for sequences of many rows only,
+    from the size of its workspace: a part has D sums and two numbers for each
+    token and head."""
+    cu = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    need = ops._lib.load().cvsa_chunk_attention_workspace_bytes(
+        (ctypes.c_int32 * len(cu))(*cu), len(lens), Hk * G, Hk, D, bs, W, 0)
+    splits = max(1, need // (cu[-1] * Hk * G * (4 * D + 8)))
+    return splits, -(-W * bs // (splits * 128)) * 128
+
+
+MANY = [  # chunks, tokens before, heads of the group, width of the table
+    ([600, 80], [1400, 900], 1, 128),    # 128-row tiles at D = 64
+    ([70, 300], [5000, 200], 4, 5000),   # the table of a much longer context
+    ([100, 17, 40], [3000, 1, 700], 4, 200),
+]
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("lens,before,G,W", MANY)
+def test_many_rows_in_several_splits(gpu, D, lens, before, G, W):
+    """Rows whose keys lie in one split, in several, and in a part of the last;
+    some of them tell complete tiles and parts of one call apart."""
+    g = _gen(D + W)
+    splits, split_len = _splits(lens, 1, G, D, 16, W)
+    assert splits > 1 and lens[0] + before[0] > split_len > 128
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, 16, 1, G, W)
+    for causal in (True, False):
+        out, lse = _attend(gpu, q, kc, vc, bt, ctx, lens, G, causal=causal, return_lse=True)
+        ref.check_attend(out, ref.attend(q, kc, vc, bt, ctx, lens, G, causal), lse)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("lens,before,G,W", MANY + [([3, 1], [700, 50], 7, None),
+                                                    ([40, 40], [60, 0], 4, None),
+                                                    ([5, 2], [2000, 900], 4, 600)])
+def test_infinite_values_keep_their_kind(gpu, D, lens, before, G, W):
+    """Columns of V that hold infinities of either sign and NaN, alone and
+    together, at keys that all rows see (in the first split and a later one)
+    and at keys that only later tokens see: each row gets what it sees."""
+    g = _gen(D + len(lens) + lens[0])
+    bs, inf, nan = 16, math.inf, math.nan
+    q, kc, vc, bt, ctx = _attend_inputs(g, lens, before, D, bs, 1, G, W)
+    columns = [{0: inf}, {0: -inf}, {0: nan}, {0: inf, 1: -inf}, {0: -inf, 1: inf},
+               {0: inf, 1: inf}, {0: inf, 1: nan}, {0: nan, 1: -inf}, {1: -inf}]
+    n, b0 = lens[0], before[0]
+    for i, (early, late) in enumerate(((3, b0 - 5), (b0 // 2, b0 + n // 2), (b0, b0 + n - 1))):
+        for j, column in enumerate(columns):
+            for at, value in column.items():
+                p = late if at else early
+                vc[bt[0, p // bs].long(), p % bs, 0, 9 * i + j] = value
+    assert 9 * 3 <= D
+    for causal in (True, False):
+        out = _attend(gpu, q, kc, vc, bt, ctx, lens, G, causal=causal)
+        ref.check_kinds(out, ref.attend(q, kc, vc, bt, ctx, lens, G, causal))
 
 
 def test_scores_of_any_size(gpu):
