@@ -32,7 +32,8 @@ struct RotaryArgs {
   float eps;
   int tokens, H_q, H_kv;
   int groups, per_wave, segs;  // passes of a token, of a wave, waves of a token
-  const int32_t *positions;    // without APPEND
+  const void *positions;       // without APPEND: int32 or, wide, int64
+  bool wide;
   // APPEND
   uint16_t *k_cache, *v_cache;
   int64_t num_blocks;
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
   };
   request(g0);
 
-  int pos;
+  int64_t pos;
   int64_t slot = -1;  // token's row in the cache, -1: not written
   if constexpr (APPEND) {
     // The sequence of token t: the last b with cu[b] <= t, 64 candidates a
@@ -210,17 +211,20 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
       n = min(step, n - k * step);
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    pos = a.context_lens[b] - (a.cu[b + 1] - t);
-    if (pos >= 0) {
-      const int page = pos / a.block_size;
+    const int at = a.context_lens[b] - (a.cu[b + 1] - t);
+    pos = at;
+    if (at >= 0) {
+      const int page = at / a.block_size;
       if (page < a.W) {
         const int blk = a.block_tables[b * a.bt_sb + page];
         if (blk >= 0 && blk < a.num_blocks)
-          slot = (int64_t)blk * a.block_size + (pos - page * a.block_size);
+          slot = (int64_t)blk * a.block_size + (at - page * a.block_size);
       }
     }
   } else {
-    pos = a.positions ? a.positions[t] : 0;
+    pos = !a.positions ? 0
+          : a.wide     ? static_cast<const int64_t *>(a.positions)[t]
+                       : static_cast<const int32_t *>(a.positions)[t];
   }
 
   // Cosines and sines of the lane's pairs; NaN at a position that the table
@@ -229,7 +233,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
 #pragma unroll
   for (int e = 0; e < 8; ++e) cs[e] = sn[e] = __builtin_nanf("");
   if (a.table && pos >= 0 && pos < a.table_len) {
-    const float *row = a.table + (int64_t)pos * a.R;
+    const float *row = a.table + pos * a.R;
     const int half = a.R / 2;
     if (PAIRS) {  // 4 pairs of each vector
       if (r0) {
@@ -451,14 +455,16 @@ static int check_rotary(const char *who, const RotaryArgs &a, int32_t dtype, int
 
 extern "C" int cvsa_qk_norm_rope(const void *q, int64_t q_stride_t, int64_t q_stride_h,
                                  const void *k, int64_t k_stride_t, int64_t k_stride_h,
-                                 int32_t dtype, const int32_t *positions, const float *table,
-                                 int64_t table_len, int32_t rot_dim, int32_t interleaved,
-                                 const void *q_weight, const void *k_weight,
+                                 int32_t dtype, const void *positions, int32_t positions_bytes,
+                                 const float *table, int64_t table_len, int32_t rot_dim,
+                                 int32_t interleaved, const void *q_weight, const void *k_weight,
                                  int32_t weight_dtype, float eps, int32_t tokens, int32_t H_q,
                                  int32_t H_kv, int32_t D, void *q_out, void *k_out,
                                  void *stream) {
   CVSA_REQUIRE(q && q_out && (!k || k_out) && (!table || positions), CVSA_ERR_INVALID,
                "qk_norm_rope: null pointer argument");
+  CVSA_REQUIRE(!table || positions_bytes == 4 || positions_bytes == 8, CVSA_ERR_INVALID,
+               "qk_norm_rope: positions of %d bytes, not 4 or 8", positions_bytes);
   RotaryArgs a = {};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h; a.q_out = q_out;
   if (k) {
@@ -467,6 +473,7 @@ extern "C" int cvsa_qk_norm_rope(const void *q, int64_t q_stride_t, int64_t q_st
   a.table = table; a.table_len = table_len; a.R = rot_dim;
   a.q_w = q_weight; a.k_w = k ? k_weight : nullptr; a.w_dtype = weight_dtype; a.eps = eps;
   a.tokens = tokens; a.H_q = H_q; a.H_kv = H_kv; a.positions = positions;
+  a.wide = positions_bytes == 8;
   const int rc = check_rotary("qk_norm_rope", a, dtype, D, interleaved);
   if (rc != CVSA_OK) return rc;
   enqueue_rotary<false>(a, dtype, D, interleaved, stream);

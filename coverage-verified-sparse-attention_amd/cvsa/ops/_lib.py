@@ -10,7 +10,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parents[1] / "libcvsa_hip.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 CVSA_OK = 0
 CVSA_ERR_INVALID = -1
@@ -128,7 +128,7 @@ SIGNATURES = {
     "cvsa_step_plan_destroy": (None, [_p]),
     "cvsa_step_plan_selection_changed": (ctypes.c_int, [_p]),
     "cvsa_qk_norm_rope": (ctypes.c_int, [
-        _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p, _i32, _f32,
+        _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i32, _p, _i64, _i32, _i32, _p, _p, _i32, _f32,
         _i32, _i32, _i32, _i32, _p, _p, _p]),
     "cvsa_append_chunk_kv": (ctypes.c_int, [
         _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _i64, _p, _i64, _i32,

@@ -22,7 +22,6 @@ from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_se
                _i32, _lib, _ptr, check)
 
 _BF16 = torch.bfloat16
-_OUTSIDE = (1 << 31) - 1  # a position past every table
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.uint16,
              torch.uint32, torch.uint64)
 
@@ -80,9 +79,6 @@ class RotaryTable:
         if table.shape[1] < 16 or table.shape[1] % 16:
             raise NotImplementedError(f"rotary table: rot_dim {table.shape[1]} is not a "
                                       "multiple of 16")
-        if table.shape[0] > _OUTSIDE:
-            raise NotImplementedError(f"rotary table: {table.shape[0]} positions (at most "
-                                      f"{_OUTSIDE})")
         self.table = table.contiguous()
         if self.table.data_ptr() % 16:
             self.table = self.table.clone()
@@ -205,14 +201,15 @@ def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, cont
 
 
 def _positions(t: torch.Tensor) -> torch.Tensor:
-    """Positions as the kernels read them.  Those that int32 cannot hold stay
-    outside every table instead of wrapping to another position."""
-    if t.dtype in (torch.uint32, torch.uint64):
-        # Read as signed, what is past their range is negative.
-        t = t.view(torch.int32 if t.dtype is torch.uint32 else torch.int64)
-    if t.dtype is torch.int64:
-        t = t.clamp(-1, _OUTSIDE)
-    return _i32(t)
+    """Positions as the kernel reads them: int32 or int64, never narrowed to
+    another position."""
+    if t.dtype is torch.uint64:
+        t = t.view(torch.int64)  # those past its range: negative, outside the table
+    elif t.dtype is torch.uint32:
+        t = t.to(torch.int64)
+    elif t.dtype is not torch.int64:
+        t = t.to(torch.int32)
+    return t.contiguous()
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
@@ -255,8 +252,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
     k_out = None if k is None else q.new_empty((T, H_kv, D))
     if T:
         _call(dev, who, _lib.load().cvsa_qk_norm_rope, *q_at, *k_at, _DTYPE_CODE[q.dtype],
-              _ptr(positions) if rotary else None, *rot, _ptr(qw), _ptr(kw), wcode, float(eps), T,
-              H_q, H_kv, D, q_out.data_ptr(), _ptr(k_out))
+              *((positions.data_ptr(), positions.element_size()) if rotary else (None, 4)), *rot,
+              _ptr(qw), _ptr(kw), wcode, float(eps), T, H_q, H_kv, D, q_out.data_ptr(),
+              _ptr(k_out))
     return q_out, k_out
 
 

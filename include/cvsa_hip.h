@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define CVSA_ABI_VERSION 15
+#define CVSA_ABI_VERSION 16
 
 enum {
   CVSA_OK = 0,
@@ -662,12 +662,13 @@ void cvsa_step_plan_destroy(cvsa_step_plan *plan);
 
 /* Norm x * rsqrt(mean(x^2) + eps) * weight of every head's row of q
  * [tokens, H_q, D] and k [tokens, H_kv, D] (or NULL), then the rotation by
- * the token's entry of positions ([tokens] int32, unused without a table).
+ * the token's entry of positions ([tokens] integers of 4 or 8 bytes, unused
+ * without a table).
  * q_out / k_out: contiguous, of the inputs' dtype (CVSA_DTYPE_*). */
 int cvsa_qk_norm_rope(const void *q, int64_t q_stride_t, int64_t q_stride_h,
                       const void *k, int64_t k_stride_t, int64_t k_stride_h,
-                      int32_t dtype, const int32_t *positions, const float *table,
-                      int64_t table_len, int32_t rot_dim, int32_t interleaved,
+                      int32_t dtype, const void *positions, int32_t positions_bytes,
+                      const float *table, int64_t table_len, int32_t rot_dim, int32_t interleaved,
                       const void *q_weight, const void *k_weight, int32_t weight_dtype,
                       float eps, int32_t tokens, int32_t H_q, int32_t H_kv, int32_t D,
                       void *q_out, void *k_out, void *stream);

@@ -268,6 +268,15 @@ def test_c_append_refuses(over, code, word):
     assert word in lib.cvsa_last_error()
 
 
+@pytest.mark.parametrize("size", [0, 2, 16])
+def test_c_norm_rope_refuses_positions_of_another_size(size):
+    lib = _lib_or_skip()
+    args = [P[0], HK * D, D, None, 0, 0, 0, P[1], size, P[2], 8, D, 0, None, None, 0, 1e-6, 3, HK,
+            0, D, P[3], None, None]
+    assert lib.cvsa_qk_norm_rope(*args) == _lib.CVSA_ERR_INVALID
+    assert b"positions" in lib.cvsa_last_error()
+
+
 def test_c_reserve_refuses():
     lib = _lib_or_skip()
     good = [P[0], W, W, P[1], P[2], P[3], 2, 0, NB, BS]
@@ -331,24 +340,23 @@ def test_manager_refuses_a_head_dimension_first(calls):
 def _position_reader(monkeypatch):
     """qk_norm_rope on CPU tensors; the positions that its launch was given."""
     seen = []
-    at = 7  # after three arguments of q, three of k and the dtype code
 
     def call(dev, who, fn, *args, keep=None):
-        seen.append(list((ctypes.c_int32 * args[16]).from_address(args[at])))
+        at, size, tokens = args[7], args[8], args[17]
+        kind = {4: ctypes.c_int32, 8: ctypes.c_int64}[size]
+        seen.append(list((kind * tokens).from_address(at)))
 
     monkeypatch.setattr(chunk, "_call", call)
     return seen
 
 
-@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
 def test_positions_past_32_bits_stay_outside_the_table(calls, monkeypatch, dtype):
     """A position that int32 cannot hold must not come back as another one."""
     seen = _position_reader(monkeypatch)
-    far = [7, 2 ** 32 + 5, 2 ** 31, 2 ** 62 + 1, 79]
-    if dtype == torch.int64:
-        far += [-1, -2 ** 32 + 5, -2 ** 63]
-    else:
-        far += [2 ** 63 + 5, 2 ** 64 - 1]
+    far = {torch.int64: [7, 2 ** 32 + 5, 2 ** 31, 2 ** 62 + 1, 79, -1, -2 ** 32 + 5, -2 ** 63],
+           torch.uint32: [7, 2 ** 31, 2 ** 31 + 5, 2 ** 32 - 1, 79],
+           torch.uint64: [7, 2 ** 32 + 5, 2 ** 63 + 5, 2 ** 64 - 1, 79]}[dtype]
     T = len(far)
     pos = torch.tensor(far, dtype=dtype)
     table = ops.RotaryTable.build(D, 80, device="cpu")
@@ -360,12 +368,19 @@ def test_positions_past_32_bits_stay_outside_the_table(calls, monkeypatch, dtype
     assert [len(got) for got in seen] == [T, T]
 
 
-@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32])
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.uint16, torch.int32])
 def test_narrow_positions_are_kept(calls, monkeypatch, dtype):
     seen = _position_reader(monkeypatch)
     pos = torch.tensor([0, 5, 79], dtype=dtype)
     ops.qk_norm_rope(_bf(3, 1, D), None, pos, ops.RotaryTable.build(D, 80, device="cpu"))
     assert seen == [[0, 5, 79]]
+
+
+def test_wide_positions_are_read_in_place(calls):
+    """No launch in front of the call's own."""
+    pos = torch.arange(3)
+    ops.qk_norm_rope(_bf(3, 1, D), None, pos, ops.RotaryTable.build(D, 80, device="cpu"))
+    assert calls[0][1][7:9] == (pos.data_ptr(), 8)
 
 
 @pytest.mark.parametrize("dtype", [torch.bool, torch.complex64, torch.float32])
@@ -374,11 +389,6 @@ def test_positions_that_are_no_integers_are_refused(calls, dtype):
         ops.qk_norm_rope(_bf(3, 1, D), None, torch.zeros(3, dtype=dtype),
                          ops.RotaryTable.build(D, 80, device="cpu"))
     assert not calls
-
-
-def test_a_table_of_more_positions_than_int32_is_refused():
-    with pytest.raises(NotImplementedError, match="positions"):
-        ops.RotaryTable(torch.empty(1 << 31, 16, device="meta"))
 
 
 # ------------------------------------------------------------ strides
