@@ -109,6 +109,8 @@ def capturing(dev: torch.device) -> bool:
     """Whether dev's current stream records a graph."""
     if dev.type != "cuda":
         return False
+    if torch._C._cuda_getDevice() == dev.index:
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(dev):
         return torch.cuda.is_current_stream_capturing()
 

@@ -269,6 +269,9 @@ class SequenceKVManager:
         written by ops.append_chunk_kv.  Not while the stream is captured: a
         replay would give the same blocks out again, without this manager's
         count of them."""
+        if ops.chunk.capturing(self.block_tables.device):
+            raise RuntimeError("a manager's pages cannot be taken in a captured graph: reserve "
+                               "them before it, capture ops.append_chunk_kv")
         need, pages = self._plan_chunk(layout)
         ops.reserve_chunk(self.block_tables, self.context_lens, self._pages_allocated_dev, layout,
                           self.cache._next_free, self.cache._total_blocks, self.block_size)
@@ -278,10 +281,7 @@ class SequenceKVManager:
 
     def _plan_chunk(self, layout):
         """(blocks a chunk takes, pages allocated after it); refuses a chunk
-        that the tables or the pool cannot hold, and a captured one."""
-        if ops.chunk.capturing(self.block_tables.device):
-            raise RuntimeError("a manager's pages cannot be taken in a captured graph: reserve "
-                               "them before it, capture ops.append_chunk_kv")
+        that the tables or the pool cannot hold."""
         if layout.batch != self.batch_size:
             raise ValueError(f"the layout has {layout.batch} sequences, the manager "
                              f"{self.batch_size}")
