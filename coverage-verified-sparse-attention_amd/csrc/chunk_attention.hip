@@ -339,6 +339,10 @@ static bool chunk_shape_ok(const int32_t *cu, int32_t B, int32_t H_q, int32_t H_
          (int64_t)cu[B] * H_q < (1LL << 31);
 }
 
+// Most keys of a sequence, as far as the host knows.  Contexts are on the device,
+// so without the caller's bound the splits of many rows are cut for sequences that
+// fill the table: in a table for 128 K keys, 32 heads on 8 of 128, 512 tokens at 4 K
+// keys take 88 us and 100 at 8 K 159, with the bound 49 and 35.
 static int64_t chunk_max_keys(int32_t W, int32_t block_size, int32_t max_context_len) {
   const int64_t all = (int64_t)W * block_size;
   return max_context_len > 0 ? std::min<int64_t>(all, max_context_len) : all;

@@ -18,10 +18,15 @@
 //  - no maximum in a step (see weights()).
 //
 // D = 32 and 256: a workgroup takes 128 rows, four waves in step, each its own
-// overlap.  So it does at D = 64 for prompts from near their start: smaller
-// tiles waste less of the causal mask and end closer together, though a step takes
-// longer: 2048 tokens from the start 34 us for 40, 16 prompts of up to 1000 after
-// 2000 175 for 189, but 4096 tokens after as many 243 for 231 (32 heads on 8).
+// overlap.  4096 tokens after as many, 32 heads on 8: 179 us at D = 32 (vector
+// instructions active in 77% of the cycles, the matrix pipe in 26%) and 1028 at D =
+// 256 (802 TFLOP/s; vector 43%, matrix 33%, LDS 17%: no pipe is full, the one wave
+// of a SIMD takes them in turns).
+//
+// 128 rows also at D = 64 for prompts from near their start: smaller tiles waste
+// less of the causal mask and end closer together, though a step takes longer:
+// 2048 tokens from the start 34 us for 40, 16 prompts of up to 1000 after 2000 175
+// for 189, but 4096 tokens after as many 243 for 231 (32 heads on 8).
 #pragma once
 #include "chunk_common.h"
 

@@ -20,7 +20,10 @@
 // Measured with the join, heads of 128: 32 sequences of 8 K keys, one token each,
 // 193 us, 5.6 TB/s (a copy of 1 GB reaches 5.1); one sequence of 128 K keys 104 us,
 // 5.2 TB/s; 8 drafts of 5 tokens at 32 K keys 112 us, 4.8 TB/s.  What is left is
-// the kernel's start (6 us to the first products) and the join (5 to 7 us).
+// the kernel's start (6 us to the first products) and the join (5 to 7 us).  The
+// decode kernels, which take single tokens only, need 88 us for the one sequence
+// (14 for one of 8 K keys, 15 here), and keep the weights of the second product in
+// two bf16 parts where these round them to one.
 #pragma once
 #include "chunk_common.h"
 

@@ -396,9 +396,13 @@ static void launch_rotary_d(const RotaryArgs &a, int D, int pairs, bool once, hi
 }
 
 // Passes of a token and how many a wave takes: all of them once the tokens
-// alone make enough waves to fill the GPU, one otherwise.  Then the outputs also
-// outgrow the caches and are stored past them: 8191 tokens of 28 + 4 heads of
-// 128 take 29.7 us, 35.6 with ordinary stores.
+// alone make enough waves to fill the GPU (2048), one otherwise.  With so many
+// tokens the outputs are also stored past the caches: 8191 tokens of 28 + 4 heads
+// of 128 take 29.7 us, 35.6 with ordinary stores.  The rule looks at the tokens
+// alone, not at the bytes.  2047 tokens (neither) and 2048 (both), heads of 128:
+// 1 + 1 heads 10.3 and 10.1 us, 32 + 8 10.6 and 10.0, 128 + 16 27.2 and 27.1, and
+// 64 + 8 heads of fp32, whose 75 MB in and 75 MB out fit the last-level cache from
+// pass to pass, 26.0 and 32.4.
 template <bool APPEND>
 static void enqueue_rotary(RotaryArgs &a, int dtype, int D, int pairs, void *stream) {
   const int rows = 64 / (D / 16);

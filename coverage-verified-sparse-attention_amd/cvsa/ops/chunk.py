@@ -388,13 +388,16 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     blocks outside the pool or past the block table take no part; a query
     that sees no key gives zeros and a log-sum-exp of -inf.  ``scale``
     defaults to D^-0.5.  ``max_context_len`` (most keys of a sequence, where
-    the caller knows) only shapes the launch.  With ``return_lse`` the natural
+    the caller knows) only shapes the launch: without it chunks of more than a
+    few tokens are cut for contexts that fill the block table, and take up to
+    several times as long where the table is much wider.  With ``return_lse`` the natural
     log-sum-exps [T, H_q] fp32 of the scaled scores are returned too.  Rows
     past layout.total are zero in a new output and left as they are in ``out``
     (contiguous bf16 of q's shape; a contiguous q itself will do).
 
     Scores, sums and outputs are held in 32 bits; the weights of the second
-    product are rounded to bf16.
+    product are rounded to bf16 (:func:`dense_decode`, for batches of single
+    tokens, keeps 16 bits of them).
     """
     who = "chunk_attention"
     dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out)

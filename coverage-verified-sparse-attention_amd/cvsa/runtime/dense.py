@@ -41,8 +41,9 @@ class DenseAttentionBackend:
                 causal=True, scale=None, max_context_len=0):
         """Attention of a chunk of new tokens already in the cache:
         [T, H_q, D] queries laid out by ``layout`` (ops.ChunkLayout) ->
-        [T, H_q, D].  No counterpart in the reference's backends, which only
-        decode."""
+        [T, H_q, D].  Pass ``max_context_len``, the longest context, where the
+        block tables are wider than the contexts (a manager's are).  No
+        counterpart in the reference's backends, which only decode."""
         return ops.chunk_attention(q, k_cache, v_cache, block_tables, context_lens, layout,
                                    self.num_kv_heads, self.num_q_per_kv, self.block_size,
                                    causal=causal, scale=scale, max_context_len=max_context_len)

@@ -718,7 +718,8 @@ size_t cvsa_chunk_attention_workspace_bytes(const int32_t *cu_host, int32_t B, i
  * cu_host: the same offsets in host memory.  out: [cu[B], H_q, D] bf16
  * contiguous; lse: [cu[B], H_q] fp32 (natural logarithm) or NULL.  The
  * workspace needs no initialisation and is free again when the call's kernels
- * have run.  max_context_len only shapes the launch. */
+ * have run.  max_context_len only shapes the launch: a bound near the longest
+ * context keeps chunks of many tokens from being cut for the whole table. */
 int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
                          const uint16_t *k_cache, const uint16_t *v_cache,
                          int64_t num_blocks, const int32_t *block_tables,
