@@ -1,8 +1,7 @@
 // Attention of a chunk of new tokens over the paged cache: the join of split
 // keys, the launch plan and the entry points.  Sequences that bring few rows
 // (chunk_stream.h) and many (chunk_prefill.h) get a launch each.
-#include "chunk_prefill.h"
-#include "chunk_stream.h"
+#include "chunk_launch.h"
 
 #include <algorithm>
 #include <cmath>
@@ -157,14 +156,6 @@ static void launch_join(const ChunkArgs &a, const ChunkClass &c, hipStream_t s) 
                      dim3(kJoinThreads), 0, s, a, c, groups);
 }
 
-// Rows of a sequence and KV head that the stream kernel takes at most: two
-// tiles of a wave (one at D = 256, whose two tiles' outputs alone would fill a
-// wave's registers).
-template <int D>
-constexpr int chunk_few_rows() {
-  return D == 256 ? 32 : 64;
-}
-
 struct ChunkPlan {
   ChunkClass few, many;  // tiles 0: no such sequence
   bool join_few, join_many;
@@ -221,7 +212,7 @@ static int plan_splits(const ChunkClass &c, int H_q, int H_kv, int64_t max_keys,
   return splits;
 }
 
-template <int D>
+template <int D, bool F8>
 static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t max_keys) {
   const int G = H_q / H_kv;
   ChunkPlan p = {};
@@ -262,13 +253,13 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   if (sequences > 1) p.many.only = -1;
   // Few rows: a range for each workgroup that fits the GPU, of one unit at least;
   // up to 256 keys, a step or two of the waves, are not worth a join.
-  const int unit_log2 = D == 256 ? 6 : 7;
-  static_assert(chunk_stream_waves<D>() * 32 == (D == 256 ? 64 : 128), "a step of the waves");
+  constexpr int unit_log2 = chunk_stream_waves<D, F8>() == 2 ? 6 : 7;
+  static_assert(chunk_stream_waves<D, F8>() * 32 == 1 << unit_log2, "a step of the waves");
   const bool whole = max_keys <= 256;
   p.few.unit_log2 = p.many.unit_log2 = whole ? 31 : unit_log2;
   const int64_t units =
       (int64_t)p.few.tiles * (whole ? 1 : (max_keys + (1 << unit_log2) - 1) >> unit_log2);
-  const int fit = most_few > 32 ? chunk_stream_fit<D, 2>() : chunk_stream_fit<D, 1>();
+  const int fit = most_few > 32 ? chunk_stream_fit<D, 2, F8>() : chunk_stream_fit<D, 1, F8>();
   p.few.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 * fit / H_kv, units));
   p.join_few = p.few.tiles > 0 && p.few.splits > 1 && !whole;
   int64_t splits = 1;
@@ -289,12 +280,13 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   return p;
 }
 
+template <bool F8>
 static ChunkPlan plan_chunk_d(const int32_t *cu, int B, int H_q, int H_kv, int D,
                               int64_t max_keys) {
-  if (D == 32) return plan_chunk<32>(cu, B, H_q, H_kv, max_keys);
-  if (D == 64) return plan_chunk<64>(cu, B, H_q, H_kv, max_keys);
-  if (D == 128) return plan_chunk<128>(cu, B, H_q, H_kv, max_keys);
-  return plan_chunk<256>(cu, B, H_q, H_kv, max_keys);
+  if (D == 32) return plan_chunk<32, F8>(cu, B, H_q, H_kv, max_keys);
+  if (D == 64) return plan_chunk<64, F8>(cu, B, H_q, H_kv, max_keys);
+  if (D == 128) return plan_chunk<128, F8>(cu, B, H_q, H_kv, max_keys);
+  return plan_chunk<256, F8>(cu, B, H_q, H_kv, max_keys);
 }
 
 static int64_t chunk_grid(const ChunkClass &c, int H_kv) {
@@ -303,26 +295,16 @@ static int64_t chunk_grid(const ChunkClass &c, int H_kv) {
 
 template <int D>
 static void launch_chunk(const ChunkArgs &a, const ChunkPlan &p, hipStream_t s) {
+  const bool f8 = a.k_scales != nullptr;
   if (p.many.tiles > 0) {
-    const dim3 grid((unsigned)chunk_grid(p.many, a.H_kv));
-    if constexpr (D == 64 || D == 128) {
-      if (p.many.tile_rows == 256)
-        hipLaunchKernelGGL((chunk_prefill_kernel<D, 8>), grid, dim3(512), 0, s, a, p.many);
-    }
-    if constexpr (D != 128) {
-      if (p.many.tile_rows == 128)
-        hipLaunchKernelGGL((chunk_prefill_kernel<D, 4>), grid, dim3(256), 0, s, a, p.many);
-    }
+    const unsigned grid = (unsigned)chunk_grid(p.many, a.H_kv);
+    if (f8) launch_chunk_prefill<D, true>(a, p.many, grid, s);
+    else launch_chunk_prefill<D, false>(a, p.many, grid, s);
     if (p.join_many) launch_join<D, false>(a, p.many, s);
   }
   if (p.few.tiles > 0) {
-    const dim3 grid((unsigned)(p.few.splits * a.H_kv)), block(chunk_stream_waves<D>() * 64);
-    if constexpr (chunk_few_rows<D>() > 32) {
-      if (p.few.tile_rows > 32)
-        hipLaunchKernelGGL((chunk_stream_kernel<D, 2>), grid, block, 0, s, a, p.few);
-    }
-    if (p.few.tile_rows <= 32)
-      hipLaunchKernelGGL((chunk_stream_kernel<D, 1>), grid, block, 0, s, a, p.few);
+    if (f8) launch_chunk_stream<D, true>(a, p.few, s);
+    else launch_chunk_stream<D, false>(a, p.few, s);
     if (p.join_few) launch_join<D, true>(a, p.few, s);
   }
 }
@@ -352,67 +334,85 @@ static int64_t chunk_max_keys(int32_t W, int32_t block_size, int32_t max_context
 
 using namespace cvsa;
 
+template <bool F8>
+static size_t chunk_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q, int32_t H_kv,
+                                    int32_t D, int32_t block_size, int32_t W,
+                                    int32_t max_context_len) {
+  if (!chunk_shape_ok(cu_host, B, H_q, H_kv, D, block_size, W) || cu_host[B] == 0) return 0;
+  return plan_chunk_d<F8>(cu_host, B, H_q, H_kv, D,
+                          chunk_max_keys(W, block_size, max_context_len))
+      .bytes;
+}
+
 extern "C" size_t cvsa_chunk_attention_workspace_bytes(const int32_t *cu_host, int32_t B,
                                                        int32_t H_q, int32_t H_kv, int32_t D,
                                                        int32_t block_size, int32_t W,
                                                        int32_t max_context_len) {
-  if (!chunk_shape_ok(cu_host, B, H_q, H_kv, D, block_size, W) || cu_host[B] == 0) return 0;
-  return plan_chunk_d(cu_host, B, H_q, H_kv, D, chunk_max_keys(W, block_size, max_context_len))
-      .bytes;
+  return chunk_workspace_bytes<false>(cu_host, B, H_q, H_kv, D, block_size, W, max_context_len);
 }
 
-extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
-                                    const uint16_t *k_cache, const uint16_t *v_cache,
-                                    int64_t num_blocks, const int32_t *block_tables,
-                                    int64_t bt_stride_b, const int32_t *context_lens,
-                                    const int32_t *cu_seqlens, const int32_t *cu_host, int32_t B,
-                                    int32_t H_q, int32_t H_kv, int32_t D, int32_t block_size,
-                                    int32_t W, int32_t max_context_len, float scale,
-                                    int32_t causal, uint16_t *out, float *lse, void *workspace,
-                                    size_t workspace_bytes, void *stream) {
+extern "C" size_t cvsa_chunk_attention8_workspace_bytes(const int32_t *cu_host, int32_t B,
+                                                        int32_t H_q, int32_t H_kv, int32_t D,
+                                                        int32_t block_size, int32_t W,
+                                                        int32_t max_context_len) {
+  return chunk_workspace_bytes<true>(cu_host, B, H_q, H_kv, D, block_size, W, max_context_len);
+}
+
+// Over caches of bf16, or of 8 bits (with scales).
+static int chunk_attention(const char *who, const uint16_t *q, int64_t q_stride_t,
+                           int64_t q_stride_h, const void *k_cache, const void *v_cache,
+                           const uint8_t *k_scales, const uint8_t *v_scales, int64_t num_blocks,
+                           const int32_t *block_tables, int64_t bt_stride_b,
+                           const int32_t *context_lens, const int32_t *cu_seqlens,
+                           const int32_t *cu_host, int32_t B, int32_t H_q, int32_t H_kv, int32_t D,
+                           int32_t block_size, int32_t W, int32_t max_context_len, float scale,
+                           int32_t causal, uint16_t *out, float *lse, void *workspace,
+                           size_t workspace_bytes, void *stream) {
   CVSA_REQUIRE(q && k_cache && v_cache && block_tables && context_lens && cu_seqlens && cu_host &&
                    out,
-               CVSA_ERR_INVALID, "chunk_attention: null pointer argument");
+               CVSA_ERR_INVALID, "%s: null pointer argument", who);
   CVSA_REQUIRE(head_dim_supported(D), CVSA_ERR_UNSUPPORTED,
-               "chunk_attention: D=%d not in {32, 64, 128, 256}", D);
+               "%s: D=%d not in {32, 64, 128, 256}", who, D);
   CVSA_REQUIRE(block_size_supported(block_size), CVSA_ERR_UNSUPPORTED,
-               "chunk_attention: block_size=%d not in {8, 16, 32, 64, 128}", block_size);
+               "%s: block_size=%d not in {8, 16, 32, 64, 128}", who, block_size);
   CVSA_REQUIRE(H_kv > 0 && H_q > 0 && H_q % H_kv == 0, CVSA_ERR_INVALID,
-               "chunk_attention: head counts H_q=%d H_kv=%d", H_q, H_kv);
+               "%s: head counts H_q=%d H_kv=%d", who, H_q, H_kv);
   CVSA_REQUIRE(H_q / H_kv <= 128 && W <= kMaxPagesWide, CVSA_ERR_UNSUPPORTED,
-               "chunk_attention: G=%d (at most 128) or W=%d (at most %d) not supported",
+               "%s: G=%d (at most 128) or W=%d (at most %d) not supported", who,
                H_q / H_kv, W, kMaxPagesWide);
   CVSA_REQUIRE(chunk_shape_ok(cu_host, B, H_q, H_kv, D, block_size, W) && num_blocks > 0 &&
                    bt_stride_b >= W,
-               CVSA_ERR_INVALID, "chunk_attention: bad sizes or chunk offsets (B=%d W=%d)", B, W);
+               CVSA_ERR_INVALID, "%s: bad sizes or chunk offsets (B=%d W=%d)", who, B, W);
   CVSA_REQUIRE((int64_t)block_size * H_kv * D < (1 << 30), CVSA_ERR_UNSUPPORTED,
-               "chunk_attention: a block of %d tokens of %d heads is too large", block_size, H_kv);
+               "%s: a block of %d tokens of %d heads is too large", who, block_size, H_kv);
   CVSA_REQUIRE(scale > 0.f && scale < INFINITY, CVSA_ERR_INVALID,
-               "chunk_attention: scale must be positive and finite");
+               "%s: scale must be positive and finite", who);
   CVSA_REQUIRE(max_context_len >= 0 && (causal == 0 || causal == 1), CVSA_ERR_INVALID,
-               "chunk_attention: bad max_context_len=%d or causal=%d", max_context_len, causal);
+               "%s: bad max_context_len=%d or causal=%d", who, max_context_len, causal);
   CVSA_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) ==
                        0 &&
                    q_stride_t % 8 == 0 && q_stride_h % 8 == 0,
-               CVSA_ERR_INVALID, "chunk_attention: rows must be 16-byte aligned");
+               CVSA_ERR_INVALID, "%s: rows must be 16-byte aligned", who);
   const int32_t tokens = cu_host[B];
   if (tokens == 0) return CVSA_OK;
-  ChunkPlan p = plan_chunk_d(cu_host, B, H_q, H_kv, D,
-                             chunk_max_keys(W, block_size, max_context_len));
+  const int64_t max_keys = chunk_max_keys(W, block_size, max_context_len);
+  ChunkPlan p = k_scales ? plan_chunk_d<true>(cu_host, B, H_q, H_kv, D, max_keys)
+                         : plan_chunk_d<false>(cu_host, B, H_q, H_kv, D, max_keys);
   CVSA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes &&
                                 ((uintptr_t)workspace & 255) == 0),
                CVSA_ERR_WORKSPACE,
-               "chunk_attention: needs a 256-byte aligned workspace of %zu bytes", p.bytes);
+               "%s: needs a 256-byte aligned workspace of %zu bytes", who, p.bytes);
   CVSA_REQUIRE(chunk_grid(p.many, H_kv) < (1LL << 31) &&
                    (int64_t)p.few.tiles * ((int64_t)W * block_size / 64 + 1) < (1LL << 31),
-               CVSA_ERR_UNSUPPORTED, "chunk_attention: too many row tiles or keys");
+               CVSA_ERR_UNSUPPORTED, "%s: too many row tiles or keys", who);
   for (ChunkClass *c : {&p.few, &p.many}) {
     c->part_ml = (float2 *)((char *)workspace + (size_t)c->part_ml);
     c->part_o = (float *)((char *)workspace + (size_t)c->part_o);
   }
   ChunkArgs a = {};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
-  a.k_cache = k_cache; a.v_cache = v_cache;
+  a.k_cache = (const uint16_t *)k_cache; a.v_cache = (const uint16_t *)v_cache;
+  a.k_scales = k_scales; a.v_scales = v_scales;
   a.num_blocks = (int)std::min<int64_t>(num_blocks, INT32_MAX);
   a.block_tables = block_tables; a.bt_sb = bt_stride_b; a.W = W;
   a.context_lens = context_lens; a.cu = cu_seqlens;
@@ -426,5 +426,38 @@ extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64
   else if (D == 64) launch_chunk<64>(a, p, s);
   else if (D == 128) launch_chunk<128>(a, p, s);
   else launch_chunk<256>(a, p, s);
-  return cvsa_host::check_launch("chunk_attention");
+  return cvsa_host::check_launch(who);
+}
+
+extern "C" int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
+                                    const uint16_t *k_cache, const uint16_t *v_cache,
+                                    int64_t num_blocks, const int32_t *block_tables,
+                                    int64_t bt_stride_b, const int32_t *context_lens,
+                                    const int32_t *cu_seqlens, const int32_t *cu_host, int32_t B,
+                                    int32_t H_q, int32_t H_kv, int32_t D, int32_t block_size,
+                                    int32_t W, int32_t max_context_len, float scale,
+                                    int32_t causal, uint16_t *out, float *lse, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+  return chunk_attention("chunk_attention", q, q_stride_t, q_stride_h, k_cache, v_cache, nullptr,
+                         nullptr, num_blocks, block_tables, bt_stride_b, context_lens, cu_seqlens,
+                         cu_host, B, H_q, H_kv, D, block_size, W, max_context_len, scale, causal,
+                         out, lse, workspace, workspace_bytes, stream);
+}
+
+extern "C" int cvsa_chunk_attention8(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
+                                     const uint8_t *k_cache, const uint8_t *v_cache,
+                                     const uint8_t *k_scales, const uint8_t *v_scales,
+                                     int64_t num_blocks, const int32_t *block_tables,
+                                     int64_t bt_stride_b, const int32_t *context_lens,
+                                     const int32_t *cu_seqlens, const int32_t *cu_host, int32_t B,
+                                     int32_t H_q, int32_t H_kv, int32_t D, int32_t block_size,
+                                     int32_t W, int32_t max_context_len, float scale,
+                                     int32_t causal, uint16_t *out, float *lse, void *workspace,
+                                     size_t workspace_bytes, void *stream) {
+  CVSA_REQUIRE(k_scales && v_scales, CVSA_ERR_INVALID,
+               "chunk_attention8: null pointer argument");
+  return chunk_attention("chunk_attention8", q, q_stride_t, q_stride_h, k_cache, v_cache, k_scales,
+                         v_scales, num_blocks, block_tables, bt_stride_b, context_lens, cu_seqlens,
+                         cu_host, B, H_q, H_kv, D, block_size, W, max_context_len, scale, causal,
+                         out, lse, workspace, workspace_bytes, stream);
 }

@@ -33,7 +33,6 @@
 #include "cvsa_common.h"
 
 #include <type_traits>
-#include <utility>
 
 namespace cvsa {
 
@@ -58,7 +57,8 @@ struct ChunkClass {
 struct ChunkArgs {
   const uint16_t *q;
   int64_t q_st, q_sh;
-  const uint16_t *k_cache, *v_cache;
+  const uint16_t *k_cache, *v_cache;     // of 8 bits: bytes, with a scale for each
+  const uint8_t *k_scales, *v_scales;    // block and head, [num_blocks, H_kv] (null: bf16)
   int num_blocks;
   const int32_t *block_tables;
   int64_t bt_sb;
@@ -76,15 +76,6 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 chunk_bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short chunk_short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) chunk_short4_t chunk_lds_short4;
-
-template <int N, class F, int... I>
-__device__ __forceinline__ void unrolled(F f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void unrolled(F f) {
-  unrolled<N>(f, std::make_integer_sequence<int, N>());
-}
 
 // Key and row ranges of a row tile.
 struct ChunkTile {
@@ -244,15 +235,18 @@ __device__ __forceinline__ ChunkRow chunk_row(const ChunkArgs &a, const ChunkTil
   return r;
 }
 
-// Q^T as the second operand: row l % 32, 8 columns from 16 ks + 8 (l / 32).
-template <int D>
+// Q^T as the second operand: row l % 32, 8 columns from 16 ks + 8 (l / 32), or
+// WIDE (as 16-byte reads of 8-bit keys have them) from 32 (ks / 2) + 16 (l / 32) +
+// 8 (ks % 2).
+template <int D, bool WIDE = false>
 __device__ __forceinline__ void chunk_load_q(const ChunkArgs &a, const ChunkTile &t,
                                              const ChunkRow &r, chunk_bf16x8_t (&q)[D / 16]) {
   const uint16_t *p = a.q + (int64_t)(t.first + r.tok) * a.q_st + r.head * a.q_sh +
-                      ((threadIdx.x >> 5) & 1) * 8;
+                      ((threadIdx.x >> 5) & 1) * (WIDE ? 16 : 8);
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks)
-    q[ks] = *reinterpret_cast<const chunk_bf16x8_t *>(p + ks * 16);
+    q[ks] = *reinterpret_cast<const chunk_bf16x8_t *>(
+        p + (WIDE ? ks / 2 * 32 + ks % 2 * 8 : ks * 16));
 }
 
 // Place of 16-byte vector ch of row r of a tile: 16 rows (32 or 64 at D = 64
@@ -263,7 +257,8 @@ __device__ __forceinline__ int chunk_swizzle(int r, int ch) {
   constexpr int CPR = D / 8;
   if constexpr (CPR >= 16) return ch ^ (((r & 3) << 2) | ((r >> 2) & 3));
   else if constexpr (CPR == 8) return ch ^ (((r & 2) << 1) | ((r >> 2) & 3));
-  else return ch ^ ((r >> 2) & 3);
+  else if constexpr (CPR == 4) return ch ^ ((r >> 2) & 3);
+  else return ch ^ ((r >> 3) & 1);
 }
 
 // Bytes from a tile's start to what the lane reads of it: K of row l % 32 (and
@@ -291,6 +286,11 @@ __device__ __forceinline__ uint4 chunk_read_v(char *lo, char *hi) {
   const uint2 y =
       __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((chunk_lds_short4 *)hi));
   return make_uint4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ uint2 chunk_read_v8(char *at) {
+  typedef int int2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       (__attribute__((address_space(3))) int2_t *)at));
 }
 
 // The places of a lane's reads, from a tile's start.  At D = 256 the second half
@@ -326,6 +326,46 @@ struct ChunkPlaces {
     return chunk_read_v(tile + v[d % DU][0] + at, tile + v[d % DU][1] + at);
   }
 };
+
+// The same of a tile of 8-bit values: rows of D bytes, whose vectors are permuted
+// as those of bf16 rows of D / 2.  K: 16 columns from 32 j + 16 (l / 32) of row l %
+// 32, two steps of the product.  V, by the transposing read of bytes (16 lanes
+// give the addresses of 8 rows of 16 bytes, each gets a column): column 32 d + l %
+// 32 of the keys 4 (l / 32) .. + 4 and 8 on, all 8 in one read.
+template <int D>
+struct ChunkPlaces8 {
+  static constexpr int N = D / 32;
+  uint32_t k[N], v[N];
+
+  __device__ __forceinline__ void init(uint32_t tile) {
+    const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, i = (lane & 15) >> 1;
+    const int r = (i & 3) + 8 * (i >> 2) + 4 * half;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      k[j] = tile + l31 * D + chunk_swizzle<D / 2>(l31, 2 * j + half) * 16;
+      v[j] = tile + r * D + chunk_swizzle<D / 2>(r, 2 * j + ((lane >> 4) & 1)) * 16 +
+             (lane & 1) * 8;
+    }
+  }
+  __device__ __forceinline__ void renew() {  // see ChunkPlaces
+#pragma unroll
+    for (int j = 0; j < N; ++j) asm volatile("" : "+v"(k[j]), "+v"(v[j]));
+  }
+};
+
+// 4 values of 8 bits times 2^(exponent of scale), exactly, as bf16.
+__device__ __forceinline__ uint2 chunk_from_8(uint32_t w, float scale) {
+  const bf16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+  const bf16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+  return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+__device__ __forceinline__ uint4 chunk_from_8(uint2 w, float scale0, float scale1) {
+  const uint2 x = chunk_from_8(w.x, scale0), y = chunk_from_8(w.y, scale1);
+  return make_uint4(x.x, x.y, y.x, y.y);
+}
+// The power of two that a scale's byte stands for (255, NaN: infinity, of which the
+// conversion makes NaN).
+__device__ __forceinline__ float chunk_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 __device__ __forceinline__ f32x16_t chunk_mfma(const uint4 &x, const uint4 &y, const f32x16_t &c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(chunk_bf16x8_t, x),
@@ -377,6 +417,30 @@ struct ChunkTaken {
       }
       any = 1;
     }
+  }
+  // A vector of 8-bit values, which have no infinities; all are NaN with such a
+  // scale.
+  __device__ __forceinline__ void clean8(uint4 *at, bool is_key, bool bad_scale, int key,
+                                         int col) {
+    uint32_t w[4] = {at->x, at->y, at->z, at->w};
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t nan = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (bad_scale || (w[i] >> (8 * e) & 0x7fu) == 0x7fu) nan |= 0xffu << (8 * e);
+      if (!is_key) {
+        w[i] = 0;
+      } else if (nan != 0) {
+        for (int e = 0; e < 4; ++e)
+          if (nan >> (8 * e) & 1) atomicMin(&first[2][col + 4 * i + e], key);
+        w[i] &= ~nan;
+        bad = 1;
+      }
+    }
+    if (!is_key || bad) *at = make_uint4(w[0], w[1], w[2], w[3]);
+    if (bad) any = 1;
   }
   // Back to the rows that see them.
   __device__ __forceinline__ void restore(int last_key, f32x16_t (&o)[D / 32]) const {

@@ -37,13 +37,49 @@ constexpr int chunk_step_keys() {
   return D == 256 ? 32 : 64;
 }
 
-// NW waves with 32 rows each.
-template <int D, int NW>
+// A thread's share of a step's 8-bit K or V: BYTES of them (8 or 16, of one row),
+// loaded into registers and written to LDS as bf16.
+template <int BYTES>
+struct ChunkRaw {
+  uint32_t w[BYTES / 4];
+  uint32_t scale;  // its byte
+
+  // From byte off of block blk; the block's scale of the head is `scales` on.
+  __device__ __forceinline__ void load(const uint16_t *cache, const uint8_t *scales, int blk,
+                                       uint32_t block_bytes, uint32_t off, int H_kv) {
+    const char *p = (const char *)cache + (uint64_t)blk * block_bytes + off;
+    if constexpr (BYTES == 16) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(p);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2 *>(p);
+      w[0] = v.x; w[1] = v.y;
+    }
+    scale = scales[(int64_t)blk * H_kv];
+  }
+  // To columns col .. of row r of a bf16 tile.
+  template <int D>
+  __device__ __forceinline__ void store(uint16_t *tile, int r, int col) const {
+    const float s = chunk_scale(scale);
+#pragma unroll
+    for (int i = 0; i < BYTES / 8; ++i)
+      *reinterpret_cast<uint4 *>(tile + r * D + chunk_swizzle<D>(r, col / 8 + i) * 8) =
+          chunk_from_8(make_uint2(w[2 * i], w[2 * i + 1]), s, s);
+  }
+};
+
+// NW waves with 32 rows each.  F8: K and V are of 8 bits.  Nothing but their way
+// into LDS differs: they pass through registers, where the matrix instructions'
+// bf16 is made of them once for all rows of the workgroup (16 conversions and 4
+// LDS writes a wave and step at D = 128), and are loaded a step earlier for it.
+template <int D, int NW, bool F8>
 __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : D == 32 ? 3 : 2) void
 chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   constexpr int NT = NW * 64, KT = chunk_step_keys<D>();
   constexpr int CPR = D / 8, NC = KT * CPR;
   constexpr int P = NC / NT;  // vectors of K and of V per thread and step
+  // 8 bits: values of a load, threads of a row, loads per thread and step.
+  constexpr int EV = KT * D / NT < 16 ? 8 : 16, TPR = D / EV, P8 = KT * D / NT / EV;
   constexpr int KB = KT / 32, KS = D / 16, DB = D / 32;
   static_assert(NC % NT == 0, "a step's vectors");
   constexpr int kStage = KT * D;  // elements of a step's K or V
@@ -68,7 +104,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
 
   const int32_t *const bt = a.block_tables + t.seq * a.bt_sb;
   const int bs_mask = (1 << a.bs_log2) - 1;
-  const int row_bytes = a.H_kv * D * 2;
+  const int row_bytes = a.H_kv * D * (F8 ? 1 : 2);
   const uint32_t block_bytes = (uint32_t)row_bytes << a.bs_log2;
 
   // Blocks.  Lane i looks up key i of a step for the whole wave, a step ahead
@@ -80,6 +116,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   // All of the first lookups are under way before the first is waited for, and
   // before Q.
   const int found0 = lookup_keys(0), found1 = lookup_keys(1), found2 = lookup_keys(2);
+  const int found3 = F8 && NW == 8 ? lookup_keys(3) : 0;
 
   const bool live = t.row0 + wave * 32 < t.rows;  // the wave has rows
   const ChunkRow row = chunk_row(a, t, h, t.row0 + wave * 32 + (lane & 31), k1);
@@ -108,11 +145,21 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
   auto whole = [&](int s, uint64_t keys) { return k0 + (s + 1) * KT <= full_keys && ~keys == 0; };
   auto clean = [&](int s, uint64_t keys, uint16_t *lds) {
     if (whole(s, keys)) return;
-    unrolled<P>([&](auto pi) {
-      const int c = tid + decltype(pi)::value * NT, r = c / CPR;
-      s_taken.clean(reinterpret_cast<uint4 *>(lds + c * 8), keys >> r & 1, k0 + s * KT + r,
-                    chunk_swizzle<D>(r, c % CPR) * 8);
-    });
+    if constexpr (F8) {
+      unrolled<P>([&](auto pi) {
+        constexpr int i = decltype(pi)::value % (EV / 8);
+        const int c = tid + decltype(pi)::value / (EV / 8) * NT, r = c / TPR;
+        const int ch = c % TPR * (EV / 8) + i;
+        s_taken.clean(reinterpret_cast<uint4 *>(lds + r * D + chunk_swizzle<D>(r, ch) * 8),
+                      keys >> r & 1, k0 + s * KT + r, ch * 8);
+      });
+    } else {
+      unrolled<P>([&](auto pi) {
+        const int c = tid + decltype(pi)::value * NT, r = c / CPR;
+        s_taken.clean(reinterpret_cast<uint4 *>(lds + c * 8), keys >> r & 1, k0 + s * KT + r,
+                      chunk_swizzle<D>(r, c % CPR) * 8);
+      });
+    }
   };
   // Every load of this wave has arrived.
   auto arrived = []() {
@@ -180,6 +227,21 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       row_off[p] = (r & bs_mask) * row_bytes + (h * D + chunk_swizzle<D>(r, c % CPR) * 8) * 2;
     }
     const uint32_t odd_off = a.bs_log2 == 7 ? 64 * row_bytes : 0;
+    // 8 bits: eight threads of a row, so a wave's rows lie in one block too.
+    static_assert(!F8 || (TPR == 8 && P8 == 1), "a block per load");
+    const int r8 = tid / 8, c8 = tid % 8 * EV;
+    const uint32_t off8 = (r8 & bs_mask) * row_bytes + h * D + c8;
+    ChunkRaw<EV> raw_k, raw_v;
+    auto load8 = [&](const uint16_t *cache, const uint8_t *scales, int blk, int odd) {
+      ChunkRaw<EV> x;
+      x.load(cache, scales + h, blk, block_bytes, off8 + (odd ? odd_off : 0), a.H_kv);
+      return x;
+    };
+    auto locate8 = [&](int s, int found, int &blk) {
+      const bool ok = in_pool(s, found);
+      blk = __builtin_amdgcn_readlane(ok ? found : 0, wave * 8);
+      return __ballot(ok);
+    };
     auto locate = [&](int s, int found, uint32_t (&blk)[P]) {
       const bool ok = in_pool(s, found);
       const int at = ok ? found : 0;
@@ -197,7 +259,9 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
     // multiplies in half 2 s + 1.  Buffers of V of step s - 1 and K of step s
     // are free after half 2 s; in half 2 s + 1 both groups start the loads of V
     // of step s + 1 and K of step s + 2 into them, each among what it computes
-    // then, and after half 2 s + 2 both have waited for theirs.
+    // then, and after half 2 s + 2 both have waited for theirs.  Of 8-bit values
+    // they write these into them then, loaded a step before, and start the loads of
+    // the step after.
     static_assert(P <= KB, "a load to 16 keys' weights");
     constexpr int kEvery = (2 * KB * DB + KB * KS) / (2 * P) < 5
                                ? (2 * KB * DB + KB * KS) / (2 * P) : 5;  // products to a load
@@ -206,18 +270,33 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       f32x16_t st[KB];
       uint32_t blk1[P], blk2[P];  // of steps s + 1 and s + 2
       uint64_t key0, key1, key2;  // keys of steps s to s + 2
-      int found;                  // blocks of step s + 2
+      int found;                  // blocks of step s + 2 (8 bits: s + 3)
+      uint64_t key3 = 0;          // 8 bits: keys and blocks of steps s + 2 and s + 3
+      int blk_v = 0, blk_k = 0;
       auto step = [&](int s, auto parity, uint16_t *k_cur, uint16_t *k_next, uint16_t *v_cur,
                       uint16_t *v_next) {
         constexpr int A = decltype(parity)::value;
         // The i-th of the 2 P loads that step s starts.
         auto next_load = [&](int i) {
-          if (i < P) load(a.v_cache, blk1[i], 1 - A, v_next, i);
+          if constexpr (F8) {
+            if (i == 0) {
+              raw_v.template store<D>(v_next, r8, c8);
+              raw_v = load8(a.v_cache, a.v_scales, blk_v, A);
+            } else if (i == 1) {
+              raw_k.template store<D>(k_cur, r8, c8);
+              raw_k = load8(a.k_cache, a.k_scales, blk_k, 1 - A);
+            }
+          } else if (i < P) load(a.v_cache, blk1[i], 1 - A, v_next, i);
           else if (i < 2 * P) load(a.k_cache, blk2[i - P], A, k_cur, i - P);
         };
         auto next_blocks = [&]() {
-          key2 = locate(s + 2, found, blk2);
-          found = lookup_keys(s + 3);
+          if constexpr (F8) {
+            key3 = locate8(s + 3, found, blk_k);
+            found = lookup_keys(s + 4);
+          } else {
+            key2 = locate(s + 2, found, blk2);
+            found = lookup_keys(s + 3);
+          }
         };
         uint4 pw[2 * KB];
         if (LATE) next_blocks();
@@ -234,7 +313,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
           for (int i = 0; i < 2 * P; ++i) next_load(i);
         }
         if (!LATE) {
-          arrived();
+          if (!F8) arrived();
           clean(s, key0, v_cur);
         }
         barrier();
@@ -251,7 +330,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
           for (int i = 0; i < 2 * P; ++i) next_load(i);
         }
         if (LATE) {
-          arrived();
+          if (!F8) arrived();
           clean(s + 1, key1, v_next);
         }
         barrier();
@@ -259,18 +338,38 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
         for (int p = 0; p < P; ++p) blk1[p] = blk2[p];
         key0 = key1;
         key1 = key2;
+        if constexpr (F8) {
+          key2 = key3;
+          blk_v = blk_k;
+        }
       };
-      key0 = locate(0, found0, blk2);
+      if constexpr (F8) {
+        int b0, b1;
+        key0 = locate8(0, found0, b0);
+        key1 = locate8(1, found1, b1);
+        key2 = locate8(2, found2, blk_v);
+        raw_k = load8(a.k_cache, a.k_scales, b0, 0);
+        const ChunkRaw<EV> v0 = load8(a.v_cache, a.v_scales, b0, 0);
+        const ChunkRaw<EV> k1 = load8(a.k_cache, a.k_scales, b1, 1);
+        raw_k.template store<D>(s_k0, r8, c8);
+        raw_v = load8(a.v_cache, a.v_scales, b1, 1);
+        raw_k = load8(a.k_cache, a.k_scales, blk_v, 0);
+        v0.template store<D>(s_v0, r8, c8);
+        k1.template store<D>(s_k1, r8, c8);
+        found = found3;
+      } else {
+        key0 = locate(0, found0, blk2);
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        load(a.k_cache, blk2[p], 0, s_k0, p);
-        load(a.v_cache, blk2[p], 0, s_v0, p);
+        for (int p = 0; p < P; ++p) {
+          load(a.k_cache, blk2[p], 0, s_k0, p);
+          load(a.v_cache, blk2[p], 0, s_v0, p);
+        }
+        key1 = locate(1, found1, blk1);
+#pragma unroll
+        for (int p = 0; p < P; ++p) load(a.k_cache, blk1[p], 1, s_k1, p);
+        found = found2;
+        arrived();
       }
-      key1 = locate(1, found1, blk1);
-#pragma unroll
-      for (int p = 0; p < P; ++p) load(a.k_cache, blk1[p], 1, s_k1, p);
-      found = found2;
-      arrived();
       if (LATE) clean(0, key0, s_v0);
       barrier();
       if (live) first_scores(s_k0, st);
@@ -281,7 +380,7 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
           step(s + 1, std::integral_constant<int, 1>(), s_k1, s_k0, s_v1, s_v0);
       }
       if (!LATE) barrier();
-      arrived();  // no load may outlive the workgroup's LDS
+      if (!F8) arrived();  // no load may outlive the workgroup's LDS
     };
     if (steps > 0) {
       if (wave >= 4) walk(std::true_type());
@@ -320,6 +419,25 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
     auto load = [&](const uint16_t *cache, int s, int at, uint16_t *lds) {
 #pragma unroll
       for (int p = 0; p < P; ++p) load_one(cache, s, at, lds, p);
+    };
+    // 8 bits: into registers in the step before the one that starts by writing
+    // them to LDS.
+    ChunkRaw<EV> raw_k[P8], raw_v[P8];
+    auto load8 = [&](const uint16_t *cache, const uint8_t *scales, int s, int at,
+                     ChunkRaw<EV> (&x)[P8]) {
+#pragma unroll
+      for (int p = 0; p < P8; ++p) {
+        const int c = tid + p * NT, r = c / TPR;
+        x[p].load(cache, scales + h, __shfl(at, r, 64), block_bytes,
+                  ((k0 + s * KT + r) & bs_mask) * row_bytes + h * D + c % TPR * EV, a.H_kv);
+      }
+    };
+    auto store8 = [&](const ChunkRaw<EV> (&x)[P8], uint16_t *lds) {
+#pragma unroll
+      for (int p = 0; p < P8; ++p) {
+        const int c = tid + p * NT;
+        x[p].template store<D>(lds, c / TPR, c % TPR * EV);
+      }
     };
     constexpr int NK = KB * KS, NV = 2 * KB * DB, NE = 16 * KB, kAhead = 4;
     uint4 f[kAhead + 1];
@@ -391,14 +509,24 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
     auto step = [&](int s, uint16_t *k_cur, uint16_t *k_next, uint16_t *v_cur, uint16_t *v_next,
                     f32x16_t (&cur)[KB], f32x16_t (&nxt)[KB]) {
       at.renew();
-      arrived();
+      if constexpr (F8) {
+        store8(raw_v, v_cur);
+        store8(raw_k, k_next);
+      } else {
+        arrived();
+      }
       clean(s, key0, v_cur);
       barrier();
       int at2;
       key2 = locate(s + 2, found, at2);
       found = lookup_keys(s + 3);
-      load(a.v_cache, s + 1, at1, v_next);
-      load(a.k_cache, s + 2, at2, k_cur);
+      if constexpr (F8) {
+        load8(a.v_cache, a.v_scales, s + 1, at1, raw_v);
+        load8(a.k_cache, a.k_scales, s + 2, at2, raw_k);
+      } else {
+        load(a.v_cache, s + 1, at1, v_next);
+        load(a.k_cache, s + 2, at2, k_cur);
+      }
       at1 = at2;
       if (live) {
         if (!whole(s, key0)) chunk_mask(cur, key0, k0 + s * KT, row.last_key);
@@ -415,17 +543,24 @@ chunk_prefill_kernel(const ChunkArgs a, const ChunkClass cl) {
       found = found2;
       key0 = locate(0, found0, at0);
       key1 = locate(1, found1, at1);
-      load(a.k_cache, 0, at0, s_k0);
-      load(a.v_cache, 0, at0, s_v0);
-      if (steps > 1) load(a.k_cache, 1, at1, s_k1);
-      arrived();
+      if constexpr (F8) {
+        load8(a.k_cache, a.k_scales, 0, at0, raw_k);
+        load8(a.v_cache, a.v_scales, 0, at0, raw_v);
+        store8(raw_k, s_k0);
+        load8(a.k_cache, a.k_scales, 1, at1, raw_k);
+      } else {
+        load(a.k_cache, 0, at0, s_k0);
+        load(a.v_cache, 0, at0, s_v0);
+        if (steps > 1) load(a.k_cache, 1, at1, s_k1);
+        arrived();
+      }
       barrier();
       if (live) scores(s_k0, st0);
       for (int s = 0; s < steps; s += 2) {
         step(s, s_k0, s_k1, s_v0, s_v1, st0, st1);
         if (s + 1 < steps) step(s + 1, s_k1, s_k0, s_v1, s_v0, st1, st0);
       }
-      arrived();  // no load may outlive the workgroup's LDS
+      if (!F8) arrived();  // no load may outlive the workgroup's LDS
     }
   }
   __syncthreads();  // the last note of a taken-out value

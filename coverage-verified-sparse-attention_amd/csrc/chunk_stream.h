@@ -29,27 +29,29 @@
 
 namespace cvsa {
 
-template <int D>
+template <int D, bool F8>
 constexpr int chunk_stream_waves() {
-  return D == 256 ? 2 : 4;
+  return D == 256 && !F8 ? 2 : 4;
 }
 
 // Workgroups of a CU: by LDS one at D >= 128, two at 64; by registers at 32.  With
 // two row tiles one at 64 as well, whose fewer parts gain more than twice the
 // waves do: 61 us for 66 (8 drafts of 5 tokens at 32 K keys, 28 heads on 4).
-template <int D, int RT>
+template <int D, int RT, bool F8>
 constexpr int chunk_stream_fit() {
+  if (F8) return D == 256 ? 1 : 3 - RT;
   return D >= 128 ? 1 : D == 64 ? 3 - RT : 4 - RT;
 }
 
-template <int D, int RT>
-__global__ __launch_bounds__(chunk_stream_waves<D>() * 64, (chunk_stream_fit<D, RT>())) void
+template <int D, int RT, bool F8>
+__global__ __launch_bounds__((chunk_stream_waves<D, F8>() * 64), (chunk_stream_fit<D, RT, F8>())) void
 chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
-  constexpr int NW = chunk_stream_waves<D>(), NT = NW * 64, KT = 32;
-  constexpr int CPR = D / 8, RPL = 64 / CPR;  // rows of a load
-  constexpr int P = KT / RPL;                 // loads of a tile of K or V
+  constexpr int NW = chunk_stream_waves<D, F8>(), NT = NW * 64, KT = 32;
+  constexpr int DV = F8 ? D / 2 : D;           // a row's bytes are those of DV bf16 values
+  constexpr int CPR = DV / 8, RPL = 64 / CPR;  // rows of a load
+  constexpr int P = KT / RPL;                  // loads of a tile of K or V
   constexpr int KS = D / 16, DB = D / 32;
-  constexpr int kTile = KT * D;
+  constexpr int kTile = KT * DV;
   __shared__ __align__(16) uint16_t s_k0[NW * kTile], s_k1[NW * kTile], s_v0[NW * kTile],
       s_v1[NW * kTile];
   __shared__ float2 s_ml[NW - 1][RT * 32];
@@ -77,15 +79,15 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     const int k0 = u0 << cl.unit_log2, k1 = u1 < units ? u1 << cl.unit_log2 : t.keys;
 
     const int bs_mask = (1 << a.bs_log2) - 1;
-    const int row_bytes = a.H_kv * D * 2;
+    const int row_bytes = a.H_kv * DV * 2;
     const uint32_t block_bytes = (uint32_t)row_bytes << a.bs_log2;
     uint32_t row_off[P];  // of the lane's vector of each load, in the block of the load's rows
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int r = p * RPL + lane / CPR;
-      row_off[p] = lane / CPR * row_bytes + (h * D + chunk_swizzle<D>(r, lane % CPR) * 8) * 2;
+      row_off[p] = lane / CPR * row_bytes + (h * DV + chunk_swizzle<DV>(r, lane % CPR) * 8) * 2;
     }
-    ChunkPlaces<D> place;
+    std::conditional_t<F8, ChunkPlaces8<D>, ChunkPlaces<D>> place;
     place.init(wave * kTile * 2);
 
     ChunkRow row[RT];
@@ -94,7 +96,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       row[r] = chunk_row(a, t, h, t.row0 + r * 32 + l31, k1);
-      chunk_load_q<D>(a, t, row[r], q[r]);
+      chunk_load_q<D, F8>(a, t, row[r], q[r]);
       state[r].init();
     }
     const int full_keys = a.causal ? min(t.pos0 + t.row0 / a.G + 1, k1) : k1;  // all rows see
@@ -124,7 +126,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
           const uint32_t blk = __shfl(at, r, 64);
           const char *from = (const char *)cache + (uint64_t)blk * block_bytes +
                              (uint32_t)(((first_key(s) + r) & bs_mask) * row_bytes) +
-                             (h * D + chunk_swizzle<D>(r, lane % CPR) * 8) * 2;
+                             (h * DV + chunk_swizzle<DV>(r, lane % CPR) * 8) * 2;
           __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                            (__attribute__((address_space(3))) void *)to, 16, 0, 0);
         }
@@ -137,6 +139,11 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     int at2;                    // blocks of tile s + 2
     uint64_t key0, key1, key2;  // keys of tiles s to s + 2
     int found;                  // looked up of tile s + 3
+    // 8 bits: bytes of the scales of the lane's key in tiles s to s + 2.
+    uint32_t ks0 = 0, ks1 = 0, ks2 = 0, vs0 = 0, vs1 = 0, vs2 = 0;
+    auto scale_of = [&](const uint8_t *scales, int at) {
+      return (uint32_t)scales[(int64_t)at * a.H_kv + h];
+    };
     auto locate = [&](int s, int looked_up, int &at) {
       const bool ok = first_key(s) + l31 < k1 && (uint32_t)looked_up < (uint32_t)a.num_blocks;
       at = ok ? looked_up : 0;
@@ -146,18 +153,37 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
       place.renew();
       const int ahead = lookup(s + 3);
       f32x16_t st[RT][1];
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const uint4 k = place.read_k((const char *)k_cur, 0, ks);
+      auto k_product = [&](const uint4 &k, int ks) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
           st[r][0] = chunk_mfma(k, __builtin_bit_cast(uint4, q[r][ks]), ks ? st[r][0] : f32x16_t{});
+      };
+      if constexpr (F8) {
+        const float scale = chunk_scale(ks0);
+#pragma unroll
+        for (int j = 0; j < DB; ++j) {
+          const uint4 w = chunk_read_k((const char *)k_cur + place.k[j]);
+          k_product(chunk_from_8(make_uint2(w.x, w.y), scale, scale), 2 * j);
+          k_product(chunk_from_8(make_uint2(w.z, w.w), scale, scale), 2 * j + 1);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) k_product(place.read_k((const char *)k_cur, 0, ks), ks);
       }
       __builtin_amdgcn_sched_barrier(0);  // K has been read
       key2 = locate(s + 2, found, at2);
       request(a.k_cache, s + 2, at2, k_cur);
+      if constexpr (F8) {
+        ks2 = scale_of(a.k_scales, at2);
+        vs2 = scale_of(a.v_scales, at2);
+      }
       found = ahead;
-      const bool whole = first_key(s) + KT <= full_keys && ~key0 == 0;
+      bool whole = first_key(s) + KT <= full_keys && ~key0 == 0;
+      uint64_t bad_scale = 0;
+      if constexpr (F8) {
+        bad_scale = __ballot(vs0 == 255u);
+        whole = whole && bad_scale == 0;
+      }
       if (!whole) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) chunk_mask(st[r], key0, first_key(s), row[r].last_key);
@@ -171,22 +197,44 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
 #pragma unroll 1
         for (int p = 0; p < P; ++p) {
           const int r = p * RPL + lane / CPR;
-          s_taken.clean(reinterpret_cast<uint4 *>(v_cur + wave * kTile + p * 512 + lane * 8),
-                        key0 >> r & 1, first_key(s) + r, chunk_swizzle<D>(r, lane % CPR) * 8);
+          uint4 *const at = reinterpret_cast<uint4 *>(v_cur + wave * kTile + p * 512 + lane * 8);
+          if constexpr (F8)
+            s_taken.clean8(at, key0 >> r & 1, bad_scale >> r & 1, first_key(s) + r,
+                           chunk_swizzle<DV>(r, lane % CPR) * 16);
+          else
+            s_taken.clean(at, key0 >> r & 1, first_key(s) + r,
+                          chunk_swizzle<D>(r, lane % CPR) * 8);
         }
       }
+      // 8 bits: a scale for 8 keys, which lie in one page; of keys that are none,
+      // and of pages whose scale is NaN, the values are zeros now.
+      const uint32_t mine = (key0 >> l31 & 1) && vs0 != 255u ? vs0 : 127u;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        float scale[2];
+        if constexpr (F8) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            scale[i] = chunk_scale(__builtin_amdgcn_readlane(mine, 16 * j + 8 * i));
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const uint4 v = place.read_v((char *)v_cur, j, d);
+          uint4 v;
+          if constexpr (F8) v = chunk_from_8(chunk_read_v8((char *)v_cur + place.v[d] + 16 * j * D),
+                                             scale[0], scale[1]);
+          else v = place.read_v((char *)v_cur, j, d);
 #pragma unroll
           for (int r = 0; r < RT; ++r) state[r].o[d] = chunk_mfma(v, pw[r][j], state[r].o[d]);
         }
+      }
       __builtin_amdgcn_sched_barrier(0);  // V has been read
       request(a.v_cache, s + 2, at2, v_cur);
       key0 = key1;
       key1 = key2;
+      ks0 = ks1;
+      ks1 = ks2;
+      vs0 = vs1;
+      vs1 = vs2;
     };
     if (steps > 0) {
       int at;
@@ -194,9 +242,17 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
       found = lookup(2);
       key0 = locate(0, f0, at);
       request(a.k_cache, 0, at, s_k0);
+      if constexpr (F8) {
+        ks0 = scale_of(a.k_scales, at);
+        vs0 = scale_of(a.v_scales, at);
+      }
       request(a.v_cache, 0, at, s_v0);
       key1 = locate(1, f1, at);
       request(a.k_cache, 1, at, s_k1);
+      if constexpr (F8) {
+        ks1 = scale_of(a.k_scales, at);
+        vs1 = scale_of(a.v_scales, at);
+      }
       request(a.v_cache, 1, at, s_v1);
       for (int s = 0; s < steps; s += 2) {
         step(s, s_k0, s_v0);
@@ -209,59 +265,64 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     }
 
     // The waves' states, joined in order by the first: an array of K or V for
-    // each other wave, float4 i of row r at place i ^ (r % 8).
-    static_assert(NW <= 4 && NW * kTile * 2 >= RT * 32 * D * 4, "room to join");
+    // each other wave, float4 i of row r at place i ^ (r % 8); JR row tiles at a
+    // time.
+    constexpr int JR = F8 ? 1 : RT;
+    static_assert(NW <= 4 && NW * kTile * 2 >= JR * 32 * D * 4, "room to join");
     auto room = [&](int w) {
       return reinterpret_cast<float4 *>(w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
     };
     auto spot = [&](int r, int d, int g) {
-      return (r * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
+      return (r % JR * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
     };
 #pragma unroll
     for (int r = 0; r < RT; ++r) state[r].finish();
-    __syncthreads();
-    if (wave > 0) {
-      float4 *const so = room(wave);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        if (half == 0) s_ml[wave - 1][r * 32 + l31] = make_float2(state[r].m, state[r].l);
+    for (int r0 = 0; r0 < RT; r0 += JR) {
+      __syncthreads();
+      if (wave > 0) {
+        float4 *const so = room(wave);
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int r = r0; r < r0 + JR; ++r) {
+          if (half == 0) s_ml[wave - 1][r * 32 + l31] = make_float2(state[r].m, state[r].l);
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
-            so[spot(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
-                                             state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              so[spot(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
+                                               state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
+        }
       }
-    }
-    __syncthreads();
-    if (wave == 0) {
+      __syncthreads();
+      if (wave == 0) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        for (int w = 1; w < NW; ++w) {
-          const float4 *const so = room(w);
-          const float2 ml = s_ml[w - 1][r * 32 + l31];
-          const float nm = fmaxf(state[r].m, ml.x);
-          const float a0 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[r].m - nm);
-          const float a1 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - nm);
-          state[r].m = nm;
-          state[r].l = state[r].l * a0 + ml.y * a1;
+        for (int r = r0; r < r0 + JR; ++r) {
+          for (int w = 1; w < NW; ++w) {
+            const float4 *const so = room(w);
+            const float2 ml = s_ml[w - 1][r * 32 + l31];
+            const float nm = fmaxf(state[r].m, ml.x);
+            const float a0 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[r].m - nm);
+            const float a1 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - nm);
+            state[r].m = nm;
+            state[r].l = state[r].l * a0 + ml.y * a1;
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
+            for (int d = 0; d < DB; ++d) {
+              __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float4 v = so[spot(r, d, g)];
-              state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
-              state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
-              state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
-              state[r].o[d][4 * g + 3] = state[r].o[d][4 * g + 3] * a0 + v.w * a1;
+              for (int g = 0; g < 4; ++g) {
+                const float4 v = so[spot(r, d, g)];
+                state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
+                state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
+                state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
+                state[r].o[d][4 * g + 3] = state[r].o[d][4 * g + 3] * a0 + v.w * a1;
+              }
             }
           }
+          s_taken.restore(row[r].last_key, state[r].o);
+          const int64_t part = (int64_t)(2 * (int)range + (u0 == 0)) * a.H_kv + h;
+          if (u0 == 0 && u1 == units) state[r].store(a, t, row[r]);
+          else state[r].store_part(cl, row[r], part * cl.tile_rows + r * 32 + l31);
         }
-        s_taken.restore(row[r].last_key, state[r].o);
-        const int64_t part = (int64_t)(2 * (int)range + (u0 == 0)) * a.H_kv + h;
-        if (u0 == 0 && u1 == units) state[r].store(a, t, row[r]);
-        else state[r].store_part(cl, row[r], part * cl.tile_rows + r * 32 + l31);
       }
     }
     __syncthreads();  // the buffers and s_taken are the next sequence's

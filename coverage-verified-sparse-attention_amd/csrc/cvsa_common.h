@@ -7,6 +7,9 @@
 #include <stddef.h>
 #include <math.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "../../include/cvsa_hip.h"
 
 namespace cvsa {
@@ -159,6 +162,16 @@ __device__ __forceinline__ void lds_barrier() {
 
 // exp(x) through the hardware base-2 exponential.
 __device__ __forceinline__ float fast_exp(float x) { return exp2f(x * 1.4426950408889634f); }
+
+// f(0) .. f(N - 1), the index known to the compiler.
+template <int N, class F, int... I>
+__device__ __forceinline__ void unrolled(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled<N>(f, std::make_integer_sequence<int, N>());
+}
 
 // ------------------------------------------------------------- lane moves
 // DPP controls (gfx9 encoding).

@@ -51,6 +51,8 @@ __all__ = [
     "prepare_append_chunk",
     "reserve_chunk",
     "chunk_attention",
+    "add_key_weights",
+    "evict_tokens",
 ]
 
 _DTYPE_CODE = {
@@ -1317,3 +1319,4 @@ class AppendCall:
 # Chunks of new tokens (uses the helpers above).
 from .chunk import (ChunkLayout, RotaryTable, append_chunk_kv, chunk_attention,  # noqa: E402
                     prepare_append_chunk, qk_norm_rope, reserve_chunk)
+from .eviction import add_key_weights, evict_tokens  # noqa: E402

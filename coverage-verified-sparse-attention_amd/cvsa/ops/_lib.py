@@ -10,7 +10,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parents[1] / "libcvsa_hip.so"
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 CVSA_OK = 0
 CVSA_ERR_INVALID = -1
@@ -141,6 +141,23 @@ SIGNATURES = {
     "cvsa_chunk_attention": (ctypes.c_int, [
         _p, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32,
         _i32, _f32, _i32, _p, _p, _p, _sz, _p]),
+    "cvsa_append_chunk_kv8": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _i64, _p, _i64,
+        _i32, _p, _p, _i32, _i32, _p, _i64, _i32, _i32, _p, _p, _i32, _f32, _i32, _i32, _i32,
+        _i32, _p, _p]),
+    "cvsa_chunk_attention8_workspace_bytes": (_sz, [
+        _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "cvsa_chunk_attention8": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
+        _i32, _i32, _f32, _i32, _p, _p, _p, _sz, _p]),
+    "cvsa_add_key_weights_workspace_bytes": (_sz, [_p, _i32, _i32, _i32, _i64, _i32]),
+    "cvsa_add_key_weights": (ctypes.c_int, [
+        _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32,
+        _i32, _i32, _f32, _i32, _i32, _p, _sz, _p]),
+    "cvsa_evict_tokens_workspace_bytes": (_sz, [_i32] * 8),
+    "cvsa_evict_tokens": (ctypes.c_int, [
+        _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32,
+        _i32, _p, _p, _sz, _p]),
 }
 
 _LIB = None

@@ -8,6 +8,10 @@ rotate the queries in the same launch; :func:`chunk_attention` attends the
 queries over the cache.  :func:`qk_norm_rope` is the norm and rotation alone,
 for keys that stay outside the cache.
 
+The cache is bf16, or holds 8 bits a value: e4m3 payloads with a power of two
+for each block and head (``k_scales`` and ``v_scales``, see
+:func:`append_chunk_kv`), half the bytes to keep and to read.
+
 None of these has a counterpart in the reference, whose harness leaves
 prefill to the model it wraps.  They serve; there is no backward pass.
 """
@@ -22,6 +26,7 @@ from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_se
                _i32, _lib, _ptr, check)
 
 _BF16 = torch.bfloat16
+_F8, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.uint16,
              torch.uint32, torch.uint64)
 
@@ -56,7 +61,7 @@ class ChunkLayout:
         self.cu_host = (ctypes.c_int32 * len(cu))(*cu)
         self.cu_seqlens = torch.tensor(cu, dtype=torch.int32, device=device)
         self.device = self.cu_seqlens.device
-        self._workspace_bytes = {}  # of chunk_attention, by the call's sizes
+        self._workspace_bytes = {}  # by the call's sizes
 
 
 class RotaryTable:
@@ -260,10 +265,28 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor],
     return q_out, k_out
 
 
-def _check_caches(who, k_cache, v_cache, block_size):
+def _check_cache8(who, name, cache, scales):
+    """A cache of 8 bits and its scales."""
+    if cache.dim() != 4 or cache.dtype is not _F8 or not cache.is_contiguous() \
+            or cache.data_ptr() & 15:
+        raise ValueError(f"{who}: {name}_cache must be contiguous, 16-byte aligned float8_e4m3fn "
+                         "[num_blocks, block_size, H_kv, D] with scales, got "
+                         f"{tuple(cache.shape)} {cache.dtype}")
+    want = (cache.shape[0], cache.shape[2])
+    if scales is None:
+        raise ValueError(f"{who}: {name}_cache is of 8 bits, {name}_scales are missing")
+    if scales.shape != want or scales.dtype is not _SCALE or not scales.is_contiguous():
+        raise ValueError(f"{who}: {name}_scales must be contiguous float8_e8m0fnu {want}, got "
+                         f"{tuple(scales.shape)} {scales.dtype}")
+
+
+def _check_caches(who, k_cache, v_cache, block_size, k_scales=None, v_scales=None):
     """The caches' (num_blocks, H_kv, D)."""
     shape = k_cache.shape
-    if len(shape) != 4 or k_cache.dtype is not _BF16 or v_cache.dtype is not _BF16 \
+    if k_scales is not None or v_scales is not None or k_cache.dtype is _F8:
+        _check_cache8(who, "k", k_cache, k_scales)
+        _check_cache8(who, "v", v_cache, v_scales)
+    elif len(shape) != 4 or k_cache.dtype is not _BF16 or v_cache.dtype is not _BF16 \
             or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         _check_cache(k_cache)
         _check_cache(v_cache, "v_cache")
@@ -275,14 +298,15 @@ def _check_caches(who, k_cache, v_cache, block_size):
 
 
 def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, layout, block_size,
-                         rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None):
+                         rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None,
+                         k_scales=None, v_scales=None):
     """The checks of :func:`append_chunk_kv` without its launch: returns
     (launch, q_out); launch() enqueues it, on the same stream.  The tables may
     change in place in between; k, v, q and the weights may not."""
     who = "append_chunk_kv"
     dev = _same_device(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
-                       rotary.table if rotary else None)
-    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
+                       rotary.table if rotary else None, k_scales, v_scales)
+    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size, k_scales, v_scales)
     bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
     T, eps = layout.total, float(eps)
@@ -311,9 +335,12 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
         b, stride, c = bt, bt_stride, ctx
         if copied and not at_once:
             b, stride, c = _tables(who, layout, dev, block_tables, context_lens)
+        L = _lib.load()
+        fn, scales = (L.cvsa_append_chunk_kv, ()) if k_scales is None else (
+            L.cvsa_append_chunk_kv8, (k_scales.data_ptr(), v_scales.data_ptr()))
         # k, v and q are held here: they may be copies.
-        _call(dev, who, _lib.load().cvsa_append_chunk_kv, *k_at, *v_at, *q_at,
-              _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks,
+        _call(dev, who, fn, *k_at, *v_at, *q_at,
+              _DTYPE_CODE[k.dtype], k_cache.data_ptr(), v_cache.data_ptr(), *scales, num_blocks,
               b.data_ptr(), stride, W, c.data_ptr(), layout.cu_seqlens.data_ptr(), B, T,
               *rot, _ptr(qw), _ptr(kw), wcode, eps, H_q, H_kv, D, block_size,
               _ptr(q_out), keep=(k, v, q, rotary))
@@ -326,7 +353,9 @@ def append_chunk_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
                     rotary: Optional[RotaryTable] = None,
                     k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
                     q: Optional[torch.Tensor] = None,
-                    q_weight: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                    q_weight: Optional[torch.Tensor] = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Write a chunk's keys and values [T, H_kv, D] to the paged cache.
 
     ``context_lens`` counts the chunk's tokens already and the block tables
@@ -340,9 +369,20 @@ def append_chunk_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     cache is bf16.  A token whose position is negative, past the block table
     or in a block outside the pool is not written.  Rows past layout.total
     are not read; the returned q is zero there.
+
+    With ``k_scales`` and ``v_scales`` ([num_blocks, H_kv] float8_e8m0fnu,
+    powers of two) the caches are float8_e4m3fn, and a value is payload times
+    its block's and head's scale.  A page whose first token is written gets
+    the smallest scale 2^e, -110 <= e <= 119, with which its new finite values
+    do not pass 448 (larger ones become 448 * 2^119); one that held tokens
+    before keeps its scale, or takes a larger one if the new tokens need it,
+    to which its tokens are brought (a shift, exact but for values that become
+    subnormal).  Payloads are rounded to nearest even; infinite and NaN values
+    become NaN.  No two sequences may append to one block.
     """
     launch, q_out = prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens,
-                                         layout, block_size, rotary, k_weight, eps, q, q_weight)
+                                         layout, block_size, rotary, k_weight, eps, q, q_weight,
+                                         k_scales, v_scales)
     launch(at_once=True)
     return q_out
 
@@ -378,7 +418,9 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     layout: ChunkLayout, num_kv_heads: int, num_q_per_kv: int, block_size: int,
                     causal: bool = True, scale: Optional[float] = None,
                     max_context_len: int = 0, return_lse: bool = False,
-                    out: Optional[torch.Tensor] = None):
+                    out: Optional[torch.Tensor] = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None):
     """Attention of a chunk's queries over the paged cache -> [T, H_q, D] bf16.
 
     q [T, H_q, D] bf16, any token and head strides.  ``context_lens`` counts
@@ -398,10 +440,14 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Scores, sums and outputs are held in 32 bits; the weights of the second
     product are rounded to bf16 (:func:`dense_decode`, for batches of single
     tokens, keeps 16 bits of them).
+
+    With ``k_scales`` and ``v_scales`` the caches are of 8 bits (see
+    :func:`append_chunk_kv`); their values are brought to bf16, exactly, and
+    the rest is the same.  A scale of NaN makes its block's values NaN.
     """
     who = "chunk_attention"
-    dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out)
-    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size)
+    dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out, k_scales, v_scales)
+    num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size, k_scales, v_scales)
     if H_kv != num_kv_heads:
         raise ValueError(f"{who}: head counts do not match the caches")
     bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
@@ -432,12 +478,16 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         # Allocated for the call, so no two calls, streams or captured graphs
         # share it.
         sizes = (H_q, H_kv, D, block_size, W, max_context_len)
-        need = layout._workspace_bytes.get(sizes)
+        key = sizes if k_scales is None else (*sizes, 8)
+        need = layout._workspace_bytes.get(key)
         if need is None:
-            need = L.cvsa_chunk_attention_workspace_bytes(layout.cu_host, B, *sizes)
-            layout._workspace_bytes[sizes] = need
+            size_of = L.cvsa_chunk_attention_workspace_bytes if k_scales is None \
+                else L.cvsa_chunk_attention8_workspace_bytes
+            need = layout._workspace_bytes[key] = size_of(layout.cu_host, B, *sizes)
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-        _call(dev, who, L.cvsa_chunk_attention, *q_at, k_cache.data_ptr(), v_cache.data_ptr(),
+        fn, scales = (L.cvsa_chunk_attention, ()) if k_scales is None else (
+            L.cvsa_chunk_attention8, (k_scales.data_ptr(), v_scales.data_ptr()))
+        _call(dev, who, fn, *q_at, k_cache.data_ptr(), v_cache.data_ptr(), *scales,
               num_blocks, bt.data_ptr(), bt_stride, ctx.data_ptr(), layout.cu_seqlens.data_ptr(),
               layout.cu_host, B, H_q, num_kv_heads, D, block_size, W, max_context_len, scale,
               int(bool(causal)), out.data_ptr(), _ptr(lse), _ptr(ws), need)

@@ -14,6 +14,11 @@ read; ``append_token_kv`` / ``append_tokens_kv`` launch the HIP append kernel
 Block tables accept any block ids, so randomly permuted physical pages work.
 If ``block_tables`` / ``context_lens`` are edited directly, call
 ``sync_host_state()`` before the next append.
+
+A cache of dtype float8_e4m3fn holds 8 bits a value with a scale for each block
+and head (ops.append_chunk_kv); the same methods append to it, and
+ops.chunk_attention reads it.  ``evict_tokens`` cuts sequences to the tokens of
+the most attention weight (ops.evict_tokens), in caches of both types.
 """
 from __future__ import annotations
 
@@ -51,6 +56,11 @@ class PagedKVCache:
                                    device=device)
         self.v_cache = torch.zeros(num_blocks, block_size, num_kv_heads, head_dim, dtype=dtype,
                                    device=device)
+        self.k_scales = self.v_scales = None
+        if dtype is torch.float8_e4m3fn:  # scales of one; each first token of a page sets its own
+            self.k_scales, self.v_scales = (
+                torch.full((num_blocks, num_kv_heads), 127, dtype=torch.uint8, device=device).view(
+                    torch.float8_e8m0fnu) for _ in range(2))
         self._next_free = 0
         self._total_blocks = num_blocks
 
@@ -74,14 +84,21 @@ class PagedKVCache:
 
     def write_kv(self, block_id: int, token_offset: int, k: torch.Tensor, v: torch.Tensor):
         """One token's [H_kv, D] K/V rows (kv_cache.py:64-70)."""
+        self._refuse_8_bits()
         self.k_cache[block_id, token_offset] = k
         self.v_cache[block_id, token_offset] = v
 
     def write_kv_block(self, block_id: int, k_block: torch.Tensor, v_block: torch.Tensor,
                        n_tokens: int):
         """The first n_tokens rows of a block (kv_cache.py:72-80)."""
+        self._refuse_8_bits()
         self.k_cache[block_id, :n_tokens] = k_block[:n_tokens]
         self.v_cache[block_id, :n_tokens] = v_block[:n_tokens]
+
+    def _refuse_8_bits(self):
+        if self.k_scales is not None:
+            raise ValueError("rows of an 8-bit cache need their page's scale: append them through "
+                             "a SequenceKVManager or ops.append_chunk_kv")
 
     def reset(self):
         """Free all blocks without zeroing (kv_cache.py:82-84)."""
@@ -136,6 +153,13 @@ class SequenceKVManager:
         n_pages = (seq_len + bs - 1) // bs
         block_ids = self.cache.allocate_blocks(n_pages)
         self.block_tables[seq_idx, :n_pages] = block_ids
+        if self.cache.k_scales is not None:
+            self.context_lens[seq_idx] = seq_len
+            self._write_8_bits(k_all, v_all, seq_idx, [seq_len])
+            self._pages_allocated[seq_idx] = n_pages
+            self._pages_allocated_dev[seq_idx] = n_pages
+            self._ctx_host[seq_idx] = seq_len
+            return
         full = seq_len // bs
         if full:
             ids = block_ids[:full].long()
@@ -151,6 +175,14 @@ class SequenceKVManager:
         self._pages_allocated[seq_idx] = n_pages
         self._pages_allocated_dev[seq_idx] = n_pages
         self._ctx_host[seq_idx] = seq_len
+
+    def _write_8_bits(self, k, v, first, lens):
+        """Tokens of sequences first .. that the tables count already."""
+        last = first + len(lens)
+        ops.append_chunk_kv(k, v, self.cache.k_cache, self.cache.v_cache,
+                            self.block_tables[first:last], self.context_lens[first:last],
+                            ops.ChunkLayout(lens, self.cache.config.device), self.block_size,
+                            k_scales=self.cache.k_scales, v_scales=self.cache.v_scales)
 
     def _plan_append(self, seqs) -> int:
         """Blocks the append of one token to each of `seqs` allocates."""
@@ -194,7 +226,7 @@ class SequenceKVManager:
             want = self._fuse_shape = (torch.Size((self.batch_size, c.shape[2], c.shape[3])),
                                        c, c.device)
         return (k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
-                and k.shape == want[0] and v.shape == want[0] and k.device == want[2]
+                and c.dtype == torch.bfloat16 and k.shape == want[0] and v.shape == want[0] and k.device == want[2]
                 and v.device == want[2] and k.is_contiguous() and v.is_contiguous()
                 and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0)
 
@@ -247,6 +279,10 @@ class SequenceKVManager:
     def _append(self, seq_begin: int, k: torch.Tensor, v: torch.Tensor):
         n = k.shape[0]
         seqs = range(seq_begin, seq_begin + n)
+        if self.cache.k_scales is not None:
+            lens = [int(s in seqs) for s in range(self.batch_size)]
+            self.append_chunk_kv(k, v, ops.ChunkLayout(lens, self.cache.config.device))
+            return
         need = self._plan_append(seqs)
         buffers = (self.cache.k_cache, self.cache.v_cache, self.block_tables, self.context_lens,
                    self._pages_allocated_dev)
@@ -315,7 +351,36 @@ class SequenceKVManager:
                                  f"{rotary.max_positions}")
         launch, q_out = ops.prepare_append_chunk(
             k, v, self.cache.k_cache, self.cache.v_cache, self.block_tables, self.context_lens,
-            layout, self.block_size, rotary, k_weight, eps, q, q_weight)
+            layout, self.block_size, rotary, k_weight, eps, q, q_weight, self.cache.k_scales,
+            self.cache.v_scales)
         self.reserve_chunk(layout)
         launch()
         return q_out
+
+    def evict_tokens(self, weights: torch.Tensor, keep: int, sinks: int = 0,
+                     recent: int = 0) -> torch.Tensor:
+        """Cut every sequence to its ``keep`` tokens of the most attention weight
+        (ops.evict_tokens), and its length (:meth:`cut`); returns the old slot
+        of each new one.  With a cache per layer, ops.evict_tokens per layer
+        and :meth:`cut` once is the same."""
+        self._check_cut(keep)
+        kept = ops.evict_tokens(weights, self.cache.k_cache, self.cache.v_cache,
+                                self.block_tables, self.context_lens, keep, self.block_size,
+                                sinks, recent, self.cache.k_scales, self.cache.v_scales)
+        self.cut(keep)
+        return kept
+
+    def cut(self, keep: int) -> None:
+        """Take no context as longer than ``keep`` tokens.  Pages stay with their
+        sequences, for the tokens to come.  Not while the stream is captured: a
+        replay would cut without this manager's count."""
+        self._check_cut(keep)
+        self.context_lens.clamp_(max=keep)
+        self._ctx_host = [min(c, keep) for c in self._ctx_host]
+
+    def _check_cut(self, keep):
+        if keep < 1:
+            raise ValueError(f"a cut to {keep} tokens")
+        if ops.chunk.capturing(self.block_tables.device):
+            raise RuntimeError("a manager's lengths cannot be cut in a captured graph: capture "
+                               "ops.evict_tokens, cut behind it")

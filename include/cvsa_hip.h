@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define CVSA_ABI_VERSION 16
+#define CVSA_ABI_VERSION 17
 
 enum {
   CVSA_OK = 0,
@@ -691,6 +691,31 @@ int cvsa_append_chunk_kv(const void *k, int64_t k_stride_t, int64_t k_stride_h,
                          int32_t weight_dtype, float eps, int32_t H_q, int32_t H_kv,
                          int32_t D, int32_t block_size, void *q_out, void *stream);
 
+/* Caches of 8 bits: k_cache and v_cache hold e4m3 payloads (no infinities),
+ * [num_blocks, block_size, H_kv, D] bytes, 16-byte aligned; k_scales and v_scales,
+ * [num_blocks, H_kv] bytes x, a power of two 2^(x - 127) for each block and head
+ * (255: NaN).  A value is payload * scale.
+ *
+ * cvsa_append_chunk_kv with such caches.  A page and head whose first token is
+ * written gets the smallest scale 2^e, -110 <= e <= 119, with which its new finite
+ * values do not pass 448 (past 448 * 2^119 they become that); one that held tokens
+ * before keeps its scale or gets a larger one, to which these are brought.
+ * Payloads are rounded to nearest even; infinities and NaN become NaN.  Rows and
+ * scales of other pages, and rows behind a context's end, are left as they are.  No
+ * two sequences of the call may append to one block. */
+int cvsa_append_chunk_kv8(const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                          const void *v, int64_t v_stride_t, int64_t v_stride_h,
+                          const void *q, int64_t q_stride_t, int64_t q_stride_h,
+                          int32_t dtype, uint8_t *k_cache, uint8_t *v_cache,
+                          uint8_t *k_scales, uint8_t *v_scales,
+                          int64_t num_blocks, const int32_t *block_tables,
+                          int64_t bt_stride_b, int32_t W, const int32_t *context_lens,
+                          const int32_t *cu_seqlens, int32_t B, int32_t tokens,
+                          const float *table, int64_t table_len, int32_t rot_dim,
+                          int32_t interleaved, const void *q_weight, const void *k_weight,
+                          int32_t weight_dtype, float eps, int32_t H_q, int32_t H_kv,
+                          int32_t D, int32_t block_size, void *q_out, void *stream);
+
 /* Pages for a chunk: adds each sequence's chunk length to context_lens and
  * gives its new pages the blocks from next_free_block on, by the rule of
  * append_token_kv (kv_cache.py:133-150) applied to each token, sequence after
@@ -729,6 +754,68 @@ int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride
                          int32_t W, int32_t max_context_len, float scale, int32_t causal,
                          uint16_t *out, float *lse, void *workspace,
                          size_t workspace_bytes, void *stream);
+
+/* cvsa_chunk_attention over caches of 8 bits (see cvsa_append_chunk_kv8), which are
+ * brought to bf16, exactly, on their way to the products.  The workspace's size is
+ * its own. */
+size_t cvsa_chunk_attention8_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
+                                             int32_t H_kv, int32_t D, int32_t block_size,
+                                             int32_t W, int32_t max_context_len);
+int cvsa_chunk_attention8(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h,
+                          const uint8_t *k_cache, const uint8_t *v_cache,
+                          const uint8_t *k_scales, const uint8_t *v_scales,
+                          int64_t num_blocks, const int32_t *block_tables,
+                          int64_t bt_stride_b, const int32_t *context_lens,
+                          const int32_t *cu_seqlens, const int32_t *cu_host, int32_t B,
+                          int32_t H_q, int32_t H_kv, int32_t D, int32_t block_size,
+                          int32_t W, int32_t max_context_len, float scale, int32_t causal,
+                          uint16_t *out, float *lse, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Weights of the keys: for each sequence b and KV head h, weights[b][h][j] of the
+ * key at position j becomes (j is one of the chunk's tokens ? 0 : itself) plus the
+ * sum of exp(scale q . k_j - lse) over the rows (token, query head of h's group) that
+ * see key j, of the sequence's last `window` tokens or, with 0, of all of its chunk.
+ * weights: [B, H_kv, S] fp32 contiguous, S >= W * block_size; entries past a
+ * context, and those of sequences without tokens in the chunk, are left as they
+ * are.  lse: [cu[B], H_q] fp32, what cvsa_chunk_attention gives; a row whose lse is
+ * -inf saw nothing and gives nothing.  Keys of blocks outside the pool get nothing.
+ * k_cache: bf16, or with k_scales 8 bits (cvsa_append_chunk_kv8).  Equal calls give
+ * equal results.  The workspace needs no initialisation. */
+size_t cvsa_add_key_weights_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
+                                            int32_t H_kv, int64_t S, int32_t window);
+int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q, int64_t q_stride_t,
+                         int64_t q_stride_h, const float *lse, const void *k_cache,
+                         const uint8_t *k_scales, int64_t num_blocks,
+                         const int32_t *block_tables, int64_t bt_stride_b,
+                         const int32_t *context_lens, const int32_t *cu_seqlens,
+                         const int32_t *cu_host, int32_t B, int32_t H_q, int32_t H_kv,
+                         int32_t D, int32_t block_size, int32_t W, float scale,
+                         int32_t causal, int32_t window, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* Cuts each sequence of more than `keep` tokens to `keep`, for each KV head by
+ * itself: its first `sinks` tokens stay, its last `recent` and, of those between,
+ * the ones of the largest weights (ties: the lowest slot; NaN is above all).
+ * Slots below keep - recent whose token stays keep it; the others of them get the
+ * kept tokens from slots keep - recent on, in order; the last `recent` tokens go to
+ * slots keep - recent .. keep, in order.  Keys, values and weights move; what is
+ * behind slot keep is left as it is.  context_lens and block_tables are read, not
+ * changed: the caller takes min(context, keep) as the new lengths.  Caches of bf16,
+ * or with scales of 8 bits: a page that tokens come to gets the largest scale of its
+ * tokens' pages, to which their payloads are brought.  kept: [B, H_kv, keep], the
+ * old slot of each new one (-1 past a shorter context).  Pages must belong to one
+ * sequence; a token whose block is outside the pool is not moved.  The workspace
+ * (256-byte aligned; cache_bits 16 or 8) needs no initialisation. */
+size_t cvsa_evict_tokens_workspace_bytes(int32_t B, int32_t H_kv, int32_t D, int32_t block_size,
+                                         int32_t cache_bits, int32_t keep, int32_t sinks,
+                                         int32_t recent);
+int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void *v_cache,
+                      uint8_t *k_scales, uint8_t *v_scales, int64_t num_blocks,
+                      const int32_t *block_tables, int64_t bt_stride_b, int32_t W,
+                      const int32_t *context_lens, int32_t B, int32_t H_kv, int32_t D,
+                      int32_t block_size, int32_t keep, int32_t sinks, int32_t recent,
+                      int32_t *kept, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
