@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kAppendThreads) void append8_kernel(const RotaryArg
   int blk = -1;
   int64_t token0 = 0;                   // of row 0
   if (unit < e.units) {
-    b = last_sequence(a.B, [&](int b) {
+    b = last_that(a.B, [&](int b) {
       return (int64_t)(a.cu[b] >> e.bs_log2) + 2 * (int64_t)b <= unit;
     });
     const int first = a.cu[b], n = a.cu[b + 1] - first, ctx = a.context_lens[b];

@@ -304,6 +304,22 @@ __device__ __forceinline__ uint32_t wave_incl_scan_u32(uint32_t v) {
   return v + (row >= 1 ? t0 : 0u) + (row >= 2 ? t1 : 0u) + (row >= 3 ? t2 : 0u);
 }
 
+// The last of n numbers that first(b) holds for, as it does for the first ones of
+// them, 64 candidates a look; the same in all lanes.
+template <class F>
+__device__ __forceinline__ int last_that(int n, F first) {
+  const int lane = threadIdx.x & 63;
+  int b = 0;
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const bool le = lane * step < n && first(b + lane * step);
+    const int k = __popcll(__ballot(le)) - 1;
+    b += k * step;
+    n = min(step, n - k * step);
+  }
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
 // Sum over lanes that share (lane mod W): adds the 64/W lanes
 // {l, l+W, l+2W, ...}.  All those lanes end with the same value.
 template <int W>

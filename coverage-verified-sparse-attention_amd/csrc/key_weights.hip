@@ -20,12 +20,14 @@
 // no LDS, no barrier.  The keys of all sequences, end to end, are cut into equal
 // ranges, one for each wave that fits the GPU.
 //
-// Many rows: the matrix and vector pipes bound it (32 exponentials of a wave to 16
-// products at D = 128).  A workgroup keeps 256 keys in registers, 64 a wave, and the
-// rows pass by through LDS, 64 at a time, so a row is read once for 256 keys and an
-// LDS read feeds two products.  Rows are cut into segments, a (segment, 256 keys)
-// pair is a job; jobs whose rows see none of their keys are left out.  If a
-// sequence has several segments their sums are joined in order by a second kernel.
+// Many rows: the vector and matrix pipes bound it (32 exponentials of a wave, with a
+// fused multiply and an addition each, to 16 products at D = 128), so the products
+// of the next 32 rows stand between the exponentials of these.  A workgroup keeps a
+// tile of 256 keys in registers, 64 a wave, and the rows that see any of them pass by
+// through LDS, 128 at a time: a row is read once for 256 keys and an LDS read feeds
+// two products.  The passes of all tiles, end to end, are cut into equal ranges, one
+// for each workgroup, which so loads one or two tiles of keys; a tile that several
+// ranges share is joined in order by a second kernel.
 #include "chunk_common.h"
 
 #include <algorithm>
@@ -50,18 +52,11 @@ struct WeighArgs {
   int causal, window;     // window: tokens of a sequence that count, 0: all
   float *weights;         // [B, H_kv, S]
   int64_t S;
-  // Sequences of few rows have at most few_rows of them, those of many more.
-  int few_rows;
-  // Many rows.
-  int segment;            // rows
-  int max_segments;       // of a sequence
-  float *parts;           // [B, H_kv, max_segments, S] where max_segments > 1
+  float *parts;           // many rows: [range][H_kv][2][kWeighKeys] sums of shared tiles
 };
 
 constexpr int kWeighFewRows = 32;
-constexpr int kWeighKeys = 256;      // of a job of many rows
-constexpr int kWeighRows = 64;       // that pass by together
-constexpr int kMaxSegments = 32;
+constexpr int kWeighKeys = 256;  // of a tile of many rows
 
 // A sequence's rows that count, 0 .. rows, from its token `skip` on.
 struct WeighSeq {
@@ -78,7 +73,7 @@ __device__ __forceinline__ WeighSeq weigh_look(const WeighArgs &a, int b, bool f
   s.pos0 = ctx - count;
   s.before = ctx - len;
   s.rows = count * a.G;
-  if (len > 0 && (s.rows <= a.few_rows) == few)
+  if (len > 0 && (s.rows <= kWeighFewRows) == few)
     s.keys = max(0, min(ctx, a.W << a.bs_log2));
   else
     s.rows = 0;
@@ -105,6 +100,31 @@ struct WeighKeys {
     } else {
       return w[ks];
     }
+  }
+};
+
+// The queries' operand of step ks, in the columns that the keys have: bytes from a
+// tile's start to row l % 32.  At D = 256 the second half of the columns is 256
+// bytes on.
+template <int D, bool F8>
+struct WeighPlaces {
+  static constexpr int N = D == 256 ? 8 : D / 16;
+  uint32_t at[N];
+
+  __device__ __forceinline__ void init() {
+    const int l31 = threadIdx.x & 31, half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int ks = 0; ks < N; ++ks) {
+      const int ch = F8 ? ks / 2 * 4 + half * 2 + ks % 2 : 2 * ks + half;
+      at[ks] = (l31 * D + chunk_swizzle<D>(l31, ch) * 8) * 2;
+    }
+  }
+  __device__ __forceinline__ void renew() {  // see ChunkPlaces
+#pragma unroll
+    for (int ks = 0; ks < N; ++ks) asm volatile("" : "+v"(at[ks]));
+  }
+  __device__ __forceinline__ uint4 read(const char *tile, int ks) const {
+    return chunk_read_k(tile + at[ks % N] + ks / N * 256);
   }
 };
 
@@ -256,109 +276,186 @@ __global__ __launch_bounds__(256, (weigh_few_fit<D, F8>())) void weigh_few_kerne
   }
 }
 
-// Segment `seg` of a sequence of many rows: the keys that its last row sees.
-__device__ __forceinline__ int weigh_segment_keys(const WeighArgs &a, int pos0, int keys, int rows,
-                                                  int seg) {
-  if (seg * a.segment >= rows) return 0;
-  const int last = (min((seg + 1) * a.segment, rows) - 1) / a.G;
-  return a.causal ? max(0, min(keys, pos0 + last + 1)) : keys;
+// Rows that pass by together.
+template <int D>
+constexpr int weigh_rows() {
+  return D == 256 ? 64 : 128;
 }
+
+// Passes of a sequence's tiles: `full` of each of the tiles that all rows see in part
+// at least, then `step` fewer from tile to tile.  (Rows come G to a token, so the
+// rows before a tile's first token are a multiple of the rows of a pass.)
+struct WeighPasses {
+  int tiles, old;  // tiles, of which all rows see the first old ones
+  uint32_t full, first, step;  // first: what tile 0 would have, were it of the latter
+
+  __device__ __forceinline__ WeighPasses(const WeighArgs &a, const WeighSeq &s, int pass_rows) {
+    tiles = s.rows > 0 ? (s.keys + kWeighKeys - 1) / kWeighKeys : 0;
+    full = (uint32_t)(s.rows + pass_rows - 1) / pass_rows;
+    old = a.causal ? min(tiles, s.pos0 < 0 ? 0 : s.pos0 / kWeighKeys + 1) : tiles;
+    step = kWeighKeys / pass_rows * a.G;
+    // (rows + pos0 G) / pass_rows rounded up, the sum not negative where it is used
+    const int64_t seen = max((int64_t)0, s.rows + (int64_t)s.pos0 * a.G);
+    first = (uint32_t)((seen + pass_rows - 1) / pass_rows);
+  }
+  __device__ __forceinline__ uint32_t of(int tile) const {
+    return tile < old ? full : first - tile * step;
+  }
+  // Of the tiles before this one.
+  __device__ __forceinline__ uint32_t before(int tile) const {
+    const uint32_t a = min(tile, old), n = tile - a;
+    // first - (a + i) step for i < n
+    return a * full + n * (first - a * step) - (uint32_t)((uint64_t)n * (n - 1) / 2) * step;
+  }
+  __device__ __forceinline__ uint32_t all() const { return before(tiles); }
+};
+
+// The ranges of all passes of a head, the first `more` a pass longer.
+struct WeighRanges {
+  uint32_t n, len, more;
+
+  __device__ __forceinline__ WeighRanges(uint32_t ranges, uint32_t passes) {
+    n = ranges;
+    len = passes / ranges;
+    more = passes - len * ranges;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t r) const { return r * len + min(r, more); }
+  __device__ __forceinline__ uint32_t of(uint32_t pass) const {
+    const uint32_t longer = more * (len + 1);
+    return pass < longer ? pass / (len + 1) : more + (pass - longer) / max(len, 1u);
+  }
+};
 
 template <int D, bool F8>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const WeighArgs a) {
-  constexpr int KS = D / 16, CPR = D / 8, RB = kWeighRows;
-  constexpr int NV = RB * CPR / 256;  // vectors of a thread, of the rows that pass by
+  constexpr int KS = D / 16, CPR = D / 8, RB = weigh_rows<D>(), TILES = RB / 32;
+  constexpr int NV = RB * CPR / 256;  // vectors of a thread, of a pass
   static_assert(NV >= 1, "a vector for each thread");
-  __shared__ __align__(16) uint16_t s_q[2][RB * D];
-  __shared__ __align__(16) float s_lse[2][RB];
+  // Two arrays: a load into one does not hold up reads of the other.
+  __shared__ __align__(16) uint16_t s_q0[RB * D], s_q1[RB * D];
+  __shared__ __align__(16) float s_lse[4][RB];
+  __shared__ int s_low[4][2];  // whether some are -inf, by wave
+  constexpr int kAhead = KS < 3 ? KS : 3;
 
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // KV heads vary fastest: workgroups go round the XCDs, so one XCD's cache sees the
+  // keys and queries of few heads.
+  const int h = blockIdx.x % a.H_kv;
+  const uint32_t range = blockIdx.x / a.H_kv;
   const WeighSeq own = weigh_look(a, lane, false);
-  auto jobs_of = [&](const WeighSeq &s) {
-    uint32_t n = 0;
-    for (int seg = 0; seg < a.max_segments; ++seg)
-      n += (uint32_t)(weigh_segment_keys(a, s.pos0, s.keys, s.rows, seg) + kWeighKeys - 1) /
-           kWeighKeys;
-    return n;
-  };
-  const uint32_t own_jobs = jobs_of(own);
+  uint32_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const WeighPasses p(a, b0 == 0 ? own : weigh_look(a, b0 + lane, false), RB);
+    total += __builtin_amdgcn_readfirstlane(wave_sum_u32(p.all()));
+  }
+  const WeighRanges ranges(gridDim.x / a.H_kv, total);
+  const uint32_t begin = ranges.start(range), end = ranges.start(range + 1);
 
-  for (uint32_t id = blockIdx.x;; id += gridDim.x) {
-    const int h = id % a.H_kv;
-    uint32_t job = id / a.H_kv;
-    // The job's sequence, segment and keys.
-    int seq = -1;
-    WeighSeq s = {};
-    for (int b0 = 0; b0 < a.B; b0 += kWave) {
-      const WeighSeq look = b0 == 0 ? own : weigh_look(a, b0 + lane, false);
-      const uint32_t n = b0 == 0 ? own_jobs : jobs_of(look);
-      const uint32_t incl = wave_incl_scan_u32(n);
-      const uint32_t all = __builtin_amdgcn_readlane(incl, 63);
-      if (job < all) {
-        const int l = __popcll(__ballot(incl <= job));
-        seq = b0 + l;
-        s.first = __builtin_amdgcn_readlane(look.first, l);
-        s.pos0 = __builtin_amdgcn_readlane(look.pos0, l);
-        s.keys = __builtin_amdgcn_readlane(look.keys, l);
-        s.rows = __builtin_amdgcn_readlane(look.rows, l);
-        s.before = __builtin_amdgcn_readlane(look.before, l);
-        job -= __builtin_amdgcn_readlane(incl - n, l);
-        break;
-      }
-      job -= all;
-    }
-    if (seq < 0) return;
-    int seg, tile;
-    {
-      const uint32_t n = lane < a.max_segments
-                             ? (uint32_t)(weigh_segment_keys(a, s.pos0, s.keys, s.rows, lane) +
-                                          kWeighKeys - 1) / kWeighKeys
-                             : 0u;
-      const uint32_t incl = wave_incl_scan_u32(n);
-      seg = __popcll(__ballot(incl <= job));
-      tile = (int)(job - __builtin_amdgcn_readlane(incl - n, seg));
-    }
+  // Tokens and heads from a thread's first row to its others, and to the next pass.
+  int step_tok[NV], step_g[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    step_tok[i] = i * 256 / CPR / a.G;
+    step_g[i] = i * 256 / CPR - step_tok[i] * a.G;
+  }
+  // The wave's loads into LDS have arrived; a barrier alone does not wait for them.
+  auto loaded = []() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+  };
+  if (tid < 8) s_low[tid / 2][tid % 2] = 0;  // of one wave only where RB is 64
+  __syncthreads();
+  const int pass_tok = RB / a.G, pass_g = RB - pass_tok * a.G;
+
+  // Passes pass0 .. pass1 of a tile's rows, which are those from its first key's on.
+  auto walk = [&](int seq, const WeighSeq &s, int tile, int pass0, int pass1, bool shared)
+      __attribute__((always_inline)) {
     const int key0 = tile * kWeighKeys;
-    const int row1 = min((seg + 1) * a.segment, s.rows);
-    int row0 = seg * a.segment;
-    // Rows before see none of the keys; whole passes of rows.
-    if (a.causal && key0 > s.pos0)
-      row0 = max(row0, (int)min((int64_t)(key0 - s.pos0) * a.G, (int64_t)row1 - 1) / RB * RB);
+    const int tile_tok = a.causal ? max(0, key0 - s.pos0) : 0;
+    // Rows count from the tile's first; those of the range.
+    const int all_rows = s.rows - tile_tok * a.G;
+    const int row0 = pass0 * RB, row1 = min(pass1 * RB, all_rows);
+    const int pos0 = s.pos0 + tile_tok;
+    const int first_tok = row0 / a.G, first_g = row0 - first_tok * a.G;
     const int32_t *const bt = a.block_tables + seq * a.bt_sb;
 
-    // Rows that pass by: the thread's vectors and, of the first threads, a
-    // log-sum-exp.
-    uint4 next[NV];
-    float next_lse = 0.f;
-    auto at_row = [&](int r) {  // its token and head
-      const int row = min(r, row1 - 1), tok = row / a.G;
-      return make_int2(s.first + tok, h * a.G + row - tok * a.G);
+    // Rows that pass by, straight into LDS: the thread's vectors, 16 bytes each,
+    // whose places are permuted as chunk_swizzle has them; and, of pass p, log-sum-
+    // exps for s_lse[p % 4].  The thread's first row lies `off` bytes from the pass's
+    // first token, whose head base_g is the pass's first row; from pass to pass
+    // without a division, in 32 bits.
+    const char *base = (const char *)(a.q + (int64_t)(s.first + tile_tok + first_tok) * a.q_st +
+                                      (int64_t)h * a.G * a.q_sh);
+    int base_g = first_g;
+    auto row_bytes = [&](int tok, int g) {
+      return (uint32_t)tok * (uint32_t)a.q_st * 2 + (uint32_t)g * (uint32_t)a.q_sh * 2;
     };
-    auto request = [&](int r0) {
+    const uint32_t wrap = row_bytes(1, 0) - row_bytes(0, a.G);
+    const int tid_tok = (first_g + tid / CPR) / a.G;
+    int g = first_g + tid / CPR - tid_tok * a.G;
+    uint32_t off = row_bytes(tid_tok, g);
+    auto request = [&](int r0, uint16_t *buf) __attribute__((always_inline)) {
       unrolled<NV>([&](auto n) {
         constexpr int i = decltype(n)::value;
-        const int c = tid + i * 256;
-        const int2 at = at_row(r0 + c / CPR);
-        next[i] = *reinterpret_cast<const uint4 *>(a.q + (int64_t)at.x * a.q_st +
-                                                   (int64_t)at.y * a.q_sh + c % CPR * 8);
+        const int r = (tid + i * 256) / CPR;
+        uint32_t at = off + row_bytes(step_tok[i], step_g[i]);
+        at += g + step_g[i] >= a.G ? wrap : 0u;
+        at = r0 + r < row1 ? at : 0;  // past the last: the first
+        const char *from = base + at + chunk_swizzle<D>(r, tid % CPR) * 16;
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)from,
+            (__attribute__((address_space(3))) void *)(buf + (i * 256 + wave * 64) * 8), 16, 0, 0);
       });
-      if (tid < RB) {
-        const int2 at = at_row(r0 + tid);
-        const float x = a.lse[(int64_t)at.x * a.H_q + at.y];
+      base_g += pass_g;
+      const bool next = base_g >= a.G;
+      base_g -= next ? a.G : 0;
+      base += (int64_t)(pass_tok + next) * a.q_st * 2;
+      g += pass_g;
+      off += row_bytes(0, pass_g) - (next ? row_bytes(1, 0) : 0u);
+      if (g >= a.G) {
+        g -= a.G;
+        off += wrap;
+      }
+    };
+    float next_lse = 0.f;
+    const int lse_tok = (first_g + tid % RB) / a.G;
+    int lse_g = first_g + tid % RB - lse_tok * a.G;
+    const float *lse_at = a.lse +
+                          (int64_t)(s.first + tile_tok + first_tok + lse_tok) * a.H_q + h * a.G +
+                          lse_g;
+    auto request_lse = [&](int r0) __attribute__((always_inline)) {
+      if (tid >= RB) return;
+      next_lse = -INFINITY;
+      if (r0 + tid < row1) {
+        const float x = *lse_at;
         // A row that saw nothing gives nothing.
         next_lse = x == -INFINITY ? -INFINITY : -x * a.lse_factor;
       }
+      lse_at += (int64_t)pass_tok * a.H_q + pass_g;
+      lse_g += pass_g;
+      if (lse_g >= a.G) {
+        lse_g -= a.G;
+        lse_at += a.H_q - a.G;
+      }
     };
-    auto store = [&](int buf) {
-      unrolled<NV>([&](auto n) {
-        constexpr int i = decltype(n)::value;
-        const int c = tid + i * 256, r = c / CPR;
-        *reinterpret_cast<uint4 *>(&s_q[buf][r * D + chunk_swizzle<D>(r, c % CPR) * 8]) = next[i];
-      });
-      if (tid < RB) s_lse[buf][tid] = next_lse;
+    auto store_lse = [&](int pass) {
+      if (tid >= RB) return;
+      s_lse[pass % 4][tid] = next_lse;
+      const bool low = __ballot(next_lse == -INFINITY) != 0;
+      if (lane == 0) s_low[pass % 4][wave] = low ? 1 : 0;
     };
-    request(row0);
+    // The buffers are free: nobody reads what the last tile left.
+    const int passes = (row1 - row0 + RB - 1) / RB;
+    request(row0, s_q0);
+    request_lse(row0);
+    store_lse(0);
+    if (passes > 1) {
+      request(row0 + RB, s_q1);
+      request_lse(row0 + RB);
+      store_lse(1);
+    }
 
     // The wave's keys, as the second operand: bf16, the scales apart.
     uint4 k[2][KS];
@@ -375,11 +472,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
       all_ok = all_ok && at.ok;
       const char *p = weigh_row<D, F8>(a, at.blk, at.ok ? key : 0, h);
       if constexpr (F8) {
-        // Columns as the bf16 rows of LDS have them.
+        WeighKeys<D, true> raw;
+        raw.load(p, half);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          k[i][ks] = chunk_from_8(*reinterpret_cast<const uint2 *>(p + ks * 16 + half * 8), 1.f,
-                                  1.f);
+        for (int ks = 0; ks < KS; ++ks) k[i][ks] = raw.get(ks);
         c[i] = a.c * chunk_scale(a.k_scales[(int64_t)at.blk * a.H_kv + h]);
       } else {
 #pragma unroll
@@ -387,129 +483,270 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
           k[i][ks] = *reinterpret_cast<const uint4 *>(p + ks * 32 + half * 16);
         c[i] = a.c;
       }
-      min_row[i] = a.causal && key > s.pos0
-                       ? (int)min((int64_t)(key - s.pos0) * a.G, (int64_t)0x7fffffff) : 0;
+      min_row[i] = a.causal && key > pos0 ? min(key - pos0, kWeighKeys) * a.G : 0;
     }
     // Rows from here on see all of the wave's keys.
     const int last_key = key0 + wave * 64 + 63;
-    const int full_row = a.causal && last_key > s.pos0
-                             ? (int)min((int64_t)(last_key - s.pos0) * a.G, (int64_t)0x7fffffff)
-                             : 0;
+    const int full_row = a.causal && last_key > pos0 ? min(last_key - pos0, kWeighKeys) * a.G : 0;
+    // Rows before see none of them.
+    const int first_key = key0 + wave * 64;
+    const int first_row =
+        a.causal && first_key > pos0 ? min(first_key - pos0, kWeighKeys) * a.G : 0;
     const bool keys_ok = __ballot(!all_ok) == 0;
 
     float sum[2] = {0.f, 0.f};
-    store(0);
+    loaded();
     __syncthreads();
-    int buf = 0;
-    for (int r0 = row0; r0 < row1; r0 += RB, buf ^= 1) {
-      if (r0 + RB < row1) request(r0 + RB);
+    WeighPlaces<D, F8> place;
+    place.init();
+    uint4 f[kAhead + 1];  // of the queries, read ahead of their products
+    auto fetch = [&](const uint16_t *rows, auto n) {
+      constexpr int ks = decltype(n)::value;
+      if constexpr (ks < KS) f[ks % (kAhead + 1)] = place.read((const char *)rows, ks);
+    };
+    auto product = [&](f32x16_t (&st)[2], auto n) {
+      constexpr int ks = decltype(n)::value;
 #pragma unroll
-      for (int rt = 0; rt < RB / 32; ++rt) {
-        f32x16_t st[2];
+      for (int i = 0; i < 2; ++i)
+        st[i] = chunk_mfma(f[ks % (kAhead + 1)], k[i][ks], ks ? st[i] : f32x16_t{});
+    };
+    // Exponentials of st, the scores of 32 rows, between the products of the next 32;
+    // neg: the first of the rows' terms, and then of the next ones'.
+    float4 neg;
+    // MASK: of the scores that are not all seen, those that are count.
+    auto weigh = [&](const f32x16_t (&st)[2], int base, const float *lse, f32x16_t (&nxt)[2],
+                     const uint16_t *rows, const float *next_lse, auto mask)
+        __attribute__((always_inline)) {
+      constexpr bool MASK = decltype(mask)::value;
+      place.renew();
+      unrolled<kAhead>([&](auto n) { fetch(rows, n); });
+      // Eight scores, four rows of both of the lane's keys, at a time; each is added
+      // one later: an addition right behind the exponential would wait.
+      float part[2][4], last = 0.f;
+      float4 next_neg;
+      const int low[2] = {min_row[0] - base - 4 * half, min_row[1] - base - 4 * half};
+      auto add = [&](auto n, float p) {
+        constexpr int m = decltype(n)::value, i = m % 8 / 4, x = m % 4;
+        part[i][x] = m / 8 == 0 ? p : part[i][x] + p;
+      };
+      unrolled<32>([&](auto n) {
+        constexpr int m = decltype(n)::value, g = m / 8, i = m % 8 / 4, x = m % 4;
+        // The products end early, so that the next exponentials do not wait.
+        constexpr int p0 = m < 28 ? m * KS / 28 : KS, p1 = m < 28 ? (m + 1) * KS / 28 : KS;
+        if constexpr (m % 8 == 0)
+          next_neg = *reinterpret_cast<const float4 *>(
+              (g < 3 ? lse + 8 * (g + 1) : next_lse) + 4 * half);
+        unrolled<p1 - p0>([&](auto o) {
+          constexpr int ks = p0 + decltype(o)::value;
+          product(nxt, std::integral_constant<int, ks>());
+          fetch(rows, std::integral_constant<int, ks + kAhead>());
+        });
+        const float ref = x == 0 ? neg.x : x == 1 ? neg.y : x == 2 ? neg.z : neg.w;
+        float p = __builtin_amdgcn_exp2f(fmaf(st[i][4 * g + x], c[i], ref));
+        // Rows past the last, and those that saw nothing, have a term of -inf.
+        if constexpr (MASK) p = 8 * g + x >= low[i] && ref != -INFINITY ? p : 0.f;
+        if constexpr (m > 0) add(std::integral_constant<int, m - 1>(), last);
+        last = p;
+        if constexpr (m % 8 == 7) neg = next_neg;
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      add(std::integral_constant<int, 31>(), last);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const uint4 x = chunk_read_k((const char *)&s_q[buf][rt * 32 * D] + chunk_k_place<D>(ks));
-#pragma unroll
-          for (int i = 0; i < 2; ++i) st[i] = chunk_mfma(x, k[i][ks], ks ? st[i] : f32x16_t{});
-        }
-        float neg[16];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 v =
-              *reinterpret_cast<const float4 *>(&s_lse[buf][rt * 32 + 8 * g + 4 * half]);
-          neg[4 * g] = v.x; neg[4 * g + 1] = v.y; neg[4 * g + 2] = v.z; neg[4 * g + 3] = v.w;
-        }
-        const int base = r0 + rt * 32;
-        const bool whole = keys_ok && base >= full_row && base + 32 <= row1;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            p[e] = __builtin_amdgcn_exp2f(fmaf(st[i][e], c[i], neg[e]));
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int r = base + 8 * (e / 4) + 4 * half + e % 4;
-              p[e] = r >= min_row[i] && r < row1 && neg[e] != -INFINITY ? p[e] : 0.f;
-            }
-          }
-          sum[i] += sum16(p);
-        }
+      for (int i = 0; i < 2; ++i)
+        sum[i] += (part[i][0] + part[i][1]) + (part[i][2] + part[i][3]);
+    };
+    auto rows32 = [&](const f32x16_t (&st)[2], int base, const float *lse, f32x16_t (&nxt)[2],
+                      const uint16_t *rows, const float *next_lse, bool all)
+        __attribute__((always_inline)) {
+      if (keys_ok && all && base >= full_row) {
+        weigh(st, base, lse, nxt, rows, next_lse, std::false_type());
+      } else if (base + 32 > first_row) {
+        weigh(st, base, lse, nxt, rows, next_lse, std::true_type());
+      } else {  // none of them sees any of the wave's keys
+        neg = *reinterpret_cast<const float4 *>(next_lse + 4 * half);
+        if (base + 64 > first_row)
+          unrolled<KS>([&](auto n) {
+            fetch(rows, n);
+            product(nxt, n);
+          });
       }
-      if (r0 + RB < row1) store(buf ^ 1);
+    };
+    // Pass p: the weights of 32 rows with the products of the next 32, at last of the
+    // first ones of pass p + 1, whose rows arrive meanwhile; those of pass p + 2 take
+    // the buffer of pass p.
+    f32x16_t st0[2], st1[2];
+    unrolled<KS>([&](auto n) {
+      fetch(s_q0, n);
+      product(st0, n);
+    });
+    neg = *reinterpret_cast<const float4 *>(s_lse[0] + 4 * half);
+    auto pass = [&](int p, uint16_t *cur, uint16_t *next) __attribute__((always_inline)) {
+      const int r0 = row0 + p * RB;
+      const float *const lse = s_lse[p % 4];
+      const bool all = __builtin_amdgcn_readfirstlane(s_low[p % 4][0] | s_low[p % 4][1]) == 0;
+      unrolled<TILES - 1>([&](auto n) __attribute__((always_inline)) {
+        constexpr int i = decltype(n)::value;
+        if constexpr (i % 2 == 0)
+          rows32(st0, r0 + 32 * i, lse + 32 * i, st1, cur + 32 * (i + 1) * D, lse + 32 * (i + 1),
+                 all);
+        else
+          rows32(st1, r0 + 32 * i, lse + 32 * i, st0, cur + 32 * (i + 1) * D, lse + 32 * (i + 1),
+                 all);
+      });
+      loaded();
       __syncthreads();
+      const bool more = p + 2 < passes;
+      if (more) {
+        request(r0 + 2 * RB, cur);
+        request_lse(r0 + 2 * RB);
+      }
+      constexpr int i = TILES - 1;
+      rows32(st1, r0 + 32 * i, lse + 32 * i, st0, next, s_lse[(p + 1) % 4], all);
+      if (more) store_lse(p + 2);
+    };
+    static_assert(TILES % 2 == 0, "two sets of scores in turn");
+    for (int p = 0; p < passes; p += 2) {
+      pass(p, s_q0, s_q1);
+      if (p + 1 < passes) pass(p + 1, s_q1, s_q0);
     }
+    __syncthreads();  // the buffers are the next tile's
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float u, v;
       xchg32(sum[i], u, v);
-      const int key = key0 + wave * 64 + i * 32 + l31;
-      const float total = ok[i] ? u + v : 0.f;
-      if (half == 0 && key < s.keys) {
-        const int64_t at = ((int64_t)seq * a.H_kv + h);
-        if (s.rows > a.segment)
-          a.parts[(at * a.max_segments + seg) * a.S + key] = total;
-        else
-          a.weights[at * a.S + key] = (key < s.before ? a.weights[at * a.S + key] : 0.f) + total;
+      const int at = wave * 64 + i * 32 + l31, key = key0 + at;
+      const float all = ok[i] ? u + v : 0.f;
+      if (half != 0) continue;
+      if (shared) {
+        a.parts[(((int64_t)range * a.H_kv + h) * 2 + (pass0 == 0)) * kWeighKeys + at] = all;
+      } else if (key < s.keys) {
+        float *const w = a.weights + ((int64_t)seq * a.H_kv + h) * a.S + key;
+        *w = (key < s.before ? *w : 0.f) + all;
       }
     }
+  };
+
+  uint32_t before = 0;
+  for (int b0 = 0; b0 < a.B && before < end; b0 += kWave) {
+    const WeighSeq mine = b0 == 0 ? own : weigh_look(a, b0 + lane, false);
+    const uint32_t passes = WeighPasses(a, mine, RB).all();
+    const uint32_t incl = wave_incl_scan_u32(passes), last = before + incl, start = last - passes;
+    uint64_t todo = __ballot(passes > 0 && start < end && last > begin);
+    while (todo != 0) {
+      const int l = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      WeighSeq s;
+      s.first = __builtin_amdgcn_readlane(mine.first, l);
+      s.pos0 = __builtin_amdgcn_readlane(mine.pos0, l);
+      s.keys = __builtin_amdgcn_readlane(mine.keys, l);
+      s.rows = __builtin_amdgcn_readlane(mine.rows, l);
+      s.before = __builtin_amdgcn_readlane(mine.before, l);
+      const WeighPasses p(a, s, RB);
+      const uint32_t from = __builtin_amdgcn_readlane(start, l);
+      const uint32_t p0 = begin > from ? begin - from : 0, p1 = min(end - from, p.all());
+      // The last tile that starts at p0 or before.
+      int tile = last_that(p.tiles, [&](int n) { return p.before(n) <= p0; });
+      for (; tile < p.tiles && p.before(tile) < p1; ++tile) {
+        const uint32_t first = p.before(tile), n = p.of(tile);
+        const uint32_t a0 = p0 > first ? p0 - first : 0, a1 = min(p1 - first, n);
+        walk(b0 + l, s, tile, (int)a0, (int)a1, a0 > 0 || a1 < n);
+      }
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
 }
 
-// The segments' sums, in order.
-__global__ __launch_bounds__(256) void weigh_join_kernel(const WeighArgs a) {
-  const int seq = blockIdx.z, h = blockIdx.y;
-  const int first = a.cu[seq], len = a.cu[seq + 1] - first, ctx = a.context_lens[seq];
-  const int count = a.window > 0 ? min(len, a.window) : len, rows = count * a.G;
-  if (rows <= a.few_rows || rows <= a.segment) return;
-  const int keys = max(0, min(ctx, a.W << a.bs_log2)), pos0 = ctx - count;
-  const int segs = (rows + a.segment - 1) / a.segment;
-  const int64_t at = (int64_t)seq * a.H_kv + h;
-  for (int key = blockIdx.x * 256 + threadIdx.x; key < keys; key += gridDim.x * 256) {
-    float sum = key < ctx - len ? a.weights[at * a.S + key] : 0.f;
-    // Whole jobs of 256 keys were written.
-    int seg = 0;
-    while (seg < segs && (key & -kWeighKeys) >= weigh_segment_keys(a, pos0, keys, rows, seg)) ++seg;
-    for (; seg < segs; ++seg) sum += a.parts[(at * a.max_segments + seg) * a.S + key];
-    a.weights[at * a.S + key] = sum;
+// The parts of tiles that several ranges share, in order.
+template <int D>
+__global__ __launch_bounds__(kWeighKeys) void weigh_join_kernel(const WeighArgs a, int n_ranges) {
+  constexpr int RB = weigh_rows<D>();
+  const int lane = threadIdx.x & 63, h = blockIdx.y;
+  // Tiles of all sequences, end to end; their passes before them.
+  uint32_t total = 0;
+  int seq = -1, want = blockIdx.x;
+  uint32_t first = 0;
+  WeighSeq s = {};
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const WeighSeq mine = weigh_look(a, b0 + lane, false);
+    const WeighPasses p(a, mine, RB);
+    const uint32_t passes = p.all(), incl = wave_incl_scan_u32(passes);
+    const uint32_t tiles = wave_incl_scan_u32((uint32_t)p.tiles);
+    const int all_tiles = __builtin_amdgcn_readlane(tiles, 63);
+    if (seq < 0 && want < all_tiles) {
+      const int l = __popcll(__ballot((int)tiles <= want));
+      seq = b0 + l;
+      s.pos0 = __builtin_amdgcn_readlane(mine.pos0, l);
+      s.keys = __builtin_amdgcn_readlane(mine.keys, l);
+      s.rows = __builtin_amdgcn_readlane(mine.rows, l);
+      s.before = __builtin_amdgcn_readlane(mine.before, l);
+      first = total + __builtin_amdgcn_readlane(incl - passes, l);
+      want -= __builtin_amdgcn_readlane(tiles - (uint32_t)p.tiles, l);
+    } else if (seq < 0) {
+      want -= all_tiles;
+    }
+    total += __builtin_amdgcn_readlane(incl, 63);
   }
+  if (seq < 0) return;
+  const WeighPasses p(a, s, RB);
+  const WeighRanges ranges((uint32_t)n_ranges, total);
+  first += p.before(want);
+  const uint32_t r0 = ranges.of(first), r1 = ranges.of(first + p.of(want) - 1);
+  const int key = want * kWeighKeys + threadIdx.x;
+  if (r0 == r1 || key >= s.keys) return;
+  float *const w = a.weights + ((int64_t)seq * a.H_kv + h) * a.S + key;
+  const float was = key < s.before ? *w : 0.f;
+  float sum = 0.f;
+  auto part = [&](uint32_t r) {
+    return a.parts + (((int64_t)r * a.H_kv + h) * 2 + (r == r0)) * kWeighKeys + threadIdx.x;
+  };
+  for (uint32_t r = r0; r <= r1; r += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r + i <= r1 ? *part(r + i) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
+  }
+  *w = was + sum;
 }
 
 struct WeighPlan {
   bool few, many;
-  int segment, max_segments;
+  int ranges;       // of a head, many rows
+  int64_t tiles;    // of all sequences of many rows, at most
+  int64_t passes;   // likewise
   size_t bytes;
 };
 
-static WeighPlan plan_weigh(const int32_t *cu, int B, int G, int H_kv, int window, int64_t S) {
+static WeighPlan plan_weigh(const int32_t *cu, int B, int G, int H_kv, int D, int window,
+                            int64_t keys) {
   WeighPlan p = {};
-  int64_t most = 0;
+  const int pass_rows = D == 256 ? weigh_rows<256>() : weigh_rows<128>();
+  const int64_t tiles = (keys + kWeighKeys - 1) / kWeighKeys;
   for (int b = 0; b < B; ++b) {
     const int len = cu[b + 1] - cu[b];
     const int64_t rows = (int64_t)(window > 0 ? std::min(len, window) : len) * G;
     if (rows == 0) continue;
-    if (rows <= kWeighFewRows) p.few = true;
-    else p.many = true;
-    most = std::max(most, rows);
+    if (rows <= kWeighFewRows) {
+      p.few = true;
+      continue;
+    }
+    p.many = true;
+    p.tiles += tiles;
+    p.passes += tiles * ((rows + pass_rows - 1) / pass_rows);
   }
-  // Segments of 512 rows, or as long as the most segments need.
-  p.segment = (int)std::max<int64_t>(512, ((most + kMaxSegments - 1) / kMaxSegments + 63) / 64 * 64);
-  p.max_segments = (int)std::max<int64_t>(1, (most + p.segment - 1) / p.segment);
-  if (p.many && p.max_segments > 1)
-    p.bytes = (size_t)B * H_kv * p.max_segments * (size_t)S * sizeof(float);
+  // A range for each workgroup that fits the GPU.
+  p.ranges = std::max(1, 256 * (D == 256 ? 1 : 2) / H_kv);
+  if (p.many) p.bytes = (size_t)p.ranges * H_kv * 2 * kWeighKeys * sizeof(float);
   return p;
 }
 
 template <int D, bool F8>
 static void launch_weigh(const WeighArgs &a, const WeighPlan &p, hipStream_t s) {
   if (p.many) {
-    const unsigned wgs = 256 * (D == 256 ? 1 : 2);
-    hipLaunchKernelGGL((weigh_many_kernel<D, F8>), dim3(wgs), dim3(256), 0, s, a);
-    if (p.max_segments > 1) {
-      const unsigned x = (unsigned)std::min<int64_t>(64, (a.S + 255) / 256);
-      hipLaunchKernelGGL(weigh_join_kernel, dim3(x, a.H_kv, a.B), dim3(256), 0, s, a);
-    }
+    hipLaunchKernelGGL((weigh_many_kernel<D, F8>), dim3((unsigned)(p.ranges * a.H_kv)), dim3(256),
+                       0, s, a);
+    hipLaunchKernelGGL(weigh_join_kernel<D>, dim3((unsigned)p.tiles, (unsigned)a.H_kv),
+                       dim3(kWeighKeys), 0, s, a, p.ranges);
   }
   if (p.few) {
     const unsigned wgs =
@@ -541,10 +778,10 @@ static bool weigh_shape_ok(const int32_t *cu, int32_t B, int32_t H_q, int32_t H_
 using namespace cvsa;
 
 extern "C" size_t cvsa_add_key_weights_workspace_bytes(const int32_t *cu_host, int32_t B,
-                                                       int32_t H_q, int32_t H_kv, int64_t S,
-                                                       int32_t window) {
+                                                       int32_t H_q, int32_t H_kv, int32_t D,
+                                                       int64_t S, int32_t window) {
   if (!weigh_shape_ok(cu_host, B, H_q, H_kv, S, window)) return 0;
-  return plan_weigh(cu_host, B, H_q / H_kv, H_kv, window, S).bytes;
+  return plan_weigh(cu_host, B, H_q / H_kv, H_kv, D, window, S).bytes;
 }
 
 extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q,
@@ -580,8 +817,15 @@ extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q
   CVSA_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache) & 15) == 0 && q_stride_t % 8 == 0 &&
                    q_stride_h % 8 == 0,
                CVSA_ERR_INVALID, "add_key_weights: rows must be 16-byte aligned");
-  const WeighPlan p = plan_weigh(cu_host, B, H_q / H_kv, H_kv, window, S);
+  const WeighPlan p =
+      plan_weigh(cu_host, B, H_q / H_kv, H_kv, D, window, (int64_t)W * block_size);
   if (!p.few && !p.many) return CVSA_OK;
+  CVSA_REQUIRE(p.passes < (1LL << 31), CVSA_ERR_UNSUPPORTED,
+               "add_key_weights: too many queries and keys");
+  // Offsets among the rows that pass by together are of 32 bits.
+  CVSA_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && q_stride_t < (1 << 23) &&
+                   q_stride_h < (1 << 23),
+               CVSA_ERR_UNSUPPORTED, "add_key_weights: queries too far apart");
   CVSA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), CVSA_ERR_WORKSPACE,
                "add_key_weights: needs a workspace of %zu bytes", p.bytes);
   WeighArgs a = {};
@@ -597,8 +841,6 @@ extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q
   a.lse_factor = (float)((double)a.c / scale);
   a.causal = causal; a.window = window;
   a.weights = weights; a.S = S;
-  a.few_rows = kWeighFewRows;
-  a.segment = p.segment; a.max_segments = p.max_segments;
   a.parts = (float *)workspace;
   const hipStream_t s = (hipStream_t)stream;
   if (k_scales) launch_weigh_d<true>(a, p, D, s);

@@ -216,22 +216,6 @@ struct RotaryPlace {
   }
 };
 
-// The last of n sequences that first(b) holds for, as it does for the first ones
-// of them, 64 candidates a look.
-template <class F>
-__device__ __forceinline__ int last_sequence(int n, F first) {
-  const int lane = threadIdx.x & 63;
-  int b = 0;
-  while (n > 1) {
-    const int step = (n + 63) / 64;
-    const bool le = lane * step < n && first(b + lane * step);
-    const int k = __popcll(__ballot(le)) - 1;
-    b += k * step;
-    n = min(step, n - k * step);
-  }
-  return __builtin_amdgcn_readfirstlane(b);
-}
-
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryBatch = 3;  // passes whose rows are requested together
 
@@ -288,7 +272,7 @@ __device__ __forceinline__ void rotary_rows(const RotaryArgs &a, int64_t w) {
   int64_t pos;
   int64_t slot = -1;  // token's row in the cache, -1: not written
   if constexpr (APPEND) {
-    const int b = last_sequence(a.B, [&](int b) { return a.cu[b] <= t; });
+    const int b = last_that(a.B, [&](int b) { return a.cu[b] <= t; });
     const int place = a.context_lens[b] - (a.cu[b + 1] - t);
     pos = place;
     if (place >= 0) {

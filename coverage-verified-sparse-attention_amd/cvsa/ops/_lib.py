@@ -150,7 +150,7 @@ SIGNATURES = {
     "cvsa_chunk_attention8": (ctypes.c_int, [
         _p, _i64, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
         _i32, _i32, _f32, _i32, _p, _p, _p, _sz, _p]),
-    "cvsa_add_key_weights_workspace_bytes": (_sz, [_p, _i32, _i32, _i32, _i64, _i32]),
+    "cvsa_add_key_weights_workspace_bytes": (_sz, [_p, _i32, _i32, _i32, _i32, _i64, _i32]),
     "cvsa_add_key_weights": (ctypes.c_int, [
         _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32,
         _i32, _i32, _f32, _i32, _i32, _p, _sz, _p]),

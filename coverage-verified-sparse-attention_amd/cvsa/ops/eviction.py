@@ -75,7 +75,7 @@ def add_key_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor,
         L = _lib.load()
         # Allocated for the call, so no two calls, streams or captured graphs
         # share it.
-        key = ("add_key_weights", H_q, H_kv, S, window)
+        key = ("add_key_weights", H_q, H_kv, D, S, window)
         need = layout._workspace_bytes.get(key)
         if need is None:
             need = L.cvsa_add_key_weights_workspace_bytes(layout.cu_host, B, *key[1:])

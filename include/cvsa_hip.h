@@ -783,7 +783,8 @@ int cvsa_chunk_attention8(const uint16_t *q, int64_t q_stride_t, int64_t q_strid
  * k_cache: bf16, or with k_scales 8 bits (cvsa_append_chunk_kv8).  Equal calls give
  * equal results.  The workspace needs no initialisation. */
 size_t cvsa_add_key_weights_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
-                                            int32_t H_kv, int64_t S, int32_t window);
+                                            int32_t H_kv, int32_t D, int64_t S,
+                                            int32_t window);
 int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q, int64_t q_stride_t,
                          int64_t q_stride_h, const float *lse, const void *k_cache,
                          const uint8_t *k_scales, int64_t num_blocks,

@@ -287,12 +287,12 @@ def test_c_weigh_asks_for_its_workspace():
         assert _weigh(lib, cu=cu) == INVALID
     assert _weigh(lib, cu=(0, 0)) == _lib.CVSA_OK
     cu = (ctypes.c_int32 * 2)(0, 2000)
-    need = lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, W * BS, 0)
+    need = lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, D, W * BS, 0)
     assert need > 0
     for over in (dict(), dict(ws=P[9], bytes=need - 1)):
         assert _weigh(lib, cu=(0, 2000), **over) == _lib.CVSA_ERR_WORKSPACE
     # the last few tokens alone need none
-    assert lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, W * BS, 64) == 0
+    assert lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, D, W * BS, 64) == 0
 
 
 def _evict(lib, **over):
