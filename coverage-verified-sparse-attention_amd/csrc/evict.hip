@@ -9,12 +9,16 @@
 // in order, so that the next call finds them there.  That moves the fewest rows: a
 // token in the middle moves only if its slot is cut off.
 //
-// First launch: a workgroup for each sequence and head finds the m-th largest
-// weight by its bits, 11, 11 and 10 at a time (histograms in LDS), then walks the
-// slots once in order and writes down which old slot each new one gets.  A
-// destination is a source itself only among slots keep - recent .. keep; other
-// workgroups of the launch copy these rows aside.  Second launch: a wave for each
-// page with arrivals, keys and values apart, no order among them.
+// The m-th largest weight is found by its bits, 11, 11 and 10 at a time (histograms
+// in LDS); then a walk over the slots in order writes down which old slot each new
+// one gets.  Rows of up to 16384 slots (by the tables' width): one workgroup for each
+// sequence and head has its weights in registers.  Longer ones: chunks of 8192 slots
+// have a workgroup each, a launch for each histogram and one for the walk, in which
+// every chunk adds up the others' counts (131072 slots, 8 heads: one workgroup each
+// 167 us, so XX us).
+// A destination is a source itself only among slots keep - recent .. keep: other
+// workgroups of the first launch copy these aside.  In the last launch a wave for
+// each page moves its arrivals, keys and values apart, in no order.
 //
 // 8 bits: a page with arrivals gets the largest scale of its tokens' pages; payloads
 // are shifted to it, which rounds only what becomes subnormal.
@@ -39,19 +43,30 @@ struct EvictArgs {
   int B, H_kv, row_bytes;  // of a token and head
   int keep, sinks, recent;
   int32_t *kept;           // [B, H_kv, keep]
-  // Workspace, each [B, H_kv, ...].
-  int32_t *holes;          // [keep]
-  float *moved_weights;    // [keep]
-  uint8_t *moved_scales;   // [2, keep]: bytes of the scales of the sources' pages
-  int32_t *pages;          // [1 + pages]: pages with arrivals, their number first
+  int select_wgs;          // workgroups of a launch before those that copy aside
+  // Workspace, each [B, H_kv, ...].  What slots keep - recent .. keep hold, and the
+  // scales of the pages from the first of these slots' to the last's.
   char *aside;             // [2, recent, row_bytes]
-  unsigned plan_wgs;       // workgroups before those that copy aside
+  float *aside_weights;    // [recent]
+  uint8_t *aside_scales;   // [2, aside_pages]
+  int aside_pages;
+  int32_t *holes;          // [keep] slots to be filled
+  // Short rows.
+  int32_t *pages;          // [1 + pages]: pages with arrivals, their number first
+  // Long rows: of chunks.
+  int chunks;              // of a row of the tables
+  uint16_t *hist;          // [3, chunks, kBins]
+  uint32_t *above;         // [chunks]: weights above the bins chosen so far
+  uint32_t *state;         // [4]: bins and what is still wanted, after passes 1 and 2
+  int32_t *tails;          // [keep]: kept slots from keep - recent on, the last first
+  int32_t *n_holes;        // [1]
 };
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / kWave;
 constexpr int kBins = 2048, kCopies = 4;
-constexpr int kSlots = 4;  // of a thread and step
+constexpr int kChunk = 8 * kEvictThreads;       // slots
+constexpr int kShortRow = 16 * kEvictThreads;
 
 __device__ __forceinline__ int evict_context(const EvictArgs &a, int b) {
   return max(0, min(a.context_lens[b], a.W << a.bs_log2));
@@ -73,7 +88,11 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
 }
 
-// Sums over the workgroup of each wave's total before this one, and in all.
+// Bits that a pass looks at.
+__host__ __device__ constexpr int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__host__ __device__ constexpr int pass_bits(int pass) { return pass == 2 ? 10 : 11; }
+
+// Sums over the workgroup: of the threads before this one, and of all.
 struct EvictScan {
   uint32_t before, all;
 };
@@ -93,35 +112,118 @@ __device__ __forceinline__ EvictScan evict_scan(uint32_t v, uint32_t *s) {
   return r;
 }
 
-__device__ __forceinline__ void evict_copy_aside(const EvictArgs &a) {
-  // A thread for each 16 bytes of keys and of values.
-  const int per_row = a.row_bytes / 16;
-  const int64_t i = (int64_t)(blockIdx.x - a.plan_wgs) * kEvictThreads + threadIdx.x;
-  const int64_t rows = i / per_row;
-  const int part = (int)(i - rows * per_row) * 16;
-  const int64_t bh = rows / a.recent;
-  const int n = (int)(rows - bh * a.recent), b = (int)(bh / a.H_kv), h = (int)(bh % a.H_kv);
-  if (b >= a.B || evict_context(a, b) <= a.keep) return;
-  const int slot = a.keep - a.recent + n, blk = evict_block(a, b, slot);
-  if (blk < 0) return;
-  const int64_t from = evict_row(a, blk, slot, h) + part;
-  char *const to = a.aside + ((bh * 2) * a.recent + n) * a.row_bytes + part;
-  *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(a.k_cache + from);
-  *reinterpret_cast<uint4 *>(to + (int64_t)a.recent * a.row_bytes) =
-      *reinterpret_cast<const uint4 *>(a.v_cache + from);
+// The bin that holds the want-th largest, and how many are above it, from the
+// thread's two bins 2047 - 2 t (n0) and the one below (n1).
+struct EvictBin {
+  uint32_t bin, above;
+};
+__device__ __forceinline__ EvictBin evict_find(uint32_t n0, uint32_t n1, int bits, uint32_t want,
+                                               uint32_t *s_sum, uint32_t *s_bin) {
+  const EvictScan s = evict_scan(n0 + n1, s_sum);
+  if (s.before < want && want <= s.before + n0 + n1) {
+    const bool second = want > s.before + n0;
+    s_bin[0] = (uint32_t)((1 << bits) - 1 - 2 * (int)threadIdx.x - (second ? 1 : 0));
+    s_bin[1] = s.before + (second ? n0 : 0u);
+  }
+  __syncthreads();
+  const EvictBin r = {s_bin[0], s_bin[1]};
+  __syncthreads();
+  return r;
 }
 
+// A thread's share of the slots: four together in each of N steps of the workgroup.
+template <int N>
+struct EvictKeys {
+  uint32_t key[4 * N];
+
+  static __device__ __forceinline__ int slot(int first, int i) {
+    return first + i / 4 * 4 * kEvictThreads + 4 * (int)threadIdx.x + i % 4;
+  }
+  // Slots first .. of a row, those of begin .. end.
+  __device__ __forceinline__ void load(const float *w, int first, int begin, int end) {
+    float v[4 * N];
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      const int j = slot(first, i);
+      v[i] = j >= begin && j < end ? w[j] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) key[i] = weight_key(v[i]);
+  }
+  // Counts of those whose bits `known` are `prefix`, by the next ones, into hist.
+  __device__ __forceinline__ void count(uint32_t *hist, int pass, uint32_t known, uint32_t prefix,
+                                        int first, int begin, int end) const {
+    const uint32_t mask = (1u << pass_bits(pass)) - 1;
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      const int j = slot(first, i);
+      if (j >= begin && j < end && (key[i] & known) == prefix)
+        atomicAdd(&hist[key[i] >> pass_shift(pass) & mask], 1u);
+    }
+  }
+};
+
+__device__ __forceinline__ void evict_clear(uint32_t (*hist)[kBins]) {
+  for (int i = threadIdx.x; i < kCopies * kBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
+  __syncthreads();
+}
+// A thread's two bins from the top, over the copies.
+__device__ __forceinline__ void evict_bins(const uint32_t (*hist)[kBins], int bits, uint32_t &n0,
+                                           uint32_t &n1) {
+  const int top = (1 << bits) - 1 - 2 * (int)threadIdx.x;
+  n0 = n1 = 0;
+  if (top <= 0) return;
+#pragma unroll
+  for (int c = 0; c < kCopies; ++c) {
+    n0 += hist[c][top];
+    n1 += hist[c][top - 1];
+  }
+}
+
+__device__ __forceinline__ void evict_copy_aside(const EvictArgs &a) {
+  // A thread for each 16 bytes of keys and of values, then one for each page.
+  const int per_row = a.row_bytes / 16, front = a.keep - a.recent;
+  const int64_t n_bh = (int64_t)a.B * a.H_kv, n_rows = n_bh * a.recent;
+  int64_t i = (int64_t)((int)blockIdx.x - a.select_wgs) * kEvictThreads + threadIdx.x;
+  if (i < n_rows * per_row) {
+    const int64_t row = i / per_row, bh = row / a.recent;
+    const int part = (int)(i - row * per_row), n = (int)(row - bh * a.recent);
+    const int b = (int)(bh / a.H_kv), h = (int)(bh % a.H_kv);
+    if (evict_context(a, b) <= a.keep) return;
+    const int slot = front + n, blk = evict_block(a, b, slot);
+    if (part == 0) a.aside_weights[row] = a.weights[bh * a.S + slot];
+    if (blk < 0) return;
+    const int64_t from = evict_row(a, blk, slot, h) + part * 16;
+    char *const to = a.aside + ((bh * 2) * a.recent + n) * a.row_bytes + part * 16;
+    *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(a.k_cache + from);
+    *reinterpret_cast<uint4 *>(to + (int64_t)a.recent * a.row_bytes) =
+        *reinterpret_cast<const uint4 *>(a.v_cache + from);
+    return;
+  }
+  i -= n_rows * per_row;
+  if (!a.k_scales || i >= n_bh * a.aside_pages) return;
+  const int64_t bh = i / a.aside_pages;
+  const int n = (int)(i - bh * a.aside_pages), b = (int)(bh / a.H_kv), h = (int)(bh % a.H_kv);
+  if (evict_context(a, b) <= a.keep) return;
+  const int blk = evict_block(a, b, ((front >> a.bs_log2) + n) << a.bs_log2);
+  if (blk < 0) return;
+  a.aside_scales[bh * 2 * a.aside_pages + n] = a.k_scales[(int64_t)blk * a.H_kv + h];
+  a.aside_scales[(bh * 2 + 1) * a.aside_pages + n] = a.v_scales[(int64_t)blk * a.H_kv + h];
+}
+
+// Short rows: old slots of the new ones, and the pages with arrivals; N steps of 4096
+// slots.
+template <int N>
 __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictArgs a) {
-  if (blockIdx.x >= a.plan_wgs) {
+  if ((int)blockIdx.x >= a.select_wgs) {
     evict_copy_aside(a);
     return;
   }
   __shared__ uint32_t s_hist[kCopies][kBins];
-  __shared__ uint32_t s_sum[kEvictWaves];
-  __shared__ uint32_t s_bin, s_above;
-  const int tid = threadIdx.x;
+  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2], s_step[N][kEvictWaves];
+  const int tid = threadIdx.x, wave = tid >> 6;
   const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / a.H_kv), h = (int)(bh % a.H_kv);
+  const int b = (int)(bh / a.H_kv);
   const int ctx = evict_context(a, b);
   float *const w = a.weights + bh * a.S;
   int32_t *const kept = a.kept + bh * a.keep, *const holes = a.holes + bh * a.keep;
@@ -133,154 +235,354 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
     return;
   }
   const int front = a.keep - a.recent, back = ctx - a.recent;
-  uint32_t want = (uint32_t)(front - a.sinks);  // of the middle, which has more
+  EvictKeys<N> keys;
+  keys.load(w, 0, a.sinks, back);
 
-  // The want-th largest: `threshold`, of whose equals the first `want` stay.
-  uint32_t threshold = 0xffffffffu, known = 0;
-  if (want == 0) {
-    // None of the middle: nothing is above this, and none of its equals stays.
-  } else {
+  // The want-th largest of the middle: `threshold`, of whose equals the first `want`
+  // stay.  None wanted: nothing is above this, and none of its equals stays.
+  uint32_t want = (uint32_t)(front - a.sinks), threshold = 0xffffffffu;
+  if (want > 0) {
+    uint32_t known = 0;
     threshold = 0;
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kCopies * kBins; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+      evict_clear(s_hist);
+      keys.count(s_hist[wave % kCopies], pass, known, threshold, 0, a.sinks, back);
       __syncthreads();
-      uint32_t *const hist = s_hist[(tid >> 6) % kCopies];
-      for (int j = a.sinks + tid; j < back; j += kEvictThreads) {
-        const uint32_t k = weight_key(w[j]);
-        if ((k & known) == threshold) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
-      }
-      __syncthreads();
-      // Bins from the largest on, two a thread.
-      const int top = (1 << bits) - 1 - 2 * tid;
-      uint32_t n0 = 0, n1 = 0;
-      if (top > 0) {
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-          n0 += s_hist[c][top];
-          n1 += s_hist[c][top - 1];
-        }
-      }
-      const EvictScan s = evict_scan(n0 + n1, s_sum);
-      if (s.before < want && want <= s.before + n0 + n1) {
-        const bool second = want > s.before + n0;
-        s_bin = (uint32_t)(second ? top - 1 : top);
-        s_above = s.before + (second ? n0 : 0u);
-      }
-      __syncthreads();
-      threshold |= s_bin << shift;
-      known |= ((1u << bits) - 1) << shift;
-      want -= s_above;
-      __syncthreads();
+      uint32_t n0, n1;
+      evict_bins(s_hist, pass_bits(pass), n0, n1);
+      const EvictBin at = evict_find(n0, n1, pass_bits(pass), want, s_sum, s_bin);
+      threshold |= at.bin << pass_shift(pass);
+      known |= ((1u << pass_bits(pass)) - 1) << pass_shift(pass);
+      want -= at.above;
     }
   }
 
   // The slots in order: the kept ones below `front` stay, the others are holes; the
-  // kept ones behind fill them.
+  // kept ones behind fill them.  Counts of larger and (high half) equal weights.
   for (int j = tid; j < a.sinks; j += kEvictThreads) kept[j] = j;
   for (int j = tid; j < a.recent; j += kEvictThreads) kept[front + j] = back + j;
-  uint32_t above = 0, equal = 0;  // before the step
-  uint32_t stay = 0;              // kept ones below front
-  auto walk = [&](int begin, int end, bool tail) {
-    for (int j0 = begin; j0 < end; j0 += kEvictThreads * kSlots) {
-      const int first = j0 + tid * kSlots;
-      uint32_t key[kSlots];
-      uint32_t count = 0;
+  uint32_t count[N], incl[N];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        key[i] = first + i < end ? weight_key(w[first + i]) : 0u;
-        if (first + i < end)
-          count += (key[i] > threshold ? 1u : 0u) + (key[i] == threshold ? 0x10000u : 0u);
-      }
-      const EvictScan s = evict_scan(count, s_sum);
-      uint32_t gt = above + (s.before & 0xffffu), eq = equal + (s.before >> 16);
+  for (int n = 0; n < N; ++n) {
+    count[n] = 0;
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        const int slot = first + i;
-        if (slot >= end) break;
-        const bool keep = key[i] > threshold || (key[i] == threshold && eq < want);
-        const uint32_t rank = gt + min(eq, want);  // kept ones before
-        if (!tail) {
-          if (keep) kept[slot] = slot;
-          else holes[(uint32_t)(slot - a.sinks) - rank] = slot;
-        } else if (keep) {
-          kept[holes[rank - stay]] = slot;
-        }
-        gt += key[i] > threshold ? 1u : 0u;
-        eq += key[i] == threshold ? 1u : 0u;
-      }
-      above += s.all & 0xffffu;
-      equal += s.all >> 16;
+    for (int i = 4 * n; i < 4 * n + 4; ++i) {
+      const int j = keys.slot(0, i);
+      if (j >= a.sinks && j < back)
+        count[n] += keys.key[i] > threshold ? 1u : keys.key[i] == threshold ? 0x10000u : 0u;
     }
-  };
-  walk(a.sinks, front, false);
-  stay = above + min(equal, want);
+    incl[n] = wave_incl_scan_u32(count[n]);
+    if ((tid & 63) == 63) s_step[n][wave] = incl[n];
+  }
   __syncthreads();
-  walk(front, back, true);
-  __syncthreads();
-
-  // What moves: its weight and the scales of where it comes from.
-  float *const moved = a.moved_weights + bh * a.keep;
-  uint8_t *const scales = a.moved_scales + bh * 2 * a.keep;
-  for (int j = tid; j < a.keep; j += kEvictThreads) {
-    const int src = kept[j];
-    if (src == j) continue;
-    moved[j] = w[src];
-    if (a.k_scales) {
-      const int blk = evict_block(a, b, src);
-      scales[j] = blk < 0 ? 0 : a.k_scales[(int64_t)blk * a.H_kv + h];
-      scales[a.keep + j] = blk < 0 ? 0 : a.v_scales[(int64_t)blk * a.H_kv + h];
+  // Kept ones before each of the thread's slots, and below front.
+  uint32_t above = 0, equal = 0, rank[4 * N], stay = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t gt = above, eq = equal;
+#pragma unroll
+    for (int v = 0; v < kEvictWaves; ++v) {
+      const uint32_t x = s_step[n][v];
+      gt += v < wave ? x & 0xffffu : 0u;
+      eq += v < wave ? x >> 16 : 0u;
+      above += x & 0xffffu;
+      equal += x >> 16;
+    }
+    gt += (incl[n] - count[n]) & 0xffffu;
+    eq += (incl[n] - count[n]) >> 16;
+#pragma unroll
+    for (int i = 4 * n; i < 4 * n + 4; ++i) {
+      const int j = keys.slot(0, i);
+      const bool in = j >= a.sinks && j < back, larger = in && keys.key[i] > threshold;
+      const bool same = in && keys.key[i] == threshold;
+      rank[i] = gt + min(eq, want);
+      const bool keep = larger || (same && eq < want);
+      if (j == front) s_bin[0] = rank[i];  // the next slot after those that may stay
+      if (in && j < front) {
+        if (keep) kept[j] = j;
+        else holes[(uint32_t)(j - a.sinks) - rank[i]] = j;
+      }
+      if (!keep || j < front) rank[i] = 0xffffffffu;
+      gt += larger ? 1u : 0u;
+      eq += same ? 1u : 0u;
     }
   }
   __syncthreads();
-  for (int j = tid; j < a.keep; j += kEvictThreads)
-    if (kept[j] != j) w[j] = moved[j];
-  // Pages with arrivals.
+  stay = s_bin[0];
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i)
+    if (rank[i] != 0xffffffffu) kept[holes[rank[i] - stay]] = keys.slot(0, i);
+  __syncthreads();
+
+  // Pages with arrivals: those of holes, and from front on all.
+  uint32_t *const flags = &s_hist[0][0];
+  static_assert(kCopies * kBins >= kShortRow / 8, "a flag for each page");
+  for (int p = tid; p < n_pages; p += kEvictThreads)
+    flags[p] = a.recent > 0 && p >= front >> a.bs_log2 ? 1u : 0u;
+  __syncthreads();
+  const int n_holes = front - a.sinks - (int)stay;
+  for (int n = tid; n < n_holes; n += kEvictThreads) flags[holes[n] >> a.bs_log2] = 1u;
+  __syncthreads();
   int listed = 0;
   for (int p0 = 0; p0 < n_pages; p0 += kEvictThreads) {
     const int p = p0 + tid;
-    bool any = false;
-    if (p < n_pages) {
-      const int end = min((p + 1) << a.bs_log2, a.keep);
-      for (int j = p << a.bs_log2; j < end; ++j) any = any || kept[j] != j;
-    }
-    const EvictScan s = evict_scan(any ? 1u : 0u, s_sum);
+    const uint32_t any = p < n_pages ? flags[p] : 0u;
+    const EvictScan s = evict_scan(any, s_sum);
     if (any) pages[1 + listed + s.before] = p;
     listed += (int)s.all;
   }
   if (tid == 0) pages[0] = listed;
 }
 
-// Rows of a page's arrivals, and in 8 bits the page's scale and its other rows.
-// Keys by even waves, values by odd ones.
-template <bool F8>
+// Long rows: the bins that pass `pass` chooses from the histograms of all chunks.
+__device__ __forceinline__ EvictBin evict_choose(const EvictArgs &a, int64_t bh, int pass,
+                                                 int chunks, uint32_t want, uint32_t *s_sum,
+                                                 uint32_t *s_bin) {
+  const int top = (1 << pass_bits(pass)) - 1 - 2 * (int)threadIdx.x;
+  uint32_t n0 = 0, n1 = 0;
+  if (top > 0) {
+    const uint16_t *const h = a.hist + (bh * 3 + pass) * (int64_t)a.chunks * kBins + top - 1;
+    for (int c0 = 0; c0 < chunks; c0 += 16) {
+      uint32_t two[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        two[c] = *reinterpret_cast<const uint32_t *>(h + (int64_t)min(c0 + c, chunks - 1) * kBins);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        if (c0 + c >= chunks) two[c] = 0;
+        n0 += two[c] >> 16;
+        n1 += two[c] & 0xffffu;
+      }
+    }
+  }
+  return evict_find(n0, n1, pass_bits(pass), want, s_sum, s_bin);
+}
+
+// A chunk's histogram of the bits of a pass, of the weights in the bins chosen before.
+template <int PASS>
+__global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictArgs a) {
+  if (PASS == 0 && (int)blockIdx.x >= a.select_wgs) {
+    evict_copy_aside(a);
+    return;
+  }
+  __shared__ uint32_t s_hist[kCopies][kBins];
+  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2];
+  const int64_t bh = blockIdx.x / a.chunks;
+  const int chunk = (int)(blockIdx.x % a.chunks), first = chunk * kChunk;
+  const int ctx = evict_context(a, (int)(bh / a.H_kv));
+  const int front = a.keep - a.recent, back = ctx - a.recent;
+  if (ctx <= a.keep || first >= back || front == a.sinks) return;
+  EvictKeys<2> keys;
+  keys.load(a.weights + bh * a.S, first, a.sinks, back);
+  uint32_t prefix = 0, known = 0;
+  if constexpr (PASS > 0) {
+    uint32_t *const state = a.state + bh * 4;
+    uint32_t want = (uint32_t)(front - a.sinks);
+    if constexpr (PASS == 2) {
+      prefix = state[0] << pass_shift(0);
+      known = ((1u << pass_bits(0)) - 1) << pass_shift(0);
+      want = state[1];
+    }
+    const EvictBin at = evict_choose(a, bh, PASS - 1, (back + kChunk - 1) / kChunk, want, s_sum,
+                                     s_bin);
+    if (chunk == 0 && threadIdx.x == 0) {
+      state[2 * PASS - 2] = at.bin;
+      state[2 * PASS - 1] = want - at.above;
+    }
+    // The chunk's weights above that bin, of those in the bins before.
+    const uint32_t mask = (1u << pass_bits(PASS - 1)) - 1;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = keys.slot(first, i);
+      if (j >= a.sinks && j < back && (keys.key[i] & known) == prefix &&
+          (keys.key[i] >> pass_shift(PASS - 1) & mask) > at.bin)
+        ++n;
+    }
+    const uint32_t all = evict_scan(n, s_sum).all;
+    uint32_t *const above = a.above + bh * a.chunks + chunk;
+    if (threadIdx.x == 0) *above = PASS == 1 ? all : *above + all;
+    prefix |= at.bin << pass_shift(PASS - 1);
+    known |= mask << pass_shift(PASS - 1);
+  }
+  evict_clear(s_hist);
+  keys.count(s_hist[(threadIdx.x >> 6) % kCopies], PASS, known, prefix, first, a.sinks, back);
+  __syncthreads();
+  uint32_t n0, n1;
+  evict_bins(s_hist, pass_bits(PASS), n0, n1);
+  const int top = (1 << pass_bits(PASS)) - 1 - 2 * (int)threadIdx.x;
+  if (top > 0)  // of at most 8192 slots: 16 bits
+    *reinterpret_cast<uint32_t *>(
+        a.hist + ((bh * 3 + PASS) * (int64_t)a.chunks + chunk) * kBins + top - 1) = n0 << 16 | n1;
+}
+
+// A chunk's slots in order: where the kept ones are, holes and what fills them.  A
+// hole n is -2 - n in kept.
+__global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictArgs a) {
+  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2], s_before[2][kEvictWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t bh = blockIdx.x / a.chunks;
+  const int chunk = (int)(blockIdx.x % a.chunks), first = chunk * kChunk;
+  const int ctx = evict_context(a, (int)(bh / a.H_kv));
+  const int front = a.keep - a.recent, back = ctx - a.recent;
+  if (ctx <= a.keep || first >= back) return;
+  EvictKeys<2> keys;
+  keys.load(a.weights + bh * a.S, first, a.sinks, back);
+  const uint32_t m = (uint32_t)(front - a.sinks);  // kept ones of the middle
+  uint32_t threshold = 0xffffffffu, want = 0;
+  uint32_t gt = 0, eq = 0;  // larger and equal ones in the chunks before
+  if (m > 0) {
+    const uint32_t *const state = a.state + bh * 4;
+    want = state[3];
+    const EvictBin at = evict_choose(a, bh, 2, (back + kChunk - 1) / kChunk, want, s_sum, s_bin);
+    want -= at.above;
+    threshold = state[0] << pass_shift(0) | state[2] << pass_shift(1) | at.bin;
+    for (int c = wave; c < chunk; c += kEvictWaves) {
+      const uint16_t *const h = a.hist + ((bh * 3 + 2) * (int64_t)a.chunks + c) * kBins;
+      static_assert(1 << pass_bits(2) == 16 * kWave, "16 bins of a lane");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int bin = (i * kWave + lane) * 8;
+        const uint4 v = *reinterpret_cast<const uint4 *>(h + bin);
+        const uint32_t two[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t n = two[k / 2] >> (k % 2 * 16) & 0xffffu;
+          gt += (uint32_t)(bin + k) > at.bin ? n : 0u;
+          eq += (uint32_t)(bin + k) == at.bin ? n : 0u;
+        }
+      }
+      if (lane == 0) gt += a.above[bh * a.chunks + c];
+    }
+    gt = wave_sum_u32(gt);
+    eq = wave_sum_u32(eq);
+    if (lane == 0) {
+      s_before[0][wave] = gt;
+      s_before[1][wave] = eq;
+    }
+    __syncthreads();
+    gt = eq = 0;
+    for (int v = 0; v < kEvictWaves; ++v) {
+      gt += s_before[0][v];
+      eq += s_before[1][v];
+    }
+  }
+  int32_t *const kept = a.kept + bh * a.keep, *const holes = a.holes + bh * a.keep;
+  int32_t *const tails = a.tails + bh * a.keep;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    uint32_t count = 0;
+#pragma unroll
+    for (int i = 4 * n; i < 4 * n + 4; ++i) {
+      const int j = keys.slot(first, i);
+      if (j >= a.sinks && j < back)
+        count += keys.key[i] > threshold ? 1u : keys.key[i] == threshold ? 0x10000u : 0u;
+    }
+    const EvictScan s = evict_scan(count, s_sum);
+    uint32_t g = gt + (s.before & 0xffffu), e = eq + (s.before >> 16);
+#pragma unroll
+    for (int i = 4 * n; i < 4 * n + 4; ++i) {
+      const int j = keys.slot(first, i);
+      if (j < a.sinks || j >= back) continue;
+      const bool larger = keys.key[i] > threshold, same = keys.key[i] == threshold;
+      const uint32_t rank = g + min(e, want);
+      const bool keep = larger || (same && e < want);
+      if (j == front) a.n_holes[bh] = (int32_t)(m - rank);
+      if (j < front) {
+        const int32_t hole = (int32_t)((uint32_t)(j - a.sinks) - rank);
+        kept[j] = keep ? j : -2 - hole;
+        if (!keep) holes[hole] = j;
+      } else if (keep) {
+        tails[m - 1 - rank] = j;
+      }
+      g += larger ? 1u : 0u;
+      e += same ? 1u : 0u;
+    }
+    gt += s.all & 0xffffu;
+    eq += s.all >> 16;
+  }
+}
+
+// Rows of a page's arrivals and their weights, and in 8 bits the page's scale and its
+// other rows.  Keys (and weights) by even waves, values by odd ones.
+template <bool F8, bool LONG>
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int wgs_each) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t bh = blockIdx.x / wgs_each;
-  const int b = (int)(bh / a.H_kv), h = (int)(bh % a.H_kv);
+  // Heads vary fastest: they move the same tokens often, whose rows lie side by side.
+  const int h = (int)(blockIdx.x % a.H_kv), wg = (int)(blockIdx.x / a.H_kv % wgs_each);
+  const int b = (int)(blockIdx.x / a.H_kv / wgs_each);
+  const int64_t bh = (int64_t)b * a.H_kv + h;
   const bool values = wave & 1;
   const int bs = 1 << a.bs_log2, n_pages = (a.keep + bs - 1) >> a.bs_log2;
-  const int32_t *const kept = a.kept + bh * a.keep;
-  const int32_t *const pages = a.pages + bh * (1 + n_pages);
-  const int listed = pages[0];
+  const int ctx = LONG ? evict_context(a, b) : 0, front = a.keep - a.recent;
+  const int last_page = (a.keep - 1) >> a.bs_log2;
+  int32_t *const kept = a.kept + bh * a.keep;
+  float *const w = a.weights + bh * a.S;
+  const int32_t *const pages = LONG ? nullptr : a.pages + bh * (1 + n_pages);
+  const int listed = LONG ? n_pages : pages[0];
   char *const cache = values ? a.v_cache : a.k_cache;
   const char *const aside = a.aside + (bh * 2 + values) * a.recent * (int64_t)a.row_bytes;
   const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
   const int part = lane % per_row * 16, sub = lane / per_row;
-  for (int i = (int)(blockIdx.x % wgs_each) * 2 + wave / 2; i < listed; i += wgs_each * 2) {
-    const int page = pages[1 + i], slot0 = page << a.bs_log2;
-    const int blk = evict_block(a, b, slot0);
-    if (blk < 0) continue;
+  int i = wg * 2 + wave / 2;
+  // Looked up before it is known whether there is one: one wait for both.
+  int next = LONG ? 0 : pages[1 + min(i, n_pages - 1)];
+  for (; i < listed; i += wgs_each * 2) {
+    const int page = LONG ? i : next, slot0 = page << a.bs_log2;
+    if (!LONG) next = pages[1 + min(i + wgs_each * 2, n_pages - 1)];
     const int count = min(bs, a.keep - slot0);
-    int byte = 0, old = 0;
+    const int blk = LONG && ctx <= a.keep ? -1 : evict_block(a, b, slot0);
+    // The lane's slots: where they come from (the place itself: it stays), the blocks.
+    int src[2], from[2];
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = lane + 64 * n, slot = slot0 + r;
+      src[n] = slot;
+      from[n] = blk;
+      if (r >= count) continue;
+      if constexpr (LONG) {
+        if (ctx <= a.keep) {
+          if (!values) kept[slot] = slot < ctx ? slot : -1;
+          continue;
+        }
+        if (slot >= front) {
+          src[n] = slot + ctx - a.keep;
+        } else if (slot >= a.sinks) {
+          const int at = kept[slot];  // the other wave may have put the answer there
+          src[n] = at >= 0 ? at : (a.tails + bh * a.keep)[a.n_holes[bh] - 1 - (-2 - at)];
+        }
+        if (!values && (slot < a.sinks || slot >= front || src[n] != slot)) kept[slot] = src[n];
+      } else {
+        src[n] = kept[slot];
+      }
+      if (src[n] == slot) continue;
+      any = true;
+      from[n] = evict_block(a, b, src[n]);
+      if (!values)
+        w[slot] = src[n] < a.keep ? a.aside_weights[bh * a.recent + src[n] - front] : w[src[n]];
+    }
+    if (blk < 0 || __ballot(any) == 0) continue;
+    int byte = 0, old = 0, scale[2] = {0, 0};  // scales' bytes: new, the page's, the rows'
     if constexpr (F8) {
-      const uint8_t *const from = a.moved_scales + (bh * 2 + values) * a.keep;
-      uint8_t *const at = (values ? a.v_scales : a.k_scales) + (int64_t)blk * a.H_kv + h;
+      uint8_t *const scales = values ? a.v_scales : a.k_scales;
+      const uint8_t *const were = a.aside_scales + (bh * 2 + values) * a.aside_pages -
+                                  (front >> a.bs_log2);
+      uint8_t *const at = scales + (int64_t)blk * a.H_kv + h;
       old = *at;
       uint32_t top = 0;
-      for (int r = lane; r < count; r += 64)
-        top = max(top, kept[slot0 + r] == slot0 + r ? (uint32_t)old : (uint32_t)from[slot0 + r]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int r = lane + 64 * n, p = src[n] >> a.bs_log2;
+        if (r >= count) continue;
+        // Pages that get arrivals themselves may have another scale by now.
+        scale[n] = src[n] == slot0 + r ? old
+                   : from[n] < 0       ? 0
+                   : p <= last_page    ? were[p]
+                                       : scales[(int64_t)from[n] * a.H_kv + h];
+        top = max(top, (uint32_t)scale[n]);
+      }
       byte = (int)wave_max_u32(top);
       if (lane == 0 && byte != old) *at = (uint8_t)byte;
     }
@@ -293,26 +595,23 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
       unrolled<kBatch>([&](auto n) {
         constexpr int g = decltype(n)::value;
         const int r = r0 + g * rows + sub, slot = slot0 + r;
+        const bool high = r >= 64;
+        const int x = __shfl(src[0], r & 63, 64), x1 = __shfl(src[1], r & 63, 64);
+        const int y = __shfl(from[0], r & 63, 64), y1 = __shfl(from[1], r & 63, 64);
+        const int s = high ? x1 : x, blk_s = high ? y1 : y;
         v[g] = make_uint4(0, 0, 0, 0);
-        write[g] = false;
         shift[g] = 0;
-        if (r >= count) return;
-        const int src = kept[slot];
-        const char *p = nullptr;
-        if (src == slot) {  // stays; its payload, where the scale has changed
-          if (!F8 || byte == old) return;
-          shift[g] = old - byte;
-          p = cache + evict_row(a, blk, slot, h);
-        } else {
-          const int from = evict_block(a, b, src);
-          if (from < 0) return;
-          if constexpr (F8)
-            shift[g] = a.moved_scales[(bh * 2 + values) * a.keep + slot] - byte;
-          p = src < a.keep ? aside + (int64_t)(src - (a.keep - a.recent)) * a.row_bytes
-                           : cache + evict_row(a, from, src, h);
+        if constexpr (F8) {
+          const int z = __shfl(scale[0], r & 63, 64), z1 = __shfl(scale[1], r & 63, 64);
+          shift[g] = (high ? z1 : z) - byte;
         }
+        // One that stays, only where its payload changes with the scale.
+        write[g] = r < count && (s != slot ? blk_s >= 0 : F8 && byte != old);
+        if (!write[g]) return;
+        const char *const p =
+            s != slot && s < a.keep ? aside + (int64_t)(s - front) * a.row_bytes
+                                    : cache + evict_row(a, blk_s, s, h);
         v[g] = *reinterpret_cast<const uint4 *>(p + part);
-        write[g] = true;
       });
       unrolled<kBatch>([&](auto n) {
         constexpr int g = decltype(n)::value;
@@ -328,21 +627,37 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
 }
 
 struct EvictPlan {
-  size_t holes, weights, scales, pages, aside, bytes;
+  bool long_rows;
+  int chunks, aside_pages;
+  size_t aside, aside_weights, aside_scales, holes, pages, hist, above, state, tails, n_holes;
+  size_t bytes;
 };
 
-static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int keep, int recent, bool f8) {
+// keys: of a row of the tables.
+static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int64_t keys, int keep, int recent,
+                            bool f8) {
   EvictPlan p = {};
   auto take = [&](size_t n) {
     const size_t at = p.bytes;
     p.bytes += (n + 255) / 256 * 256;
     return at;
   };
-  p.holes = take((size_t)bh * keep * 4);
-  p.weights = take((size_t)bh * keep * 4);
-  p.scales = take(f8 ? (size_t)bh * keep * 2 : 0);
-  p.pages = take((size_t)bh * (1 + (keep + bs - 1) / bs) * 4);
+  p.long_rows = keys > kShortRow;
+  p.chunks = (int)((keys + kChunk - 1) / kChunk);
+  p.aside_pages = std::max(0, (keep - 1) / bs - (keep - recent) / bs + 1);
   p.aside = take((size_t)bh * 2 * recent * row_bytes);
+  p.aside_weights = take((size_t)bh * recent * 4);
+  p.aside_scales = take(f8 ? (size_t)bh * 2 * p.aside_pages : 0);
+  p.holes = take((size_t)bh * keep * 4);
+  if (p.long_rows) {
+    p.hist = take((size_t)bh * 3 * p.chunks * kBins * 2);
+    p.above = take((size_t)bh * p.chunks * 4);
+    p.state = take((size_t)bh * 16);
+    p.tails = take((size_t)bh * keep * 4);
+    p.n_holes = take((size_t)bh * 4);
+  } else {
+    p.pages = take((size_t)bh * (1 + (keep + bs - 1) / bs) * 4);
+  }
   return p;
 }
 
@@ -358,11 +673,14 @@ static bool evict_sizes_ok(int32_t B, int32_t H_kv, int32_t D, int32_t block_siz
 using namespace cvsa;
 
 extern "C" size_t cvsa_evict_tokens_workspace_bytes(int32_t B, int32_t H_kv, int32_t D,
-                                                    int32_t block_size, int32_t cache_bits,
-                                                    int32_t keep, int32_t sinks, int32_t recent) {
-  if (!evict_sizes_ok(B, H_kv, D, block_size, keep, sinks, recent)) return 0;
-  return plan_evict((int64_t)B * H_kv, D * cache_bits / 8, block_size, keep, recent,
-                    cache_bits == 8)
+                                                    int32_t block_size, int32_t W,
+                                                    int32_t cache_bits, int32_t keep,
+                                                    int32_t sinks, int32_t recent) {
+  if (!evict_sizes_ok(B, H_kv, D, block_size, keep, sinks, recent) || W <= 0 ||
+      W > kMaxPagesWide || (cache_bits != 8 && cache_bits != 16))
+    return 0;
+  return plan_evict((int64_t)B * H_kv, D * cache_bits / 8, block_size, (int64_t)W * block_size,
+                    keep, recent, cache_bits == 8)
       .bytes;
 }
 
@@ -394,13 +712,18 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
                "evict_tokens: caches must be 16-byte aligned");
   const int64_t bh = (int64_t)B * H_kv;
   const int row_bytes = D * (k_scales ? 1 : 2);
-  const EvictPlan p = plan_evict(bh, row_bytes, block_size, keep, recent, k_scales != nullptr);
+  // More than the tables hold keeps all.
+  const int64_t keys = (int64_t)W * block_size;
+  const EvictPlan p = plan_evict(bh, row_bytes, block_size, keys, keep, recent,
+                                 k_scales != nullptr);
   CVSA_REQUIRE(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
                CVSA_ERR_WORKSPACE,
                "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", p.bytes);
-  const int64_t aside = bh * recent * (row_bytes / 16);
-  CVSA_REQUIRE(aside / kEvictThreads + bh < (1LL << 31) - 1, CVSA_ERR_UNSUPPORTED,
-               "evict_tokens: too many recent tokens");
+  const int64_t aside = bh * recent * (row_bytes / 16) + (k_scales ? bh * p.aside_pages : 0);
+  const int64_t aside_wgs = (aside + kEvictThreads - 1) / kEvictThreads;
+  const int64_t select_wgs = p.long_rows ? bh * p.chunks : bh;
+  CVSA_REQUIRE(aside_wgs + select_wgs < (1LL << 31), CVSA_ERR_UNSUPPORTED,
+               "evict_tokens: too many sequences, heads or recent tokens");
   EvictArgs a = {};
   a.weights = weights; a.S = S;
   a.k_cache = (char *)k_cache; a.v_cache = (char *)v_cache;
@@ -413,21 +736,40 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
   a.keep = keep; a.sinks = sinks; a.recent = recent;
   a.kept = kept;
   char *const ws = (char *)workspace;
-  a.holes = (int32_t *)(ws + p.holes);
-  a.moved_weights = (float *)(ws + p.weights);
-  a.moved_scales = (uint8_t *)(ws + p.scales);
-  a.pages = (int32_t *)(ws + p.pages);
   a.aside = ws + p.aside;
-  a.plan_wgs = (unsigned)bh;
+  a.aside_weights = (float *)(ws + p.aside_weights);
+  a.aside_scales = (uint8_t *)(ws + p.aside_scales);
+  a.aside_pages = p.aside_pages;
+  a.holes = (int32_t *)(ws + p.holes);
+  a.pages = (int32_t *)(ws + p.pages);
+  a.chunks = p.chunks;
+  a.hist = (uint16_t *)(ws + p.hist);
+  a.above = (uint32_t *)(ws + p.above);
+  a.state = (uint32_t *)(ws + p.state);
+  a.tails = (int32_t *)(ws + p.tails);
+  a.n_holes = (int32_t *)(ws + p.n_holes);
+  a.select_wgs = (int)select_wgs;
   const hipStream_t s = (hipStream_t)stream;
-  const unsigned wgs = (unsigned)(bh + (aside + kEvictThreads - 1) / kEvictThreads);
-  hipLaunchKernelGGL(evict_plan_kernel, dim3(wgs), dim3(kEvictThreads), 0, s, a);
-  // Two pages at once in a workgroup; enough of them to fill the GPU, or one for
-  // each two pages.
-  const int n_pages = (keep + block_size - 1) / block_size;
-  const int each = (int)std::max<int64_t>(1, std::min<int64_t>((n_pages + 1) / 2, 4096 / bh));
+  const dim3 select((unsigned)select_wgs), first((unsigned)(select_wgs + aside_wgs));
+  const dim3 threads(kEvictThreads);
+  if (p.long_rows) {
+    hipLaunchKernelGGL(evict_count_kernel<0>, first, threads, 0, s, a);
+    hipLaunchKernelGGL(evict_count_kernel<1>, select, threads, 0, s, a);
+    hipLaunchKernelGGL(evict_count_kernel<2>, select, threads, 0, s, a);
+    hipLaunchKernelGGL(evict_walk_kernel, select, threads, 0, s, a);
+  } else if (keys <= 4 * kEvictThreads) {
+    hipLaunchKernelGGL(evict_plan_kernel<1>, first, threads, 0, s, a);
+  } else if (keys <= 8 * kEvictThreads) {
+    hipLaunchKernelGGL(evict_plan_kernel<2>, first, threads, 0, s, a);
+  } else {
+    hipLaunchKernelGGL(evict_plan_kernel<4>, first, threads, 0, s, a);
+  }
+  // Two pages at once in a workgroup, in turn past 8192 workgroups.
+  const int64_t n_pages = (keep + block_size - 1) / block_size;
+  const int each = (int)std::max<int64_t>(1, std::min<int64_t>((n_pages + 1) / 2, 8192 / bh));
   const dim3 grid((unsigned)(bh * each));
-  if (k_scales) hipLaunchKernelGGL(evict_move_kernel<true>, grid, dim3(256), 0, s, a, each);
-  else hipLaunchKernelGGL(evict_move_kernel<false>, grid, dim3(256), 0, s, a, each);
+  auto move = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, each); };
+  if (p.long_rows) k_scales ? move(evict_move_kernel<true, true>) : move(evict_move_kernel<false, true>);
+  else k_scales ? move(evict_move_kernel<true, false>) : move(evict_move_kernel<false, false>);
   return cvsa_host::check_launch("evict_tokens");
 }

@@ -154,7 +154,7 @@ SIGNATURES = {
     "cvsa_add_key_weights": (ctypes.c_int, [
         _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i32, _i32, _i32, _i32,
         _i32, _i32, _f32, _i32, _i32, _p, _sz, _p]),
-    "cvsa_evict_tokens_workspace_bytes": (_sz, [_i32] * 8),
+    "cvsa_evict_tokens_workspace_bytes": (_sz, [_i32] * 9),
     "cvsa_evict_tokens": (ctypes.c_int, [
         _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _i32, _p, _i32, _i32, _i32, _i32, _i32, _i32,
         _i32, _p, _p, _sz, _p]),

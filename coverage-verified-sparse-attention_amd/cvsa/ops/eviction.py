@@ -125,7 +125,7 @@ def evict_tokens(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         raise ValueError(f"{who}: {sinks} first and {recent} last tokens of {keep} kept")
     kept = torch.empty(B, H_kv, keep, device=dev, dtype=torch.int32)
     L = _lib.load()
-    need = L.cvsa_evict_tokens_workspace_bytes(B, H_kv, D, block_size,
+    need = L.cvsa_evict_tokens_workspace_bytes(B, H_kv, D, block_size, W,
                                                16 if k_scales is None else 8, keep, sinks, recent)
     ws = torch.empty(need, device=dev, dtype=torch.uint8)
     _call(dev, who, L.cvsa_evict_tokens, weights.data_ptr(), S, k_cache.data_ptr(),

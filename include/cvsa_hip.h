@@ -809,8 +809,8 @@ int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q, int64_t q
  * sequence; a token whose block is outside the pool is not moved.  The workspace
  * (256-byte aligned; cache_bits 16 or 8) needs no initialisation. */
 size_t cvsa_evict_tokens_workspace_bytes(int32_t B, int32_t H_kv, int32_t D, int32_t block_size,
-                                         int32_t cache_bits, int32_t keep, int32_t sinks,
-                                         int32_t recent);
+                                         int32_t W, int32_t cache_bits, int32_t keep,
+                                         int32_t sinks, int32_t recent);
 int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void *v_cache,
                       uint8_t *k_scales, uint8_t *v_scales, int64_t num_blocks,
                       const int32_t *block_tables, int64_t bt_stride_b, int32_t W,

@@ -193,6 +193,7 @@ def evicted(weights, caches, block_tables, context_lens, keep, sinks, recent, sc
                 rows = c[sb.clamp(0, nb - 1), src % bs, h].clone()
                 if scales:
                     e = bytes_[i][sb.clamp(0, nb - 1), h].clone()
+                    e[(sb < 0) | (sb >= nb)] = 0  # no row, so no scale
                     for p in range(-(-keep // bs)):
                         part = slice(p * bs, min((p + 1) * bs, keep))
                         if not moved[part].any() or not 0 <= int(bt[b, p]) < nb:

@@ -529,6 +529,24 @@ def test_evict_long_rows(gpu, bits):
     _check_evict(gpu, bt, ctx, k, v, torch.zeros_like(w), 4000, 16, 4, 300)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_evict_rows_of_chunks(gpu, bits):
+    """Tables of more than 16384 keys: rows of several chunks, of one, empty ones, cuts
+    in the first chunk and in later ones, equal weights over several chunks."""
+    g = _gen(bits)
+    bt, ctx, k, v, w = _evict_inputs(g, [20000, 9000, 5, 17000], 64, 2, 32, bits)
+    for keep, sinks, recent in ((8192, 4, 256), (16500, 0, 0), (8200, 3, 8000), (100, 100, 0),
+                                (1, 0, 0), (30000, 1, 2), (17000, 8192, 8192)):
+        _check_evict(gpu, bt, ctx, k, v, w, keep, 64, sinks, recent)
+    w[:, :, ::2] = 1.0
+    _check_evict(gpu, bt, ctx, k, v, w, 9500, 64, 4, 100)
+    _check_evict(gpu, bt, ctx, k, v, torch.zeros_like(w), 8193, 64, 1, 1)
+    w[0, 0, :12] = torch.tensor([math.nan, -math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-45,
+                                 -1e-45, -1.0, 3e38, -3e38, math.nan])
+    bt[0, 5], bt[3, 200] = -1, 10 ** 7
+    _check_evict(gpu, bt, ctx, k, v, w, 12000, 64, 0, 33)
+
+
 def test_evict_weights_of_every_kind(gpu):
     g = _gen(9)
     bt, ctx, k, v, w = _evict_inputs(g, [200], 16, 2, 64, 8)

@@ -292,7 +292,7 @@ def test_c_weigh_asks_for_its_workspace():
     for over in (dict(), dict(ws=P[9], bytes=need - 1)):
         assert _weigh(lib, cu=(0, 2000), **over) == _lib.CVSA_ERR_WORKSPACE
     # the last few tokens alone need none
-    assert lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, D, W * BS, 64) == 0
+    assert lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, D, W * BS, 8) == 0
 
 
 def _evict(lib, **over):
