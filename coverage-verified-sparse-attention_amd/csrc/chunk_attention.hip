@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kJoinThreads) void chunk_join_kernel(const ChunkArg
   int64_t second;
   if (RANGES) {
     const ChunkRanges ranges(c, total);
-    const int r0 = ranges.of(unit0), r1 = ranges.of(unit0 + units - 1);
+    const int r0 = ranges.of(unit0 + c.extra_units), r1 = ranges.of(unit0 + units - 1);
     const int h = head / a.G, place = tok * a.G + head % a.G;
     parts = r1 - r0 + 1;
     part0 = ((int64_t)(2 * r0 + 1) * a.H_kv + h) * c.tile_rows + place;
@@ -257,6 +257,9 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   static_assert(chunk_stream_waves<D, F8>() * 32 == 1 << unit_log2, "a step of the waves");
   const bool whole = max_keys <= 256;
   p.few.unit_log2 = p.many.unit_log2 = whole ? 31 : unit_log2;
+  // A sequence's start and end cost a workgroup about as much as 3 units of 128 keys of
+  // 8 bits: counted so, 32 single tokens over up to 8 K keys take 62 us, 67 without.
+  p.few.extra_units = F8 && !whole ? 3 : 0;
   const int64_t units =
       (int64_t)p.few.tiles * (whole ? 1 : (max_keys + (1 << unit_log2) - 1) >> unit_log2);
   const int fit = most_few > 32 ? chunk_stream_fit<D, 2, F8>() : chunk_stream_fit<D, 1, F8>();
@@ -403,7 +406,7 @@ static int chunk_attention(const char *who, const uint16_t *q, int64_t q_stride_
                CVSA_ERR_WORKSPACE,
                "%s: needs a 256-byte aligned workspace of %zu bytes", who, p.bytes);
   CVSA_REQUIRE(chunk_grid(p.many, H_kv) < (1LL << 31) &&
-                   (int64_t)p.few.tiles * ((int64_t)W * block_size / 64 + 1) < (1LL << 31),
+                   (int64_t)p.few.tiles * ((int64_t)W * block_size / 64 + 4) < (1LL << 31),
                CVSA_ERR_UNSUPPORTED, "%s: too many row tiles or keys", who);
   for (ChunkClass *c : {&p.few, &p.many}) {
     c->part_ml = (float2 *)((char *)workspace + (size_t)c->part_ml);

@@ -47,6 +47,7 @@ struct ChunkClass {
   int tile_rows, tiles;
   int splits, split_len;
   int unit_log2;    // few rows: keys of a unit, 31: a unit has all of a sequence
+  int extra_units;  // few rows: without keys, before each sequence's, for its start
   int tokens;       // of these sequences
   int only, only_first, only_len;  // many rows: the one such sequence, -1: several
   int same_len;     // what every sequence brings, 0: they differ
@@ -105,7 +106,7 @@ __device__ __forceinline__ ChunkSeq chunk_look(const ChunkArgs &a, const ChunkCl
   s.ctx = a.context_lens[b];
   s.keys = max(0, min(s.ctx, a.W << a.bs_log2));
   if (s.len * a.G < c.min_rows || s.len * a.G > c.max_rows) s.len = 0;
-  else s.units = (max(s.keys - 1, 0) >> c.unit_log2) + 1;
+  else s.units = (max(s.keys - 1, 0) >> c.unit_log2) + 1 + c.extra_units;
   return s;
 }
 

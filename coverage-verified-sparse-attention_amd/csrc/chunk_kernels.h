@@ -17,13 +17,19 @@ void launch_chunk_prefill(const ChunkArgs &a, const ChunkClass &c, unsigned grid
 
 template <int D, bool F8>
 void launch_chunk_stream(const ChunkArgs &a, const ChunkClass &c, hipStream_t s) {
-  const dim3 grid((unsigned)(c.splits * a.H_kv)), block(chunk_stream_waves<D, F8>() * 64);
-  if constexpr (chunk_few_rows<D>() > 32) {
-    if (c.tile_rows > 32)
-      hipLaunchKernelGGL((chunk_stream_kernel<D, 2, F8>), grid, block, 0, s, a, c);
+  const unsigned wgs = (unsigned)(c.splits * a.H_kv);
+  const dim3 block(chunk_stream_waves<D, F8>() * 64);
+  if constexpr (F8) {
+    hipLaunchKernelGGL((chunk_stream_kernel<D, 1, F8>), dim3(wgs, c.tile_rows / 32), block, 0, s,
+                       a, c);
+  } else {
+    if constexpr (chunk_few_rows<D>() > 32) {
+      if (c.tile_rows > 32)
+        hipLaunchKernelGGL((chunk_stream_kernel<D, 2, F8>), dim3(wgs), block, 0, s, a, c);
+    }
+    if (c.tile_rows <= 32)
+      hipLaunchKernelGGL((chunk_stream_kernel<D, 1, F8>), dim3(wgs), block, 0, s, a, c);
   }
-  if (c.tile_rows <= 32)
-    hipLaunchKernelGGL((chunk_stream_kernel<D, 1, F8>), grid, block, 0, s, a, c);
 }
 
 #define CVSA_CHUNK_LAUNCHES(D)                                                             \

@@ -34,6 +34,12 @@ constexpr int chunk_stream_waves() {
   return D == 256 && !F8 ? 2 : 4;
 }
 
+// Over 8 bits each row tile has a workgroup of its own; those of the same keys run
+// next to each other on one XCD, whose L2 the second reads.  (Both tiles in a wave:
+// its registers are moved to and fro, and one wave to a SIMD takes its conversions,
+// products and waits in turns: 8 drafts of 5 tokens at 32 K keys, 28 heads on 4, 77 us
+// for 71.)
+//
 // Workgroups of a CU: by LDS one at D >= 128, two at 64; by registers at 32.  With
 // two row tiles one at 64 as well, whose fewer parts gain more than twice the
 // waves do: 61 us for 66 (8 drafts of 5 tokens at 32 K keys, 28 heads on 4).
@@ -44,9 +50,11 @@ constexpr int chunk_stream_fit() {
 }
 
 template <int D, int RT, bool F8>
-__global__ __launch_bounds__((chunk_stream_waves<D, F8>() * 64), (chunk_stream_fit<D, RT, F8>())) void
+__global__ __launch_bounds__((chunk_stream_waves<D, F8>() * 64),
+                             (chunk_stream_fit<D, RT, F8>())) void
 chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   constexpr int NW = chunk_stream_waves<D, F8>(), NT = NW * 64, KT = 32;
+  static_assert(!F8 || RT == 1, "8 bits: a workgroup for each row tile");
   constexpr int DV = F8 ? D / 2 : D;           // a row's bytes are those of DV bf16 values
   constexpr int CPR = DV / 8, RPL = 64 / CPR;  // rows of a load
   constexpr int P = KT / RPL;                  // loads of a tile of K or V
@@ -58,7 +66,11 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   __shared__ ChunkTaken<D> s_taken;
 
   const int tid = threadIdx.x;
-  const uint32_t range = blockIdx.x / a.H_kv;
+  // Over 8 bits the heads of a range go to one XCD: each of its rows has 128 bytes at
+  // D = 128, and an XCD that reads all heads' draws on all of its L2's channels (plain
+  // reads of such rows: 5.2 TB/s with an XCD for each head, 5.6 so).
+  const uint32_t n_ranges = gridDim.x / a.H_kv;
+  const uint32_t range = F8 ? blockIdx.x % n_ranges : blockIdx.x / a.H_kv;
   const ChunkSeq first = chunk_look(a, cl, tid & 63);
   uint32_t total = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave)
@@ -72,11 +84,12 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   auto walk = [&](const ChunkTile &t, int u0, int u1, int units) {
     // New to the compiler for each sequence, or it keeps everything that
     // follows from the lane and the head over the loop, and spills.
-    int id = tid, h = blockIdx.x % a.H_kv;
+    int id = tid, h = F8 ? blockIdx.x / n_ranges : blockIdx.x % a.H_kv;
     asm volatile("" : "+v"(id), "+s"(h));
     const int lane = id & 63, wave = __builtin_amdgcn_readfirstlane(id >> 6);
     const int l31 = lane & 31, half = lane >> 5;
-    const int k0 = u0 << cl.unit_log2, k1 = u1 < units ? u1 << cl.unit_log2 : t.keys;
+    const int k0 = max(u0 - cl.extra_units, 0) << cl.unit_log2;
+    const int k1 = u1 < units ? (u1 - cl.extra_units) << cl.unit_log2 : t.keys;
 
     const int bs_mask = (1 << a.bs_log2) - 1;
     const int row_bytes = a.H_kv * DV * 2;
@@ -185,6 +198,8 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
         whole = whole && bad_scale == 0;
       }
       if (!whole) {
+        // A branch to the compiler: it would make selects of it for every tile.
+        if constexpr (F8) asm volatile("");
 #pragma unroll
         for (int r = 0; r < RT; ++r) chunk_mask(st[r], key0, first_key(s), row[r].last_key);
       }
@@ -265,64 +280,59 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
     }
 
     // The waves' states, joined in order by the first: an array of K or V for
-    // each other wave, float4 i of row r at place i ^ (r % 8); JR row tiles at a
-    // time.
-    constexpr int JR = F8 ? 1 : RT;
-    static_assert(NW <= 4 && NW * kTile * 2 >= JR * 32 * D * 4, "room to join");
+    // each other wave, float4 i of row r at place i ^ (r % 8).
+    static_assert(NW <= 4 && NW * kTile * 2 >= RT * 32 * D * 4, "room to join");
     auto room = [&](int w) {
       return reinterpret_cast<float4 *>(w == 1 ? s_k1 : w == 2 ? s_v0 : s_v1);
     };
     auto spot = [&](int r, int d, int g) {
-      return (r % JR * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
+      return (r * 32 + l31) * (D / 4) + ((8 * d + 2 * g + half) ^ (l31 & 7));
     };
 #pragma unroll
     for (int r = 0; r < RT; ++r) state[r].finish();
+    __syncthreads();
+    if (wave > 0) {
+      float4 *const so = room(wave);
 #pragma unroll
-    for (int r0 = 0; r0 < RT; r0 += JR) {
-      __syncthreads();
-      if (wave > 0) {
-        float4 *const so = room(wave);
+      for (int r = 0; r < RT; ++r) {
+        if (half == 0) s_ml[wave - 1][r * 32 + l31] = make_float2(state[r].m, state[r].l);
 #pragma unroll
-        for (int r = r0; r < r0 + JR; ++r) {
-          if (half == 0) s_ml[wave - 1][r * 32 + l31] = make_float2(state[r].m, state[r].l);
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              so[spot(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
-                                               state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
-        }
+          for (int g = 0; g < 4; ++g)
+            so[spot(r, d, g)] = make_float4(state[r].o[d][4 * g], state[r].o[d][4 * g + 1],
+                                             state[r].o[d][4 * g + 2], state[r].o[d][4 * g + 3]);
       }
-      __syncthreads();
-      if (wave == 0) {
+    }
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
-        for (int r = r0; r < r0 + JR; ++r) {
-          for (int w = 1; w < NW; ++w) {
-            const float4 *const so = room(w);
-            const float2 ml = s_ml[w - 1][r * 32 + l31];
-            const float nm = fmaxf(state[r].m, ml.x);
-            const float a0 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[r].m - nm);
-            const float a1 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - nm);
-            state[r].m = nm;
-            state[r].l = state[r].l * a0 + ml.y * a1;
+      for (int r = 0; r < RT; ++r) {
+        for (int w = 1; w < NW; ++w) {
+          const float4 *const so = room(w);
+          const float2 ml = s_ml[w - 1][r * 32 + l31];
+          const float nm = fmaxf(state[r].m, ml.x);
+          const float a0 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(state[r].m - nm);
+          const float a1 = nm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - nm);
+          state[r].m = nm;
+          state[r].l = state[r].l * a0 + ml.y * a1;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
+          for (int d = 0; d < DB; ++d) {
+            __builtin_amdgcn_sched_barrier(0);  // few reads at once: registers
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const float4 v = so[spot(r, d, g)];
-                state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
-                state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
-                state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
-                state[r].o[d][4 * g + 3] = state[r].o[d][4 * g + 3] * a0 + v.w * a1;
-              }
+            for (int g = 0; g < 4; ++g) {
+              const float4 v = so[spot(r, d, g)];
+              state[r].o[d][4 * g] = state[r].o[d][4 * g] * a0 + v.x * a1;
+              state[r].o[d][4 * g + 1] = state[r].o[d][4 * g + 1] * a0 + v.y * a1;
+              state[r].o[d][4 * g + 2] = state[r].o[d][4 * g + 2] * a0 + v.z * a1;
+              state[r].o[d][4 * g + 3] = state[r].o[d][4 * g + 3] * a0 + v.w * a1;
             }
           }
-          s_taken.restore(row[r].last_key, state[r].o);
-          const int64_t part = (int64_t)(2 * (int)range + (u0 == 0)) * a.H_kv + h;
-          if (u0 == 0 && u1 == units) state[r].store(a, t, row[r]);
-          else state[r].store_part(cl, row[r], part * cl.tile_rows + r * 32 + l31);
         }
+        s_taken.restore(row[r].last_key, state[r].o);
+        const int64_t part = (int64_t)(2 * (int)range + (k0 == 0)) * a.H_kv + h;
+        if (k0 == 0 && u1 == units) state[r].store(a, t, row[r]);
+        else state[r].store_part(cl, row[r], part * cl.tile_rows + t.row0 + r * 32 + l31);
       }
     }
     __syncthreads();  // the buffers and s_taken are the next sequence's
@@ -346,8 +356,13 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
       t.keys = __builtin_amdgcn_readlane(mine.keys, l);
       const int units = __builtin_amdgcn_readlane(mine.units, l);
       const uint32_t from = before + __builtin_amdgcn_readlane(incl, l) - units;
-      walk(t, (int)(begin > from ? begin - from : 0),
-           end < from + units ? (int)(end - from) : units, units);
+      const int u1 = end < from + units ? (int)(end - from) : units;
+      if (u1 <= cl.extra_units) continue;  // none of its keys
+      if constexpr (F8) {
+        t.row0 = blockIdx.y * 32;
+        if (t.row0 >= t.rows) continue;
+      }
+      walk(t, (int)(begin > from ? begin - from : 0), u1, units);
     }
     before += __builtin_amdgcn_readlane(incl, 63);
   }
