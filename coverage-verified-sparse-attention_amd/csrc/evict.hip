@@ -18,7 +18,7 @@
 // 167 us, so XX us).
 // A destination is a source itself only among slots keep - recent .. keep: other
 // workgroups of the first launch copy these aside.  In the last launch a wave for
-// each page moves its arrivals, keys and values apart, in no order.
+// each page moves its arrivals, in no order.
 //
 // 8 bits: a page with arrivals gets the largest scale of its tokens' pages; payloads
 // are shifted to it, which rounds only what becomes subnormal.
@@ -503,8 +503,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
   }
 }
 
-// Rows of a page's arrivals and their weights, and in 8 bits the page's scale and its
-// other rows.  Keys (and weights) by even waves, values by odd ones.
+// Rows of a page's arrivals and their weights, and in 8 bits the page's scales and its
+// other rows; a wave for each page.
 template <bool F8, bool LONG>
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int wgs_each) {
   const int lane = threadIdx.x & 63;
@@ -513,7 +513,6 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
   const int h = (int)(blockIdx.x % a.H_kv), wg = (int)(blockIdx.x / a.H_kv % wgs_each);
   const int b = (int)(blockIdx.x / a.H_kv / wgs_each);
   const int64_t bh = (int64_t)b * a.H_kv + h;
-  const bool values = wave & 1;
   const int bs = 1 << a.bs_log2, n_pages = (a.keep + bs - 1) >> a.bs_log2;
   const int ctx = LONG ? evict_context(a, b) : 0, front = a.keep - a.recent;
   const int last_page = (a.keep - 1) >> a.bs_log2;
@@ -521,16 +520,15 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
   float *const w = a.weights + bh * a.S;
   const int32_t *const pages = LONG ? nullptr : a.pages + bh * (1 + n_pages);
   const int listed = LONG ? n_pages : pages[0];
-  char *const cache = values ? a.v_cache : a.k_cache;
-  const char *const aside = a.aside + (bh * 2 + values) * a.recent * (int64_t)a.row_bytes;
+  const char *const aside = a.aside + bh * 2 * a.recent * (int64_t)a.row_bytes;
   const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
   const int part = lane % per_row * 16, sub = lane / per_row;
-  int i = wg * 2 + wave / 2;
+  int i = wg * 4 + wave;
   // Looked up before it is known whether there is one: one wait for both.
   int next = LONG ? 0 : pages[1 + min(i, n_pages - 1)];
-  for (; i < listed; i += wgs_each * 2) {
+  for (; i < listed; i += wgs_each * 4) {
     const int page = LONG ? i : next, slot0 = page << a.bs_log2;
-    if (!LONG) next = pages[1 + min(i + wgs_each * 2, n_pages - 1)];
+    if (!LONG) next = pages[1 + min(i + wgs_each * 4, n_pages - 1)];
     const int count = min(bs, a.keep - slot0);
     const int blk = LONG && ctx <= a.keep ? -1 : evict_block(a, b, slot0);
     // The lane's slots: where they come from (the place itself: it stays), the blocks.
@@ -544,83 +542,95 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
       if (r >= count) continue;
       if constexpr (LONG) {
         if (ctx <= a.keep) {
-          if (!values) kept[slot] = slot < ctx ? slot : -1;
+          kept[slot] = slot < ctx ? slot : -1;
           continue;
         }
         if (slot >= front) {
           src[n] = slot + ctx - a.keep;
         } else if (slot >= a.sinks) {
-          const int at = kept[slot];  // the other wave may have put the answer there
+          const int at = kept[slot];
           src[n] = at >= 0 ? at : (a.tails + bh * a.keep)[a.n_holes[bh] - 1 - (-2 - at)];
         }
-        if (!values && (slot < a.sinks || slot >= front || src[n] != slot)) kept[slot] = src[n];
+        if (slot < a.sinks || src[n] != slot) kept[slot] = src[n];
       } else {
         src[n] = kept[slot];
       }
       if (src[n] == slot) continue;
       any = true;
       from[n] = evict_block(a, b, src[n]);
-      if (!values)
-        w[slot] = src[n] < a.keep ? a.aside_weights[bh * a.recent + src[n] - front] : w[src[n]];
+      w[slot] = src[n] < a.keep ? a.aside_weights[bh * a.recent + src[n] - front] : w[src[n]];
     }
     if (blk < 0 || __ballot(any) == 0) continue;
-    int byte = 0, old = 0, scale[2] = {0, 0};  // scales' bytes: new, the page's, the rows'
+    // Scales' bytes of keys and values: the page's, its new ones, the rows'.
+    int old[2] = {0, 0}, byte[2] = {0, 0}, scale[2][2] = {{0, 0}, {0, 0}};
     if constexpr (F8) {
-      uint8_t *const scales = values ? a.v_scales : a.k_scales;
-      const uint8_t *const were = a.aside_scales + (bh * 2 + values) * a.aside_pages -
-                                  (front >> a.bs_log2);
-      uint8_t *const at = scales + (int64_t)blk * a.H_kv + h;
-      old = *at;
-      uint32_t top = 0;
+      uint32_t top[2] = {0, 0};
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int r = lane + 64 * n, p = src[n] >> a.bs_log2;
-        if (r >= count) continue;
-        // Pages that get arrivals themselves may have another scale by now.
-        scale[n] = src[n] == slot0 + r ? old
-                   : from[n] < 0       ? 0
-                   : p <= last_page    ? were[p]
-                                       : scales[(int64_t)from[n] * a.H_kv + h];
-        top = max(top, (uint32_t)scale[n]);
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint8_t *const scales = kv ? a.v_scales : a.k_scales;
+        const uint8_t *const were = a.aside_scales + (bh * 2 + kv) * a.aside_pages -
+                                    (front >> a.bs_log2);
+        old[kv] = scales[(int64_t)blk * a.H_kv + h];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int r = lane + 64 * n, p = src[n] >> a.bs_log2;
+          if (r >= count) continue;
+          // Pages that get arrivals themselves may have another scale by now.
+          scale[kv][n] = src[n] == slot0 + r ? old[kv]
+                         : from[n] < 0       ? 0
+                         : p <= last_page    ? were[p]
+                                             : scales[(int64_t)from[n] * a.H_kv + h];
+          top[kv] = max(top[kv], (uint32_t)scale[kv][n]);
+        }
       }
-      byte = (int)wave_max_u32(top);
-      if (lane == 0 && byte != old) *at = (uint8_t)byte;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        byte[kv] = (int)wave_max_u32(top[kv]);
+        if (lane == 0 && byte[kv] != old[kv])
+          (kv ? a.v_scales : a.k_scales)[(int64_t)blk * a.H_kv + h] = (uint8_t)byte[kv];
+      }
     }
-    // Up to four groups of rows are read before they are written.
-    constexpr int kBatch = 4;
+    // Two groups of rows of both are read before they are written.
+    constexpr int kBatch = 2;
     for (int r0 = 0; r0 < count; r0 += rows * kBatch) {
-      uint4 v[kBatch];
-      int shift[kBatch];
-      bool write[kBatch];
+      uint4 v[kBatch][2];
+      int shift[kBatch][2];
+      bool write[kBatch][2];
       unrolled<kBatch>([&](auto n) {
         constexpr int g = decltype(n)::value;
         const int r = r0 + g * rows + sub, slot = slot0 + r;
         const bool high = r >= 64;
-        const int x = __shfl(src[0], r & 63, 64), x1 = __shfl(src[1], r & 63, 64);
-        const int y = __shfl(from[0], r & 63, 64), y1 = __shfl(from[1], r & 63, 64);
-        const int s = high ? x1 : x, blk_s = high ? y1 : y;
-        v[g] = make_uint4(0, 0, 0, 0);
-        shift[g] = 0;
-        if constexpr (F8) {
-          const int z = __shfl(scale[0], r & 63, 64), z1 = __shfl(scale[1], r & 63, 64);
-          shift[g] = (high ? z1 : z) - byte;
+        auto of_row = [&](const int (&x)[2]) {
+          const int lo = __shfl(x[0], r & 63, 64), hi = __shfl(x[1], r & 63, 64);
+          return high ? hi : lo;
+        };
+        const int s = of_row(src), s_blk = of_row(from);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          v[g][kv] = make_uint4(0, 0, 0, 0);
+          shift[g][kv] = F8 ? of_row(scale[kv]) - byte[kv] : 0;
+          // One that stays, only where its payload changes with the scale.
+          write[g][kv] = r < count && (s != slot ? s_blk >= 0 : F8 && byte[kv] != old[kv]);
+          if (!write[g][kv]) continue;
+          const char *const p =
+              s != slot && s < a.keep
+                  ? aside + ((int64_t)kv * a.recent + (s - front)) * a.row_bytes
+                  : (kv ? a.v_cache : a.k_cache) + evict_row(a, s_blk, s, h);
+          v[g][kv] = *reinterpret_cast<const uint4 *>(p + part);
         }
-        // One that stays, only where its payload changes with the scale.
-        write[g] = r < count && (s != slot ? blk_s >= 0 : F8 && byte != old);
-        if (!write[g]) return;
-        const char *const p =
-            s != slot && s < a.keep ? aside + (int64_t)(s - front) * a.row_bytes
-                                    : cache + evict_row(a, blk_s, s, h);
-        v[g] = *reinterpret_cast<const uint4 *>(p + part);
       });
       unrolled<kBatch>([&](auto n) {
         constexpr int g = decltype(n)::value;
-        if (!write[g]) return;
         const int slot = slot0 + r0 + g * rows + sub;
-        if constexpr (F8) {
-          if (shift[g] != 0) v[g] = shifted_8_bits(v[g], shift[g]);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!write[g][kv]) continue;
+          if constexpr (F8) {
+            if (shift[g][kv] != 0) v[g][kv] = shifted_8_bits(v[g][kv], shift[g][kv]);
+          }
+          *reinterpret_cast<uint4 *>((kv ? a.v_cache : a.k_cache) + evict_row(a, blk, slot, h) +
+                                     part) = v[g][kv];
         }
-        *reinterpret_cast<uint4 *>(cache + evict_row(a, blk, slot, h) + part) = v[g];
       });
     }
   }
@@ -764,9 +774,9 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
   } else {
     hipLaunchKernelGGL(evict_plan_kernel<4>, first, threads, 0, s, a);
   }
-  // Two pages at once in a workgroup, in turn past 8192 workgroups.
+  // Four pages at once in a workgroup, in turn past 8192 workgroups.
   const int64_t n_pages = (keep + block_size - 1) / block_size;
-  const int each = (int)std::max<int64_t>(1, std::min<int64_t>((n_pages + 1) / 2, 8192 / bh));
+  const int each = (int)std::max<int64_t>(1, std::min<int64_t>((n_pages + 3) / 4, 8192 / bh));
   const dim3 grid((unsigned)(bh * each));
   auto move = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, each); };
   if (p.long_rows) k_scales ? move(evict_move_kernel<true, true>) : move(evict_move_kernel<false, true>);

@@ -165,8 +165,10 @@ __global__ __launch_bounds__(256, (weigh_few_fit<D, F8>())) void weigh_few_kerne
   constexpr int KS = D / 16;
   const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.x % a.H_kv;
-  const uint32_t range = blockIdx.x / a.H_kv * 4 + wave, ranges = gridDim.x / a.H_kv * 4;
+  // The heads of a range go to one XCD: see the chunk attention of few rows.
+  const uint32_t n_wgs = gridDim.x / a.H_kv;
+  const int h = blockIdx.x / n_wgs;
+  const uint32_t range = blockIdx.x % n_wgs * 4 + wave, ranges = n_wgs * 4;
 
   // The wave's units of 32 keys.
   const WeighSeq own = weigh_look(a, lane, true);
