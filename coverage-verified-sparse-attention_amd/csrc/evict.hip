@@ -15,10 +15,15 @@
 // sequence and head has its weights in registers.  Longer ones: chunks of 8192 slots
 // have a workgroup each, a launch for each histogram and one for the walk, in which
 // every chunk adds up the others' counts (131072 slots, 8 heads: one workgroup each
-// 167 us, so XX us).
+// 167 us, so 30 before the rows are moved).
 // A destination is a source itself only among slots keep - recent .. keep: other
 // workgroups of the first launch copy these aside.  In the last launch a wave for
-// each page moves its arrivals, in no order.
+// 64 slots moves their arrivals, in no order.
+//
+// Measured: 32 sequences of 8 heads, 4160 tokens to 4096, 256 of them recent, 8 bits: 19
+// us for the plan and what is copied aside (6 of them; 4 are the searches) and 22 to
+// move, for 51 MB.  131072 to 16384, 8 heads of bf16: 7 + 7 + 7 + 9 and 13, for 125 MB.
+// Both are chains of short dependent steps, not bound by a rate.
 //
 // 8 bits: a page with arrivals gets the largest scale of its tokens' pages; payloads
 // are shifted to it, which rounds only what becomes subnormal.
@@ -50,11 +55,11 @@ struct EvictArgs {
   float *aside_weights;    // [recent]
   uint8_t *aside_scales;   // [2, aside_pages]
   int aside_pages;
-  int32_t *holes;          // [keep] slots to be filled
   // Short rows.
   int32_t *pages;          // [1 + pages]: pages with arrivals, their number first
   // Long rows: of chunks.
   int chunks;              // of a row of the tables
+  int32_t *holes;          // [keep] slots to be filled
   uint16_t *hist;          // [3, chunks, kBins]
   uint32_t *above;         // [chunks]: weights above the bins chosen so far
   uint32_t *state;         // [4]: bins and what is still wanted, after passes 1 and 2
@@ -76,9 +81,10 @@ __device__ __forceinline__ int evict_block(const EvictArgs &a, int b, int slot) 
   const int blk = a.block_tables[b * a.bt_sb + (slot >> a.bs_log2)];
   return (uint32_t)blk < (uint64_t)a.num_blocks ? blk : -1;
 }
+// Row of a slot and head in the caches.
 __device__ __forceinline__ int64_t evict_row(const EvictArgs &a, int blk, int slot, int h) {
   const int64_t token = ((int64_t)blk << a.bs_log2) + (slot & ((1 << a.bs_log2) - 1));
-  return (token * a.H_kv + h) * a.row_bytes;
+  return token * a.H_kv + h;
 }
 
 // Weights' order as unsigned numbers; NaN is above all, zeros are equal.
@@ -92,7 +98,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 __host__ __device__ constexpr int pass_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __host__ __device__ constexpr int pass_bits(int pass) { return pass == 2 ? 10 : 11; }
 
-// Sums over the workgroup: of the threads before this one, and of all.
+// Sums over the workgroup: of the threads before this one, and of all.  s is used
+// again only after another barrier.
 struct EvictScan {
   uint32_t before, all;
 };
@@ -108,7 +115,6 @@ __device__ __forceinline__ EvictScan evict_scan(uint32_t v, uint32_t *s) {
     r.before += w < wave ? x : 0u;
     r.all += x;
   }
-  __syncthreads();
   return r;
 }
 
@@ -117,18 +123,19 @@ __device__ __forceinline__ EvictScan evict_scan(uint32_t v, uint32_t *s) {
 struct EvictBin {
   uint32_t bin, above;
 };
+struct EvictFind {  // LDS of one search
+  uint32_t sum[kEvictWaves], bin, above;
+};
 __device__ __forceinline__ EvictBin evict_find(uint32_t n0, uint32_t n1, int bits, uint32_t want,
-                                               uint32_t *s_sum, uint32_t *s_bin) {
-  const EvictScan s = evict_scan(n0 + n1, s_sum);
+                                               EvictFind &f) {
+  const EvictScan s = evict_scan(n0 + n1, f.sum);
   if (s.before < want && want <= s.before + n0 + n1) {
     const bool second = want > s.before + n0;
-    s_bin[0] = (uint32_t)((1 << bits) - 1 - 2 * (int)threadIdx.x - (second ? 1 : 0));
-    s_bin[1] = s.before + (second ? n0 : 0u);
+    f.bin = (uint32_t)((1 << bits) - 1 - 2 * (int)threadIdx.x - (second ? 1 : 0));
+    f.above = s.before + (second ? n0 : 0u);
   }
   __syncthreads();
-  const EvictBin r = {s_bin[0], s_bin[1]};
-  __syncthreads();
-  return r;
+  return {f.bin, f.above};
 }
 
 // A thread's share of the slots: four together in each of N steps of the workgroup.
@@ -163,20 +170,25 @@ struct EvictKeys {
   }
 };
 
-__device__ __forceinline__ void evict_clear(uint32_t (*hist)[kBins]) {
-  for (int i = threadIdx.x; i < kCopies * kBins; i += kEvictThreads) (&hist[0][0])[i] = 0;
-  __syncthreads();
+// Clears n words (a multiple of 4) of LDS; the caller waits.
+__device__ __forceinline__ void evict_clear(void *s, int n) {
+  for (int i = threadIdx.x; i < n / 4; i += kEvictThreads)
+    reinterpret_cast<uint4 *>(s)[i] = make_uint4(0, 0, 0, 0);
 }
-// A thread's two bins from the top, over the copies.
-__device__ __forceinline__ void evict_bins(const uint32_t (*hist)[kBins], int bits, uint32_t &n0,
+// A thread's two bins from the top, over the copies, which it leaves cleared.
+template <int BITS>
+__device__ __forceinline__ void evict_bins(uint32_t (*hist)[1 << BITS], uint32_t &n0,
                                            uint32_t &n1) {
-  const int top = (1 << bits) - 1 - 2 * (int)threadIdx.x;
+  const int top = (1 << BITS) - 1 - 2 * (int)threadIdx.x;
   n0 = n1 = 0;
   if (top <= 0) return;
 #pragma unroll
   for (int c = 0; c < kCopies; ++c) {
-    n0 += hist[c][top];
-    n1 += hist[c][top - 1];
+    uint2 &at = *reinterpret_cast<uint2 *>(&hist[c][top - 1]);
+    const uint2 two = at;
+    at = make_uint2(0, 0);
+    n0 += two.y;
+    n1 += two.x;
   }
 }
 
@@ -193,7 +205,7 @@ __device__ __forceinline__ void evict_copy_aside(const EvictArgs &a) {
     const int slot = front + n, blk = evict_block(a, b, slot);
     if (part == 0) a.aside_weights[row] = a.weights[bh * a.S + slot];
     if (blk < 0) return;
-    const int64_t from = evict_row(a, blk, slot, h) + part * 16;
+    const int64_t from = evict_row(a, blk, slot, h) * a.row_bytes + part * 16;
     char *const to = a.aside + ((bh * 2) * a.recent + n) * a.row_bytes + part * 16;
     *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(a.k_cache + from);
     *reinterpret_cast<uint4 *>(to + (int64_t)a.recent * a.row_bytes) =
@@ -219,14 +231,25 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
     evict_copy_aside(a);
     return;
   }
-  __shared__ uint32_t s_hist[kCopies][kBins];
-  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2], s_step[N][kEvictWaves];
+  // Histograms, the passes' in turn, as each leaves its own cleared; after them, in
+  // their place, the holes.
+  constexpr int kPages = N * 4 * kEvictThreads / 8;
+  __shared__ __align__(16) union {
+    uint32_t hist[2][kCopies][kBins];
+    uint16_t holes[N * 4 * kEvictThreads];
+  } s;
+  __shared__ __align__(16) uint8_t s_page[kPages];
+  __shared__ EvictFind s_find[3];
+  __shared__ uint32_t s_step[N][kEvictWaves], s_sum[2][kEvictWaves], s_stay;
   const int tid = threadIdx.x, wave = tid >> 6;
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / a.H_kv);
-  const int ctx = evict_context(a, b);
   float *const w = a.weights + bh * a.S;
-  int32_t *const kept = a.kept + bh * a.keep, *const holes = a.holes + bh * a.keep;
+  EvictKeys<N> keys;
+  // Of all the tables' slots: the context's length is on its way yet.
+  keys.load(w, 0, 0, a.W << a.bs_log2);
+  const int ctx = evict_context(a, b);
+  int32_t *const kept = a.kept + bh * a.keep;
   const int n_pages = (a.keep + (1 << a.bs_log2) - 1) >> a.bs_log2;
   int32_t *const pages = a.pages + bh * (1 + n_pages);
   if (ctx <= a.keep) {  // nothing to cut
@@ -235,8 +258,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
     return;
   }
   const int front = a.keep - a.recent, back = ctx - a.recent;
-  EvictKeys<N> keys;
-  keys.load(w, 0, a.sinks, back);
+  evict_clear(s.hist, 2 * kCopies * kBins);
+  evict_clear(s_page, kPages / 4);
+  __syncthreads();
 
   // The want-th largest of the middle: `threshold`, of whose equals the first `want`
   // stay.  None wanted: nothing is above this, and none of its equals stays.
@@ -244,17 +268,20 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
   if (want > 0) {
     uint32_t known = 0;
     threshold = 0;
-    for (int pass = 0; pass < 3; ++pass) {
-      evict_clear(s_hist);
-      keys.count(s_hist[wave % kCopies], pass, known, threshold, 0, a.sinks, back);
+    unrolled<3>([&](auto n) __attribute__((always_inline)) {
+      constexpr int pass = decltype(n)::value;
+      constexpr int bits = pass_bits(pass);
+      uint32_t(*const hist)[1 << bits] = reinterpret_cast<uint32_t(*)[1 << bits]>(
+          &s.hist[pass % 2][0][0]);
+      keys.count(hist[wave % kCopies], pass, known, threshold, 0, a.sinks, back);
       __syncthreads();
       uint32_t n0, n1;
-      evict_bins(s_hist, pass_bits(pass), n0, n1);
-      const EvictBin at = evict_find(n0, n1, pass_bits(pass), want, s_sum, s_bin);
+      evict_bins<bits>(hist, n0, n1);
+      const EvictBin at = evict_find(n0, n1, bits, want, s_find[pass]);
       threshold |= at.bin << pass_shift(pass);
-      known |= ((1u << pass_bits(pass)) - 1) << pass_shift(pass);
+      known |= ((1u << bits) - 1) << pass_shift(pass);
       want -= at.above;
-    }
+    });
   }
 
   // The slots in order: the kept ones below `front` stay, the others are holes; the
@@ -276,7 +303,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
   }
   __syncthreads();
   // Kept ones before each of the thread's slots, and below front.
-  uint32_t above = 0, equal = 0, rank[4 * N], stay = 0;
+  uint32_t above = 0, equal = 0, rank[4 * N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     uint32_t gt = above, eq = equal;
@@ -297,10 +324,14 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
       const bool same = in && keys.key[i] == threshold;
       rank[i] = gt + min(eq, want);
       const bool keep = larger || (same && eq < want);
-      if (j == front) s_bin[0] = rank[i];  // the next slot after those that may stay
+      if (j == front) s_stay = rank[i];  // the next slot after those that may stay
       if (in && j < front) {
-        if (keep) kept[j] = j;
-        else holes[(uint32_t)(j - a.sinks) - rank[i]] = j;
+        if (keep) {
+          kept[j] = j;
+        } else {
+          s.holes[(uint32_t)(j - a.sinks) - rank[i]] = (uint16_t)j;
+          s_page[j >> a.bs_log2] = 1;
+        }
       }
       if (!keep || j < front) rank[i] = 0xffffffffu;
       gt += larger ? 1u : 0u;
@@ -308,36 +339,26 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
     }
   }
   __syncthreads();
-  stay = s_bin[0];
+  const uint32_t stay = s_stay;
 #pragma unroll
   for (int i = 0; i < 4 * N; ++i)
-    if (rank[i] != 0xffffffffu) kept[holes[rank[i] - stay]] = keys.slot(0, i);
-  __syncthreads();
+    if (rank[i] != 0xffffffffu) kept[s.holes[rank[i] - stay]] = keys.slot(0, i);
 
   // Pages with arrivals: those of holes, and from front on all.
-  uint32_t *const flags = &s_hist[0][0];
-  static_assert(kCopies * kBins >= kShortRow / 8, "a flag for each page");
-  for (int p = tid; p < n_pages; p += kEvictThreads)
-    flags[p] = a.recent > 0 && p >= front >> a.bs_log2 ? 1u : 0u;
-  __syncthreads();
-  const int n_holes = front - a.sinks - (int)stay;
-  for (int n = tid; n < n_holes; n += kEvictThreads) flags[holes[n] >> a.bs_log2] = 1u;
-  __syncthreads();
   int listed = 0;
-  for (int p0 = 0; p0 < n_pages; p0 += kEvictThreads) {
+  for (int p0 = 0, turn = 0; p0 < n_pages; p0 += kEvictThreads, turn ^= 1) {
     const int p = p0 + tid;
-    const uint32_t any = p < n_pages ? flags[p] : 0u;
-    const EvictScan s = evict_scan(any, s_sum);
-    if (any) pages[1 + listed + s.before] = p;
-    listed += (int)s.all;
+    const bool any = p < n_pages && (s_page[p] || (a.recent > 0 && p >= front >> a.bs_log2));
+    const EvictScan sum = evict_scan(any ? 1u : 0u, s_sum[turn]);
+    if (any) pages[1 + listed + sum.before] = p;
+    listed += (int)sum.all;
   }
   if (tid == 0) pages[0] = listed;
 }
 
 // Long rows: the bins that pass `pass` chooses from the histograms of all chunks.
 __device__ __forceinline__ EvictBin evict_choose(const EvictArgs &a, int64_t bh, int pass,
-                                                 int chunks, uint32_t want, uint32_t *s_sum,
-                                                 uint32_t *s_bin) {
+                                                 int chunks, uint32_t want, EvictFind &f) {
   const int top = (1 << pass_bits(pass)) - 1 - 2 * (int)threadIdx.x;
   uint32_t n0 = 0, n1 = 0;
   if (top > 0) {
@@ -355,7 +376,7 @@ __device__ __forceinline__ EvictBin evict_choose(const EvictArgs &a, int64_t bh,
       }
     }
   }
-  return evict_find(n0, n1, pass_bits(pass), want, s_sum, s_bin);
+  return evict_find(n0, n1, pass_bits(pass), want, f);
 }
 
 // A chunk's histogram of the bits of a pass, of the weights in the bins chosen before.
@@ -365,8 +386,10 @@ __global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictA
     evict_copy_aside(a);
     return;
   }
-  __shared__ uint32_t s_hist[kCopies][kBins];
-  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2];
+  constexpr int kBits = pass_bits(PASS);
+  __shared__ __align__(16) uint32_t s_hist[kCopies][1 << kBits];
+  __shared__ EvictFind s_find;
+  __shared__ uint32_t s_sum[kEvictWaves];
   const int64_t bh = blockIdx.x / a.chunks;
   const int chunk = (int)(blockIdx.x % a.chunks), first = chunk * kChunk;
   const int ctx = evict_context(a, (int)(bh / a.H_kv));
@@ -374,6 +397,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictA
   if (ctx <= a.keep || first >= back || front == a.sinks) return;
   EvictKeys<2> keys;
   keys.load(a.weights + bh * a.S, first, a.sinks, back);
+  evict_clear(s_hist, kCopies << kBits);
   uint32_t prefix = 0, known = 0;
   if constexpr (PASS > 0) {
     uint32_t *const state = a.state + bh * 4;
@@ -383,8 +407,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictA
       known = ((1u << pass_bits(0)) - 1) << pass_shift(0);
       want = state[1];
     }
-    const EvictBin at = evict_choose(a, bh, PASS - 1, (back + kChunk - 1) / kChunk, want, s_sum,
-                                     s_bin);
+    const EvictBin at =
+        evict_choose(a, bh, PASS - 1, (back + kChunk - 1) / kChunk, want, s_find);
     if (chunk == 0 && threadIdx.x == 0) {
       state[2 * PASS - 2] = at.bin;
       state[2 * PASS - 1] = want - at.above;
@@ -405,12 +429,12 @@ __global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictA
     prefix |= at.bin << pass_shift(PASS - 1);
     known |= mask << pass_shift(PASS - 1);
   }
-  evict_clear(s_hist);
+  if (PASS == 0) __syncthreads();  // later ones have waited in the search
   keys.count(s_hist[(threadIdx.x >> 6) % kCopies], PASS, known, prefix, first, a.sinks, back);
   __syncthreads();
   uint32_t n0, n1;
-  evict_bins(s_hist, pass_bits(PASS), n0, n1);
-  const int top = (1 << pass_bits(PASS)) - 1 - 2 * (int)threadIdx.x;
+  evict_bins<kBits>(s_hist, n0, n1);
+  const int top = (1 << kBits) - 1 - 2 * (int)threadIdx.x;
   if (top > 0)  // of at most 8192 slots: 16 bits
     *reinterpret_cast<uint32_t *>(
         a.hist + ((bh * 3 + PASS) * (int64_t)a.chunks + chunk) * kBins + top - 1) = n0 << 16 | n1;
@@ -419,7 +443,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_count_kernel(const EvictA
 // A chunk's slots in order: where the kept ones are, holes and what fills them.  A
 // hole n is -2 - n in kept.
 __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictArgs a) {
-  __shared__ uint32_t s_sum[kEvictWaves], s_bin[2], s_before[2][kEvictWaves];
+  __shared__ EvictFind s_find;
+  __shared__ uint32_t s_sum[2][kEvictWaves], s_before[2][kEvictWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t bh = blockIdx.x / a.chunks;
   const int chunk = (int)(blockIdx.x % a.chunks), first = chunk * kChunk;
@@ -434,7 +459,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
   if (m > 0) {
     const uint32_t *const state = a.state + bh * 4;
     want = state[3];
-    const EvictBin at = evict_choose(a, bh, 2, (back + kChunk - 1) / kChunk, want, s_sum, s_bin);
+    const EvictBin at = evict_choose(a, bh, 2, (back + kChunk - 1) / kChunk, want, s_find);
     want -= at.above;
     threshold = state[0] << pass_shift(0) | state[2] << pass_shift(1) | at.bin;
     for (int c = wave; c < chunk; c += kEvictWaves) {
@@ -478,7 +503,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
       if (j >= a.sinks && j < back)
         count += keys.key[i] > threshold ? 1u : keys.key[i] == threshold ? 0x10000u : 0u;
     }
-    const EvictScan s = evict_scan(count, s_sum);
+    const EvictScan s = evict_scan(count, s_sum[n]);
     uint32_t g = gt + (s.before & 0xffffu), e = eq + (s.before >> 16);
 #pragma unroll
     for (int i = 4 * n; i < 4 * n + 4; ++i) {
@@ -503,8 +528,21 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
   }
 }
 
-// Rows of a page's arrivals and their weights, and in 8 bits the page's scales and its
-// other rows; a wave for each page.
+__device__ __forceinline__ int64_t shfl_i64(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__shfl((int)v, lane, 64);
+  return (int64_t)__shfl((int)(v >> 32), lane, 64) << 32 | lo;
+}
+// Most of a lane's page: the largest of the 2^log2 lanes (64 at most) that have it.
+__device__ __forceinline__ uint32_t page_max(uint32_t v, int log2) {
+  for (int m = 1; m < 1 << min(log2, 6); m *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, m, 64));
+  return v;
+}
+
+// Rows of pages' arrivals and their weights, and in 8 bits the pages' scales and their
+// other rows.  A wave for as many pages as have 64 slots together (one of 128): what
+// leads to a row is four loads, each with what the last one brought (256 rows of 4096
+// kept ones of 16 a page, 64 cut: 8 us where each page has a wave 15; 256 recent ones
+// besides, 33 MB: 17 and 21).
 template <bool F8, bool LONG>
 __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int wgs_each) {
   const int lane = threadIdx.x & 63;
@@ -523,20 +561,24 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
   const char *const aside = a.aside + bh * 2 * a.recent * (int64_t)a.row_bytes;
   const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
   const int part = lane % per_row * 16, sub = lane / per_row;
-  int i = wg * 4 + wave;
+  const int at_once = max(1, 64 >> a.bs_log2);  // pages
+  const int mine = bs < 64 ? lane >> a.bs_log2 : 0, row0 = lane & (bs - 1);
+  int i = (wg * 4 + wave) * at_once;
+  const int step = wgs_each * 4 * at_once;
   // Looked up before it is known whether there is one: one wait for both.
-  int next = LONG ? 0 : pages[1 + min(i, n_pages - 1)];
-  for (; i < listed; i += wgs_each * 4) {
-    const int page = LONG ? i : next, slot0 = page << a.bs_log2;
-    if (!LONG) next = pages[1 + min(i + wgs_each * 4, n_pages - 1)];
-    const int count = min(bs, a.keep - slot0);
-    const int blk = LONG && ctx <= a.keep ? -1 : evict_block(a, b, slot0);
+  int next = LONG ? 0 : pages[1 + min(i + mine, n_pages - 1)];
+  for (; i < listed; i += step) {
+    const bool there = i + mine < listed;
+    const int page = LONG ? i + mine : next, slot0 = page << a.bs_log2;
+    if (!LONG) next = pages[1 + min(i + step + mine, n_pages - 1)];
+    const int count = there ? min(bs, a.keep - slot0) : 0;
+    const int blk = !there || (LONG && ctx <= a.keep) ? -1 : evict_block(a, b, slot0);
     // The lane's slots: where they come from (the place itself: it stays), the blocks.
     int src[2], from[2];
     bool any = false;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int r = lane + 64 * n, slot = slot0 + r;
+      const int r = row0 + 64 * n, slot = slot0 + r;
       src[n] = slot;
       from[n] = blk;
       if (r >= count) continue;
@@ -560,79 +602,96 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
       from[n] = evict_block(a, b, src[n]);
       w[slot] = src[n] < a.keep ? a.aside_weights[bh * a.recent + src[n] - front] : w[src[n]];
     }
-    if (blk < 0 || __ballot(any) == 0) continue;
-    // Scales' bytes of keys and values: the page's, its new ones, the rows'.
-    int old[2] = {0, 0}, byte[2] = {0, 0}, scale[2][2] = {{0, 0}, {0, 0}};
+    if (__ballot(any && blk >= 0) == 0) continue;
+    // How far payloads of keys and values are shifted: to the largest scale of the
+    // page's tokens.
+    int shift[2][2] = {{0, 0}, {0, 0}};
     if constexpr (F8) {
+      int old[2] = {0, 0};
       uint32_t top[2] = {0, 0};
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const uint8_t *const scales = kv ? a.v_scales : a.k_scales;
         const uint8_t *const were = a.aside_scales + (bh * 2 + kv) * a.aside_pages -
                                     (front >> a.bs_log2);
-        old[kv] = scales[(int64_t)blk * a.H_kv + h];
+        if (blk >= 0) old[kv] = scales[(int64_t)blk * a.H_kv + h];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const int r = lane + 64 * n, p = src[n] >> a.bs_log2;
-          if (r >= count) continue;
+          const int r = row0 + 64 * n, p = src[n] >> a.bs_log2;
+          if (r >= count || blk < 0) continue;
           // Pages that get arrivals themselves may have another scale by now.
-          scale[kv][n] = src[n] == slot0 + r ? old[kv]
+          shift[kv][n] = src[n] == slot0 + r ? old[kv]
                          : from[n] < 0       ? 0
                          : p <= last_page    ? were[p]
                                              : scales[(int64_t)from[n] * a.H_kv + h];
-          top[kv] = max(top[kv], (uint32_t)scale[kv][n]);
+          top[kv] = max(top[kv], (uint32_t)shift[kv][n]);
         }
       }
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        byte[kv] = (int)wave_max_u32(top[kv]);
-        if (lane == 0 && byte[kv] != old[kv])
-          (kv ? a.v_scales : a.k_scales)[(int64_t)blk * a.H_kv + h] = (uint8_t)byte[kv];
+        const int byte = (int)page_max(top[kv], a.bs_log2);
+        if (row0 == 0 && blk >= 0 && byte != old[kv])
+          (kv ? a.v_scales : a.k_scales)[(int64_t)blk * a.H_kv + h] = (uint8_t)byte;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) shift[kv][n] -= byte;
       }
     }
-    // Two groups of rows of both are read before they are written.
-    constexpr int kBatch = 2;
-    for (int r0 = 0; r0 < count; r0 += rows * kBatch) {
-      uint4 v[kBatch][2];
-      int shift[kBatch][2];
-      bool write[kBatch][2];
-      unrolled<kBatch>([&](auto n) {
-        constexpr int g = decltype(n)::value;
-        const int r = r0 + g * rows + sub, slot = slot0 + r;
-        const bool high = r >= 64;
-        auto of_row = [&](const int (&x)[2]) {
-          const int lo = __shfl(x[0], r & 63, 64), hi = __shfl(x[1], r & 63, 64);
-          return high ? hi : lo;
-        };
-        const int s = of_row(src), s_blk = of_row(from);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          v[g][kv] = make_uint4(0, 0, 0, 0);
-          shift[g][kv] = F8 ? of_row(scale[kv]) - byte[kv] : 0;
-          // One that stays, only where its payload changes with the scale.
-          write[g][kv] = r < count && (s != slot ? s_blk >= 0 : F8 && byte[kv] != old[kv]);
-          if (!write[g][kv]) continue;
-          const char *const p =
-              s != slot && s < a.keep
-                  ? aside + ((int64_t)kv * a.recent + (s - front)) * a.row_bytes
-                  : (kv ? a.v_cache : a.k_cache) + evict_row(a, s_blk, s, h);
-          v[g][kv] = *reinterpret_cast<const uint4 *>(p + part);
-        }
-      });
-      unrolled<kBatch>([&](auto n) {
-        constexpr int g = decltype(n)::value;
-        const int slot = slot0 + r0 + g * rows + sub;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!write[g][kv]) continue;
+    // The rows to be written, those of lanes that have one: four groups of both keys
+    // and values are read before they are written.
+    constexpr int kBatch = 4;
+    unrolled<2>([&](auto half) __attribute__((always_inline)) {
+      constexpr int n = decltype(half)::value;
+      if (n == 1 && bs <= 64) return;
+      const int r = row0 + 64 * n, slot = slot0 + r;
+      const bool moves = src[n] != slot;
+      // One that stays, only where its payload changes with the scale.
+      const bool write =
+          r < count && blk >= 0 && (moves ? from[n] >= 0 : (shift[0][n] | shift[1][n]) != 0);
+      const uint64_t mask = __ballot(write);
+      const int n_rows = __popcll(mask);
+      // Their lanes first, in order.
+      const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                                        __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      const int list = __builtin_amdgcn_ds_permute(
+          (write ? before : n_rows + lane - before) * 4, lane);
+      // Rows of the caches, or -1 - n: row n of those copied aside.
+      const int64_t to = evict_row(a, blk, slot, h);
+      int64_t at = evict_row(a, from[n], src[n], h);
+      if (moves && src[n] < a.keep) at = -1 - (int64_t)(src[n] - front);
+      const int shifts = F8 ? (shift[0][n] + 256) | (shift[1][n] + 256) << 16 : 0;
+      for (int t0 = 0; t0 < n_rows; t0 += rows * kBatch) {
+        uint4 v[kBatch][2];
+        int by[kBatch];
+        int64_t to_row[kBatch];
+        unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
+          constexpr int g = decltype(group)::value;
+          const int t = t0 + g * rows + sub, of = __shfl(list, min(t, 63), 64);
+          int64_t row = shfl_i64(at, of);
+          to_row[g] = shfl_i64(to, of);
+          by[g] = F8 ? __shfl(shifts, of, 64) : 0;
+          v[g][0] = v[g][1] = make_uint4(0, 0, 0, 0);
+          if (t >= n_rows) return;
+          const bool put_aside = row < 0;
+          const char *const k = put_aside ? aside : a.k_cache;
+          const char *const v_ = put_aside ? aside + (int64_t)a.recent * a.row_bytes : a.v_cache;
+          row = (put_aside ? -1 - row : row) * a.row_bytes + part;
+          v[g][0] = *reinterpret_cast<const uint4 *>(k + row);
+          v[g][1] = *reinterpret_cast<const uint4 *>(v_ + row);
+        });
+        unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
+          constexpr int g = decltype(group)::value;
+          if (t0 + g * rows + sub >= n_rows) return;
           if constexpr (F8) {
-            if (shift[g][kv] != 0) v[g][kv] = shifted_8_bits(v[g][kv], shift[g][kv]);
+            const int k = (by[g] & 0xffff) - 256, v_ = (by[g] >> 16) - 256;
+            if (k != 0) v[g][0] = shifted_8_bits(v[g][0], k);
+            if (v_ != 0) v[g][1] = shifted_8_bits(v[g][1], v_);
           }
-          *reinterpret_cast<uint4 *>((kv ? a.v_cache : a.k_cache) + evict_row(a, blk, slot, h) +
-                                     part) = v[g][kv];
-        }
-      });
-    }
+          const int64_t row = to_row[g] * a.row_bytes + part;
+          *reinterpret_cast<uint4 *>(a.k_cache + row) = v[g][0];
+          *reinterpret_cast<uint4 *>(a.v_cache + row) = v[g][1];
+        });
+      }
+    });
   }
 }
 
@@ -658,8 +717,8 @@ static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int64_t keys, int
   p.aside = take((size_t)bh * 2 * recent * row_bytes);
   p.aside_weights = take((size_t)bh * recent * 4);
   p.aside_scales = take(f8 ? (size_t)bh * 2 * p.aside_pages : 0);
-  p.holes = take((size_t)bh * keep * 4);
   if (p.long_rows) {
+    p.holes = take((size_t)bh * keep * 4);
     p.hist = take((size_t)bh * 3 * p.chunks * kBins * 2);
     p.above = take((size_t)bh * p.chunks * 4);
     p.state = take((size_t)bh * 16);
@@ -774,9 +833,11 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
   } else {
     hipLaunchKernelGGL(evict_plan_kernel<4>, first, threads, 0, s, a);
   }
-  // Four pages at once in a workgroup, in turn past 8192 workgroups.
+  // Four waves in a workgroup, in turn past 8192 workgroups.
   const int64_t n_pages = (keep + block_size - 1) / block_size;
-  const int each = (int)std::max<int64_t>(1, std::min<int64_t>((n_pages + 3) / 4, 8192 / bh));
+  const int64_t wave_pages = std::max(1, 64 / block_size);
+  const int each = (int)std::max<int64_t>(
+      1, std::min((n_pages + 4 * wave_pages - 1) / (4 * wave_pages), 8192 / bh));
   const dim3 grid((unsigned)(bh * each));
   auto move = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, each); };
   if (p.long_rows) k_scales ? move(evict_move_kernel<true, true>) : move(evict_move_kernel<false, true>);
