@@ -267,7 +267,7 @@ extern "C" int cvsa_append_chunk_kv8(
   if (!q) once = tokens >= 2048;
   a.groups = r.groups; a.per_wave = r.per_wave; a.segs = r.segs;
   const int64_t wgs = page_wgs + (q_waves + wg_waves - 1) / wg_waves;
-  CVSA_REQUIRE(wgs < (1LL << 31), CVSA_ERR_UNSUPPORTED,
+  CVSA_REQUIRE(wgs < (1LL << 32) / (wg_waves * 64), CVSA_ERR_UNSUPPORTED,
                "append_chunk_kv8: too many tokens, sequences or heads");
   e.page_wgs = (unsigned)page_wgs;
   const dim3 grid((unsigned)wgs), block(wg_waves * 64);

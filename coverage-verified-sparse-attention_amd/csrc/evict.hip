@@ -791,7 +791,7 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
   const int64_t aside = bh * recent * (row_bytes / 16) + (k_scales ? bh * p.aside_pages : 0);
   const int64_t aside_wgs = (aside + kEvictThreads - 1) / kEvictThreads;
   const int64_t select_wgs = p.long_rows ? bh * p.chunks : bh;
-  CVSA_REQUIRE(aside_wgs + select_wgs < (1LL << 31), CVSA_ERR_UNSUPPORTED,
+  CVSA_REQUIRE(aside_wgs + select_wgs < (1LL << 32) / kEvictThreads, CVSA_ERR_UNSUPPORTED,
                "evict_tokens: too many sequences, heads or recent tokens");
   EvictArgs a = {};
   a.weights = weights; a.S = S;

@@ -822,7 +822,7 @@ extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q
   const WeighPlan p =
       plan_weigh(cu_host, B, H_q / H_kv, H_kv, D, window, (int64_t)W * block_size);
   if (!p.few && !p.many) return CVSA_OK;
-  CVSA_REQUIRE(p.passes < (1LL << 31), CVSA_ERR_UNSUPPORTED,
+  CVSA_REQUIRE(p.passes < (1LL << 31) && p.tiles < (1LL << 32) / kWeighKeys, CVSA_ERR_UNSUPPORTED,
                "add_key_weights: too many queries and keys");
   // Offsets among the rows that pass by together are of 32 bits.
   CVSA_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && q_stride_t < (1 << 23) &&

@@ -49,6 +49,8 @@ def add_key_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor,
     nothing.  ``window``: only the last tokens of each sequence's chunk count
     (0: all).  Entries past a context, and of sequences without tokens in the
     chunk, are left as they are; keys of blocks outside the pool get nothing.
+    So a chunk for which this is not called leaves its keys what their slots
+    held, and the caller sets those to 0.
     Sums are of 32 bits, in an order that does not vary.
     """
     who = "add_key_weights"

@@ -123,6 +123,7 @@ class SequenceKVManager:
         self._ctx_host = [0] * batch_size
         self._append_call = None
         self._fuse_shape = None   # (row shape, cache, device) of fusable_rows
+        self._token_layouts = {}   # (first sequence, sequences) -> ChunkLayout of a token each
 
     def adopt(self, block_tables: torch.Tensor, context_lens: torch.Tensor,
               next_free_block: int) -> None:
@@ -226,7 +227,8 @@ class SequenceKVManager:
             want = self._fuse_shape = (torch.Size((self.batch_size, c.shape[2], c.shape[3])),
                                        c, c.device)
         return (k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
-                and c.dtype == torch.bfloat16 and k.shape == want[0] and v.shape == want[0] and k.device == want[2]
+                and c.dtype == torch.bfloat16 and k.shape == want[0] and v.shape == want[0]
+                and k.device == want[2]
                 and v.device == want[2] and k.is_contiguous() and v.is_contiguous()
                 and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0)
 
@@ -280,8 +282,12 @@ class SequenceKVManager:
         n = k.shape[0]
         seqs = range(seq_begin, seq_begin + n)
         if self.cache.k_scales is not None:
-            lens = [int(s in seqs) for s in range(self.batch_size)]
-            self.append_chunk_kv(k, v, ops.ChunkLayout(lens, self.cache.config.device))
+            layout = self._token_layouts.get((seq_begin, n))
+            if layout is None:
+                lens = [int(s in seqs) for s in range(self.batch_size)]
+                layout = self._token_layouts[seq_begin, n] = ops.ChunkLayout(
+                    lens, self.cache.config.device)
+            self.append_chunk_kv(k, v, layout)
             return
         need = self._plan_append(seqs)
         buffers = (self.cache.k_cache, self.cache.v_cache, self.block_tables, self.context_lens,
@@ -363,7 +369,7 @@ class SequenceKVManager:
         (ops.evict_tokens), and its length (:meth:`cut`); returns the old slot
         of each new one.  With a cache per layer, ops.evict_tokens per layer
         and :meth:`cut` once is the same."""
-        self._check_cut(keep)
+        keep = self._check_cut(keep)
         kept = ops.evict_tokens(weights, self.cache.k_cache, self.cache.v_cache,
                                 self.block_tables, self.context_lens, keep, self.block_size,
                                 sinks, recent, self.cache.k_scales, self.cache.v_scales)
@@ -374,13 +380,15 @@ class SequenceKVManager:
         """Take no context as longer than ``keep`` tokens.  Pages stay with their
         sequences, for the tokens to come.  Not while the stream is captured: a
         replay would cut without this manager's count."""
-        self._check_cut(keep)
+        keep = self._check_cut(keep)
         self.context_lens.clamp_(max=keep)
         self._ctx_host = [min(c, keep) for c in self._ctx_host]
 
-    def _check_cut(self, keep):
+    def _check_cut(self, keep) -> int:
+        keep = int(keep)
         if keep < 1:
             raise ValueError(f"a cut to {keep} tokens")
         if ops.chunk.capturing(self.block_tables.device):
             raise RuntimeError("a manager's lengths cannot be cut in a captured graph: capture "
                                "ops.evict_tokens, cut behind it")
+        return keep

@@ -587,7 +587,176 @@ def test_evict_scales_that_far_apart(gpu):
     _check_evict(gpu, bt, ctx, k, v, w, 100, 16, 4, 30)
 
 
+def test_evict_twice_in_place(gpu):
+    """A cut of what a cut left, and one that finds nothing more to do."""
+    g = _gen(31)
+    bt, ctx, k, v, w = _evict_inputs(g, [260, 90], 16, 2, 64, 8)
+    kc, ks, vc, vs, wg, btg, cg = _gpu(gpu, *k, *v, w, bt, ctx)
+    caches, scales, weights = [k[0], v[0]], [k[1], v[1]], w
+    for keep, recent in ((200, 30), (77, 20), (77, 0)):
+        kept = ops.evict_tokens(wg, kc, vc, btg, cg, keep, 16, 3, recent, ks, vs)
+        cg.clamp_(max=keep)
+        want, weights, caches, scales = small.evicted(weights, caches, bt, ctx, keep, 3, recent,
+                                                      scales)
+        ctx = ctx.clamp(max=keep)
+        assert torch.equal(kept.cpu(), want)
+        assert torch.equal(wg.cpu(), weights)
+        for got, c in ((kc, caches[0]), (vc, caches[1])):
+            x, y = got.cpu().view(torch.uint8), c.view(torch.uint8)
+            assert ((x == y) | (x & 0x7f == 0x7f) & (y & 0x7f == 0x7f)).all()
+
+
+# ------------------------------------------------------------ sizes
+
+def test_more_sequences_than_a_wave_has_lanes(gpu):
+    """150 sequences, of none, one and many tokens, in all four."""
+    g = _gen(41)
+    bs, Hk, G, D = 8, 2, 3, 32
+    lens = [(1, 0, 2, 15)[b % 4] for b in range(150)]
+    before = [int(x) for x in torch.randint(0, 60, (150,), generator=g)]
+    totals = [a + b for a, b in zip(lens, before)]
+    q, k, v, bt, ctx = _attend_inputs(g, lens, before, bs, Hk, G, D)
+    new = [_randn(g, sum(lens), Hk, D).bfloat16() for _ in range(2)]
+    kc, ks, vc, vs, btg, cg = _gpu(gpu, *k, *v, bt, ctx)
+    ops.append_chunk_kv(new[0].to(gpu), new[1].to(gpu), kc, vc, btg, cg,
+                        ops.ChunkLayout(lens, gpu), bs, k_scales=ks, v_scales=vs)
+    for got, scales, was, y in ((kc, ks, k, new[0]), (vc, vs, v, new[1])):
+        small.check_appended(got, scales, was, small.appended(
+            y.double(), y.double().abs(), *was, bt, ctx, lens, 0.0))
+    _check_attend(gpu, q, k, v, bt, ctx, lens, G, bs)
+    w = torch.rand(150, Hk, bt.shape[1] * bs, generator=g)
+    keys = small.values(*k)
+    lse = _lse(q, keys, bt, ctx, lens, G, True)
+    _check_weigh(_weigh(gpu, w, q, lse, k, bt, ctx, lens, G, bs),
+                 *small.key_weights(w, q, lse, keys, bt, ctx, lens, G), w)
+    _check_evict(gpu, bt, ctx, k, v, w, 30, bs, 2, 9)
+
+
+@pytest.mark.parametrize("n,G", [(1, 128), (9, 33), (40, 6), (3, 100)])
+def test_weigh_groups_of_any_size(gpu, n, G):
+    """Query heads of a group that no pass of rows is a multiple of, and rows that saw
+    nothing among those of which every key is seen."""
+    g = _gen(G)
+    bs, Hk, D, before = 16, 2, 64, 700
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, [n, 2], [before, 5], bs, Hk, G, D, 8)
+    lse = _lse(q, keys, bt, ctx, [n, 2], G, True)
+    lse[torch.rand(lse.shape, generator=g) < 0.1] = -math.inf
+    for causal in (True, False):
+        got = _weigh(gpu, w, q, lse, k, bt, ctx, [n, 2], G, bs, causal=causal)
+        _check_weigh(got, *small.key_weights(w, q, lse, keys, bt, ctx, [n, 2], G, causal), w)
+
+
+def test_weigh_with_more_heads_than_compute_units(gpu):
+    g = _gen(51)
+    bs, Hk, G, D = 16, 300, 1, 32
+    for lens, before in (([1, 2], [30, 5]), ([40], [3])):
+        q, k, keys, bt, ctx, w = _weigh_inputs(g, lens, before, bs, Hk, G, D, 16)
+        lse = _lse(q, keys, bt, ctx, lens, G, True)
+        _check_weigh(_weigh(gpu, w, q, lse, k, bt, ctx, lens, G, bs),
+                     *small.key_weights(w, q, lse, keys, bt, ctx, lens, G), w)
+
+
+def test_queries_that_heads_share(gpu):
+    """A stride of zero between heads."""
+    g = _gen(61)
+    bs, Hk, G, D, lens, before = 16, 2, 4, 64, [1, 30], [40, 9]
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, lens, before, bs, Hk, G, D, 8)
+    one = q[:, :1].to(gpu).expand(-1, Hk * G, -1)
+    kc, ks, wg, btg, cg = _gpu(gpu, *k, w, bt, ctx)
+    layout = ops.ChunkLayout(lens, gpu)
+    got = [ops.chunk_attention(x, kc, kc, btg, cg, layout, Hk, G, bs, return_lse=True, k_scales=ks,
+                               v_scales=ks) for x in (one, one.contiguous())]
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    sums = [ops.add_key_weights(wg.clone(), x, got[0][1], kc, btg, cg, layout, Hk, G, bs,
+                                k_scales=ks) for x in (one, one.contiguous())]
+    assert torch.equal(*sums)
+
+
 # ------------------------------------------------------------ together
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_serving_loop(gpu, bits):
+    """A manager's prompts, then single tokens, cut again and again: positions that
+    the caller counts, every cached value that of the token which should be there, and
+    each step's attention by its formula over the cache."""
+    g = _gen(71)
+    bs, Hk, G, D, B, keep = 16, 2, 4, 64, 3, 48
+    cache = PagedKVCache(40, bs, Hk, D, device=gpu,
+                         dtype=torch.float8_e4m3fn if bits == 8 else torch.bfloat16)
+    mgr = SequenceKVManager(cache, B, 160)
+    scales = dict(k_scales=cache.k_scales, v_scales=cache.v_scales)
+    table = ops.RotaryTable.build(D, 256, device=gpu)
+    weights = torch.zeros(B, Hk, mgr.block_tables.shape[1] * bs, device=gpu)
+    norm = (1 + 0.2 * _randn(g, D)).to(gpu)
+    tokens = [[] for _ in range(B)]  # (key, value) rows of [Hk, D] as they were appended
+    ids = [[[] for _ in range(Hk)] for _ in range(B)]
+    seen = [0] * B
+
+    def step(lens):
+        layout = ops.ChunkLayout(lens, gpu)
+        T = sum(lens)
+        q, k, v = ((_randn(g, T, n, D) * torch.exp(_randn(g, T, 1, 1))).bfloat16().to(gpu)
+                   for n in (Hk * G, Hk, Hk))
+        pos = torch.cat([torch.arange(s, s + n) for s, n in zip(seen, lens)]).to(gpu)
+        q, k = ops.qk_norm_rope(q, k, pos, table, norm, norm)
+        mgr.append_chunk_kv(k, v, layout)
+        at = 0
+        for b, n in enumerate(lens):
+            for i in range(n):
+                for h in range(Hk):
+                    ids[b][h].append(len(tokens[b]))
+                tokens[b].append((k[at + i].double().cpu(), v[at + i].double().cpu()))
+            at += n
+            seen[b] += n
+        out, lse = ops.chunk_attention(q, cache.k_cache, cache.v_cache, mgr.block_tables,
+                                       mgr.context_lens, layout, Hk, G, bs, return_lse=True,
+                                       **scales)
+        ops.add_key_weights(weights, q, lse, cache.k_cache, mgr.block_tables, mgr.context_lens,
+                            layout, Hk, G, bs, k_scales=cache.k_scales)
+        values = [small.values(c.cpu(), s.cpu()) if bits == 8 else c.double().cpu() for c, s in
+                  ((cache.k_cache, cache.k_scales), (cache.v_cache, cache.v_scales))]
+        bt, ctx = mgr.block_tables.cpu(), mgr.context_lens.cpu()
+        assert ctx.tolist() == [len(x[0]) for x in ids] == mgr._ctx_host
+        ref.check_attend(out, ref.attend(q.cpu(), *values, bt, ctx, lens, G, True), lse)
+        for b in range(B):
+            slot = torch.arange(int(ctx[b]))
+            blk = bt[b].long()[slot // bs]
+            for h in range(Hk):
+                for i, (got, s) in enumerate(zip(values, scales.values())):
+                    want = torch.stack([tokens[b][t][i][h] for t in ids[b][h]])
+                    x = got[blk, slot % bs, h]
+                    if bits == 16:
+                        assert torch.equal(x, want)
+                        continue
+                    # One rounding to e4m3, then shifts to ever larger scales, each off by
+                    # at most half of the smallest step, 2^-10 of its scale: 2 2^-10 of the
+                    # last one together.
+                    unit = torch.exp2(small.scale_bytes(s).double() - 127)[blk, h][:, None]
+                    assert ((x - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -9 * unit).all()
+
+    def cut():
+        before = weights.cpu()
+        old = mgr.context_lens.cpu()
+        kept = mgr.evict_tokens(weights, keep, 4, 16).cpu()
+        for b in range(B):
+            for h in range(Hk):
+                slots = kept[b, h].tolist()[:min(keep, int(old[b]))]
+                ids[b][h] = [ids[b][h][j] for j in slots]
+                # nothing that is gone weighs more than what stays in the middle
+                n = int(old[b])
+                middle = set(range(4, max(4, n - 16)))
+                gone = [float(before[b, h, j]) for j in middle - set(slots)]
+                stay = [float(before[b, h, j]) for j in middle & set(slots)]
+                assert not gone or max(gone) <= min(stay)
+
+    step([70, 5, 33])
+    cut()
+    for n in range(40):
+        step([1, int(n % 3 != 0), 2 if n == 7 else 1])
+        if n % 8 == 7:
+            cut()
+    assert mgr.context_lens.tolist() == [48, 31, 48]
+
 
 def test_two_streams_and_graph_replays(gpu):
     """All four captured once and replayed over new inputs, with eager work in

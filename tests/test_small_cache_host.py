@@ -291,6 +291,11 @@ def test_c_weigh_asks_for_its_workspace():
     assert need > 0
     for over in (dict(), dict(ws=P[9], bytes=need - 1)):
         assert _weigh(lib, cu=(0, 2000), **over) == _lib.CVSA_ERR_WORKSPACE
+    # more tiles than a launch has workgroups of 256 threads
+    many = tuple(40 * b for b in range(4001))
+    wide = dict(W=(1 << 18) - 1, sb=1 << 18, bs=128, S=1 << 25, H_q=1, H_kv=1)
+    assert _weigh(lib, cu=many, **wide) == UNSUPPORTED
+    assert b"too many" in lib.cvsa_last_error()
     # the last few tokens alone need none
     assert lib.cvsa_add_key_weights_workspace_bytes(cu, 1, HK * G, HK, D, W * BS, 8) == 0
 
@@ -311,6 +316,7 @@ def _evict(lib, **over):
     (dict(sinks=18), INVALID, b"sinks=18"), (dict(recent=-1), INVALID, b"recent=-1"),
     (dict(B=0), INVALID, b"B=0"), (dict(sb=W - 1), INVALID, b"bad sizes"),
     (dict(S=W * BS - 1), INVALID, b"weights of"), (dict(vc=P[2] + 8), INVALID, b"aligned"),
+    (dict(B=1 << 19, H_kv=16), UNSUPPORTED, b"too many"),
     (dict(bytes=16), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
     (dict(ws=None), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
     (dict(ws=P[6] + 128), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
@@ -351,6 +357,13 @@ def test_the_manager_appends_to_8_bits(calls):
     assert mgr._ctx_host == [2, 21]
     done = [c[0] for c in calls if c[0] != "cvsa_reserve_chunk"]
     assert done == ["cvsa_append_chunk_kv8"] * 3
+    # the layouts of single tokens are kept
+    first = dict(mgr._token_layouts)
+    assert {k: x.lens for k, x in first.items()} == {(0, 2): (1, 1), (0, 1): (1, 0)}
+    mgr.append_tokens_kv(rows, rows)
+    mgr.append_token_kv(1, rows[0], rows[0])
+    assert all(mgr._token_layouts[k] is x for k, x in first.items())
+    assert mgr._token_layouts[1, 1].lens == (0, 1) and mgr._ctx_host == [3, 23]
 
 
 def test_the_manager_cuts(calls, monkeypatch):
@@ -362,8 +375,10 @@ def test_the_manager_cuts(calls, monkeypatch):
     assert kept.shape == (2, HK, 12) and calls[-1][0] == "cvsa_evict_tokens"
     assert mgr._ctx_host == [12, 7] and mgr.context_lens.tolist() == [12, 7]
     assert mgr._pages_allocated == [3, 1]  # theirs still
-    mgr.cut(100)
+    mgr.cut(100.5)
     assert mgr._ctx_host == [12, 7]
+    mgr.evict_tokens(w, 12.75)
+    assert mgr._ctx_host == [12, 7] and all(type(c) is int for c in mgr._ctx_host)
     n = len(calls)
     for call in (lambda: mgr.cut(0), lambda: mgr.evict_tokens(w, 0),
                  lambda: mgr.evict_tokens(w, 5, 3, 3)):
