@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
   // Two arrays: a load into one does not hold up reads of the other.
   __shared__ __align__(16) uint16_t s_q0[RB * D], s_q1[RB * D];
   __shared__ __align__(16) float s_lse[4][RB];
-  __shared__ int s_low[4][2];  // whether some are -inf, by wave
+  __shared__ uint32_t s_low[4][TILES];  // which are -inf
   constexpr int kAhead = KS < 3 ? KS : 3;
 
   const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -354,6 +354,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
   const WeighRanges ranges(gridDim.x / a.H_kv, total);
   const uint32_t begin = ranges.start(range), end = ranges.start(range + 1);
 
+  // Of two workgroups of a CU the older one's waves go first and would end early, the
+  // other one left alone; so the younger ones are favoured for half of their passes.
+  uint32_t favoured = 2 * blockIdx.x >= gridDim.x ? (end - begin + 1) / 2 : 0;
+  if (favoured > 0) __builtin_amdgcn_s_setprio(1);
+
   // Tokens and heads from a thread's first row to its others, and to the next pass.
   int step_tok[NV], step_g[NV];
 #pragma unroll
@@ -367,8 +372,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
     __builtin_amdgcn_s_waitcnt(0x0f70);
     asm volatile("" ::: "memory");
   };
-  if (tid < 8) s_low[tid / 2][tid % 2] = 0;  // of one wave only where RB is 64
-  __syncthreads();
   const int pass_tok = RB / a.G, pass_g = RB - pass_tok * a.G;
 
   // Passes pass0 .. pass1 of a tile's rows, which are those from its first key's on.
@@ -381,7 +384,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
     const int row0 = pass0 * RB, row1 = min(pass1 * RB, all_rows);
     const int pos0 = s.pos0 + tile_tok;
     const int first_tok = row0 / a.G, first_g = row0 - first_tok * a.G;
+    // What is waited for first is asked for first: where the wave's keys are, then the
+    // rows, then the keys.
     const int32_t *const bt = a.block_tables + seq * a.bt_sb;
+    float *const weights = a.weights + ((int64_t)seq * a.H_kv + h) * a.S;
+    int found[2];
+    float was[2];  // what is added to, of the lanes that write
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = key0 + wave * 64 + i * 32 + l31;
+      found[i] = bt[min(key >> a.bs_log2, a.W - 1)];
+      was[i] = !shared && half == 0 && key < min(s.keys, s.before) ? weights[key] : 0.f;
+    }
 
     // Rows that pass by, straight into LDS: the thread's vectors, 16 bytes each,
     // whose places are permuted as chunk_swizzle has them; and, of pass p, log-sum-
@@ -421,55 +435,50 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
         off += wrap;
       }
     };
-    float next_lse = 0.f;
     const int lse_tok = (first_g + tid % RB) / a.G;
     int lse_g = first_g + tid % RB - lse_tok * a.G;
     const float *lse_at = a.lse +
                           (int64_t)(s.first + tile_tok + first_tok + lse_tok) * a.H_q + h * a.G +
                           lse_g;
     auto request_lse = [&](int r0) __attribute__((always_inline)) {
-      if (tid >= RB) return;
-      next_lse = -INFINITY;
-      if (r0 + tid < row1) {
-        const float x = *lse_at;
-        // A row that saw nothing gives nothing.
-        next_lse = x == -INFINITY ? -INFINITY : -x * a.lse_factor;
-      }
+      float x = -INFINITY;
+      if (tid >= RB) return x;
+      if (r0 + tid < row1) x = *lse_at;
       lse_at += (int64_t)pass_tok * a.H_q + pass_g;
       lse_g += pass_g;
       if (lse_g >= a.G) {
         lse_g -= a.G;
         lse_at += a.H_q - a.G;
       }
+      return x;
     };
-    auto store_lse = [&](int pass) {
+    auto store_lse = [&](int pass, float x) __attribute__((always_inline)) {
       if (tid >= RB) return;
-      s_lse[pass % 4][tid] = next_lse;
-      const bool low = __ballot(next_lse == -INFINITY) != 0;
-      if (lane == 0) s_low[pass % 4][wave] = low ? 1 : 0;
+      // A row that saw nothing gives nothing.
+      const float term = x == -INFINITY ? -INFINITY : -x * a.lse_factor;
+      s_lse[pass % 4][tid] = term;
+      const uint64_t low = __ballot(term == -INFINITY);
+      if (l31 == 0) s_low[pass % 4][tid / 32] = (uint32_t)(half ? low >> 32 : low);
     };
     // The buffers are free: nobody reads what the last tile left.
     const int passes = (row1 - row0 + RB - 1) / RB;
     request(row0, s_q0);
-    request_lse(row0);
-    store_lse(0);
+    const float lse0 = request_lse(row0);
+    float lse1 = 0.f;
     if (passes > 1) {
       request(row0 + RB, s_q1);
-      request_lse(row0 + RB);
-      store_lse(1);
+      lse1 = request_lse(row0 + RB);
     }
 
     // The wave's keys, as the second operand: bf16, the scales apart.
     uint4 k[2][KS];
     float c[2];
-    int min_row[2];
     bool ok[2];
     bool all_ok = true;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int key = key0 + wave * 64 + i * 32 + l31;
-      const WeighKeyAt at =
-          weigh_key_at(a, key, s.keys, bt[min(key >> a.bs_log2, a.W - 1)]);
+      const WeighKeyAt at = weigh_key_at(a, key, s.keys, found[i]);
       ok[i] = at.ok;
       all_ok = all_ok && at.ok;
       const char *p = weigh_row<D, F8>(a, at.blk, at.ok ? key : 0, h);
@@ -485,8 +494,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
           k[i][ks] = *reinterpret_cast<const uint4 *>(p + ks * 32 + half * 16);
         c[i] = a.c;
       }
-      min_row[i] = a.causal && key > pos0 ? min(key - pos0, kWeighKeys) * a.G : 0;
     }
+    // The first row that sees the lane's first key (the second one is 32 tokens on), or
+    // one before the tile's: the difference is cut there, its product could overflow.
+    const int min_row =
+        (a.causal ? max(key0 + wave * 64 + l31 - pos0, -kWeighKeys) : -kWeighKeys) * a.G;
     // Rows from here on see all of the wave's keys.
     const int last_key = key0 + wave * 64 + 63;
     const int full_row = a.causal && last_key > pos0 ? min(last_key - pos0, kWeighKeys) * a.G : 0;
@@ -495,6 +507,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
     const int first_row =
         a.causal && first_key > pos0 ? min(first_key - pos0, kWeighKeys) * a.G : 0;
     const bool keys_ok = __ballot(!all_ok) == 0;
+
+    store_lse(0, lse0);
+    if (passes > 1) store_lse(1, lse1);
 
     float sum[2] = {0.f, 0.f};
     loaded();
@@ -515,18 +530,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
     // Exponentials of st, the scores of 32 rows, between the products of the next 32;
     // neg: the first of the rows' terms, and then of the next ones'.
     float4 neg;
-    // MASK: of the scores that are not all seen, those that are count.
+    // MASK: of the scores that are not all seen, those that are count, but for rows past
+    // the last and those that saw nothing, whose terms are -inf (none: bits).
     auto weigh = [&](const f32x16_t (&st)[2], int base, const float *lse, f32x16_t (&nxt)[2],
-                     const uint16_t *rows, const float *next_lse, auto mask)
+                     const uint16_t *rows, const float *next_lse, auto mask, uint32_t none)
         __attribute__((always_inline)) {
       constexpr bool MASK = decltype(mask)::value;
-      place.renew();
       unrolled<kAhead>([&](auto n) { fetch(rows, n); });
       // Eight scores, four rows of both of the lane's keys, at a time; each is added
       // one later: an addition right behind the exponential would wait.
       float part[2][4], last = 0.f;
       float4 next_neg;
-      const int low[2] = {min_row[0] - base - 4 * half, min_row[1] - base - 4 * half};
+      // Bits 8 g + x of the lane's rows that see its keys and count.
+      uint32_t seen[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        seen[i] = ~0u << min(max(0, min_row + i * 32 * a.G - base - 4 * half), 31) &
+                  ~(none >> 4 * half);
       auto add = [&](auto n, float p) {
         constexpr int m = decltype(n)::value, i = m % 8 / 4, x = m % 4;
         part[i][x] = m / 8 == 0 ? p : part[i][x] + p;
@@ -545,8 +565,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
         });
         const float ref = x == 0 ? neg.x : x == 1 ? neg.y : x == 2 ? neg.z : neg.w;
         float p = __builtin_amdgcn_exp2f(fmaf(st[i][4 * g + x], c[i], ref));
-        // Rows past the last, and those that saw nothing, have a term of -inf.
-        if constexpr (MASK) p = 8 * g + x >= low[i] && ref != -INFINITY ? p : 0.f;
+        if constexpr (MASK) {
+          int on;  // the builtin becomes a comparison and a selection
+          asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(on) : "v"(seen[i]), "n"(8 * g + x));
+          p = __int_as_float(__float_as_int(p) & on);
+        }
         if constexpr (m > 0) add(std::integral_constant<int, m - 1>(), last);
         last = p;
         if constexpr (m % 8 == 7) neg = next_neg;
@@ -558,12 +581,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
         sum[i] += (part[i][0] + part[i][1]) + (part[i][2] + part[i][3]);
     };
     auto rows32 = [&](const f32x16_t (&st)[2], int base, const float *lse, f32x16_t (&nxt)[2],
-                      const uint16_t *rows, const float *next_lse, bool all)
+                      const uint16_t *rows, const float *next_lse, uint32_t none)
         __attribute__((always_inline)) {
-      if (keys_ok && all && base >= full_row) {
-        weigh(st, base, lse, nxt, rows, next_lse, std::false_type());
+      place.renew();
+      if (keys_ok && none == 0 && base >= full_row) {
+        weigh(st, base, lse, nxt, rows, next_lse, std::false_type(), none);
       } else if (base + 32 > first_row) {
-        weigh(st, base, lse, nxt, rows, next_lse, std::true_type());
+        weigh(st, base, lse, nxt, rows, next_lse, std::true_type(), none);
       } else {  // none of them sees any of the wave's keys
         neg = *reinterpret_cast<const float4 *>(next_lse + 4 * half);
         if (base + 64 > first_row)
@@ -585,26 +609,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
     auto pass = [&](int p, uint16_t *cur, uint16_t *next) __attribute__((always_inline)) {
       const int r0 = row0 + p * RB;
       const float *const lse = s_lse[p % 4];
-      const bool all = __builtin_amdgcn_readfirstlane(s_low[p % 4][0] | s_low[p % 4][1]) == 0;
+      auto none = [&](int i) { return (uint32_t)__builtin_amdgcn_readfirstlane(s_low[p % 4][i]); };
       unrolled<TILES - 1>([&](auto n) __attribute__((always_inline)) {
         constexpr int i = decltype(n)::value;
         if constexpr (i % 2 == 0)
           rows32(st0, r0 + 32 * i, lse + 32 * i, st1, cur + 32 * (i + 1) * D, lse + 32 * (i + 1),
-                 all);
+                 none(i));
         else
           rows32(st1, r0 + 32 * i, lse + 32 * i, st0, cur + 32 * (i + 1) * D, lse + 32 * (i + 1),
-                 all);
+                 none(i));
       });
       loaded();
       __syncthreads();
       const bool more = p + 2 < passes;
+      float next_lse = 0.f;
       if (more) {
         request(r0 + 2 * RB, cur);
-        request_lse(r0 + 2 * RB);
+        next_lse = request_lse(r0 + 2 * RB);
       }
       constexpr int i = TILES - 1;
-      rows32(st1, r0 + 32 * i, lse + 32 * i, st0, next, s_lse[(p + 1) % 4], all);
-      if (more) store_lse(p + 2);
+      rows32(st1, r0 + 32 * i, lse + 32 * i, st0, next, s_lse[(p + 1) % 4], none(i));
+      if (more) store_lse(p + 2, next_lse);
+      if (favoured > 0 && --favoured == 0) __builtin_amdgcn_s_setprio(0);
     };
     static_assert(TILES % 2 == 0, "two sets of scores in turn");
     for (int p = 0; p < passes; p += 2) {
@@ -622,8 +648,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
       if (shared) {
         a.parts[(((int64_t)range * a.H_kv + h) * 2 + (pass0 == 0)) * kWeighKeys + at] = all;
       } else if (key < s.keys) {
-        float *const w = a.weights + ((int64_t)seq * a.H_kv + h) * a.S + key;
-        *w = (key < s.before ? *w : 0.f) + all;
+        weights[key] = was[i] + all;
       }
     }
   };

@@ -152,11 +152,18 @@ class SequenceKVManager:
         seq_len = k_all.shape[0]
         bs = self.block_size
         n_pages = (seq_len + bs - 1) // bs
+        launch = None
+        if self.cache.k_scales is not None:  # checked before a block is taken
+            launch, _ = ops.prepare_append_chunk(
+                k_all, v_all, self.cache.k_cache, self.cache.v_cache,
+                self.block_tables[seq_idx][None], self.context_lens[seq_idx][None],
+                ops.ChunkLayout([seq_len], self.cache.config.device), bs,
+                k_scales=self.cache.k_scales, v_scales=self.cache.v_scales)
         block_ids = self.cache.allocate_blocks(n_pages)
         self.block_tables[seq_idx, :n_pages] = block_ids
-        if self.cache.k_scales is not None:
+        if launch is not None:
             self.context_lens[seq_idx] = seq_len
-            self._write_8_bits(k_all, v_all, seq_idx, [seq_len])
+            launch()
             self._pages_allocated[seq_idx] = n_pages
             self._pages_allocated_dev[seq_idx] = n_pages
             self._ctx_host[seq_idx] = seq_len
@@ -176,14 +183,6 @@ class SequenceKVManager:
         self._pages_allocated[seq_idx] = n_pages
         self._pages_allocated_dev[seq_idx] = n_pages
         self._ctx_host[seq_idx] = seq_len
-
-    def _write_8_bits(self, k, v, first, lens):
-        """Tokens of sequences first .. that the tables count already."""
-        last = first + len(lens)
-        ops.append_chunk_kv(k, v, self.cache.k_cache, self.cache.v_cache,
-                            self.block_tables[first:last], self.context_lens[first:last],
-                            ops.ChunkLayout(lens, self.cache.config.device), self.block_size,
-                            k_scales=self.cache.k_scales, v_scales=self.cache.v_scales)
 
     def _plan_append(self, seqs) -> int:
         """Blocks the append of one token to each of `seqs` allocates."""

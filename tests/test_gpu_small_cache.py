@@ -9,6 +9,7 @@ import torch
 import chunk_reference as ref
 import small_cache_reference as small
 from cvsa import ops
+from cvsa.runtime.dense import DenseAttentionBackend
 from cvsa.runtime.kv_cache import PagedKVCache, SequenceKVManager
 
 pytestmark = pytest.mark.gpu
@@ -831,3 +832,40 @@ def test_two_streams_and_graph_replays(gpu):
     for seed, x, (out, kept) in zip((2, 3), states, got):
         for a, b in zip([out, kept] + x.state(), want[seed]):
             assert torch.equal(a, b)
+
+
+def test_the_managers_other_appends(gpu):
+    """Prompts and single tokens without a layout, before and after a cut, are what a
+    chunk writes; the backend's prefill is the attention over them."""
+    g = _gen(81)
+    bs, Hk, D, B = 16, 2, 64, 2
+    k, v = (_randn(g, 60, Hk, D).bfloat16().to(gpu) for _ in range(2))
+    caches = [PagedKVCache(16, bs, Hk, D, dtype=torch.float8_e4m3fn, device=gpu) for _ in "ab"]
+    one, other = (SequenceKVManager(c, B, 96) for c in caches)
+    one.prefill_kv(0, k[:37], v[:37])
+    one.prefill_kv(1, k[37:42], v[37:42])
+    other.append_chunk_kv(k[:37], v[:37], ops.ChunkLayout([37, 0], gpu))
+    other.append_chunk_kv(k[37:42], v[37:42], ops.ChunkLayout([0, 5], gpu))
+    w = torch.rand(B, Hk, one.block_tables.shape[1] * bs, generator=g).to(gpu)
+    for m in (one, other):
+        assert m.evict_tokens(w.clone(), 20, 1, 3).shape == (B, Hk, 20)
+    one.append_tokens_kv(k[42:44], v[42:44])
+    one.append_token_kv(1, k[44], v[44])
+    one.append_token_kv(0, k[45], v[45])
+    other.append_chunk_kv(k[42:44], v[42:44], ops.ChunkLayout([1, 1], gpu))
+    other.append_chunk_kv(k[44:45], v[44:45], ops.ChunkLayout([0, 1], gpu))
+    other.append_chunk_kv(k[45:46], v[45:46], ops.ChunkLayout([1, 0], gpu))
+    assert one._ctx_host == other._ctx_host == one.context_lens.tolist() == [22, 7]
+    a, b = caches
+    for x, y in ((a.k_cache, b.k_cache), (a.v_cache, b.v_cache), (a.k_scales, b.k_scales),
+                 (a.v_scales, b.v_scales)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    q = _randn(g, 2, 8, D).bfloat16().to(gpu)
+    layout = ops.ChunkLayout([1, 1], gpu)
+    got = DenseAttentionBackend(Hk, Hk * 4, D, bs).prefill(
+        q, a.k_cache, a.v_cache, one.block_tables, one.context_lens, layout, max_context_len=22,
+        k_scales=a.k_scales, v_scales=a.v_scales)
+    want = ops.chunk_attention(q, a.k_cache, a.v_cache, one.block_tables, one.context_lens, layout,
+                               Hk, 4, bs, max_context_len=22, k_scales=a.k_scales,
+                               v_scales=a.v_scales)
+    assert torch.equal(got, want)

@@ -366,6 +366,20 @@ def test_the_manager_appends_to_8_bits(calls):
     assert mgr._token_layouts[1, 1].lens == (0, 1) and mgr._ctx_host == [3, 23]
 
 
+def test_a_refused_prompt_takes_no_block(calls):
+    cache, mgr = _manager()
+    for k, v in ((_bf(20, HK, D), _bf(19, HK, D)), (_bf(20, HK, D), _bf(20, HK, D).float()),
+                 (_bf(20, HK, D + 8), _bf(20, HK, D + 8)), (_bf(20, HK + 1, D), _bf(20, HK, D))):
+        with pytest.raises(ValueError):
+            mgr.prefill_kv(0, k, v)
+    assert cache._next_free == 0 and mgr._ctx_host == [0, 0] and not calls
+    assert mgr.context_lens.tolist() == [0, 0]
+    mgr.prefill_kv(1, _bf(0, HK, D), _bf(0, HK, D))
+    assert mgr._ctx_host == [0, 0] and not calls
+    mgr.prefill_kv(-1, _bf(17, HK, D), _bf(17, HK, D))  # the last sequence
+    assert mgr._ctx_host == [0, 17] and len(calls) == 1
+
+
 def test_the_manager_cuts(calls, monkeypatch):
     cache, mgr = _manager()
     mgr.prefill_kv(0, _bf(40, HK, D), _bf(40, HK, D))
