@@ -16,13 +16,16 @@
 // have a workgroup each, a launch for each histogram and one for the walk, in which
 // every chunk adds up the others' counts (131072 slots, 8 heads: one workgroup each
 // 167 us, so 30 before the rows are moved).
-// A destination is a source itself only among slots keep - recent .. keep: other
-// workgroups of the first launch copy these aside.  In the last launch a wave for
-// 64 slots moves their arrivals, in no order.
 //
-// Measured: 32 sequences of 8 heads, 4160 tokens to 4096, 256 of them recent, 8 bits: 19
-// us for the plan and what is copied aside (6 of them; 4 are the searches) and 22 to
-// move, for 51 MB.  131072 to 16384, 8 heads of bf16: 7 + 7 + 7 + 9 and 13, for 125 MB.
+// A destination is a source itself only among slots keep - recent .. keep.  Where there
+// are many sequences and heads, the workgroup that planned moves the rows too: those of
+// the holes, then the window's in rounds, in order, each read before it is written.
+// Else a wave for each 64 slots moves their arrivals in a launch of its own, in no
+// order, and workgroups of the first launch copy the window's rows aside.
+//
+// Measured: 32 sequences of 8 heads, 4160 tokens to 4096, 256 of them recent, 8 bits: 26
+// to 30 us in one launch for 51 MB (23 where the caches hold some of them; 12 until the
+// rows are known); 131072 to 16384, 8 heads of bf16: 7 + 7 + 7 + 9 and 13, for 125 MB.
 // Both are chains of short dependent steps, not bound by a rate.
 //
 // 8 bits: a page with arrivals gets the largest scale of its tokens' pages; payloads
@@ -223,21 +226,147 @@ __device__ __forceinline__ void evict_copy_aside(const EvictArgs &a) {
   a.aside_scales[(bh * 2 + 1) * a.aside_pages + n] = a.v_scales[(int64_t)blk * a.H_kv + h];
 }
 
-// Short rows: old slots of the new ones, and the pages with arrivals; N steps of 4096
-// slots.
-template <int N>
+__device__ __forceinline__ int64_t shfl_i64(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__shfl((int)v, lane, 64);
+  return (int64_t)__shfl((int)(v >> 32), lane, 64) << 32 | lo;
+}
+// Most of a lane's page: the largest of the 2^log2 lanes (64 at most) that have it.
+__device__ __forceinline__ uint32_t page_max(uint32_t v, int log2) {
+  for (int m = 1; m < 1 << min(log2, 6); m *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, m, 64));
+  return v;
+}
+
+// What a lane's page gets: where its slots' rows come from.
+struct EvictPage {
+  int page, slot0, count, blk;  // count slots; blk -1: none of the pool
+  int src[2], from[2];          // of the lane's slots: old slots (themselves: they stay), blocks
+  int shift[2][2];              // of keys' and values' payloads
+  int byte[2];                  // the page's scales, where they change (-1)
+};
+
+// The page's scales, and how far payloads are shifted: to the largest scale of the
+// page's tokens.  were: of keys and values, those of pages up to last_page, which may
+// have got others by now (null: none has).
+__device__ __forceinline__ void evict_scales(const EvictArgs &a, int h, int row0,
+                                             const uint8_t *were_k, const uint8_t *were_v,
+                                             EvictPage &p) {
+  const int last_page = (a.keep - 1) >> a.bs_log2;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint8_t *const scales = kv ? a.v_scales : a.k_scales;
+    const uint8_t *const were = kv ? were_v : were_k;
+    const int old = p.blk >= 0 ? scales[(int64_t)p.blk * a.H_kv + h] : 0;
+    uint32_t top = 0;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = row0 + 64 * n, of = p.src[n] >> a.bs_log2;
+      p.shift[kv][n] = 0;
+      if (r >= p.count || p.blk < 0) continue;
+      p.shift[kv][n] = p.src[n] == p.slot0 + r   ? old
+                       : p.from[n] < 0           ? 0
+                       : were && of <= last_page ? were[of]
+                                                 : scales[(int64_t)p.from[n] * a.H_kv + h];
+      top = max(top, (uint32_t)p.shift[kv][n]);
+    }
+    const int byte = (int)page_max(top, a.bs_log2);
+    p.byte[kv] = byte != old ? byte : -1;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) p.shift[kv][n] -= byte;
+  }
+}
+__device__ __forceinline__ void evict_put_scales(const EvictArgs &a, int h, int row0,
+                                                 const EvictPage &p) {
+  if (row0 != 0 || p.blk < 0) return;
+  if (p.byte[0] >= 0) a.k_scales[(int64_t)p.blk * a.H_kv + h] = (uint8_t)p.byte[0];
+  if (p.byte[1] >= 0) a.v_scales[(int64_t)p.blk * a.H_kv + h] = (uint8_t)p.byte[1];
+}
+// Whether the row of the lane's slot n is written: one that stays, only where its
+// payload changes with the scale.
+__device__ __forceinline__ bool evict_writes(const EvictPage &p, int row0, int n) {
+  const int r = row0 + 64 * n;
+  return r < p.count && p.blk >= 0 &&
+         (p.src[n] != p.slot0 + r ? p.from[n] >= 0 : (p.shift[0][n] | p.shift[1][n]) != 0);
+}
+
+// Moves the rows that a wave's lanes have to write, each of its slots; four groups of
+// both keys and values are read before they are written.  ASIDE: old slots front ..
+// keep are read where they were copied to.
+template <bool F8, bool ASIDE>
+__device__ __forceinline__ void evict_move_rows(const EvictArgs &a, int h, int row0,
+                                                const EvictPage &p, const char *aside,
+                                                int front) {
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 63;
+  const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
+  const int part = lane % per_row * 16, sub = lane / per_row;
+  unrolled<2>([&](auto half) __attribute__((always_inline)) {
+    constexpr int n = decltype(half)::value;
+    if (n == 1 && a.bs_log2 <= 6) return;
+    const int slot = p.slot0 + row0 + 64 * n;
+    const bool write = evict_writes(p, row0, n);
+    const uint64_t mask = __ballot(write);
+    const int n_rows = __popcll(mask);
+    // Their lanes first, in order.
+    const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    const int list = __builtin_amdgcn_ds_permute(
+        (write ? before : n_rows + lane - before) * 4, lane);
+    // Rows of the caches, or -1 - n: row n of those copied aside.
+    const int64_t to = evict_row(a, p.blk, slot, h);
+    int64_t at = evict_row(a, p.from[n], p.src[n], h);
+    if (ASIDE && p.src[n] != slot && p.src[n] < a.keep) at = -1 - (int64_t)(p.src[n] - front);
+    const int shifts = F8 ? (p.shift[0][n] + 256) | (p.shift[1][n] + 256) << 16 : 0;
+    for (int t0 = 0; t0 < n_rows; t0 += rows * kBatch) {
+      uint4 v[kBatch][2];
+      int by[kBatch];
+      int64_t to_row[kBatch];
+      unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
+        constexpr int g = decltype(group)::value;
+        const int t = t0 + g * rows + sub, of = __shfl(list, min(t, 63), 64);
+        int64_t row = shfl_i64(at, of);
+        to_row[g] = shfl_i64(to, of);
+        by[g] = F8 ? __shfl(shifts, of, 64) : 0;
+        v[g][0] = v[g][1] = make_uint4(0, 0, 0, 0);
+        if (t >= n_rows) return;
+        const bool put_aside = ASIDE && row < 0;
+        const char *const k = put_aside ? aside : a.k_cache;
+        const char *const v_ = put_aside ? aside + (int64_t)a.recent * a.row_bytes : a.v_cache;
+        row = (put_aside ? -1 - row : row) * a.row_bytes + part;
+        v[g][0] = *reinterpret_cast<const uint4 *>(k + row);
+        v[g][1] = *reinterpret_cast<const uint4 *>(v_ + row);
+      });
+      unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
+        constexpr int g = decltype(group)::value;
+        if (t0 + g * rows + sub >= n_rows) return;
+        if constexpr (F8) {
+          const int k = (by[g] & 0xffff) - 256, v_ = (by[g] >> 16) - 256;
+          if (k != 0) v[g][0] = shifted_8_bits(v[g][0], k);
+          if (v_ != 0) v[g][1] = shifted_8_bits(v[g][1], v_);
+        }
+        const int64_t row = to_row[g] * a.row_bytes + part;
+        *reinterpret_cast<uint4 *>(a.k_cache + row) = v[g][0];
+        *reinterpret_cast<uint4 *>(a.v_cache + row) = v[g][1];
+      });
+    }
+  });
+}
+
+// Short rows: old slots of the new ones; N steps of 4096 slots.  Then the pages with
+// arrivals (MOVE 0), or their rows are moved here (1, and 2: of 8 bits).
+template <int N, int MOVE>
 __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictArgs a) {
-  if ((int)blockIdx.x >= a.select_wgs) {
+  if (MOVE == 0 && (int)blockIdx.x >= a.select_wgs) {
     evict_copy_aside(a);
     return;
   }
   // Histograms, the passes' in turn, as each leaves its own cleared; after them, in
-  // their place, the holes.
-  constexpr int kPages = N * 4 * kEvictThreads / 8;
+  // their place, the holes and the old slots.
+  constexpr int kSlots = N * 4 * kEvictThreads, kPages = kSlots / 8;
   __shared__ __align__(16) union {
     uint32_t hist[2][kCopies][kBins];
-    uint16_t holes[N * 4 * kEvictThreads];
+    uint16_t slots[2][kSlots];
   } s;
+  uint16_t *const holes = s.slots[0], *const src = s.slots[1];
   __shared__ __align__(16) uint8_t s_page[kPages];
   __shared__ EvictFind s_find[3];
   __shared__ uint32_t s_step[N][kEvictWaves], s_sum[2][kEvictWaves], s_stay;
@@ -251,10 +380,10 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
   const int ctx = evict_context(a, b);
   int32_t *const kept = a.kept + bh * a.keep;
   const int n_pages = (a.keep + (1 << a.bs_log2) - 1) >> a.bs_log2;
-  int32_t *const pages = a.pages + bh * (1 + n_pages);
+  int32_t *const pages = MOVE ? nullptr : a.pages + bh * (1 + n_pages);
   if (ctx <= a.keep) {  // nothing to cut
     for (int j = tid; j < a.keep; j += kEvictThreads) kept[j] = j < ctx ? j : -1;
-    if (tid == 0) pages[0] = 0;
+    if (MOVE == 0 && tid == 0) pages[0] = 0;
     return;
   }
   const int front = a.keep - a.recent, back = ctx - a.recent;
@@ -286,8 +415,12 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
 
   // The slots in order: the kept ones below `front` stay, the others are holes; the
   // kept ones behind fill them.  Counts of larger and (high half) equal weights.
-  for (int j = tid; j < a.sinks; j += kEvictThreads) kept[j] = j;
-  for (int j = tid; j < a.recent; j += kEvictThreads) kept[front + j] = back + j;
+  auto put = [&](int slot, int old) {
+    kept[slot] = old;
+    if (MOVE) src[slot] = (uint16_t)old;
+  };
+  for (int j = tid; j < a.sinks; j += kEvictThreads) put(j, j);
+  for (int j = tid; j < a.recent; j += kEvictThreads) put(front + j, back + j);
   uint32_t count[N], incl[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -327,9 +460,9 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
       if (j == front) s_stay = rank[i];  // the next slot after those that may stay
       if (in && j < front) {
         if (keep) {
-          kept[j] = j;
+          put(j, j);
         } else {
-          s.holes[(uint32_t)(j - a.sinks) - rank[i]] = (uint16_t)j;
+          holes[(uint32_t)(j - a.sinks) - rank[i]] = (uint16_t)j;
           s_page[j >> a.bs_log2] = 1;
         }
       }
@@ -342,18 +475,103 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
   const uint32_t stay = s_stay;
 #pragma unroll
   for (int i = 0; i < 4 * N; ++i)
-    if (rank[i] != 0xffffffffu) kept[s.holes[rank[i] - stay]] = keys.slot(0, i);
+    if (rank[i] != 0xffffffffu) put(holes[rank[i] - stay], keys.slot(0, i));
 
   // Pages with arrivals: those of holes, and from front on all.
+  const int window = front >> a.bs_log2;  // its first page
+  __shared__ uint16_t s_list[MOVE ? kPages : 1];
   int listed = 0;
   for (int p0 = 0, turn = 0; p0 < n_pages; p0 += kEvictThreads, turn ^= 1) {
     const int p = p0 + tid;
-    const bool any = p < n_pages && (s_page[p] || (a.recent > 0 && p >= front >> a.bs_log2));
+    const bool any = p < n_pages && (MOVE ? p < window && s_page[p]
+                                          : s_page[p] || (a.recent > 0 && p >= window));
     const EvictScan sum = evict_scan(any ? 1u : 0u, s_sum[turn]);
-    if (any) pages[1 + listed + sum.before] = p;
+    if (any && MOVE) s_list[listed + sum.before] = (uint16_t)p;
+    if (any && !MOVE) pages[1 + listed + sum.before] = p;
     listed += (int)sum.all;
   }
-  if (tid == 0) pages[0] = listed;
+  if constexpr (MOVE == 0) {
+    if (tid == 0) pages[0] = listed;
+  } else {
+    constexpr bool F8 = MOVE == 2;
+    __syncthreads();
+    const int h = (int)(bh % a.H_kv), lane = tid & 63, bs = 1 << a.bs_log2;
+    const int at_once = 64 >> a.bs_log2;  // pages of a wave, of 64 slots at most
+    const int mine = lane >> a.bs_log2, row0 = lane & (bs - 1);
+    auto look = [&](bool there, int page) __attribute__((always_inline)) {
+      EvictPage p = {page, page << a.bs_log2, 0, -1};
+      if (there) {
+        p.count = min(bs, a.keep - p.slot0);
+        p.blk = evict_block(a, b, p.slot0);
+      }
+      const int slot = p.slot0 + row0;
+      p.src[0] = row0 < p.count ? src[slot] : slot;
+      p.from[0] = p.src[0] != slot ? evict_block(a, b, p.src[0]) : p.blk;
+      p.src[1] = slot + 64;
+      p.from[1] = -1;
+      p.shift[0][0] = p.shift[1][0] = p.shift[0][1] = p.shift[1][1] = 0;
+      return p;
+    };
+    // Those before the window's are no sources.
+    for (int i = wave * at_once; i < listed; i += kEvictWaves * at_once) {
+      const bool there = i + mine < listed;
+      EvictPage p = look(there, s_list[there ? i + mine : 0]);
+      const int slot = p.slot0 + row0;
+      if (p.src[0] != slot) w[slot] = w[p.src[0]];
+      if constexpr (F8) {
+        evict_scales(a, h, row0, nullptr, nullptr, p);
+        evict_put_scales(a, h, row0, p);
+      }
+      evict_move_rows<F8, false>(a, h, row0, p, nullptr, front);
+    }
+    __syncthreads();
+    // The window's, in rounds, each read before it is written.  What a round reads lies
+    // at the slots that it writes or behind them, so rounds before have not written it.
+    const int per = min(at_once, max(1, (n_pages - window + kEvictWaves - 1) / kEvictWaves));
+    const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
+    const int part = lane % per_row * 16, sub = lane / per_row;
+    constexpr int kSteps = 16;  // rows of 256 bytes at most
+    for (int q0 = window; q0 < n_pages; q0 += kEvictWaves * per) {
+      const int page = q0 + wave * per + mine;
+      EvictPage p = look(mine < per && page < n_pages, page);
+      const int slot = p.slot0 + row0;
+      const bool moves = p.src[0] != slot;
+      const float weight = moves ? w[p.src[0]] : 0.f;
+      if constexpr (F8) evict_scales(a, h, row0, nullptr, nullptr, p);
+      const int write = evict_writes(p, row0, 0) ? 1 : 0;
+      const int64_t at = evict_row(a, p.from[0], p.src[0], h), to = evict_row(a, p.blk, slot, h);
+      const int slots = per << a.bs_log2;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        char *const cache = kv ? a.v_cache : a.k_cache;
+        uint4 v[kSteps];
+        unrolled<kSteps>([&](auto step) __attribute__((always_inline)) {
+          constexpr int n = decltype(step)::value;
+          v[n] = make_uint4(0, 0, 0, 0);
+          if (n * rows >= slots) return;
+          const int of = n * rows + sub;
+          const int64_t row = shfl_i64(at, of);
+          if (__shfl(write, of, 64))
+            v[n] = *reinterpret_cast<const uint4 *>(cache + row * a.row_bytes + part);
+        });
+        __syncthreads();
+        if (kv == 0) {
+          if (moves) w[slot] = weight;
+          if constexpr (F8) evict_put_scales(a, h, row0, p);
+        }
+        unrolled<kSteps>([&](auto step) __attribute__((always_inline)) {
+          constexpr int n = decltype(step)::value;
+          if (n * rows >= slots) return;
+          const int of = n * rows + sub;
+          const int64_t row = shfl_i64(to, of);
+          const int by = F8 ? __shfl(p.shift[kv][0], of, 64) : 0;
+          if (!__shfl(write, of, 64)) return;
+          if (F8 && by != 0) v[n] = shifted_8_bits(v[n], by);
+          *reinterpret_cast<uint4 *>(cache + row * a.row_bytes + part) = v[n];
+        });
+      }
+    }
+  }
 }
 
 // Long rows: the bins that pass `pass` chooses from the histograms of all chunks.
@@ -528,16 +746,6 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
   }
 }
 
-__device__ __forceinline__ int64_t shfl_i64(int64_t v, int lane) {
-  const uint32_t lo = (uint32_t)__shfl((int)v, lane, 64);
-  return (int64_t)__shfl((int)(v >> 32), lane, 64) << 32 | lo;
-}
-// Most of a lane's page: the largest of the 2^log2 lanes (64 at most) that have it.
-__device__ __forceinline__ uint32_t page_max(uint32_t v, int log2) {
-  for (int m = 1; m < 1 << min(log2, 6); m *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, m, 64));
-  return v;
-}
-
 // Rows of pages' arrivals and their weights, and in 8 bits the pages' scales and their
 // other rows.  A wave for as many pages as have 64 slots together (one of 128): what
 // leads to a row is four loads, each with what the last one brought (256 rows of 4096
@@ -553,14 +761,11 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
   const int64_t bh = (int64_t)b * a.H_kv + h;
   const int bs = 1 << a.bs_log2, n_pages = (a.keep + bs - 1) >> a.bs_log2;
   const int ctx = LONG ? evict_context(a, b) : 0, front = a.keep - a.recent;
-  const int last_page = (a.keep - 1) >> a.bs_log2;
   int32_t *const kept = a.kept + bh * a.keep;
   float *const w = a.weights + bh * a.S;
   const int32_t *const pages = LONG ? nullptr : a.pages + bh * (1 + n_pages);
   const int listed = LONG ? n_pages : pages[0];
   const char *const aside = a.aside + bh * 2 * a.recent * (int64_t)a.row_bytes;
-  const int per_row = a.row_bytes / 16, rows = 64 / per_row;  // lanes of a row, rows at once
-  const int part = lane % per_row * 16, sub = lane / per_row;
   const int at_once = max(1, 64 >> a.bs_log2);  // pages
   const int mine = bs < 64 ? lane >> a.bs_log2 : 0, row0 = lane & (bs - 1);
   int i = (wg * 4 + wave) * at_once;
@@ -573,14 +778,15 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
     if (!LONG) next = pages[1 + min(i + step + mine, n_pages - 1)];
     const int count = there ? min(bs, a.keep - slot0) : 0;
     const int blk = !there || (LONG && ctx <= a.keep) ? -1 : evict_block(a, b, slot0);
-    // The lane's slots: where they come from (the place itself: it stays), the blocks.
-    int src[2], from[2];
+    // The lane's slots.
+    EvictPage p = {page, slot0, count, blk};
     bool any = false;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int r = row0 + 64 * n, slot = slot0 + r;
-      src[n] = slot;
-      from[n] = blk;
+      p.src[n] = slot;
+      p.from[n] = blk;
+      p.shift[0][n] = p.shift[1][n] = 0;
       if (r >= count) continue;
       if constexpr (LONG) {
         if (ctx <= a.keep) {
@@ -588,115 +794,32 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
           continue;
         }
         if (slot >= front) {
-          src[n] = slot + ctx - a.keep;
+          p.src[n] = slot + ctx - a.keep;
         } else if (slot >= a.sinks) {
           const int at = kept[slot];
-          src[n] = at >= 0 ? at : (a.tails + bh * a.keep)[a.n_holes[bh] - 1 - (-2 - at)];
+          p.src[n] = at >= 0 ? at : (a.tails + bh * a.keep)[a.n_holes[bh] - 1 - (-2 - at)];
         }
-        if (slot < a.sinks || src[n] != slot) kept[slot] = src[n];
+        if (slot < a.sinks || p.src[n] != slot) kept[slot] = p.src[n];
       } else {
-        src[n] = kept[slot];
+        p.src[n] = kept[slot];
       }
-      if (src[n] == slot) continue;
+      if (p.src[n] == slot) continue;
       any = true;
-      from[n] = evict_block(a, b, src[n]);
-      w[slot] = src[n] < a.keep ? a.aside_weights[bh * a.recent + src[n] - front] : w[src[n]];
+      p.from[n] = evict_block(a, b, p.src[n]);
+      w[slot] = p.src[n] < a.keep ? a.aside_weights[bh * a.recent + p.src[n] - front] : w[p.src[n]];
     }
     if (__ballot(any && blk >= 0) == 0) continue;
-    // How far payloads of keys and values are shifted: to the largest scale of the
-    // page's tokens.
-    int shift[2][2] = {{0, 0}, {0, 0}};
     if constexpr (F8) {
-      int old[2] = {0, 0};
-      uint32_t top[2] = {0, 0};
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t *const scales = kv ? a.v_scales : a.k_scales;
-        const uint8_t *const were = a.aside_scales + (bh * 2 + kv) * a.aside_pages -
-                                    (front >> a.bs_log2);
-        if (blk >= 0) old[kv] = scales[(int64_t)blk * a.H_kv + h];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int r = row0 + 64 * n, p = src[n] >> a.bs_log2;
-          if (r >= count || blk < 0) continue;
-          // Pages that get arrivals themselves may have another scale by now.
-          shift[kv][n] = src[n] == slot0 + r ? old[kv]
-                         : from[n] < 0       ? 0
-                         : p <= last_page    ? were[p]
-                                             : scales[(int64_t)from[n] * a.H_kv + h];
-          top[kv] = max(top[kv], (uint32_t)shift[kv][n]);
-        }
-      }
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int byte = (int)page_max(top[kv], a.bs_log2);
-        if (row0 == 0 && blk >= 0 && byte != old[kv])
-          (kv ? a.v_scales : a.k_scales)[(int64_t)blk * a.H_kv + h] = (uint8_t)byte;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) shift[kv][n] -= byte;
-      }
+      const uint8_t *const were = a.aside_scales + bh * 2 * a.aside_pages - (front >> a.bs_log2);
+      evict_scales(a, h, row0, were, were + a.aside_pages, p);
+      evict_put_scales(a, h, row0, p);
     }
-    // The rows to be written, those of lanes that have one: four groups of both keys
-    // and values are read before they are written.
-    constexpr int kBatch = 4;
-    unrolled<2>([&](auto half) __attribute__((always_inline)) {
-      constexpr int n = decltype(half)::value;
-      if (n == 1 && bs <= 64) return;
-      const int r = row0 + 64 * n, slot = slot0 + r;
-      const bool moves = src[n] != slot;
-      // One that stays, only where its payload changes with the scale.
-      const bool write =
-          r < count && blk >= 0 && (moves ? from[n] >= 0 : (shift[0][n] | shift[1][n]) != 0);
-      const uint64_t mask = __ballot(write);
-      const int n_rows = __popcll(mask);
-      // Their lanes first, in order.
-      const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
-                                                        __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-      const int list = __builtin_amdgcn_ds_permute(
-          (write ? before : n_rows + lane - before) * 4, lane);
-      // Rows of the caches, or -1 - n: row n of those copied aside.
-      const int64_t to = evict_row(a, blk, slot, h);
-      int64_t at = evict_row(a, from[n], src[n], h);
-      if (moves && src[n] < a.keep) at = -1 - (int64_t)(src[n] - front);
-      const int shifts = F8 ? (shift[0][n] + 256) | (shift[1][n] + 256) << 16 : 0;
-      for (int t0 = 0; t0 < n_rows; t0 += rows * kBatch) {
-        uint4 v[kBatch][2];
-        int by[kBatch];
-        int64_t to_row[kBatch];
-        unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
-          constexpr int g = decltype(group)::value;
-          const int t = t0 + g * rows + sub, of = __shfl(list, min(t, 63), 64);
-          int64_t row = shfl_i64(at, of);
-          to_row[g] = shfl_i64(to, of);
-          by[g] = F8 ? __shfl(shifts, of, 64) : 0;
-          v[g][0] = v[g][1] = make_uint4(0, 0, 0, 0);
-          if (t >= n_rows) return;
-          const bool put_aside = row < 0;
-          const char *const k = put_aside ? aside : a.k_cache;
-          const char *const v_ = put_aside ? aside + (int64_t)a.recent * a.row_bytes : a.v_cache;
-          row = (put_aside ? -1 - row : row) * a.row_bytes + part;
-          v[g][0] = *reinterpret_cast<const uint4 *>(k + row);
-          v[g][1] = *reinterpret_cast<const uint4 *>(v_ + row);
-        });
-        unrolled<kBatch>([&](auto group) __attribute__((always_inline)) {
-          constexpr int g = decltype(group)::value;
-          if (t0 + g * rows + sub >= n_rows) return;
-          if constexpr (F8) {
-            const int k = (by[g] & 0xffff) - 256, v_ = (by[g] >> 16) - 256;
-            if (k != 0) v[g][0] = shifted_8_bits(v[g][0], k);
-            if (v_ != 0) v[g][1] = shifted_8_bits(v[g][1], v_);
-          }
-          const int64_t row = to_row[g] * a.row_bytes + part;
-          *reinterpret_cast<uint4 *>(a.k_cache + row) = v[g][0];
-          *reinterpret_cast<uint4 *>(a.v_cache + row) = v[g][1];
-        });
-      }
-    });
+    evict_move_rows<F8, true>(a, h, row0, p, aside, front);
   }
 }
 
 struct EvictPlan {
-  bool long_rows;
+  bool long_rows, one_launch;
   int chunks, aside_pages;
   size_t aside, aside_weights, aside_scales, holes, pages, hist, above, state, tails, n_holes;
   size_t bytes;
@@ -712,6 +835,14 @@ static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int64_t keys, int
     return at;
   };
   p.long_rows = keys > kShortRow;
+  // One launch where a workgroup for each sequence and head is one for each compute
+  // unit, or has little to move (rows at most, of keys): 256 of them, 4160 tokens to
+  // 4096, 8 bits, 22.9 us for 36.4, 128 20.9 for 27.3, 64 19.7 for 23.8, 8 19.0 for
+  // 18.0; 16384 to 8192, 256 of them 96 for 133, 128 73 for 63, 16 51 for 30.
+  const int64_t moved = recent + std::min<int64_t>(keep, std::max<int64_t>(0, keys - keep));
+  p.one_launch = !p.long_rows && row_bytes <= 256 && bs <= 64 &&
+                 (bh >= 256 || moved * row_bytes <= 1024 * bh);
+  if (p.one_launch) return p;
   p.chunks = (int)((keys + kChunk - 1) / kChunk);
   p.aside_pages = std::max(0, (keep - 1) / bs - (keep - recent) / bs + 1);
   p.aside = take((size_t)bh * 2 * recent * row_bytes);
@@ -779,16 +910,21 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
                (long long)W * block_size);
   CVSA_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, CVSA_ERR_INVALID,
                "evict_tokens: caches must be 16-byte aligned");
+  CVSA_REQUIRE(k_cache != v_cache, CVSA_ERR_INVALID,
+               "evict_tokens: keys and values must have caches of their own");
   const int64_t bh = (int64_t)B * H_kv;
   const int row_bytes = D * (k_scales ? 1 : 2);
   // More than the tables hold keeps all.
   const int64_t keys = (int64_t)W * block_size;
   const EvictPlan p = plan_evict(bh, row_bytes, block_size, keys, keep, recent,
                                  k_scales != nullptr);
-  CVSA_REQUIRE(workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0,
+  CVSA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes &&
+                                ((uintptr_t)workspace & 255) == 0),
                CVSA_ERR_WORKSPACE,
                "evict_tokens: needs a 256-byte aligned workspace of %zu bytes", p.bytes);
-  const int64_t aside = bh * recent * (row_bytes / 16) + (k_scales ? bh * p.aside_pages : 0);
+  const int64_t aside = p.one_launch ? 0
+                                     : bh * recent * (row_bytes / 16) +
+                                           (k_scales ? bh * p.aside_pages : 0);
   const int64_t aside_wgs = (aside + kEvictThreads - 1) / kEvictThreads;
   const int64_t select_wgs = p.long_rows ? bh * p.chunks : bh;
   CVSA_REQUIRE(aside_wgs + select_wgs < (1LL << 32) / kEvictThreads, CVSA_ERR_UNSUPPORTED,
@@ -826,12 +962,22 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
     hipLaunchKernelGGL(evict_count_kernel<1>, select, threads, 0, s, a);
     hipLaunchKernelGGL(evict_count_kernel<2>, select, threads, 0, s, a);
     hipLaunchKernelGGL(evict_walk_kernel, select, threads, 0, s, a);
-  } else if (keys <= 4 * kEvictThreads) {
-    hipLaunchKernelGGL(evict_plan_kernel<1>, first, threads, 0, s, a);
-  } else if (keys <= 8 * kEvictThreads) {
-    hipLaunchKernelGGL(evict_plan_kernel<2>, first, threads, 0, s, a);
   } else {
-    hipLaunchKernelGGL(evict_plan_kernel<4>, first, threads, 0, s, a);
+    auto plan = [&](auto move) {
+      constexpr int MOVE = decltype(move)::value;
+      if (keys <= 4 * kEvictThreads)
+        hipLaunchKernelGGL((evict_plan_kernel<1, MOVE>), first, threads, 0, s, a);
+      else if (keys <= 8 * kEvictThreads)
+        hipLaunchKernelGGL((evict_plan_kernel<2, MOVE>), first, threads, 0, s, a);
+      else
+        hipLaunchKernelGGL((evict_plan_kernel<4, MOVE>), first, threads, 0, s, a);
+    };
+    if (!p.one_launch) {
+      plan(std::integral_constant<int, 0>());
+    } else {
+      k_scales ? plan(std::integral_constant<int, 2>()) : plan(std::integral_constant<int, 1>());
+      return cvsa_host::check_launch("evict_tokens");
+    }
   }
   // Four waves in a workgroup, in turn past 8192 workgroups.
   const int64_t n_pages = (keep + block_size - 1) / block_size;

@@ -806,8 +806,9 @@ int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q, int64_t q
  * or with scales of 8 bits: a page that tokens come to gets the largest scale of its
  * tokens' pages, to which their payloads are brought.  kept: [B, H_kv, keep], the
  * old slot of each new one (-1 past a shorter context).  Pages must belong to one
- * sequence; a token whose block is outside the pool is not moved.  The workspace
- * (256-byte aligned; cache_bits 16 or 8) needs no initialisation. */
+ * sequence, and keys and values have caches of their own; a token whose block is
+ * outside the pool is not moved.  The workspace (256-byte aligned; cache_bits 16 or
+ * 8; none may be needed) needs no initialisation. */
 size_t cvsa_evict_tokens_workspace_bytes(int32_t B, int32_t H_kv, int32_t D, int32_t block_size,
                                          int32_t W, int32_t cache_bits, int32_t keep,
                                          int32_t sinks, int32_t recent);

@@ -548,6 +548,35 @@ def test_evict_rows_of_chunks(gpu, bits):
     _check_evict(gpu, bt, ctx, k, v, w, 12000, 64, 0, 33)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 8), (32, 64), (256, 32), (128, 128)])
+def test_evict_of_many_sequences(gpu, bits, D, bs):
+    """As many sequences and heads as have a workgroup each for everything."""
+    g = _gen(D + bs + bits + 1)
+    totals = [300, 0, 1, 97, 150, 299, 98, 33, 128, 129, 255, 256, 257, 12, 101, 200, 64, 190]
+    bt, ctx, k, v, w = _evict_inputs(g, totals, bs, 4, D, bits)
+    for keep, sinks, recent in ((97, 4, 16), (1, 0, 0), (1, 0, 1), (128, 0, 128), (96, 0, 0),
+                                (100, 7, 0), (150, 10, 140), (255, 3, 100), (64, 64, 0)):
+        _check_evict(gpu, bt, ctx, k, v, w, keep, bs, sinks, recent)
+    w[:, :, ::3] = 0.25
+    bt[0, 1], bt[4, 0], bt[9, 1] = -1, 10 ** 7, 2 ** 31 - 1
+    ctx[5] = bt.shape[1] * bs + 40
+    _check_evict(gpu, bt, ctx, k, v, w, 90, bs, 4, 20)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("total", [5000, 9000])
+def test_evict_of_many_long_rows(gpu, bits, total):
+    """Last tokens of several rounds, which move by less and by more than a page."""
+    g = _gen(total + bits)
+    totals = [total, total - 3, total - 700] + [20] * 29
+    bt, ctx, k, v, w = _evict_inputs(g, totals, 16, 8, 32, bits)
+    w[0, :, ::5] = math.nan
+    for keep, sinks, recent in ((total - 5, 4, 2500), (total - 1500, 0, 1100), (2000, 1, 1999),
+                                (total - 701, 0, 0)):
+        _check_evict(gpu, bt, ctx, k, v, w, keep, 16, sinks, recent)
+
+
 def test_evict_weights_of_every_kind(gpu):
     g = _gen(9)
     bt, ctx, k, v, w = _evict_inputs(g, [200], 16, 2, 64, 8)

@@ -317,6 +317,7 @@ def _evict(lib, **over):
     (dict(B=0), INVALID, b"B=0"), (dict(sb=W - 1), INVALID, b"bad sizes"),
     (dict(S=W * BS - 1), INVALID, b"weights of"), (dict(vc=P[2] + 8), INVALID, b"aligned"),
     (dict(B=1 << 19, H_kv=16), UNSUPPORTED, b"too many"),
+    (dict(vc=P[1]), INVALID, b"of their own"),
     (dict(bytes=16), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
     (dict(ws=None), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
     (dict(ws=P[6] + 128), _lib.CVSA_ERR_WORKSPACE, b"workspace"),
@@ -325,6 +326,16 @@ def test_c_evict_refuses(over, code, word):
     lib = _lib_or_skip()
     assert _evict(lib, **over) == code
     assert word in lib.cvsa_last_error()
+
+
+def test_c_evict_asks_for_a_workspace_only_where_two_launches_share_it():
+    lib = _lib_or_skip()
+
+    def need(B, D=128, bs=16, W=260, keep=4096, recent=256, bits=8):
+        return lib.cvsa_evict_tokens_workspace_bytes(B, 8, D, bs, W, bits, keep, 4, recent)
+    assert need(32) == need(64) == need(16) == need(32, bits=16) == 0
+    assert need(1) > 0 and need(32, W=1025) > 0 and need(32, bs=128) > 0
+    assert need(32, D=256, bits=16) > 0 and need(16, W=1024, keep=8192) > 0
 
 
 # ------------------------------------------------------------ the manager
