@@ -238,7 +238,7 @@ __device__ __forceinline__ uint32_t page_max(uint32_t v, int log2) {
 
 // What a lane's page gets: where its slots' rows come from.
 struct EvictPage {
-  int page, slot0, count, blk;  // count slots; blk -1: none of the pool
+  int slot0, count, blk;        // its first slot, how many; blk -1: none of the pool
   int src[2], from[2];          // of the lane's slots: old slots (themselves: they stay), blocks
   int shift[2][2];              // of keys' and values' payloads
   int byte[2];                  // the page's scales, where they change (-1)
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_plan_kernel(const EvictAr
     const int at_once = 64 >> a.bs_log2;  // pages of a wave, of 64 slots at most
     const int mine = lane >> a.bs_log2, row0 = lane & (bs - 1);
     auto look = [&](bool there, int page) __attribute__((always_inline)) {
-      EvictPage p = {page, page << a.bs_log2, 0, -1};
+      EvictPage p = {page << a.bs_log2, 0, -1};
       if (there) {
         p.count = min(bs, a.keep - p.slot0);
         p.blk = evict_block(a, b, p.slot0);
@@ -779,7 +779,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
     const int count = there ? min(bs, a.keep - slot0) : 0;
     const int blk = !there || (LONG && ctx <= a.keep) ? -1 : evict_block(a, b, slot0);
     // The lane's slots.
-    EvictPage p = {page, slot0, count, blk};
+    EvictPage p = {slot0, count, blk};
     bool any = false;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {

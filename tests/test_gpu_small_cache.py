@@ -702,6 +702,66 @@ def test_queries_that_heads_share(gpu):
     assert torch.equal(*sums)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_pools_past_32_bits(gpu, bits):
+    """Blocks whose bytes lie past 2^32 (and values past 2^31): all four as over a
+    small pool of the same content."""
+    g = _gen(91)
+    bs, Hk, G, D = 128, 8, 2, 128 if bits == 8 else 256
+    lens, before = [1, 40, 70], [500, 300, 0]
+    totals = [a + b for a, b in zip(lens, before)]
+    bt, ctx, nb = _tables(g, totals, bs, spare=0)
+    per = bs * Hk * D * bits // 8
+    far = 2 ** 32 // per + nb
+    ids = torch.randperm(nb, generator=g)  # alternately from the start and past 2^32
+    where = torch.where(ids % 2 == 0, ids, far - nb + ids).int()
+    wide = bt.clone()
+    wide[bt >= 0] = where[bt[bt >= 0].long()]
+    assert int(wide.max()) * per >= 2 ** 32
+    keys, vals = (small.random_cache(g, nb, bs, Hk, D) for _ in range(2))
+    if bits == 16:
+        keys, vals = ((small.values(*c).to(torch.bfloat16), None) for c in (keys, vals))
+    q, k, v = (_randn(g, sum(lens), n, D).bfloat16().to(gpu) for n in (Hk * G, Hk, Hk))
+    w = torch.rand(3, Hk, bt.shape[1] * bs, generator=g)
+    layout = ops.ChunkLayout(lens, gpu)
+
+    def run(tables, pools):
+        (kc, ks), (vc, vs) = pools
+        bt, cg, wg = tables.to(gpu), ctx.to(gpu), w.to(gpu)
+        ops.append_chunk_kv(k, v, kc, vc, bt, cg, layout, bs, k_scales=ks, v_scales=vs)
+        out, lse = ops.chunk_attention(q, kc, vc, bt, cg, layout, Hk, G, bs, return_lse=True,
+                                       k_scales=ks, v_scales=vs)
+        ops.add_key_weights(wg, q, lse, kc, bt, cg, layout, Hk, G, bs, k_scales=ks)
+        kept = ops.evict_tokens(wg, kc, vc, bt, cg, 200, bs, 4, 30, ks, vs)
+        return [out, lse, wg, kept]
+
+    def bytes_of(t):
+        return None if t is None else t.view(torch.uint8)
+
+    def pool(c, n):
+        """c's blocks at `where` of n."""
+        x, s = c
+        big = torch.zeros(n, *x.shape[1:], dtype=torch.uint8 if bits == 8 else x.dtype, device=gpu)
+        big[where.long()] = (bytes_of(x) if bits == 8 else x).to(gpu)
+        if s is None:
+            return big, None
+        scales = torch.full((n, Hk), 127, dtype=torch.uint8, device=gpu)
+        scales[where.long()] = bytes_of(s).to(gpu)
+        return big.view(x.dtype), scales.view(s.dtype)
+
+    near = [[None if t is None else t.to(gpu) for t in c] for c in (keys, vals)]
+    want = run(bt, near)
+    pools = [pool(keys, far), pool(vals, far)]
+    got = run(wide, pools)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    for c, d in zip(pools, near):
+        for x, y in zip(c, d):
+            if x is not None:
+                at = where.long().to(gpu)
+                assert torch.equal(bytes_of(x)[at], bytes_of(y))
+
+
 # ------------------------------------------------------------ together
 
 @pytest.mark.parametrize("bits", [8, 16])
