@@ -161,8 +161,14 @@ def _weights(who: str, D: int, q_weight, k_weight):
     """Norm weights [D] of one dtype (None: no norm), and its code."""
     if q_weight is None and k_weight is None:
         return None, None, 0
-    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
-        raise ValueError(f"{who}: q_weight and k_weight differ in dtype")
+    if q_weight is not None and k_weight is not None:
+        dt = k_weight.dtype
+        if q_weight.dtype is not dt:
+            raise ValueError(f"{who}: q_weight and k_weight differ in dtype")
+        if dt in _DTYPE_CODE and q_weight.shape == k_weight.shape == (D,) \
+                and q_weight.is_contiguous() and k_weight.is_contiguous() \
+                and not (q_weight.data_ptr() | k_weight.data_ptr()) & 15:
+            return q_weight, k_weight, _DTYPE_CODE[dt]
     return (_weight(who, "q_weight", q_weight, D), _weight(who, "k_weight", k_weight, D),
             _DTYPE_CODE[(k_weight if q_weight is None else q_weight).dtype])
 
@@ -283,7 +289,15 @@ def _check_cache8(who, name, cache, scales):
 def _check_caches(who, k_cache, v_cache, block_size, k_scales=None, v_scales=None):
     """The caches' (num_blocks, H_kv, D)."""
     shape = k_cache.shape
-    if k_scales is not None or v_scales is not None or k_cache.dtype is _F8:
+    if k_scales is not None and v_scales is not None and len(shape) == 4 \
+            and k_cache.dtype is v_cache.dtype is _F8 \
+            and k_scales.dtype is v_scales.dtype is _SCALE \
+            and k_scales.shape == v_scales.shape == (shape[0], shape[2]) \
+            and k_cache.is_contiguous() and v_cache.is_contiguous() \
+            and k_scales.is_contiguous() and v_scales.is_contiguous() \
+            and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        pass  # as _check_cache8 wants them: one look at each
+    elif k_scales is not None or v_scales is not None or k_cache.dtype is _F8:
         _check_cache8(who, "k", k_cache, k_scales)
         _check_cache8(who, "v", v_cache, v_scales)
     elif len(shape) != 4 or k_cache.dtype is not _BF16 or v_cache.dtype is not _BF16 \
