@@ -31,10 +31,10 @@
 //
 // Measured, heads of 128.  Few rows: a token of each of 32 sequences of 8 K keys at
 // most, 32 heads on 8, 8 bits: 33 us for 147 MB, 4.4 TB/s (a copy reaches 5.1).  Many
-// rows: 4096 tokens over themselves, 32 heads on 8, 8 bits: 90 us and 5 to join, 735
-// TFLOP/s of the product (a large one of the library 1318); the vector pipe, with 52
-// instructions to 8 products, 16 of them exponentials, is active in about 85% of the
-// cycles between the first product and the last.  The last 64 of 2048 tokens over 32768
+// rows: 4096 tokens over themselves, 32 heads on 8, 8 bits: 82 us with 4 to join, 850
+// TFLOP/s of the product (a large one of the library 1318); the vector pipe's 52
+// instructions to 8 products, 16 of them exponentials, take 400 cycles of a SIMD where
+// the products take 256, so 47 us at 2.2 GHz.  The last 64 of 2048 tokens over 32768
 // keys of bf16: 31 and 5, where half of the time a workgroup waits for its two tiles of
 // keys (a word of each line of the second one read ahead of time into the XCD's cache,
 // whose 4 MB the first ones fill: 37 for 35).
