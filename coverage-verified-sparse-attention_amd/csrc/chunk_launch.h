@@ -1,5 +1,5 @@
-// Launches of the chunk attention's kernels, without the join.  Those of each head
-// dimension and type of the cache are compiled by themselves (chunk_kernels_bf16.hip, chunk_kernels_f8.hip).
+// Launches of the chunk attention's kernels, without the join.  Those of each type of
+// the cache are compiled by themselves (chunk_kernels_bf16.hip, chunk_kernels_f8.hip).
 #pragma once
 #include "chunk_prefill.h"
 #include "chunk_stream.h"
