@@ -25,7 +25,7 @@ import torch
 from . import (_DTYPE_CODE, _block_tables, _check_cache, _check_count, _check_seqs, _device_of,
                _i32, _lib, _ptr, check)
 
-_BF16 = torch.bfloat16
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 _F8, _SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8, torch.uint16,
              torch.uint32, torch.uint64)
@@ -147,7 +147,7 @@ def _rows(who: str, name: str, t: torch.Tensor, rows: Optional[int], heads: Opti
                          f"got {dt}")
     st, sh, sd = t.stride()
     at = t.data_ptr()
-    if sd != 1 or (st | sh) & (3 if dt is torch.float32 else 7) or at & 15:
+    if sd != 1 or (st | sh) & (3 if dt is _F32 else 7) or at & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()
@@ -196,21 +196,22 @@ def _rotary(who: str, rotary: Optional[RotaryTable], D: int):
 def _tables(who: str, layout: ChunkLayout, dev: torch.device, block_tables, context_lens):
     """Block tables, their row stride and context lengths as the kernels read
     them."""
-    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 \
-            or block_tables.stride(1) != 1:
+    strides = block_tables.stride()
+    if block_tables.dtype is not _I32 or len(strides) != 2 or strides[1] != 1:
         block_tables = _block_tables(block_tables)
-    if context_lens.dtype is not torch.int32 or not context_lens.is_contiguous():
+        strides = block_tables.stride()
+    if context_lens.dtype is not _I32 or not context_lens.is_contiguous():
         context_lens = _i32(context_lens)
     B = layout.batch
     if layout.device != dev:
         raise ValueError(f"{who}: the layout is on {layout.device}, the tensors on {dev}")
-    if block_tables.shape[0] != B:
-        raise ValueError(f"{who}: the layout has {B} sequences, the tables "
-                         f"{block_tables.shape[0]}")
-    if context_lens.dim() != 1 or context_lens.shape[0] != B:
+    rows, W = block_tables.shape
+    if rows != B:
+        raise ValueError(f"{who}: the layout has {B} sequences, the tables {rows}")
+    if context_lens.shape != (B,):
         _check_seqs(who, B, None, context_lens)
     # The stride of a single row can be any number.
-    return block_tables, block_tables.stride(0) if B > 1 else block_tables.shape[1], context_lens
+    return block_tables, strides[0] if B > 1 else W, context_lens
 
 
 def _positions(t: torch.Tensor) -> torch.Tensor:

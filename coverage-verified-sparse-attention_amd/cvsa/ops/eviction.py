@@ -130,7 +130,7 @@ def evict_tokens(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     L = _lib.load()
     need = L.cvsa_evict_tokens_workspace_bytes(B, H_kv, D, block_size, W,
                                                16 if k_scales is None else 8, keep, sinks, recent)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     _call(dev, who, L.cvsa_evict_tokens, weights.data_ptr(), S, k_cache.data_ptr(),
           v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), num_blocks, bt.data_ptr(),
           bt.stride(0) if B > 1 else W, W, ctx.data_ptr(), B, H_kv, D, block_size, keep, sinks,
