@@ -18,8 +18,10 @@
 // the second operand: the weights go from one product to the next without
 // leaving the lane.  V^T comes from the row-major tile through the transposing
 // LDS read.  The weights are rounded to bf16 for the second product (as V is;
-// at most half a step, 2^-8 of each weight); their sum l is taken in 32 bits
-// before that.
+// at most half a step, 2^-8 of each weight), since that product bounds many rows
+// and would have to be made twice for more; few rows over 8 bits, which memory
+// bounds, make it twice, with the rounded weights and with what the rounding left
+// (16 bits, 2^-16 of each weight).  Their sum l is taken in 32 bits before that.
 //
 // Keys go straight into LDS, 16 bytes a lane; the vectors of row r are permuted
 // by swizzle(r), so that both the row reads of K and the transposing reads of V
@@ -382,6 +384,15 @@ __device__ __forceinline__ uint32_t chunk_cvt_bf16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
+// What the rounding to bf16 left of weights (pairs of `p` in `w`), as bf16 itself:
+// the difference is exact, so 2^-8 of 2^-8 of each is lost.
+__device__ __forceinline__ uint4 chunk_rest(const float (&p)[8], const uint4 &w) {
+  return make_uint4(chunk_cvt_bf16x2(p[0] - bf16_lo(w.x), p[1] - bf16_hi(w.x)),
+                    chunk_cvt_bf16x2(p[2] - bf16_lo(w.y), p[3] - bf16_hi(w.y)),
+                    chunk_cvt_bf16x2(p[4] - bf16_lo(w.z), p[5] - bf16_hi(w.z)),
+                    chunk_cvt_bf16x2(p[6] - bf16_lo(w.w), p[7] - bf16_hi(w.w)));
+}
+
 // Infinite and NaN elements of a bf16 pair, as masks of their bits.
 __device__ __forceinline__ uint32_t nonfinite_bf16x2(uint32_t w) {
   const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
@@ -496,11 +507,13 @@ struct ChunkState {
     l = 0.f;
   }
 
-  // exp2(c s - reference) of a step's scores as bf16 pairs; their sum.
+  // exp2(c s - reference) of a step's scores as bf16 pairs, with what their rounding
+  // left behind them if pw has room for it (PW = 4 KB); their sum.
   // before(j) precedes 16 keys' part.
-  template <int KB, class F>
+  template <int KB, int PW, class F>
   static __device__ __forceinline__ float weigh(const f32x16_t (&st)[KB], float c, float neg_ref,
-                                                uint4 (&pw)[2 * KB], F before) {
+                                                uint4 (&pw)[PW], F before) {
+    static_assert(PW == 2 * KB || PW == 4 * KB, "one part of the weights or two");
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 2 * KB; ++j) {
@@ -513,6 +526,7 @@ struct ChunkState {
       }
       pw[j] = make_uint4(chunk_cvt_bf16x2(p[0], p[1]), chunk_cvt_bf16x2(p[2], p[3]),
                          chunk_cvt_bf16x2(p[4], p[5]), chunk_cvt_bf16x2(p[6], p[7]));
+      if constexpr (PW == 4 * KB) pw[2 * KB + j] = chunk_rest(p, pw[j]);
     }
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
@@ -521,14 +535,14 @@ struct ChunkState {
   // set; it moves only when the weights of a step outgrow it (their sum in a
   // lane passes 2^20, or there is no reference yet: NaN), so that steps need no
   // maximum.  Weights of up to 2^20 have the same relative precision.
-  template <int KB, class F>
-  __device__ __forceinline__ void weights(const f32x16_t (&st)[KB], float c, uint4 (&pw)[2 * KB],
+  template <int KB, int PW, class F>
+  __device__ __forceinline__ void weights(const f32x16_t (&st)[KB], float c, uint4 (&pw)[PW],
                                           F before) {
     settle(st, c, pw, weigh(st, c, neg_m, pw, before));
   }
   // The rest of weights(), given their sum for the present reference.
-  template <int KB>
-  __device__ __forceinline__ void settle(const f32x16_t (&st)[KB], float c, uint4 (&pw)[2 * KB],
+  template <int KB, int PW>
+  __device__ __forceinline__ void settle(const f32x16_t (&st)[KB], float c, uint4 (&pw)[PW],
                                          float sum) {
     if (__ballot(!(sum < 1048576.f)) != 0) {
       float top[4] = {st[0][0], st[0][1], st[0][2], st[0][3]};

@@ -27,7 +27,10 @@
 // Over 8 bits: a token each of 32 sequences of up to 8 K keys, 32 heads on 8, 62 us and
 // 5 to join, 277 MB, 4.5 TB/s in the walk; 8 drafts of 5 tokens at 32 K keys, 28 heads
 // on 4, 71 and 6, 269 MB.  The conversions to bf16 stand before each product there: with
-// 35 rows they, the products and the loads' waits of a wave follow each other.
+// 35 rows they, the products and the loads' waits of a wave follow each other.  The
+// weights are kept in two bf16 parts there too, as no decode kernel reads such caches:
+// one part took 67.7 and 78 us with the join where two take 68.5 and 88 (the products
+// of the second parts behind those of all the first, not between them: 91).
 #pragma once
 #include "chunk_common.h"
 
@@ -207,7 +210,7 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) chunk_mask(st[r], key0, first_key(s), row[r].last_key);
       }
-      uint4 pw[RT][2];
+      uint4 pw[RT][F8 ? 4 : 2];  // 8 bits: the weights in two parts
 #pragma unroll
       for (int r = 0; r < RT; ++r) state[r].weights(st[r], a.c, pw[r], [](int) {});
       if (!whole) {
@@ -243,7 +246,10 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
                                              scale[0], scale[1]);
           else v = place.read_v((char *)v_cur, j, d);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) state[r].o[d] = chunk_mfma(v, pw[r][j], state[r].o[d]);
+          for (int r = 0; r < RT; ++r) {
+            state[r].o[d] = chunk_mfma(v, pw[r][j], state[r].o[d]);
+            if constexpr (F8) state[r].o[d] = chunk_mfma(v, pw[r][2 + j], state[r].o[d]);
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // V has been read

@@ -458,7 +458,10 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     With ``k_scales`` and ``v_scales`` the caches are of 8 bits (see
     :func:`append_chunk_kv`); their values are brought to bf16, exactly, and
-    the rest is the same.  A scale of NaN makes its block's values NaN.
+    the rest is the same, but that sequences of up to 64 rows (tokens times
+    num_q_per_kv; 32 at D = 256) keep 16 bits of the weights: single tokens
+    and drafts, which no decode kernel takes over such caches.  A scale of NaN
+    makes its block's values NaN.
     """
     who = "chunk_attention"
     dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out, k_scales, v_scales)

@@ -52,7 +52,8 @@ def check_rotated(got, want, size, dtype, D):
     assert not bad.any(), ((got - want).abs() - bound)[bad].max()
 
 
-def attend(q, k_cache, v_cache, block_tables, context_lens, lens, G, causal=True, scale=None):
+def attend(q, k_cache, v_cache, block_tables, context_lens, lens, G, causal=True, scale=None,
+           parts=1):
     """(out, lse, slack, lse_slack) in 64 bits, token by token over exactly the
     keys that each sees; slack bounds the kernel's errors.
 
@@ -62,7 +63,8 @@ def attend(q, k_cache, v_cache, block_tables, context_lens, lens, G, causal=True
     of exp2 (2^-22), and by half a step of bf16 (2^-8) in the second product,
     whose sum over n keys adds n 2^-24, with 64 roundings for moving
     references and joining splits.  All are relative to sum p |v|; the output
-    is then rounded to bf16.
+    is then rounded to bf16.  With the weights in two bf16 `parts` half a step of
+    half a step is lost (2^-16), and the sum has twice the terms.
     """
     q, kc, vc = q.double().cpu(), k_cache.double().cpu(), v_cache.double().cpu()
     bt, ctx = block_tables.cpu(), context_lens.cpu().tolist()
@@ -93,9 +95,9 @@ def attend(q, k_cache, v_cache, block_tables, context_lens, lens, G, causal=True
                 lse[at + i] = total
                 x = (s.amax(-1) - s.amin(-1)).clamp(max=150.0) / math.log(2) + 8
                 rel = (2 * (D + 8) * 2.0 ** -24 * a + x * 2.0 ** -23 + 2.0 ** -22
-                       + (seen + 64) * 2.0 ** -24)
+                       + (parts * seen + 64) * 2.0 ** -24)
                 size = (w[:, None] @ vv.abs())[:, 0]
-                slack[at + i] = ((2.0 ** -8 + 2 * rel)[:, None] * size
+                slack[at + i] = ((2.0 ** (-8 * parts) + 2 * rel)[:, None] * size
                                  + half_step(torch.bfloat16) * out[at + i].abs())
                 lse_slack[at + i] = 2 * rel + 2.0 ** -22 * total.abs()
         at += n

@@ -351,6 +351,43 @@ def test_attend_strided_queries_and_output_in_place(gpu):
     assert torch.equal(qg, want)
 
 
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_attend_few_rows_keeps_16_bits_of_the_weights(gpu, D):
+    """Half of the keys have a weight of 1 and values of 1, the others a weight just
+    above 1/2, which one bf16 rounds to it, and values of -2: what is left of the sum
+    is what that rounding loses."""
+    bs, n = 16, 64
+    for lens, before, G in (([1], [n - 1], 4), ([32 // 7], [n - 32 // 7], 7), ([1], [5000], 1)):
+        total = lens[0] + before[0]
+        bt, ctx, nb = _tables(_gen(D), [total], bs)
+        k = torch.zeros(nb, bs, 1, D)
+        k[:, 1::2, 0, 0], k[:, 1::2, 0, 1] = -0.6875, -0.1171875
+        v = torch.ones(nb, bs, 1, D)
+        v[:, 1::2] = -2.0
+        q = torch.zeros(sum(lens), G, D)
+        q[..., 0], q[..., 1] = 1.0, 2.0 ** -5
+        ones = small.to_scales(torch.full((nb, 1), 127))
+        k, v = (k.to(torch.float8_e4m3fn), ones), (v.to(torch.float8_e4m3fn), ones)
+        out, lse = _attend(gpu, q.bfloat16(), k, v, bt, ctx, lens, G, bs, scale=1.0)
+        want = ref.attend(q.bfloat16(), small.values(*k), small.values(*v), bt, ctx, lens, G,
+                          scale=1.0, parts=2)
+        ref.check_attend(out, want, lse)
+
+
+@pytest.mark.parametrize("D,most", [(32, 64), (64, 64), (128, 64), (256, 32)])
+@pytest.mark.parametrize("G", [1, 4, 7])
+def test_attend_few_rows_within_16_bits(gpu, D, most, G):
+    """As many rows as count as few, over one workgroup's keys and over many's."""
+    g = _gen(D + G)
+    bs, Hk = 16, 2
+    lens = [most // G, 1, 2]
+    x = _attend_inputs(g, lens, [40, 2500, 0], bs, Hk, G, D)
+    out, lse = _attend(gpu, *x, lens, G, bs)
+    q, k, v, bt, ctx = x
+    want = ref.attend(q, small.values(*k), small.values(*v), bt, ctx, lens, G, parts=2)
+    ref.check_attend(out, want, lse)
+
+
 # ------------------------------------------------------------ weights of keys
 
 def _weigh_inputs(g, lens, before, bs, Hk, G, D, bits, W=None):
