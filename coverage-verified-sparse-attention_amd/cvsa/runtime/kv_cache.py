@@ -281,6 +281,10 @@ class SequenceKVManager:
         n = k.shape[0]
         seqs = range(seq_begin, seq_begin + n)
         if self.cache.k_scales is not None:
+            if seq_begin < 0 or seq_begin + n > self.batch_size:
+                raise IndexError(f"sequences {seq_begin} .. {seq_begin + n} of {self.batch_size}")
+            if v.shape[0] != n:
+                raise ValueError(f"{n} rows of keys and {v.shape[0]} of values")
             layout = self._token_layouts.get((seq_begin, n))
             if layout is None:
                 lens = [int(s in seqs) for s in range(self.batch_size)]

@@ -414,3 +414,17 @@ def test_the_manager_cuts(calls, monkeypatch):
         with pytest.raises(RuntimeError, match="captured"):
             call()
     assert mgr._ctx_host == [12, 7] and len(calls) == n
+
+
+def test_a_token_of_no_sequence_is_refused(calls):
+    cache, mgr = _manager()
+    row = _bf(HK, D)
+    for s in (-1, -2, 2, 7):
+        with pytest.raises(IndexError):
+            mgr.append_token_kv(s, row, row)
+    with pytest.raises(ValueError):
+        mgr.append_tokens_kv(_bf(2, HK, D), _bf(3, HK, D))
+    assert mgr._ctx_host == [0, 0] and cache._next_free == 0 and not calls
+    assert not mgr._token_layouts
+    mgr.append_token_kv(1, row, row)
+    assert mgr._ctx_host == [0, 1]
