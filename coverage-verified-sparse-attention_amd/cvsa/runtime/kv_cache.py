@@ -154,6 +154,9 @@ class SequenceKVManager:
         n_pages = (seq_len + bs - 1) // bs
         launch = None
         if self.cache.k_scales is not None:  # checked before a block is taken
+            if n_pages > self.max_pages:
+                raise IndexError(f"a prompt of {seq_len} tokens exceeds the block table "
+                                 f"({self.max_pages} pages)")
             launch, _ = ops.prepare_append_chunk(
                 k_all, v_all, self.cache.k_cache, self.cache.v_cache,
                 self.block_tables[seq_idx][None], self.context_lens[seq_idx][None],

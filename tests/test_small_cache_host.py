@@ -428,3 +428,13 @@ def test_a_token_of_no_sequence_is_refused(calls):
     assert not mgr._token_layouts
     mgr.append_token_kv(1, row, row)
     assert mgr._ctx_host == [0, 1]
+
+
+def test_a_prompt_past_the_tables_takes_no_block(calls):
+    cache, mgr = _manager()
+    with pytest.raises(IndexError, match="block table"):
+        mgr.prefill_kv(0, _bf(5 * BS + 1, HK, D), _bf(5 * BS + 1, HK, D))
+    assert cache._next_free == 0 and mgr._ctx_host == [0, 0] and not calls
+    assert mgr.context_lens.tolist() == [0, 0]
+    mgr.prefill_kv(0, _bf(5 * BS, HK, D), _bf(5 * BS, HK, D))
+    assert cache._next_free == 5 and mgr._ctx_host == [5 * BS, 0]
