@@ -205,7 +205,8 @@ __global__ __launch_bounds__(256, (weigh_few_fit<D, F8>())) void weigh_few_kerne
       const int pos0 = __builtin_amdgcn_readlane(mine.pos0, l);
       const int keys = __builtin_amdgcn_readlane(mine.keys, l);
       const int rows = __builtin_amdgcn_readlane(mine.rows, l);
-      const int old = __builtin_amdgcn_readlane(mine.before, l);
+      // Those of the table: the context may be longer.
+      const int old = min(__builtin_amdgcn_readlane(mine.before, l), keys);
       const uint32_t from = __builtin_amdgcn_readlane(start, l);
       const int t0 = (int)(begin > from ? begin - from : 0);
       const int t1 = (int)min(end - from, (uint32_t)__builtin_amdgcn_readlane(units, l));

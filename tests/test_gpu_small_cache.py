@@ -510,6 +510,23 @@ def test_weigh_strides_and_other_scales(gpu):
     _check_weigh(got, *small.key_weights(w, q, lse, keys, bt, ctx, lens, G, scale=0.01), w)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("n", [1, 60])
+def test_weigh_context_past_the_table(gpu, bits, n):
+    """Contexts of more keys than the tables hold, which are not a multiple of a
+    tile, with weights of the tables' keys and no more."""
+    g = _gen(n + bits)
+    bs, Hk, G, D = 8, 2, 4, 64
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, [n, n], [40 - n, 40 - n] if n == 1 else [12, 20],
+                                           bs, Hk, G, D, bits)
+    w = w[..., :bt.shape[1] * bs].contiguous()
+    ctx = ctx + torch.tensor([300, 5], dtype=torch.int32)
+    for causal in (True, False):
+        lse = _lse(q, keys, bt, ctx, [n, n], G, causal)
+        got = _weigh(gpu, w, q, lse, k, bt, ctx, [n, n], G, bs, causal=causal)
+        _check_weigh(got, *small.key_weights(w, q, lse, keys, bt, ctx, [n, n], G, causal), w)
+
+
 # ------------------------------------------------------------ eviction
 
 def _evict_inputs(g, totals, bs, H, D, bits, W=None):
