@@ -861,9 +861,15 @@ extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q
   if (!p.few && !p.many) return CVSA_OK;
   CVSA_REQUIRE(p.passes < (1LL << 31) && p.tiles < (1LL << 32) / kWeighKeys, CVSA_ERR_UNSUPPORTED,
                "add_key_weights: too many queries and keys");
-  // Offsets among the rows that pass by together are of 32 bits.
-  CVSA_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && q_stride_t < (1 << 23) &&
-                   q_stride_h < (1 << 23),
+  // Many rows: the bytes from the first token of a pass to any of its rows are counted
+  // in 32 bits.  (Few rows have addresses of 64.)
+  const int64_t G = H_q / H_kv;
+  const int64_t pass_rows = D == 256 ? weigh_rows<256>() : weigh_rows<128>();
+  CVSA_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0, CVSA_ERR_INVALID,
+               "add_key_weights: negative stride of the queries");
+  CVSA_REQUIRE(!p.many || (q_stride_t < (1LL << 31) && q_stride_h < (1LL << 31) &&
+                           (pass_rows + G - 2) / G * q_stride_t + (G - 1) * q_stride_h <
+                               (1LL << 31)),
                CVSA_ERR_UNSUPPORTED, "add_key_weights: queries too far apart");
   CVSA_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), CVSA_ERR_WORKSPACE,
                "add_key_weights: needs a workspace of %zu bytes", p.bytes);

@@ -63,8 +63,12 @@ def add_key_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor,
     if bt_stride < W:  # a row that sequences share
         bt, bt_stride = bt.contiguous(), W
     S = _check_weights(who, weights, B, H_kv, W * block_size)
-    T, H_q = layout.total, num_kv_heads * num_q_per_kv
+    T, H_q, G = layout.total, num_kv_heads * num_q_per_kv, num_q_per_kv
     q, *q_at = _rows(who, "q", q, T, H_q, D, _BF16)
+    # The kernel counts in 32 bits from the first of up to 128 rows to the others.
+    if (126 + G) // G * q_at[1] + (G - 1) * q_at[2] >= 1 << 31:
+        q = q[:T].contiguous()
+        q_at = [q.data_ptr(), H_q * D, D]
     if lse.dim() != 2 or lse.shape[0] < T or lse.shape[1] != H_q or lse.dtype is not torch.float32:
         raise ValueError(f"{who}: lse must be [{T}, {H_q}] float32, got {tuple(lse.shape)} "
                          f"{lse.dtype}")

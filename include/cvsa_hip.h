@@ -780,8 +780,10 @@ int cvsa_chunk_attention8(const uint16_t *q, int64_t q_stride_t, int64_t q_strid
  * context, and those of sequences without tokens in the chunk, are left as they
  * are.  lse: [cu[B], H_q] fp32, what cvsa_chunk_attention gives; a row whose lse is
  * -inf saw nothing and gives nothing.  Keys of blocks outside the pool get nothing.
- * k_cache: bf16, or with k_scales 8 bits (cvsa_append_chunk_kv8).  Equal calls give
- * equal results.  The workspace needs no initialisation. */
+ * k_cache: bf16, or with k_scales 8 bits (cvsa_append_chunk_kv8).  Where more than 32
+ * rows of a sequence and KV head count, the rows of 128 of them (64 at D = 256) must
+ * lie within 4 GiB: ((126 + G) / G) q_stride_t + (G - 1) q_stride_h < 2^31, G = H_q /
+ * H_kv.  Equal calls give equal results.  The workspace needs no initialisation. */
 size_t cvsa_add_key_weights_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
                                             int32_t H_kv, int32_t D, int64_t S,
                                             int32_t window);

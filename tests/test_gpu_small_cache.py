@@ -527,6 +527,28 @@ def test_weigh_context_past_the_table(gpu, bits, n):
         _check_weigh(got, *small.key_weights(w, q, lse, keys, bt, ctx, [n, n], G, causal), w)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_weigh_queries_far_apart(gpu, bits):
+    """Heads 2^23 values apart (of 65536 tokens, head after head), tokens 2^23 and 2^25
+    apart: as the same queries side by side."""
+    g = _gen(bits)
+    lens, before, bs, Hk, G, D = [1, 40, 3], [100, 30, 200], 16, 2, 4, 128
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, lens, before, bs, Hk, G, D, bits)
+    lse = _lse(q, keys, bt, ctx, lens, G, True)
+    want = _weigh(gpu, w, q, lse, k, bt, ctx, lens, G, bs)
+    T, H = q.shape[:2]
+    for st, sh in ((D, 1 << 23), (1 << 23, D), (1 << 26, D)):
+        far = torch.empty((T - 1) * st + (H - 1) * sh + D, dtype=q.dtype, device=gpu)
+        far = far.as_strided((T, H, D), (st, sh, 1))
+        far.copy_(q)
+        got = _weigh(gpu, w, far, lse, k, bt, ctx, lens, G, bs)
+        assert torch.equal(got, want)
+        for window in (1, 5):
+            assert torch.equal(_weigh(gpu, w, far, lse, k, bt, ctx, lens, G, bs, window=window),
+                               _weigh(gpu, w, q, lse, k, bt, ctx, lens, G, bs, window=window))
+        del far
+
+
 # ------------------------------------------------------------ eviction
 
 def _evict_inputs(g, totals, bs, H, D, bits, W=None):

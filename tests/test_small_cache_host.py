@@ -438,3 +438,28 @@ def test_a_prompt_past_the_tables_takes_no_block(calls):
     assert mgr.context_lens.tolist() == [0, 0]
     mgr.prefill_kv(0, _bf(5 * BS, HK, D), _bf(5 * BS, HK, D))
     assert cache._next_free == 5 and mgr._ctx_host == [5 * BS, 0]
+
+
+def test_c_weigh_refuses_queries_that_32_bits_cannot_span():
+    lib = _lib_or_skip()
+    most = (1 << 31) - 1
+    for g, st, sh in ((4, HK * G * D, most // 3 // 8 * 8 + 8), (4, most // 32 // 8 * 8 + 8, D),
+                      (1, most // 127 // 8 * 8 + 8, D), (4, 1 << 40, D), (4, 8, 1 << 40)):
+        assert _weigh(lib, cu=(0, 2000), H_q=HK * g, st=st, sh=sh) == UNSUPPORTED
+        assert b"too far apart" in lib.cvsa_last_error()
+    # Those that it can are asked for their workspace.
+    for g, st, sh in ((4, D, 1 << 23), (4, 1 << 25, D), (1, 1 << 24, D), (4, 1 << 24, 1 << 28)):
+        assert _weigh(lib, cu=(0, 2000), H_q=HK * g, st=st, sh=sh) == _lib.CVSA_ERR_WORKSPACE
+    assert _weigh(lib, st=-8) == INVALID
+
+
+def test_queries_far_apart_are_copied(calls, monkeypatch):
+    """What the kernel's 32 bits cannot span is made contiguous, nothing else is."""
+    w = _weigh_args()
+    where = w["q"].data_ptr()
+    for st, sh, copied in ((HK * G * D, 1 << 23, False), (1 << 25, D, False),
+                           (1 << 26, D, True), (HK * G * D, 1 << 30, True)):
+        monkeypatch.setattr(eviction, "_rows", lambda *a: (a[2], where, st, sh))
+        ops.add_key_weights(**w)
+        at, st_, sh_ = calls[-1][1][2:5]
+        assert (st_, sh_) == ((HK * G * D, D) if copied else (st, sh))
