@@ -102,11 +102,11 @@ struct WeighKeys {
     for (int i = 0; i < N; ++i)
       w[i] = *reinterpret_cast<const uint4 *>(row + 32 * i + 16 * half);
   }
-  // The operand of step ks.
-  __device__ __forceinline__ uint4 get(int ks) const {
+  // The operand of step ks; 8 bits: times the scale, exactly, as the attention has them.
+  __device__ __forceinline__ uint4 get(int ks, float scale) const {
     if constexpr (F8) {
       const uint4 &v = w[ks / 2];
-      return chunk_from_8(ks % 2 ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y), 1.f, 1.f);
+      return chunk_from_8(ks % 2 ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y), scale, scale);
     } else {
       return w[ks];
     }
@@ -252,19 +252,20 @@ __global__ __launch_bounds__(256, (weigh_few_fit<D, F8>())) void weigh_few_kerne
       };
       auto add = [&](int t, const Tile &x) {
         f32x16_t s;
+        const float scale = chunk_scale(x.scale);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          s = chunk_mfma(__builtin_bit_cast(uint4, q[ks]), x.k.get(ks), ks ? s : f32x16_t{});
+          s = chunk_mfma(__builtin_bit_cast(uint4, q[ks]), x.k.get(ks, scale),
+                         ks ? s : f32x16_t{});
         const int key = t * 32 + l31;
         // The first row that sees the key, and the lane's rows from there on.
         const int min_row = a.causal && key > pos0 ? min(key - pos0, 1 << 20) * a.G : 0;
-        const float c = a.c * chunk_scale(x.scale);
         float p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int r = 8 * (e / 4) + e % 4;
           const bool see = (live >> e & 1) && r + 4 * half >= min_row;
-          const float v = __builtin_amdgcn_exp2f(fmaf(s[e], c, neg[e]));
+          const float v = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, neg[e]));
           p[e] = see ? v : 0.f;
         }
         float u, v;
@@ -482,9 +483,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
       lse1 = request_lse(row0 + RB);
     }
 
-    // The wave's keys, as the second operand: bf16, the scales apart.
+    // The wave's keys, as the second operand.
     uint4 k[2][KS];
-    float c[2];
     bool ok[2];
     bool all_ok = true;
 #pragma unroll
@@ -497,14 +497,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
       if constexpr (F8) {
         WeighKeys<D, true> raw;
         raw.load(p, half);
+        const float scale = chunk_scale(a.k_scales[(int64_t)at.blk * a.H_kv + h]);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) k[i][ks] = raw.get(ks);
-        c[i] = a.c * chunk_scale(a.k_scales[(int64_t)at.blk * a.H_kv + h]);
+        for (int ks = 0; ks < KS; ++ks) k[i][ks] = raw.get(ks, scale);
       } else {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           k[i][ks] = *reinterpret_cast<const uint4 *>(p + ks * 32 + half * 16);
-        c[i] = a.c;
       }
     }
     // The first row that sees the lane's first key (the second one is 32 tokens on), or
@@ -576,7 +575,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void weigh_many_kernel(const
           fetch(rows, std::integral_constant<int, ks + kAhead>());
         });
         const float ref = x == 0 ? neg.x : x == 1 ? neg.y : x == 2 ? neg.z : neg.w;
-        float p = __builtin_amdgcn_exp2f(fmaf(st[i][4 * g + x], c[i], ref));
+        float p = __builtin_amdgcn_exp2f(fmaf(st[i][4 * g + x], a.c, ref));
         if constexpr (MASK) {
           int on;  // the builtin becomes a comparison and a selection: 6 us of 97
           asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(on) : "v"(seen[i]), "n"(8 * g + x));

@@ -549,6 +549,26 @@ def test_weigh_queries_far_apart(gpu, bits):
         del far
 
 
+@pytest.mark.parametrize("n", [1, 60])
+def test_weigh_scales_of_nan_and_the_largest(gpu, n):
+    """Log-sum-exps of the caller's own: keys of a block whose scale is NaN get NaN of
+    the rows that see them, zeros at the largest scale have a score of zero."""
+    g = _gen(n)
+    bs, Hk, G, D, before = 16, 2, 4, 64, 100
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, [n], [before], bs, Hk, G, D, 8)
+    lse = torch.zeros(n, Hk * G)
+    k[1].view(torch.uint8)[bt[0, [1, (before + n - 1) // bs]].long(), 1] = 255
+    keys = small.values(*k)
+    got = _weigh(gpu, w, q, lse, k, bt, ctx, [n], G, bs, scale=0.01)
+    want, slack = small.key_weights(w, q, lse, keys, bt, ctx, [n], G, scale=0.01)
+    assert want[0, 1, bs:2 * bs].isnan().all() and not want[0, 0].isnan().any()
+    _check_weigh(got, want, torch.nan_to_num(slack, nan=0.0), w)
+    k = (torch.zeros_like(k[0].float()).to(k[0].dtype), small.to_scales(torch.full(k[1].shape, 246)))
+    got = _weigh(gpu, w, q, lse, k, bt, ctx, [n], G, bs, scale=400.0)
+    _check_weigh(got, *small.key_weights(w, q, lse, small.values(*k), bt, ctx, [n], G,
+                                         scale=400.0), w)
+
+
 # ------------------------------------------------------------ eviction
 
 def _evict_inputs(g, totals, bs, H, D, bits, W=None):
