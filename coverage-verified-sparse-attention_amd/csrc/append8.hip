@@ -234,6 +234,8 @@ extern "C" int cvsa_append_chunk_kv8(
                "append_chunk_kv8: block_size=%d not in {8, 16, 32, 64, 128}", block_size);
   CVSA_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, CVSA_ERR_INVALID,
                "append_chunk_kv8: caches must be 16-byte aligned");
+  CVSA_REQUIRE(k_cache != v_cache && k_scales != v_scales, CVSA_ERR_INVALID,
+               "append_chunk_kv8: keys and values must have caches and scales of their own");
   RotaryArgs a = {};
   a.k = k; a.k_st = k_stride_t; a.k_sh = k_stride_h;
   a.v = v; a.v_st = v_stride_t; a.v_sh = v_stride_h;

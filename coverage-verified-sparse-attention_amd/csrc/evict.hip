@@ -910,8 +910,8 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
                (long long)W * block_size);
   CVSA_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, CVSA_ERR_INVALID,
                "evict_tokens: caches must be 16-byte aligned");
-  CVSA_REQUIRE(k_cache != v_cache, CVSA_ERR_INVALID,
-               "evict_tokens: keys and values must have caches of their own");
+  CVSA_REQUIRE(k_cache != v_cache && (!k_scales || k_scales != v_scales), CVSA_ERR_INVALID,
+               "evict_tokens: keys and values must have caches and scales of their own");
   const int64_t bh = (int64_t)B * H_kv;
   const int row_bytes = D * (k_scales ? 1 : 2);
   // More than the tables hold keeps all.

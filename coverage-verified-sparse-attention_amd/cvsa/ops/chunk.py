@@ -322,6 +322,9 @@ def prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens, lay
     dev = _same_device(k, v, k_cache, v_cache, block_tables, context_lens, q, q_weight, k_weight,
                        rotary.table if rotary else None, k_scales, v_scales)
     num_blocks, H_kv, D = _check_caches(who, k_cache, v_cache, block_size, k_scales, v_scales)
+    if k_scales is not None and (k_cache.data_ptr() == v_cache.data_ptr()
+                                 or k_scales.data_ptr() == v_scales.data_ptr()):
+        raise ValueError(f"{who}: keys and values must have caches and scales of their own")
     bt, bt_stride, ctx = _tables(who, layout, dev, block_tables, context_lens)
     B, W = bt.shape
     T, eps = layout.total, float(eps)
@@ -393,7 +396,8 @@ def append_chunk_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     before keeps its scale, or takes a larger one if the new tokens need it,
     to which its tokens are brought (a shift, exact but for values that become
     subnormal).  Payloads are rounded to nearest even; infinite and NaN values
-    become NaN.  No two sequences may append to one block.
+    become NaN.  No two sequences may append to one block, and keys and values
+    have caches and scales of their own.
     """
     launch, q_out = prepare_append_chunk(k, v, k_cache, v_cache, block_tables, context_lens,
                                          layout, block_size, rotary, k_weight, eps, q, q_weight,

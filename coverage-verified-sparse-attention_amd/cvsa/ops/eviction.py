@@ -112,10 +112,10 @@ def evict_tokens(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
     The caches are changed in place, the tables are not: the caller takes
     context_lens.clamp(max=keep) as the new lengths, once for all layers.
-    Pages must belong to one sequence alone, and k_cache and v_cache must not
-    be one tensor.  In caches of 8 bits a page that
-    tokens come to gets the largest scale of its tokens' pages, to which they
-    are brought (exact but for values that become subnormal).
+    Pages must belong to one sequence alone, and keys and values have caches
+    (and scales) of their own.  In caches of 8 bits a page that tokens come to
+    gets the largest scale of its tokens' pages, to which they are brought
+    (exact but for values that become subnormal).
 
     Returns [B, H_kv, keep] int32, the old slot of each new one (-1 past a
     shorter context).

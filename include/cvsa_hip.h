@@ -702,7 +702,8 @@ int cvsa_append_chunk_kv(const void *k, int64_t k_stride_t, int64_t k_stride_h,
  * before keeps its scale or gets a larger one, to which these are brought.
  * Payloads are rounded to nearest even; infinities and NaN become NaN.  Rows and
  * scales of other pages, and rows behind a context's end, are left as they are.  No
- * two sequences of the call may append to one block. */
+ * two sequences of the call may append to one block, and keys and values have caches
+ * and scales of their own. */
 int cvsa_append_chunk_kv8(const void *k, int64_t k_stride_t, int64_t k_stride_h,
                           const void *v, int64_t v_stride_t, int64_t v_stride_h,
                           const void *q, int64_t q_stride_t, int64_t q_stride_h,
@@ -808,8 +809,8 @@ int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q, int64_t q
  * or with scales of 8 bits: a page that tokens come to gets the largest scale of its
  * tokens' pages, to which their payloads are brought.  kept: [B, H_kv, keep], the
  * old slot of each new one (-1 past a shorter context).  Pages must belong to one
- * sequence, and keys and values have caches of their own; a token whose block is
- * outside the pool is not moved.  The workspace (256-byte aligned; cache_bits 16 or
+ * sequence, and keys and values have caches and scales of their own; a token whose
+ * block is outside the pool is not moved.  The workspace (256-byte aligned; cache_bits 16 or
  * 8; none may be needed) needs no initialisation. */
 size_t cvsa_evict_tokens_workspace_bytes(int32_t B, int32_t H_kv, int32_t D, int32_t block_size,
                                          int32_t W, int32_t cache_bits, int32_t keep,

@@ -463,3 +463,24 @@ def test_queries_far_apart_are_copied(calls, monkeypatch):
         ops.add_key_weights(**w)
         at, st_, sh_ = calls[-1][1][2:5]
         assert (st_, sh_) == ((HK * G * D, D) if copied else (st, sh))
+
+
+def test_c_caches_that_are_written_are_not_shared():
+    """Keys and values would write one row, or one byte of a scale, each its own."""
+    lib = _lib_or_skip()
+    for over in (dict(vc=P[2]), dict(vs=P[7])):
+        assert _append(lib, **over) == INVALID
+        assert b"of their own" in lib.cvsa_last_error()
+    assert _evict(lib, ks=P[7], vs=P[7]) == INVALID
+    assert b"of their own" in lib.cvsa_last_error()
+
+
+def test_caches_that_are_written_are_not_shared(calls):
+    a = _append_args()
+    for over in (dict(v_cache=a["k_cache"]), dict(v_scales=a["k_scales"])):
+        with pytest.raises(ValueError, match="of their own"):
+            ops.append_chunk_kv(**{**a, **over})
+    assert not calls
+    b = _attend_args()  # reading one is fine
+    ops.chunk_attention(**{**b, "v_cache": b["k_cache"], "v_scales": b["k_scales"]})
+    assert len(calls) == 1
