@@ -38,14 +38,17 @@ class DenseAttentionBackend:
                                 work=work)
 
     def prefill(self, q, k_cache, v_cache, block_tables, context_lens, layout, layer_idx=0,
-                causal=True, scale=None, max_context_len=0, k_scales=None, v_scales=None):
+                causal=True, scale=None, max_context_len=0, k_scales=None, v_scales=None,
+                return_lse=False):
         """Attention of a chunk of new tokens already in the cache:
         [T, H_q, D] queries laid out by ``layout`` (ops.ChunkLayout) ->
         [T, H_q, D].  Pass ``max_context_len``, the longest context, where the
         block tables are wider than the contexts (a manager's are), and the
         scales of caches of 8 bits, whose decode steps are chunks of one token
-        a sequence too.  No counterpart in the reference's backends, which only decode."""
+        a sequence too.  With ``return_lse`` also the log-sum-exps [T, H_q] that
+        ops.add_key_weights takes.  No counterpart in the reference's backends,
+        which only decode."""
         return ops.chunk_attention(q, k_cache, v_cache, block_tables, context_lens, layout,
                                    self.num_kv_heads, self.num_q_per_kv, self.block_size,
                                    causal=causal, scale=scale, max_context_len=max_context_len,
-                                   k_scales=k_scales, v_scales=v_scales)
+                                   return_lse=return_lse, k_scales=k_scales, v_scales=v_scales)

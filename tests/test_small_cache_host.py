@@ -484,3 +484,18 @@ def test_caches_that_are_written_are_not_shared(calls):
     b = _attend_args()  # reading one is fine
     ops.chunk_attention(**{**b, "v_cache": b["k_cache"], "v_scales": b["k_scales"]})
     assert len(calls) == 1
+
+
+def test_the_backends_prefill_returns_what_the_weights_need(calls):
+    from cvsa.runtime.dense import DenseAttentionBackend
+    a = _attend_args()
+    dense = DenseAttentionBackend(HK, HK * G, D, BS)
+    args = [a[x] for x in ("q", "k_cache", "v_cache", "block_tables", "context_lens", "layout")]
+    kw = dict(k_scales=a["k_scales"], v_scales=a["v_scales"])
+    assert dense.prefill(*args, **kw).shape == (T, HK * G, D)
+    out, lse = dense.prefill(*args, **kw, return_lse=True)
+    assert out.shape == (T, HK * G, D) and lse.shape == (T, HK * G)
+    assert lse.dtype == torch.float32
+    w = _weigh_args()
+    ops.add_key_weights(**{**w, "lse": lse})
+    assert [c[0] for c in calls] == ["cvsa_chunk_attention8"] * 2 + ["cvsa_add_key_weights"]
