@@ -529,7 +529,7 @@ class QuestPageMeta:
     ``scores(...)`` recomputes the pages whose valid-token count changed
     and scores every page, in one launch.  Valid while keys are only
     appended; ``invalidate()`` forgets every block (needed when blocks are
-    rewritten, e.g. reused for another sequence).
+    rewritten, e.g. reused for another sequence or cut by evict_tokens).
     """
 
     def __init__(self, k_cache: torch.Tensor):

@@ -112,6 +112,8 @@ def evict_tokens(weights: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
     The caches are changed in place, the tables are not: the caller takes
     context_lens.clamp(max=keep) as the new lengths, once for all layers.
+    What was learned of pages before no longer holds: ``reset()`` a CVSABackend
+    (its selections, Quest's extremes), ``invalidate()`` a QuestPageMeta.
     Pages must belong to one sequence alone, and keys and values have caches
     (and scales) of their own.  In caches of 8 bits a page that tokens come to
     gets the largest scale of its tokens' pages, to which they are brought

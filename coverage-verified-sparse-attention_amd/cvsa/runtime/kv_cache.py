@@ -374,7 +374,8 @@ class SequenceKVManager:
         """Cut every sequence to its ``keep`` tokens of the most attention weight
         (ops.evict_tokens), and its length (:meth:`cut`); returns the old slot
         of each new one.  With a cache per layer, ops.evict_tokens per layer
-        and :meth:`cut` once is the same."""
+        and :meth:`cut` once is the same.  reset() a CVSABackend that reads the
+        cache, and invalidate() a QuestPageMeta of it."""
         keep = self._check_cut(keep)
         kept = ops.evict_tokens(weights, self.cache.k_cache, self.cache.v_cache,
                                 self.block_tables, self.context_lens, keep, self.block_size,
@@ -384,7 +385,8 @@ class SequenceKVManager:
 
     def cut(self, keep: int) -> None:
         """Take no context as longer than ``keep`` tokens.  Pages stay with their
-        sequences, for the tokens to come.  Not while the stream is captured: a
+        sequences, for the tokens to come; what a CVSABackend or a QuestPageMeta
+        has learned of them is void (reset(), invalidate()).  Not while the stream is captured: a
         replay would cut without this manager's count."""
         keep = self._check_cut(keep)
         self.context_lens.clamp_(max=keep)

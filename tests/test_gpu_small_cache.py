@@ -9,6 +9,7 @@ import torch
 import chunk_reference as ref
 import small_cache_reference as small
 from cvsa import ops
+from cvsa.backend import CVSABackend
 from cvsa.runtime.dense import DenseAttentionBackend
 from cvsa.runtime.kv_cache import PagedKVCache, SequenceKVManager
 
@@ -1054,3 +1055,48 @@ def test_the_managers_other_appends(gpu):
                                Hk, 4, bs, max_context_len=22, k_scales=a.k_scales,
                                v_scales=a.v_scales)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("selector", ["exact", "quest"])
+def test_the_sparse_backend_over_a_cut_cache(gpu, selector):
+    """Cut, reset: the backend's steps are those of one that never saw the cache before
+    the cut, from its selections of pages to Quest's extremes of them."""
+    g = _gen(111)
+    B, Hk, G, D, bs, keep = 2, 4, 4, 128, 16, 600
+    cache = PagedKVCache(300, bs, Hk, D, device=gpu)
+    mgr = SequenceKVManager(cache, B, 2048)
+    for b, n in enumerate((1900, 1500)):
+        mgr.prefill_kv(b, *(_randn(g, n, Hk, D).bfloat16().to(gpu) for _ in range(2)))
+
+    def backend():
+        return CVSABackend(Hk, Hk * G, D, bs, num_layers=1, budget_pct=0.25, lazy=True,
+                           check_interval=3, selector=selector)
+
+    def step(*backends):
+        k, v = (_randn(g, B, Hk, D).bfloat16().to(gpu) for _ in range(2))
+        mgr.append_tokens_kv(k, v)
+        q = _randn(g, B, Hk * G, D).bfloat16().to(gpu)
+        outs = []
+        for x in backends:
+            outs.append(x(q, cache.k_cache, cache.v_cache, mgr.block_tables, mgr.context_lens, 0))
+            x.step_done(0, 1)
+        return q, outs
+
+    used = backend()
+    meta = ops.QuestPageMeta(cache.k_cache)
+    for _ in range(4):
+        q, _ = step(used)
+        meta.scores(q, mgr.block_tables, mgr.context_lens, Hk, G, bs)
+    w = torch.rand(B, Hk, mgr.block_tables.shape[1] * bs, generator=g).to(gpu)
+    mgr.evict_tokens(w, keep, 4, 64)
+    used.reset()
+    meta.invalidate()
+    fresh, new = backend(), ops.QuestPageMeta(cache.k_cache)
+    for _ in range(7):
+        q, (a, b) = step(used, fresh)
+        assert torch.equal(a, b)
+        assert torch.equal(used._cached_selection[0][0], fresh._cached_selection[0][0])
+        x, y = (m.scores(q, mgr.block_tables, mgr.context_lens, Hk, G, bs) for m in (meta, new))
+        assert torch.equal(x, y)
+    assert used.get_stats() == fresh.get_stats()
+    assert mgr.context_lens.tolist() == [keep + 7, keep + 7]
