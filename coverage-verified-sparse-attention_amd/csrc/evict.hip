@@ -62,7 +62,6 @@ struct EvictArgs {
   int32_t *pages;          // [1 + pages]: pages with arrivals, their number first
   // Long rows: of chunks.
   int chunks;              // of a row of the tables
-  int32_t *holes;          // [keep] slots to be filled
   uint16_t *hist;          // [3, chunks, kBins]
   uint32_t *above;         // [chunks]: weights above the bins chosen so far
   uint32_t *state;         // [4]: bins and what is still wanted, after passes 1 and 2
@@ -710,8 +709,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
       eq += s_before[1][v];
     }
   }
-  int32_t *const kept = a.kept + bh * a.keep, *const holes = a.holes + bh * a.keep;
-  int32_t *const tails = a.tails + bh * a.keep;
+  int32_t *const kept = a.kept + bh * a.keep, *const tails = a.tails + bh * a.keep;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     uint32_t count = 0;
@@ -732,9 +730,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_walk_kernel(const EvictAr
       const bool keep = larger || (same && e < want);
       if (j == front) a.n_holes[bh] = (int32_t)(m - rank);
       if (j < front) {
-        const int32_t hole = (int32_t)((uint32_t)(j - a.sinks) - rank);
-        kept[j] = keep ? j : -2 - hole;
-        if (!keep) holes[hole] = j;
+        kept[j] = keep ? j : -2 - (int32_t)((uint32_t)(j - a.sinks) - rank);
       } else if (keep) {
         tails[m - 1 - rank] = j;
       }
@@ -821,7 +817,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictArgs a, int 
 struct EvictPlan {
   bool long_rows, one_launch;
   int chunks, aside_pages;
-  size_t aside, aside_weights, aside_scales, holes, pages, hist, above, state, tails, n_holes;
+  size_t aside, aside_weights, aside_scales, pages, hist, above, state, tails, n_holes;
   size_t bytes;
 };
 
@@ -849,7 +845,6 @@ static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int64_t keys, int
   p.aside_weights = take((size_t)bh * recent * 4);
   p.aside_scales = take(f8 ? (size_t)bh * 2 * p.aside_pages : 0);
   if (p.long_rows) {
-    p.holes = take((size_t)bh * keep * 4);
     p.hist = take((size_t)bh * 3 * p.chunks * kBins * 2);
     p.above = take((size_t)bh * p.chunks * 4);
     p.state = take((size_t)bh * 16);
@@ -945,7 +940,6 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
   a.aside_weights = (float *)(ws + p.aside_weights);
   a.aside_scales = (uint8_t *)(ws + p.aside_scales);
   a.aside_pages = p.aside_pages;
-  a.holes = (int32_t *)(ws + p.holes);
   a.pages = (int32_t *)(ws + p.pages);
   a.chunks = p.chunks;
   a.hist = (uint16_t *)(ws + p.hist);

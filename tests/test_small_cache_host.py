@@ -499,3 +499,11 @@ def test_the_backends_prefill_returns_what_the_weights_need(calls):
     w = _weigh_args()
     ops.add_key_weights(**{**w, "lse": lse})
     assert [c[0] for c in calls] == ["cvsa_chunk_attention8"] * 2 + ["cvsa_add_key_weights"]
+
+
+def test_c_evict_of_long_rows_takes_a_number_for_each_kept_slot():
+    lib = _lib_or_skip()
+
+    def need(keep):
+        return lib.cvsa_evict_tokens_workspace_bytes(1, 8, 128, 16, 2048, 16, keep, 0, 0)
+    assert need(8192) - need(4096) == 4096 * 8 * 4
