@@ -830,6 +830,12 @@ static EvictPlan plan_evict(int64_t bh, int row_bytes, int bs, int64_t keys, int
     p.bytes += (n + 255) / 256 * 256;
     return at;
   };
+  // Tables that hold no more than is kept: nothing to cut or to move, and the plan
+  // kernel alone says so.
+  if (keep >= keys) {
+    p.one_launch = true;
+    return p;
+  }
   p.long_rows = keys > kShortRow;
   // One launch where a workgroup for each sequence and head is one for each compute
   // unit, or has little to move (rows at most, of keys): 256 of them, 4160 tokens to
@@ -909,7 +915,6 @@ extern "C" int cvsa_evict_tokens(float *weights, int64_t S, void *k_cache, void 
                "evict_tokens: keys and values must have caches and scales of their own");
   const int64_t bh = (int64_t)B * H_kv;
   const int row_bytes = D * (k_scales ? 1 : 2);
-  // More than the tables hold keeps all.
   const int64_t keys = (int64_t)W * block_size;
   const EvictPlan p = plan_evict(bh, row_bytes, block_size, keys, keep, recent,
                                  k_scales != nullptr);

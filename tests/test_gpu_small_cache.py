@@ -733,6 +733,17 @@ def test_evict_twice_in_place(gpu):
             assert ((x == y) | (x & 0x7f == 0x7f) & (y & 0x7f == 0x7f)).all()
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("W,bs,D", [(300, 64, 32), (40, 128, 256), (20, 16, 128)])
+def test_evict_keeps_all_that_the_tables_hold(gpu, bits, W, bs, D):
+    g = _gen(W + bits)
+    bt, ctx, k, v, w = _evict_inputs(g, [W * bs, 0, 77], bs, 1, D, bits)
+    ctx[0] += 9  # past the table
+    for keep in (W * bs, W * bs + 100):
+        for sinks, recent in ((0, 0), (4, 64), (0, keep)):
+            _check_evict(gpu, bt, ctx, k, v, w, keep, bs, sinks, recent)
+
+
 # ------------------------------------------------------------ sizes
 
 def test_more_sequences_than_a_wave_has_lanes(gpu):

@@ -507,3 +507,11 @@ def test_c_evict_of_long_rows_takes_a_number_for_each_kept_slot():
     def need(keep):
         return lib.cvsa_evict_tokens_workspace_bytes(1, 8, 128, 16, 2048, 16, keep, 0, 0)
     assert need(8192) - need(4096) == 4096 * 8 * 4
+
+
+def test_c_evict_of_tables_that_hold_no_more_than_is_kept_needs_nothing():
+    lib = _lib_or_skip()
+    for W, bs, D, bits in ((2048, 16, 128, 16), (260, 16, 128, 8), (40, 128, 256, 16)):
+        for keep in (W * bs, W * bs + 1, 1 << 24):
+            assert lib.cvsa_evict_tokens_workspace_bytes(1, 8, D, bs, W, bits, keep, 4, 256) == 0
+        assert lib.cvsa_evict_tokens_workspace_bytes(1, 8, D, bs, W, bits, W * bs - 1, 4, 256) > 0
