@@ -570,6 +570,21 @@ def test_weigh_scales_of_nan_and_the_largest(gpu, n):
                                          scale=400.0), w)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("window", [0, 2, 50])
+def test_weigh_chunks_longer_than_their_contexts(gpu, bits, window):
+    """Tokens at negative positions see nothing and bring no key."""
+    g = _gen(bits + window)
+    lens, bs, Hk, G, D = [4, 70, 3, 40, 7], 16, 2, 4, 64
+    q, k, keys, bt, ctx, w = _weigh_inputs(g, lens, [0] * 5, bs, Hk, G, D, bits)
+    ctx = torch.tensor([2, 33, 0, -9, 7], dtype=torch.int32)
+    for causal in (True, False):
+        lse = _lse(q, keys, bt, ctx, lens, G, causal)
+        got = _weigh(gpu, w, q, lse, k, bt, ctx, lens, G, bs, causal=causal, window=window)
+        _check_weigh(got, *small.key_weights(w, q, lse, keys, bt, ctx, lens, G, causal,
+                                             window=window), w)
+
+
 # ------------------------------------------------------------ eviction
 
 def _evict_inputs(g, totals, bs, H, D, bits, W=None):
