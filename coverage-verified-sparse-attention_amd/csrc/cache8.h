@@ -14,10 +14,8 @@ __device__ __forceinline__ int scale_byte(uint32_t top) {
   const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, kLowExponent), kHighExponent) + 127;
 }
-// 2^e, 0 below the normal numbers.
-__device__ __forceinline__ float power_of_two(int e) {
-  return e < -126 ? 0.f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23);
-}
+// 2^e, subnormal ones too (the inverse of a caller's own scale of 2^127).
+__device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
 __device__ __forceinline__ bool finite_bits(uint32_t u) {
   return (u & 0x7f800000u) != 0x7f800000u;
 }

@@ -188,6 +188,29 @@ def test_append_leaves_the_rest_as_it_was(gpu):
             assert torch.equal(got[n].cpu().view(torch.uint8), was[0][n].view(torch.uint8))
 
 
+def test_append_to_pages_of_the_callers_scales(gpu):
+    """Pages that held a token under scales that the append itself does not write: the
+    largest powers of two, and the least, which grow."""
+    D, bs = 32, 8
+    bytes_ = [254, 253, 250, 247, 0, 1, 16]
+    n = len(bytes_)
+    rows = torch.zeros(n, 1, D)
+    for i, b in enumerate(bytes_):
+        rows[i, 0, :4] = torch.tensor([1.0, 1.5, -1.75, 0.25]) * 2.0 ** min(b - 127, 127)
+    bt = torch.arange(n, dtype=torch.int32)[:, None]
+    ctx = torch.full((n,), 2, dtype=torch.int32)
+    cache = (torch.ones(n, bs, 1, D).to(torch.float8_e4m3fn),
+             small.to_scales(torch.tensor(bytes_)[:, None]))
+    (kc, ks), (vc, vs) = [[t.to(gpu) for t in cache] for _ in range(2)]
+    ops.append_chunk_kv(rows.to(gpu), rows.to(gpu), kc, vc, bt.to(gpu), ctx.to(gpu),
+                        ops.ChunkLayout([1] * n, gpu), bs, k_scales=ks, v_scales=vs)
+    y = rows.double()
+    for c, s in ((kc, ks), (vc, vs)):
+        small.check_appended(c, s, cache, small.appended(y, y.abs(), *cache, bt, ctx, [1] * n, 0.0))
+        assert small.scale_bytes(s)[:, 0].tolist() == [254, 253, 250, 247, 17, 17, 17]
+        assert torch.equal(small.values(c, s)[:4, 1], y[:4, 0, None])
+
+
 # ------------------------------------------------------------ attention
 
 def _attend_inputs(g, lens, before, bs, Hk, G, D, W=None):
