@@ -375,6 +375,27 @@ def test_attend_strided_queries_and_output_in_place(gpu):
     assert torch.equal(qg, want)
 
 
+@pytest.mark.parametrize("n", [1, 80])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_attend_scales_of_every_size(gpu, n, D):
+    """Scales that only a caller's own pages have, of values that bf16 holds."""
+    bs = 16
+    q = torch.zeros(n, 1, D)
+    for byte, payload in ((0, 448.0), (1, 1.5), (8, -2.0), (16, 448.0), (250, 1.75), (254, -1.0)):
+        k = torch.zeros(8, bs, 1, D).to(torch.float8_e4m3fn)
+        v = torch.full((8, bs, 1, D), payload).to(torch.float8_e4m3fn)
+        scales = small.to_scales(torch.full((8, 1), byte))
+        # Causal: the first token sees one key, so that no sum passes 32 bits there.
+        out = ops.chunk_attention(*_gpu(gpu, q.bfloat16(), k, v,
+                                        torch.arange(8, dtype=torch.int32)[None],
+                                        torch.tensor([n], dtype=torch.int32)),
+                                  ops.ChunkLayout([n], gpu), 1, 1, bs,
+                                  k_scales=scales.to(gpu), v_scales=scales.to(gpu))
+        want = payload * 2.0 ** (byte - 127)
+        got = (out if byte < 200 else out[:1]).double().cpu()
+        assert (got / want - 1).abs().max() <= 2.0 ** -8, (byte, got.flatten()[:2], want)
+
+
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_attend_few_rows_keeps_16_bits_of_the_weights(gpu, D):
     """Half of the keys have a weight of 1 and values of 1, the others a weight just
