@@ -258,7 +258,10 @@ static ChunkPlan plan_chunk(const int32_t *cu, int B, int H_q, int H_kv, int64_t
   const bool whole = max_keys <= 256;
   p.few.unit_log2 = p.many.unit_log2 = whole ? 31 : unit_log2;
   // A sequence's start and end cost a workgroup about as much as 3 units of 128 keys of
-  // 8 bits: counted so, 32 single tokens over up to 8 K keys take 62 us, 67 without.
+  // 8 bits.  Counted so and not, 32 single tokens over up to 8 K keys, 32 heads on 8: at
+  // D = 32 29.5 us and 33.3, 64 38.7 and 43.5, 128 68.5 and 73.8, 256 126 and 133; equal
+  // sequences lose 1% (8 drafts of 5 tokens at 32 K keys, 28 heads on 4: 44 and 43, 55
+  // and 54, 90 and 89, 210 and 209).
   p.few.extra_units = F8 && !whole ? 3 : 0;
   const int64_t units =
       (int64_t)p.few.tiles * (whole ? 1 : (max_keys + (1 << unit_log2) - 1) >> unit_log2);

@@ -24,13 +24,13 @@
 // decode kernels, which take single tokens only, need 88 us for the one sequence
 // (14 for one of 8 K keys, 15 here), and keep the weights of the second product in
 // two bf16 parts where these round them to one.
-// Over 8 bits: a token each of 32 sequences of up to 8 K keys, 32 heads on 8, 62 us and
-// 5 to join, 277 MB, 4.5 TB/s in the walk; 8 drafts of 5 tokens at 32 K keys, 28 heads
-// on 4, 71 and 6, 269 MB.  The conversions to bf16 stand before each product there: with
-// 35 rows they, the products and the loads' waits of a wave follow each other.  The
+// Over 8 bits: a token each of 32 sequences of up to 8 K keys, 32 heads on 8, 63 us and
+// 5 to join, 277 MB, 4.4 TB/s in the walk; 8 drafts of 5 tokens at 32 K keys, 28 heads
+// on 4, 80 to 85 and 6, 269 MB.  The conversions to bf16 stand before each product there:
+// with 35 rows they, the products and the loads' waits of a wave follow each other.  The
 // weights are kept in two bf16 parts there too, as no decode kernel reads such caches:
-// one part took 67.7 and 78 us with the join where two take 68.5 and 88 (the products
-// of the second parts behind those of all the first, not between them: 91).
+// one part took 67.7 and 78 us with the join where two take 68.5 and 86 to 90 (the
+// products of the second parts behind those of all the first, not between them: 91).
 #pragma once
 #include "chunk_common.h"
 
@@ -41,11 +41,11 @@ constexpr int chunk_stream_waves() {
   return D == 256 && !F8 ? 2 : 4;
 }
 
-// Over 8 bits each row tile has a workgroup of its own; those of the same keys run
-// next to each other on one XCD, whose L2 the second reads.  (Both tiles in a wave:
-// its registers are moved to and fro, and one wave to a SIMD takes its conversions,
-// products and waits in turns: 8 drafts of 5 tokens at 32 K keys, 28 heads on 4, 77 us
-// for 71.)
+// Over 8 bits each row tile has a workgroup of its own; those of the same keys run on
+// one XCD, whose L2 the second reads, where the ranges and KV heads are a multiple of
+// its 8 together.  (Both tiles in a wave: its registers are moved to and fro, and one
+// wave to a SIMD takes its conversions, products and waits in turns: 8 drafts of 5
+// tokens at 32 K keys, 28 heads on 4, with one part of the weights 77 us for 71.)
 //
 // Workgroups of a CU: by LDS one at D >= 128, two at 64; by registers at 32.  With
 // two row tiles one at 64 as well, whose fewer parts gain more than twice the
@@ -75,7 +75,9 @@ chunk_stream_kernel(const ChunkArgs a, const ChunkClass cl) {
   const int tid = threadIdx.x;
   // Over 8 bits the heads of a range go to one XCD: each of its rows has 128 bytes at
   // D = 128, and an XCD that reads all heads' draws on all of its L2's channels (plain
-  // reads of such rows: 5.2 TB/s with an XCD for each head, 5.6 so).
+  // reads of such rows: 5.2 TB/s with an XCD for each head, 5.6 so).  This holds for
+  // numbers of ranges that are multiples of the 8 XCDs, as powers of two of KV heads
+  // give over many keys; with others (3 heads: 170) a range's heads are spread.
   const uint32_t n_ranges = gridDim.x / a.H_kv;
   const uint32_t range = F8 ? blockIdx.x % n_ranges : blockIdx.x / a.H_kv;
   const ChunkSeq first = chunk_look(a, cl, tid & 63);

@@ -24,9 +24,12 @@
 // order, and workgroups of the first launch copy the window's rows aside.
 //
 // Measured: 32 sequences of 8 heads, 4160 tokens to 4096, 256 of them recent, 8 bits: 26
-// to 30 us in one launch for 51 MB (23 where the caches hold some of them; 12 until the
-// rows are known); 131072 to 16384, 8 heads of bf16: 7 + 7 + 7 + 9 and 13, for 125 MB.
-// Both are chains of short dependent steps, not bound by a rate.
+// to 30 us in one launch for 51 MB (23 where the caches hold some of them, 39 where they
+// hold none; 12 until the rows are known); a first cut of 131072 to 16384, 8 heads of
+// bf16, 14600 rows a head: 7 + 7 + 7 + 10 and 28 to move 120 MB (41 from memory alone).
+// Cut again at the same length, as a loop of calls does, the heaviest tokens are in
+// front already: 8200 rows, then 5900, 4700 .., moved in 25 us to 12.  The plans are
+// chains of short dependent steps, not bound by a rate.
 //
 // 8 bits: a page with arrivals gets the largest scale of its tokens' pages; payloads
 // are shifted to it, which rounds only what becomes subnormal.

@@ -175,7 +175,8 @@ __global__ __launch_bounds__(256, (weigh_few_fit<D, F8>())) void weigh_few_kerne
   constexpr int KS = D / 16;
   const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The heads of a range go to one XCD: see the chunk attention of few rows.
+  // The heads of a range go to one XCD, where the workgroups of a head are a multiple of
+  // 8 (powers of two of KV heads): see the chunk attention of few rows.
   const uint32_t n_wgs = gridDim.x / a.H_kv;
   const int h = blockIdx.x / n_wgs;
   const uint32_t range = blockIdx.x % n_wgs * 4 + wave, ranges = n_wgs * 4;

@@ -465,7 +465,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the rest is the same, but that sequences of up to 64 rows (tokens times
     num_q_per_kv; 32 at D = 256) keep 16 bits of the weights: single tokens
     and drafts, which no decode kernel takes over such caches.  A scale of NaN
-    makes its block's values NaN.
+    makes its block's values NaN; under one past 2^119, which the append does not
+    write, values that bf16 does not hold make their outputs infinite or NaN.
     """
     who = "chunk_attention"
     dev = _same_device(q, k_cache, v_cache, block_tables, context_lens, out, k_scales, v_scales)

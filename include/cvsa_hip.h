@@ -757,8 +757,9 @@ int cvsa_chunk_attention(const uint16_t *q, int64_t q_stride_t, int64_t q_stride
                          size_t workspace_bytes, void *stream);
 
 /* cvsa_chunk_attention over caches of 8 bits (see cvsa_append_chunk_kv8), which are
- * brought to bf16, exactly, on their way to the products.  The workspace's size is
- * its own. */
+ * brought to bf16, exactly, on their way to the products (scales past 2^119 can bring
+ * them past it).  Sequences of up to 64 rows of a KV head, 32 at D = 256, keep 16 bits of
+ * the second product's weights, others 8.  The workspace's size is its own. */
 size_t cvsa_chunk_attention8_workspace_bytes(const int32_t *cu_host, int32_t B, int32_t H_q,
                                              int32_t H_kv, int32_t D, int32_t block_size,
                                              int32_t W, int32_t max_context_len);
