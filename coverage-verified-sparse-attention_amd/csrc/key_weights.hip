@@ -867,7 +867,7 @@ extern "C" int cvsa_add_key_weights(float *weights, int64_t S, const uint16_t *q
   const int64_t pass_rows = D == 256 ? weigh_rows<256>() : weigh_rows<128>();
   CVSA_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0, CVSA_ERR_INVALID,
                "add_key_weights: negative stride of the queries");
-  CVSA_REQUIRE(!p.many || (q_stride_t < (1LL << 31) && q_stride_h < (1LL << 31) &&
+  CVSA_REQUIRE(!p.many || (q_stride_t < (1LL << 31) && (G == 1 || q_stride_h < (1LL << 31)) &&
                            (pass_rows + G - 2) / G * q_stride_t + (G - 1) * q_stride_h <
                                (1LL << 31)),
                CVSA_ERR_UNSUPPORTED, "add_key_weights: queries too far apart");

@@ -450,6 +450,8 @@ def test_c_weigh_refuses_queries_that_32_bits_cannot_span():
     # Those that it can are asked for their workspace.
     for g, st, sh in ((4, D, 1 << 23), (4, 1 << 25, D), (1, 1 << 24, D), (4, 1 << 24, 1 << 28)):
         assert _weigh(lib, cu=(0, 2000), H_q=HK * g, st=st, sh=sh) == _lib.CVSA_ERR_WORKSPACE
+    # Groups of one head: none is far from its group's first.
+    assert _weigh(lib, cu=(0, 2000), H_q=HK, st=D, sh=1 << 40) == _lib.CVSA_ERR_WORKSPACE
     assert _weigh(lib, st=-8) == INVALID
 
 
