@@ -154,6 +154,7 @@ class SequenceKVManager:
         n_pages = (seq_len + bs - 1) // bs
         launch = None
         if self.cache.k_scales is not None:  # checked before a block is taken
+            self._refuse_capture()  # the layout is copied from the host
             if n_pages > self.max_pages:
                 raise IndexError(f"a prompt of {seq_len} tokens exceeds the block table "
                                  f"({self.max_pages} pages)")
@@ -290,6 +291,7 @@ class SequenceKVManager:
                 raise ValueError(f"{n} rows of keys and {v.shape[0]} of values")
             layout = self._token_layouts.get((seq_begin, n))
             if layout is None:
+                self._refuse_capture()
                 lens = [int(s in seqs) for s in range(self.batch_size)]
                 layout = self._token_layouts[seq_begin, n] = ops.ChunkLayout(
                     lens, self.cache.config.device)
@@ -317,15 +319,18 @@ class SequenceKVManager:
         written by ops.append_chunk_kv.  Not while the stream is captured: a
         replay would give the same blocks out again, without this manager's
         count of them."""
-        if ops.chunk.capturing(self.block_tables.device):
-            raise RuntimeError("a manager's pages cannot be taken in a captured graph: reserve "
-                               "them before it, capture ops.append_chunk_kv")
+        self._refuse_capture()
         need, pages = self._plan_chunk(layout)
         ops.reserve_chunk(self.block_tables, self.context_lens, self._pages_allocated_dev, layout,
                           self.cache._next_free, self.cache._total_blocks, self.block_size)
         self.cache._reserve(need)
         self._pages_allocated = pages
         self._ctx_host = [c + n for c, n in zip(self._ctx_host, layout.lens)]
+
+    def _refuse_capture(self) -> None:
+        if ops.chunk.capturing(self.block_tables.device):
+            raise RuntimeError("a manager's pages cannot be taken in a captured graph: reserve "
+                               "them before it, capture ops.append_chunk_kv")
 
     def _plan_chunk(self, layout):
         """(blocks a chunk takes, pages allocated after it); refuses a chunk

@@ -517,3 +517,21 @@ def test_c_evict_of_tables_that_hold_no_more_than_is_kept_needs_nothing():
         for keep in (W * bs, W * bs + 1, 1 << 24):
             assert lib.cvsa_evict_tokens_workspace_bytes(1, 8, D, bs, W, bits, keep, 4, 256) == 0
         assert lib.cvsa_evict_tokens_workspace_bytes(1, 8, D, bs, W, bits, W * bs - 1, 4, 256) > 0
+
+
+def test_no_append_of_the_managers_to_8_bits_is_captured(calls, monkeypatch):
+    """Refused before a layout is copied from the host, which would end the capture."""
+    cache, mgr = _manager()
+    rows = _bf(2, HK, D)
+
+    def layout(*a):
+        raise AssertionError("a copy to the device in a capture")
+    monkeypatch.setattr(kv_cache.ops.chunk, "capturing", lambda dev: True)
+    monkeypatch.setattr(kv_cache.ops, "ChunkLayout", layout)
+    for call in (lambda: mgr.append_tokens_kv(rows, rows),
+                 lambda: mgr.append_token_kv(1, rows[0], rows[0]),
+                 lambda: mgr.prefill_kv(0, _bf(20, HK, D), _bf(20, HK, D))):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    assert mgr._ctx_host == [0, 0] and cache._next_free == 0 and not calls
+    assert not mgr._token_layouts
